@@ -452,6 +452,89 @@ int ptcg_attention_bwd(int operand_dtype, const void* qkv, long ldqkv, const uns
                        const void* out, long ldo, const void* dout, long lddo, const float* lse,
                        void* dqkv, long lddqkv, float* dbias, int nseq, int L, int H,
                        void* stream);
+/* ---- decoder operators ------------------------------------------------------
+ * The operators of a decoder that reads this model's encoder rows (options,
+ * beams or drafted decks as queries, the board as states), for callers that
+ * build one beside the policy: embedding, layer norm and cross attention,
+ * forward and backward.  They take no model; they run on the current device
+ * and on `stream`, allocate nothing, wait for nothing on the host and can be
+ * captured in a CUDA graph.  Element types are PTCG_FP32 / PTCG_BF16;
+ * statistics, sums and weight gradients are fp32.  Scratch (16-byte aligned
+ * device memory of the size the _scratch call gives) holds nothing between
+ * calls; calls that may overlap, replayed graphs included, need their own.
+ * No result depends on scheduling: equal inputs give equal bits.
+ *
+ * Embedding: out[i, :] = scale * table[ids[i], :], n places, rows of `width`
+ * at pitches ldt / ldo (elements).  Ids are clamped to [0, vocab) as the
+ * model's gathers clamp theirs; a place whose id equals pad_id (>= 0; pass -1
+ * for none) gives zeros and takes no gradient.  The gradient sorts the places
+ * by id and writes every row of dtable (vocab x width fp32, pitch lddt) once:
+ *   dtable[v, :] = scale * sum of dout[i, :] over ids[i] = v, in place order
+ * (0 for a row without places; accumulate != 0 adds to what is there).
+ * Replaces the gathers and atomic scatter-adds of k_tok_cat / k_tok_cat_bwd
+ * (native/model/ptcg_model.cu:289-321, ptcg_model2.cu:36-64) for callers with
+ * their own token tables. */
+int ptcg_embedding_fwd(const void* table, int table_dtype, long ldt, int vocab, int width,
+                       const int* ids, long n, float scale, int pad_id, void* out, int out_dtype,
+                       long ldo, void* stream);
+long ptcg_embedding_bwd_scratch(long n, int vocab, int width);
+int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* ids, long n,
+                       float scale, int pad_id, float* dtable, long lddt, int vocab, int width,
+                       int accumulate, void* scratch, long scratch_bytes, void* stream);
+
+/* Layer norm over rows of `width` <= PTCG_LN_MAX_WIDTH elements:
+ * y = (x - mean) * rstd * gamma + beta, rstd = (var + eps)^(-1/2).  gamma /
+ * beta NULL mean 1 / 0; mean / rstd (one float per row, what the backward
+ * needs) may be NULL.  y may be x when the types and pitches agree.
+ * Backward: dx (x's type) = the gradient through the norm, plus dres (x's
+ * type, may be NULL: the residual stream's own gradient); dgamma / dbeta
+ * (fp32, both or neither) are written, or added to with accumulate != 0.
+ * dx may be dres, or dy when the types and pitches agree.  The reference
+ * norms with k_ln_fwd / k_ln_bwd (native/model/ptcg_kernels.cuh) inside its
+ * model only. */
+#define PTCG_LN_MAX_WIDTH 8192
+int ptcg_layer_norm_fwd(const void* x, int x_dtype, long ldx, const float* gamma,
+                        const float* beta, float eps, void* y, int y_dtype, long ldy, float* mean,
+                        float* rstd, long rows, int width, void* stream);
+long ptcg_layer_norm_bwd_scratch(long rows, int width);
+int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, int x_dtype,
+                        long ldx, const float* gamma, const float* mean, const float* rstd,
+                        const void* dres, long lddres, void* dx, long lddx, float* dgamma,
+                        float* dbeta, int accumulate, long rows, int width, void* scratch,
+                        long scratch_bytes, void* stream);
+
+/* Cross attention: `lq` query rows of each of nseq sequences over that
+ * sequence's lk key rows (an encoder's states or a cache), heads query heads
+ * in groups of heads / kv_heads per key head, head width dh 32, 64 or 128:
+ *   S = scale q k^T, P = softmax over the kept keys, out = P v,
+ *   lse[s, head, i] = log sum exp S (natural log).
+ * Key j of sequence s is kept when j < kv_len[s] (int32 per sequence, clamped
+ * to [0, lk]; NULL: lk) and keep[s * lk + j] != 0 (NULL: all).  Masked keys
+ * are not read: they may hold anything.  A query row with no kept key gets
+ * out = 0, lse = -inf and takes no gradient.  Backward (out and lse from the
+ * forward): dq, dk, dv; dk / dv are summed over a group's query heads and are
+ * zero for masked keys.  Each tensor has its own strides in elements:
+ * element (s, row, head, d) at p + s * seq + row * row + head * head + d.
+ * bf16 runs on tensor cores with fp32 sums (P and dS are rounded to bf16 as
+ * operands); fp32 is exact.  Rows must start on 16-byte boundaries (strides
+ * multiples of 16 bytes).  Beside ptcg_attention_fwd / _bwd, which take
+ * packed self-attention rows of width 32. */
+typedef struct PtcgHeads { long seq, row, head; } PtcgHeads;
+typedef struct PtcgCross {
+    int dtype, nseq, lq, lk, heads, kv_heads, dh;
+    float scale;
+    PtcgHeads q, k, v, out;              /* forward */
+    PtcgHeads dout, dq, dk, dv;          /* backward */
+} PtcgCross;
+long ptcg_cross_attention_fwd_scratch(const PtcgCross* c);
+int ptcg_cross_attention_fwd(const PtcgCross* c, const void* q, const void* k, const void* v,
+                             const unsigned char* keep, const int* kv_len, void* out, float* lse,
+                             void* scratch, long scratch_bytes, void* stream);
+long ptcg_cross_attention_bwd_scratch(const PtcgCross* c);
+int ptcg_cross_attention_bwd(const PtcgCross* c, const void* q, const void* k, const void* v,
+                             const unsigned char* keep, const int* kv_len, const void* out,
+                             const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                             void* scratch, long scratch_bytes, void* stream);
 /* The GELU and GELU' that the tensor-core GEMM epilogues evaluate (the
  * normal tail erfc(|x|/sqrt 2)/2 as the normal pdf times a degree-7
  * polynomial in |x|, fitted for this library with its error weighted by the

@@ -1,0 +1,1288 @@
+// Cross attention: query rows over an encoder's states (or a cache) of
+// another length, forward and backward, head width 32, 64 or 128.
+//   S = scale q k^T over the kept keys, lse = log sum exp S, P = exp(S - lse),
+//   out = P v;
+//   delta = dout . out, dS = P o (dout v^T - delta),
+//   dq = scale dS k, dk = scale dS^T q, dv = P^T dout.
+// There is no order between queries and keys, so the lq rows of the query
+// heads that share a key head are stacked into R = group * lq rows of one
+// problem per (sequence, key head): grouped heads fill the same tiles as more
+// queries would, and dk / dv sum over the group by themselves.
+//
+// Masked keys never reach a sum: their K and V rows are filled with zeros
+// instead of being loaded and their probabilities are set to 0, so whatever
+// they hold (NaN, infinities, rows never written) has no effect.
+#include <algorithm>
+
+#include "vec.cuh"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct CrossArgs {
+    const void *q, *k, *v, *o, *dout;
+    const uint8_t* keep;
+    const int* kv_len;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;
+    // split work: fp32 partial rows and, in the forward, their (max, sum)
+    float *part, *part2;
+    float2* part_ml;
+    PtcgHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    int lq, lk, heads, kv_heads, group, rows;      // rows = group * lq
+    int tiles, nsplit, split;                      // `split` rows of the split axis per part
+    float scale;
+};
+
+// element offset of stacked row r of key head hk in a query-like tensor
+PTCG_DEV long qrow(const CrossArgs& a, const PtcgHeads& s, int seq, int hk, int r) {
+    const int g = r / a.lq;
+    return seq * s.seq + (r - g * a.lq) * s.row + (long)(hk * a.group + g) * s.head;
+}
+PTCG_DEV long krow(const PtcgHeads& s, int seq, int hk, int j) {
+    return seq * s.seq + j * s.row + hk * s.head;
+}
+PTCG_DEV int kept_len(const CrossArgs& a, int seq) {
+    return a.kv_len ? min(max(a.kv_len[seq], 0), a.lk) : a.lk;
+}
+PTCG_DEV bool kept(const CrossArgs& a, int seq, int j, int len) {
+    return j < len && (!a.keep || a.keep[(long)seq * a.lk + j] != 0);
+}
+// block index -> (tile of the problem, part of the split axis, key head, sequence)
+struct Where { int tile, part, hk, seq; };
+PTCG_DEV Where where(const CrossArgs& a) {
+    Where w;
+    unsigned b = blockIdx.x;
+    w.tile = b % a.tiles; b /= a.tiles;
+    w.part = b % a.nsplit; b /= a.nsplit;
+    w.hk = b % a.kv_heads;
+    w.seq = b / a.kv_heads;
+    return w;
+}
+
+// ------------------------------------------------------- mma.sync pieces
+PTCG_DEV uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+PTCG_DEV void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+PTCG_DEV void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+PTCG_DEV void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+                 "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+PTCG_DEV void cp16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 :: "r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+PTCG_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> PTCG_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// bf16 tiles of DH columns without padding: the 16-byte pieces of a row are
+// permuted by the row so that the eight rows an ldmatrix phase touches fall
+// into different banks (a 64-byte row shares its 128-byte line with its
+// neighbour, hence row / 2 there)
+template <int DH> PTCG_DEV uint32_t tile_off(int row, int piece) {
+    const int x = DH == 32 ? (row >> 1) & 3 : row & 7;
+    return (uint32_t)(row * DH * 2 + ((piece ^ x) << 4));
+}
+// A fragment of rows r0 .. +15, columns 16 ks ..
+template <int DH> PTCG_DEV void frag_a(uint32_t (&f)[4], uint32_t base, int r0, int ks, int lane) {
+    const int mi = lane >> 3;
+    ldsm4(f, base + tile_off<DH>(r0 + (mi & 1) * 8 + (lane & 7), ks * 2 + (mi >> 1)));
+}
+// B fragments of B[k][n] = X[n][k]: rows n0 .. +15 of X, columns 16 ks ..
+template <int DH> PTCG_DEV void frag_bn(uint32_t (&f)[4], uint32_t base, int n0, int ks, int lane) {
+    const int mi = lane >> 3;
+    ldsm4(f, base + tile_off<DH>(n0 + (mi >> 1) * 8 + (lane & 7), ks * 2 + (mi & 1)));
+}
+// B fragments of B[k][n] = X[k][n]: rows k0 .. +15 of X, columns 16 nd ..
+template <int DH> PTCG_DEV void frag_bk(uint32_t (&f)[4], uint32_t base, int k0, int nd, int lane) {
+    const int mi = lane >> 3;
+    ldsm4t(f, base + tile_off<DH>(k0 + (mi & 1) * 8 + (lane & 7), nd * 2 + (mi >> 1)));
+}
+// stacked query rows r0 .. +N into a tile; rows past R are zeros
+template <int DH, int N, int THREADS>
+PTCG_DEV void stage_q(uint32_t dst, const bf16* src, const PtcgHeads& s, const CrossArgs& a,
+                      int seq, int hk, int r0) {
+    constexpr int P = DH / 8;
+    for (int i = threadIdx.x; i < N * P; i += THREADS) {
+        const int r = i / P, c = i % P;
+        const bool in = r0 + r < a.rows;
+        cp16(dst + tile_off<DH>(r, c), src + (in ? qrow(a, s, seq, hk, r0 + r) + c * 8 : 0), in);
+    }
+}
+// key rows j0 .. +N into a tile; rows whose bit is clear are zeros
+template <int DH, int N, int THREADS>
+PTCG_DEV void stage_k(uint32_t dst, const bf16* src, const PtcgHeads& s, int seq, int hk, int j0,
+                      const uint32_t* bits) {
+    constexpr int P = DH / 8;
+    for (int i = threadIdx.x; i < N * P; i += THREADS) {
+        const int r = i / P, c = i % P;
+        const bool in = (bits[r >> 5] >> (r & 31)) & 1;
+        cp16(dst + tile_off<DH>(r, c), src + (in ? krow(s, seq, hk, j0 + r) + c * 8 : 0), in);
+    }
+}
+PTCG_DEV float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+PTCG_DEV float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+// ---------------------------------------------------------- bf16 forward
+// A block owns 16 WM stacked rows and walks its keys 64 at a time through NST
+// cp.async stages; the running maximum, sum and output rows stay in registers
+// and P goes from the accumulators of S straight into the operand of P V
+// (rounded to bf16: 2^-9 of each probability, the size of the output's own
+// rounding).  WN = 4 is the form for at most 16 rows (single tokens): the four
+// warps take 16 keys each of every tile and are joined at the end.
+template <int DH, int WM, int WN, int NST>
+__global__ void __launch_bounds__(WM * WN * 32) k_cross_fwd(const __grid_constant__ CrossArgs a) {
+    constexpr int THREADS = WM * WN * 32, BM = WM * 16, BN = 64, KW = BN / WN, NT = KW / 8;
+    constexpr int KS = DH / 16, TILE = BN * DH * 2;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t bits[NST + 1][2];
+    const uint32_t sQ = s_addr(sm), sK = sQ + BM * DH * 2, sV = sK + NST * TILE;
+    const Where at = where(a);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wm = WN == 1 ? warp : 0, wn = WN == 1 ? 0 : warp;
+    const int r0 = at.tile * BM, len = kept_len(a, at.seq);
+    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    const int nt = (kend - kbeg + BN - 1) / BN;
+    const bf16 *K = (const bf16*)a.k, *V = (const bf16*)a.v;
+
+    auto mask_byte = [&](int j) {           // this lane's key of tile j
+        const int key = kbeg + j * BN + warp * 32 + lane;
+        return warp < 2 && key < kend && kept(a, at.seq, key, len);
+    };
+    auto put_bits = [&](int j, bool b) {
+        const uint32_t m = __ballot_sync(0xffffffffu, b);
+        if (warp < 2 && lane == 0) bits[j % (NST + 1)][warp] = m;
+    };
+    auto load = [&](int j) {
+        if (j < nt) {
+            const uint32_t* b = bits[j % (NST + 1)];
+            stage_k<DH, BN, THREADS>(sK + (j % NST) * TILE, K, a.sk, at.seq, at.hk, kbeg + j * BN, b);
+            stage_k<DH, BN, THREADS>(sV + (j % NST) * TILE, V, a.sv, at.seq, at.hk, kbeg + j * BN, b);
+        }
+        cp_commit();
+    };
+    #pragma unroll
+    for (int j = 0; j < NST; j++) put_bits(j, mask_byte(j));
+    stage_q<DH, BM, THREADS>(sQ, (const bf16*)a.q, a.sq, a, at.seq, at.hk, r0);
+    __syncthreads();
+    #pragma unroll
+    for (int j = 0; j < NST - 1; j++) load(j);
+
+    float o[DH / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    #pragma unroll
+    for (int i = 0; i < DH / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    uint32_t qf[KS][4];
+    const float sc = a.scale * LOG2E;
+    const int t = lane & 3;
+    for (int j = 0; j < nt; j++) {
+        const bool next = mask_byte(j + NST);
+        cp_wait<NST - 2>();
+        __syncthreads();
+        load(j + NST - 1);
+        if (j == 0) {
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) frag_a<DH>(qf[ks], sQ, wm * 16, ks, lane);
+        }
+        const uint32_t w0 = bits[j % (NST + 1)][0], w1 = bits[j % (NST + 1)][1];
+        // this warp's keys: all 64, or its 16
+        const uint32_t v0 = WN == 1 ? w0 : ((wn & 2 ? w1 : w0) >> ((wn & 1) * 16)) & 0xffffu;
+        const uint32_t v1 = WN == 1 ? w1 : 0u;
+        if (v0 | v1) {
+            const uint32_t kt = sK + (j % NST) * TILE, vt = sV + (j % NST) * TILE;
+            float s[NT][4];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                #pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    uint32_t b[4];
+                    frag_bn<DH>(b, kt, wn * KW + i * 16, ks, lane);
+                    mma(s[2 * i], qf[ks], b[0], b[1]);
+                    mma(s[2 * i + 1], qf[ks], b[2], b[3]);
+                }
+            }
+            if ((v0 & v1) != 0xffffffffu) {
+                #pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const uint32_t w = (i < 4 ? v0 : v1) >> ((i & 3) * 8 + 2 * t);
+                    if (!(w & 1)) s[i][0] = s[i][2] = -INFINITY;
+                    if (!(w & 2)) s[i][1] = s[i][3] = -INFINITY;
+                }
+            }
+            float x0 = -INFINITY, x1 = -INFINITY;
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                x0 = fmaxf(x0, fmaxf(s[i][0], s[i][1]));
+                x1 = fmaxf(x1, fmaxf(s[i][2], s[i][3]));
+            }
+            const float n0 = fmaxf(m0, quad_max(x0) * sc), n1 = fmaxf(m1, quad_max(x1) * sc);
+            // a row whose keys so far are all masked keeps a zero sum
+            const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
+            if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+                const float c0 = ex2_approx(m0 - u0), c1 = ex2_approx(m1 - u1);
+                l0 *= c0;
+                l1 *= c1;
+                #pragma unroll
+                for (int i = 0; i < DH / 8; i++) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
+            }
+            m0 = n0;
+            m1 = n1;
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                s[i][0] = ex2_approx(fmaf(s[i][0], sc, -u0));
+                s[i][1] = ex2_approx(fmaf(s[i][1], sc, -u0));
+                s[i][2] = ex2_approx(fmaf(s[i][2], sc, -u1));
+                s[i][3] = ex2_approx(fmaf(s[i][3], sc, -u1));
+                l0 += s[i][0] + s[i][1];
+                l1 += s[i][2] + s[i][3];
+            }
+            #pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                const uint32_t p[4] = {pack_bf2(s[2 * i][0], s[2 * i][1]), pack_bf2(s[2 * i][2], s[2 * i][3]),
+                                       pack_bf2(s[2 * i + 1][0], s[2 * i + 1][1]),
+                                       pack_bf2(s[2 * i + 1][2], s[2 * i + 1][3])};
+                #pragma unroll
+                for (int d = 0; d < KS; d++) {
+                    uint32_t b[4];
+                    frag_bk<DH>(b, vt, wn * KW + i * 16, d, lane);
+                    mma(o[2 * d], p, b[0], b[1]);
+                    mma(o[2 * d + 1], p, b[2], b[3]);
+                }
+            }
+        }
+        put_bits(j + NST, next);
+    }
+    cp_wait<0>();
+    l0 = quad_sum(l0);
+    l1 = quad_sum(l1);
+    const int g = lane >> 2;
+    if (WN > 1) {
+        // join the four warps' key shares: [WN][16] max and sum, [WN][16][DH] output
+        __syncthreads();
+        float* jm = (float*)sm;
+        float* jl = jm + WN * 16;
+        float* jo = jl + WN * 16;
+        if (t == 0) {
+            jm[wn * 16 + g] = m0; jm[wn * 16 + g + 8] = m1;
+            jl[wn * 16 + g] = l0; jl[wn * 16 + g + 8] = l1;
+        }
+        #pragma unroll
+        for (int i = 0; i < DH / 8; i++) {
+            float* p = jo + (wn * 16 + g) * DH + i * 8 + 2 * t;
+            *(float2*)p = make_float2(o[i][0], o[i][1]);
+            *(float2*)(p + 8 * DH) = make_float2(o[i][2], o[i][3]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * DH / 2; i += THREADS) {
+            const int r = i / (DH / 2), d = i % (DH / 2) * 2;
+            if (r0 + r >= a.rows) continue;
+            float m = -INFINITY, l = 0.f, y0 = 0.f, y1 = 0.f;
+            #pragma unroll
+            for (int k = 0; k < WN; k++) m = fmaxf(m, jm[k * 16 + r]);
+            const float u = m == -INFINITY ? 0.f : m;
+            #pragma unroll
+            for (int k = 0; k < WN; k++) {
+                const float c = ex2_approx(jm[k * 16 + r] - u);
+                const float2 x = *(const float2*)(jo + (k * 16 + r) * DH + d);
+                l = fmaf(jl[k * 16 + r], c, l);
+                y0 = fmaf(x.x, c, y0);
+                y1 = fmaf(x.y, c, y1);
+            }
+            const long row = ((long)at.seq * a.kv_heads + at.hk) * a.rows + r0 + r;
+            if (a.nsplit > 1) {
+                *(float2*)(a.part + (row * a.nsplit + at.part) * DH + d) = make_float2(y0, y1);
+                if (d == 0) a.part_ml[row * a.nsplit + at.part] = make_float2(m, l);
+            } else {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                *(uint32_t*)((bf16*)a.out + qrow(a, a.so, at.seq, at.hk, r0 + r) + d) =
+                    pack_bf2(y0 * inv, y1 * inv);
+                if (d == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+            }
+        }
+        return;
+    }
+    const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int r = r0 + wm * 16 + g + half * 8;
+        if (r >= a.rows) continue;
+        const long row = ((long)at.seq * a.kv_heads + at.hk) * a.rows + r;
+        const float m = half ? m1 : m0, l = half ? l1 : l0, inv = half ? i1 : i0;
+        if (a.nsplit > 1) {
+            float* p = a.part + (row * a.nsplit + at.part) * DH;
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++)
+                *(float2*)(p + i * 8 + 2 * t) = make_float2(o[i][2 * half], o[i][2 * half + 1]);
+            if (t == 0) a.part_ml[row * a.nsplit + at.part] = make_float2(m, l);
+        } else {
+            bf16* p = (bf16*)a.out + qrow(a, a.so, at.seq, at.hk, r);
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++)
+                *(uint32_t*)(p + i * 8 + 2 * t) = pack_bf2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+            if (t == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        }
+    }
+}
+
+// joins the parts of a split forward: a warp per stacked row
+template <typename T, int DH>
+__global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ CrossArgs a, long nrows) {
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= nrows) return;
+    const float2* ml = a.part_ml + row * a.nsplit;
+    float m = -INFINITY;
+    for (int i = lane; i < a.nsplit; i += 32) m = fmaxf(m, ml[i].x);
+    m = warp_max(m);
+    const float u = m == -INFINITY ? 0.f : m;
+    float l = 0.f, y[DH / 32];
+    #pragma unroll
+    for (int e = 0; e < DH / 32; e++) y[e] = 0.f;
+    const float* p = a.part + row * a.nsplit * DH + lane;
+    #pragma unroll 4
+    for (int i = 0; i < a.nsplit; i++) {
+        const float2 x = ml[i];
+        const float c = ex2_approx(x.x - u);
+        l = fmaf(x.y, c, l);
+        #pragma unroll
+        for (int e = 0; e < DH / 32; e++) y[e] = fmaf(p[(long)i * DH + e * 32], c, y[e]);
+    }
+    const long b = row / a.rows;
+    const int seq = (int)(b / a.kv_heads), hk = (int)(b % a.kv_heads), r = (int)(row - b * a.rows);
+    T* out = (T*)a.out + qrow(a, a.so, seq, hk, r) + lane;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    #pragma unroll
+    for (int e = 0; e < DH / 32; e++) out[e * 32] = from_f<T>(y[e] * inv);
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// --------------------------------------------------------- bf16 backward
+// dq: a block owns 64 stacked rows (16 a warp) with q, dout and dq in
+// registers and walks the keys; it also writes delta = dout . out for the
+// dk / dv kernel.  S is computed again from q and k: reading stored
+// probabilities would cost lk numbers a row.
+template <int DH>
+__global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossArgs a) {
+    constexpr int THREADS = 128, BM = 64, BN = DH == 128 ? 32 : 64, NT = BN / 8, KS = DH / 16;
+    constexpr int TILE = BN * DH * 2;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t bits[3][2];
+    __shared__ float s_delta[BM];
+    const uint32_t sK = s_addr(sm), sV = sK + 2 * TILE, sQ = sV + 2 * TILE, sG = sQ + BM * DH * 2;
+    const Where at = where(a);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r0 = at.tile * BM, len = kept_len(a, at.seq);
+    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    const int nt = (kend - kbeg + BN - 1) / BN;
+    const bf16 *K = (const bf16*)a.k, *V = (const bf16*)a.v;
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    auto mask_byte = [&](int j) {
+        const int key = kbeg + j * BN + warp * 32 + lane;
+        return warp < BN / 32 && key < kend && kept(a, at.seq, key, len);
+    };
+    auto put_bits = [&](int j, bool b) {
+        const uint32_t m = __ballot_sync(0xffffffffu, b);
+        if (warp < 2 && lane == 0) bits[j % 3][warp] = m;
+    };
+    auto load = [&](int j) {
+        if (j < nt) {
+            stage_k<DH, BN, THREADS>(sK + (j & 1) * TILE, K, a.sk, at.seq, at.hk, kbeg + j * BN, bits[j % 3]);
+            stage_k<DH, BN, THREADS>(sV + (j & 1) * TILE, V, a.sv, at.seq, at.hk, kbeg + j * BN, bits[j % 3]);
+        }
+        cp_commit();
+    };
+    put_bits(0, mask_byte(0));
+    put_bits(1, mask_byte(1));
+    stage_q<DH, BM, THREADS>(sQ, (const bf16*)a.q, a.sq, a, at.seq, at.hk, r0);
+    stage_q<DH, BM, THREADS>(sG, (const bf16*)a.dout, a.sdo, a, at.seq, at.hk, r0);
+    __syncthreads();
+    load(0);
+    {   // delta: two threads a row
+        const int r = threadIdx.x >> 1, h = threadIdx.x & 1;
+        float d = 0.f;
+        if (r0 + r < a.rows) {
+            const bf16* og = (const bf16*)a.o + qrow(a, a.so, at.seq, at.hk, r0 + r) + h * (DH / 2);
+            const bf16* gg = (const bf16*)a.dout + qrow(a, a.sdo, at.seq, at.hk, r0 + r) + h * (DH / 2);
+            #pragma unroll
+            for (int c = 0; c < DH / 16; c++) {
+                float x[8], y[8];
+                VecIO<bf16, 8>::ld(x, og + c * 8);
+                VecIO<bf16, 8>::ld(y, gg + c * 8);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) d = fmaf(x[e], y[e], d);
+            }
+        }
+        d += __shfl_xor_sync(0xffffffffu, d, 1);
+        if (h == 0) {
+            s_delta[r] = d;
+            if (r0 + r < a.rows && at.part == 0) a.delta[row0 + r0 + r] = d;
+        }
+    }
+    const int g = lane >> 2, t = lane & 3;
+    const int ra = r0 + warp * 16 + g, rb = ra + 8;
+    // log2-domain lse; +inf makes the probabilities of a row without keys
+    // (and of rows past the end) zero
+    float la = ra < a.rows ? a.lse[row0 + ra] : -INFINITY, lb = rb < a.rows ? a.lse[row0 + rb] : -INFINITY;
+    la = la == -INFINITY ? INFINITY : la * LOG2E;
+    lb = lb == -INFINITY ? INFINITY : lb * LOG2E;
+    const float sc = a.scale * LOG2E;
+    float dq[DH / 8][4];
+    #pragma unroll
+    for (int i = 0; i < DH / 8; i++) dq[i][0] = dq[i][1] = dq[i][2] = dq[i][3] = 0.f;
+    uint32_t qf[KS][4], gf[KS][4];
+    float da = 0.f, db = 0.f;
+    for (int j = 0; j < nt; j++) {
+        const bool next = mask_byte(j + 2);
+        cp_wait<0>();
+        __syncthreads();
+        load(j + 1);
+        if (j == 0) {
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                frag_a<DH>(qf[ks], sQ, warp * 16, ks, lane);
+                frag_a<DH>(gf[ks], sG, warp * 16, ks, lane);
+            }
+            da = s_delta[warp * 16 + g];
+            db = s_delta[warp * 16 + g + 8];
+        }
+        const uint32_t w0 = bits[j % 3][0], w1 = BN == 64 ? bits[j % 3][1] : 0u;
+        if (w0 | w1) {
+            const uint32_t kt = sK + (j & 1) * TILE, vt = sV + (j & 1) * TILE;
+            float s[NT][4], p[NT][4];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+                p[i][0] = p[i][1] = p[i][2] = p[i][3] = 0.f;
+            }
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                #pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    uint32_t b[4];
+                    frag_bn<DH>(b, kt, i * 16, ks, lane);
+                    mma(s[2 * i], qf[ks], b[0], b[1]);
+                    mma(s[2 * i + 1], qf[ks], b[2], b[3]);
+                    frag_bn<DH>(b, vt, i * 16, ks, lane);
+                    mma(p[2 * i], gf[ks], b[0], b[1]);
+                    mma(p[2 * i + 1], gf[ks], b[2], b[3]);
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const uint32_t w = (i < 4 ? w0 : w1) >> ((i & 3) * 8 + 2 * t);
+                const float e0 = w & 1 ? ex2_approx(fmaf(s[i][0], sc, -la)) : 0.f;
+                const float e1 = w & 2 ? ex2_approx(fmaf(s[i][1], sc, -la)) : 0.f;
+                const float e2 = w & 1 ? ex2_approx(fmaf(s[i][2], sc, -lb)) : 0.f;
+                const float e3 = w & 2 ? ex2_approx(fmaf(s[i][3], sc, -lb)) : 0.f;
+                s[i][0] = e0 * (p[i][0] - da);
+                s[i][1] = e1 * (p[i][1] - da);
+                s[i][2] = e2 * (p[i][2] - db);
+                s[i][3] = e3 * (p[i][3] - db);
+            }
+            #pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                const uint32_t f[4] = {pack_bf2(s[2 * i][0], s[2 * i][1]), pack_bf2(s[2 * i][2], s[2 * i][3]),
+                                       pack_bf2(s[2 * i + 1][0], s[2 * i + 1][1]),
+                                       pack_bf2(s[2 * i + 1][2], s[2 * i + 1][3])};
+                #pragma unroll
+                for (int d = 0; d < KS; d++) {
+                    uint32_t b[4];
+                    frag_bk<DH>(b, kt, i * 16, d, lane);
+                    mma(dq[2 * d], f, b[0], b[1]);
+                    mma(dq[2 * d + 1], f, b[2], b[3]);
+                }
+            }
+        }
+        put_bits(j + 2, next);
+    }
+    cp_wait<0>();
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int r = half ? rb : ra;
+        if (r >= a.rows) continue;
+        if (a.nsplit > 1) {
+            float* p = a.part + ((row0 + r) * a.nsplit + at.part) * DH;
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++)
+                *(float2*)(p + i * 8 + 2 * t) = make_float2(dq[i][2 * half] * a.scale, dq[i][2 * half + 1] * a.scale);
+        } else {
+            bf16* p = (bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r);
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++)
+                *(uint32_t*)(p + i * 8 + 2 * t) = pack_bf2(dq[i][2 * half] * a.scale, dq[i][2 * half + 1] * a.scale);
+        }
+    }
+}
+
+// dk, dv: a block owns 64 keys (16 a warp) and walks the stacked rows; S^T and
+// dP^T come out with keys as rows, so P^T and dS^T are the left operands of
+// dv += P^T dout and dk += dS^T q straight from the accumulators.
+template <int DH>
+__global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ CrossArgs a) {
+    constexpr int THREADS = 128, BK = 64, BQ = DH == 128 ? 32 : 64, NT = BQ / 8, KS = DH / 16;
+    constexpr int QT = BQ * DH * 2;
+    constexpr bool REGS = DH < 128;              // k and v fragments stay in registers
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t bits[2];
+    __shared__ float s_lse[2][BQ], s_delta[2][BQ];
+    const uint32_t sK = s_addr(sm), sV = sK + BK * DH * 2, sQ = sV + BK * DH * 2, sG = sQ + 2 * QT;
+    const Where at = where(a);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int j0 = at.tile * BK, len = kept_len(a, at.seq);
+    const int qbeg = min(at.part * a.split, a.rows), qend = min(a.rows, qbeg + a.split);
+    const int nt = (qend - qbeg + BQ - 1) / BQ;
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    {
+        const int key = j0 + warp * 32 + lane;
+        const uint32_t m = __ballot_sync(0xffffffffu, warp < 2 && kept(a, at.seq, key, len));
+        if (warp < 2 && lane == 0) bits[warp] = m;
+    }
+    __syncthreads();
+    const uint32_t w0 = bits[0], w1 = bits[1];
+    const bool any = (w0 | w1) != 0;
+    auto load = [&](int j) {
+        if (j < nt) {
+            stage_q<DH, BQ, THREADS>(sQ + (j & 1) * QT, (const bf16*)a.q, a.sq, a, at.seq, at.hk, qbeg + j * BQ);
+            stage_q<DH, BQ, THREADS>(sG + (j & 1) * QT, (const bf16*)a.dout, a.sdo, a, at.seq, at.hk, qbeg + j * BQ);
+        }
+        cp_commit();
+    };
+    float lv = 0.f, dl = 0.f;
+    auto load_stat = [&](int j) {
+        const int r = qbeg + j * BQ + threadIdx.x;
+        const bool in = threadIdx.x < BQ && r < qend;
+        lv = in ? a.lse[row0 + r] : -INFINITY;
+        lv = lv == -INFINITY ? INFINITY : lv * LOG2E;
+        dl = in ? a.delta[row0 + r] : 0.f;
+    };
+    auto put_stat = [&](int j) {
+        if (threadIdx.x < BQ) { s_lse[j & 1][threadIdx.x] = lv; s_delta[j & 1][threadIdx.x] = dl; }
+    };
+    float dk[DH / 8][4], dv[DH / 8][4];
+    #pragma unroll
+    for (int i = 0; i < DH / 8; i++) {
+        dk[i][0] = dk[i][1] = dk[i][2] = dk[i][3] = 0.f;
+        dv[i][0] = dv[i][1] = dv[i][2] = dv[i][3] = 0.f;
+    }
+    const int g = lane >> 2, t = lane & 3;
+    if (any) {
+        stage_k<DH, BK, THREADS>(sK, (const bf16*)a.k, a.sk, at.seq, at.hk, j0, bits);
+        stage_k<DH, BK, THREADS>(sV, (const bf16*)a.v, a.sv, at.seq, at.hk, j0, bits);
+        load(0);
+        load_stat(0);
+        const float sc = a.scale * LOG2E;
+        const uint32_t wk = warp & 2 ? w1 : w0;
+        const bool ka = (wk >> ((warp & 1) * 16 + g)) & 1, kb = (wk >> ((warp & 1) * 16 + g + 8)) & 1;
+        uint32_t kf[REGS ? KS : 1][4], vf[REGS ? KS : 1][4];
+        for (int j = 0; j < nt; j++) {
+            put_stat(j);
+            load_stat(j + 1);
+            cp_wait<0>();
+            __syncthreads();
+            load(j + 1);
+            if (REGS && j == 0) {
+                #pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    frag_a<DH>(kf[REGS ? ks : 0], sK, warp * 16, ks, lane);
+                    frag_a<DH>(vf[REGS ? ks : 0], sV, warp * 16, ks, lane);
+                }
+            }
+            const uint32_t qt = sQ + (j & 1) * QT, gt = sG + (j & 1) * QT;
+            float s[NT][4], p[NT][4];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+                p[i][0] = p[i][1] = p[i][2] = p[i][3] = 0.f;
+            }
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if (!REGS) {
+                    frag_a<DH>(kf[0], sK, warp * 16, ks, lane);
+                    frag_a<DH>(vf[0], sV, warp * 16, ks, lane);
+                }
+                #pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    uint32_t b[4];
+                    frag_bn<DH>(b, qt, i * 16, ks, lane);
+                    mma(s[2 * i], kf[REGS ? ks : 0], b[0], b[1]);
+                    mma(s[2 * i + 1], kf[REGS ? ks : 0], b[2], b[3]);
+                    frag_bn<DH>(b, gt, i * 16, ks, lane);
+                    mma(p[2 * i], vf[REGS ? ks : 0], b[0], b[1]);
+                    mma(p[2 * i + 1], vf[REGS ? ks : 0], b[2], b[3]);
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const int c = i * 8 + 2 * t;
+                const float x0 = s_lse[j & 1][c], x1 = s_lse[j & 1][c + 1];
+                const float d0 = s_delta[j & 1][c], d1 = s_delta[j & 1][c + 1];
+                s[i][0] = ka ? ex2_approx(fmaf(s[i][0], sc, -x0)) : 0.f;
+                s[i][1] = ka ? ex2_approx(fmaf(s[i][1], sc, -x1)) : 0.f;
+                s[i][2] = kb ? ex2_approx(fmaf(s[i][2], sc, -x0)) : 0.f;
+                s[i][3] = kb ? ex2_approx(fmaf(s[i][3], sc, -x1)) : 0.f;
+                p[i][0] = s[i][0] * (p[i][0] - d0);
+                p[i][1] = s[i][1] * (p[i][1] - d1);
+                p[i][2] = s[i][2] * (p[i][2] - d0);
+                p[i][3] = s[i][3] * (p[i][3] - d1);
+            }
+            #pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                const uint32_t pf[4] = {pack_bf2(s[2 * i][0], s[2 * i][1]), pack_bf2(s[2 * i][2], s[2 * i][3]),
+                                        pack_bf2(s[2 * i + 1][0], s[2 * i + 1][1]),
+                                        pack_bf2(s[2 * i + 1][2], s[2 * i + 1][3])};
+                const uint32_t df[4] = {pack_bf2(p[2 * i][0], p[2 * i][1]), pack_bf2(p[2 * i][2], p[2 * i][3]),
+                                        pack_bf2(p[2 * i + 1][0], p[2 * i + 1][1]),
+                                        pack_bf2(p[2 * i + 1][2], p[2 * i + 1][3])};
+                #pragma unroll
+                for (int d = 0; d < KS; d++) {
+                    uint32_t b[4];
+                    frag_bk<DH>(b, gt, i * 16, d, lane);
+                    mma(dv[2 * d], pf, b[0], b[1]);
+                    mma(dv[2 * d + 1], pf, b[2], b[3]);
+                    frag_bk<DH>(b, qt, i * 16, d, lane);
+                    mma(dk[2 * d], df, b[0], b[1]);
+                    mma(dk[2 * d + 1], df, b[2], b[3]);
+                }
+            }
+        }
+        cp_wait<0>();
+    }
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int j = j0 + warp * 16 + g + half * 8;
+        if (j >= a.lk) continue;
+        if (a.nsplit > 1) {
+            const long at_row = (((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part;
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) {
+                *(float2*)(a.part + at_row * DH + i * 8 + 2 * t) = make_float2(dk[i][2 * half] * a.scale, dk[i][2 * half + 1] * a.scale);
+                *(float2*)(a.part2 + at_row * DH + i * 8 + 2 * t) = make_float2(dv[i][2 * half], dv[i][2 * half + 1]);
+            }
+        } else {
+            bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, j);
+            bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, j);
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) {
+                *(uint32_t*)(pk + i * 8 + 2 * t) = pack_bf2(dk[i][2 * half] * a.scale, dk[i][2 * half + 1] * a.scale);
+                *(uint32_t*)(pv + i * 8 + 2 * t) = pack_bf2(dv[i][2 * half], dv[i][2 * half + 1]);
+            }
+        }
+    }
+}
+
+// sums the parts of a split gradient in order: one 4-column piece a thread.
+// keys: the rows are key rows of a.dk (from part) and a.dv (from part2),
+// else stacked rows of a.dq
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ CrossArgs a, long nrows, int keys) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long row = i / (DH / 4);
+    const int c = (int)(i % (DH / 4)) * 4;
+    if (row >= nrows) return;
+    const long per = keys ? a.lk : a.rows, b = row / per;
+    const int seq = (int)(b / a.kv_heads), hk = (int)(b % a.kv_heads), r = (int)(row - b * per);
+    for (int which = 0; which < 1 + keys; which++) {
+        const float* p = (which ? a.part2 : a.part) + row * a.nsplit * DH + c;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < a.nsplit; k++) {
+            float v[4];
+            VecIO<float, 4>::ld(v, p + (long)k * DH);
+            #pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += v[e];
+        }
+        T* out = !keys ? (T*)a.dq + qrow(a, a.sdq, seq, hk, r)
+                       : which ? (T*)a.dv + krow(a.sdv, seq, hk, r) : (T*)a.dk + krow(a.sdk, seq, hk, r);
+        VecIO<T, 4>::st(out + c, s);
+    }
+}
+
+// ------------------------------------------------------------------ fp32
+// Exact fp32 on the SIMT cores.  128 threads as 8 x 16: thread (ty, tx) owns
+// RT rows x NC columns of every product, all of which are
+//   acc[i][j] += sum_k A[k][ty RT + i] B[k][tx NC + j]
+// over tiles in shared memory, two rows at a time on the packed f32x2 path.
+template <int RT, int NC>
+PTCG_DEV void tile_mm(float (&acc)[RT][NC], const float* A, int lda, const float* B, int ldb, int K,
+                      int ty, int tx) {
+    unsigned long long c[RT / 2][NC];
+    #pragma unroll
+    for (int i = 0; i < RT / 2; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) c[i][j] = pk2(acc[2 * i][j], acc[2 * i + 1][j]);
+    const float* pa = A + ty * RT;
+    const float* pb = B + tx * NC;
+    #pragma unroll 4
+    for (int k = 0; k < K; k++, pa += lda, pb += ldb) {
+        unsigned long long x[RT / 2];
+        float y[NC];
+        if (RT >= 4) {
+            #pragma unroll
+            for (int i = 0; i < RT / 4; i++) {
+                const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(pa + 4 * i);
+                x[2 * i] = u.x;
+                x[RT >= 4 ? 2 * i + 1 : 0] = u.y;
+            }
+        } else {
+            x[0] = *reinterpret_cast<const unsigned long long*>(pa);
+        }
+        if (NC >= 4) {
+            #pragma unroll
+            for (int j = 0; j < NC / 4; j++) {
+                const float4 v = *reinterpret_cast<const float4*>(pb + 4 * j);
+                y[4 * j] = v.x; y[(4 * j + 1) % NC] = v.y; y[(4 * j + 2) % NC] = v.z; y[(4 * j + 3) % NC] = v.w;
+            }
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(pb);
+            y[0] = v.x; y[1] = v.y;
+        }
+        #pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const unsigned long long s = splat2(y[j]);
+            #pragma unroll
+            for (int i = 0; i < RT / 2; i++) c[i][j] = fma2(x[i], s, c[i][j]);
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < RT / 2; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) upk2(c[i][j], acc[2 * i][j], acc[2 * i + 1][j]);
+}
+// N rows of DH floats: transposed to T[d][row] (pitch ldt) and / or as they
+// are to X[row][d]; row(r) gives the source or null (zeros)
+template <int DH, int N, typename F>
+PTCG_DEV void stage_f32(float* T, int ldt, float* X, F row) {
+    for (int i = threadIdx.x; i < N * (DH / 4); i += 128) {
+        const int r = i % N, c = i / N * 4;
+        const float* p = row(r);
+        const float4 v = p ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (T) { T[c * ldt + r] = v.x; T[(c + 1) * ldt + r] = v.y; T[(c + 2) * ldt + r] = v.z; T[(c + 3) * ldt + r] = v.w; }
+        if (X) *reinterpret_cast<float4*>(X + r * DH + c) = v;
+    }
+}
+PTCG_DEV float row16_max(float v) {
+    #pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+PTCG_DEV float row16_sum(float v) {
+    #pragma unroll
+    for (int o = 1; o < 16; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// keys per tile of the fp32 kernels, and shared-memory pitches
+template <int DH> struct F32 { static constexpr int BN = DH == 128 ? 32 : 64, LB = BN + 4; };
+
+template <int DH, int RT>
+__global__ void __launch_bounds__(128) k_cross_fwd_f32(const __grid_constant__ CrossArgs a) {
+    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LB = F32<DH>::LB, NC = BN / 16, ND = DH / 16;
+    extern __shared__ __align__(16) float fs[];
+    __shared__ uint8_t ok[64];
+    float* Qt = fs;                  // [DH][LM]
+    float* Kt = Qt + DH * LM;        // [DH][LB]
+    float* Vs = Kt + DH * LB;        // [BN][DH]
+    float* Ps = Vs + BN * DH;        // [BN][LM]
+    const Where at = where(a);
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int r0 = at.tile * BM, len = kept_len(a, at.seq);
+    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    const float* q = (const float*)a.q;
+    stage_f32<DH, BM>(Qt, LM, nullptr, [&](int r) {
+        return r0 + r < a.rows ? q + qrow(a, a.sq, at.seq, at.hk, r0 + r) : nullptr; });
+    float o[RT][ND], m[RT], l[RT];
+    #pragma unroll
+    for (int i = 0; i < RT; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        #pragma unroll
+        for (int j = 0; j < ND; j++) o[i][j] = 0.f;
+    }
+    for (int k0 = kbeg; k0 < kend; k0 += BN) {
+        __syncthreads();
+        const bool in = threadIdx.x < BN && k0 + threadIdx.x < kend && kept(a, at.seq, k0 + threadIdx.x, len);
+        if (threadIdx.x < BN) ok[threadIdx.x] = in;
+        if (!__syncthreads_or(in)) continue;
+        stage_f32<DH, BN>(Kt, LB, nullptr, [&](int r) {
+            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, k0 + r) : nullptr; });
+        stage_f32<DH, BN>(nullptr, 0, Vs, [&](int r) {
+            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, k0 + r) : nullptr; });
+        __syncthreads();
+        float s[RT][NC];
+        #pragma unroll
+        for (int i = 0; i < RT; i++)
+            #pragma unroll
+            for (int j = 0; j < NC; j++) s[i][j] = 0.f;
+        tile_mm<RT, NC>(s, Qt, LM, Kt, LB, DH, ty, tx);
+        #pragma unroll
+        for (int i = 0; i < RT; i++) {
+            float x = -INFINITY;
+            #pragma unroll
+            for (int j = 0; j < NC; j++) {
+                s[i][j] = ok[tx * NC + j] ? s[i][j] * a.scale : -INFINITY;
+                x = fmaxf(x, s[i][j]);
+            }
+            const float n = fmaxf(m[i], row16_max(x)), u = n == -INFINITY ? 0.f : n;
+            const float c = expf(m[i] - u);
+            m[i] = n;
+            float t = 0.f;
+            #pragma unroll
+            for (int j = 0; j < NC; j++) {
+                s[i][j] = expf(s[i][j] - u);
+                t += s[i][j];
+                Ps[(tx * NC + j) * LM + ty * RT + i] = s[i][j];
+            }
+            l[i] = fmaf(l[i], c, t);
+            #pragma unroll
+            for (int j = 0; j < ND; j++) o[i][j] *= c;
+        }
+        __syncthreads();
+        tile_mm<RT, ND>(o, Ps, LM, Vs, DH, BN, ty, tx);
+    }
+    #pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const float t = row16_sum(l[i]);
+        const int r = r0 + ty * RT + i;
+        if (r >= a.rows) continue;
+        const long row = ((long)at.seq * a.kv_heads + at.hk) * a.rows + r;
+        const float inv = a.nsplit > 1 ? 1.f : t == 0.f ? 0.f : 1.f / t;
+        float* p = a.nsplit > 1 ? a.part + (row * a.nsplit + at.part) * DH
+                                : (float*)a.out + qrow(a, a.so, at.seq, at.hk, r);
+        #pragma unroll
+        for (int j = 0; j < ND; j++) p[tx * ND + j] = o[i][j] * inv;
+        if (tx == 0) {
+            // the parts carry their maximum in the log2 domain, as the bf16 kernel's do
+            if (a.nsplit > 1) a.part_ml[row * a.nsplit + at.part] = make_float2(m[i] * LOG2E, t);
+            else if (a.lse) a.lse[row] = t == 0.f ? -INFINITY : m[i] + logf(t);
+        }
+    }
+}
+
+template <int DH, int RT>
+__global__ void __launch_bounds__(128) k_cross_dq_f32(const __grid_constant__ CrossArgs a) {
+    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LB = F32<DH>::LB, NC = BN / 16, ND = DH / 16;
+    extern __shared__ __align__(16) float fs[];
+    __shared__ uint8_t ok[64];
+    __shared__ float s_lse[BM], s_delta[BM];
+    float* Qt = fs;                  // [DH][LM]
+    float* Gt = Qt + DH * LM;        // [DH][LM]
+    float* Kt = Gt + DH * LM;        // [DH][LB]
+    float* Vt = Kt + DH * LB;        // [DH][LB]
+    float* Ks = Vt + DH * LB;        // [BN][DH]
+    float* Ds = Ks + BN * DH;        // [BN][LM]
+    const Where at = where(a);
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int r0 = at.tile * BM, len = kept_len(a, at.seq);
+    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    stage_f32<DH, BM>(Qt, LM, nullptr, [&](int r) {
+        return r0 + r < a.rows ? (const float*)a.q + qrow(a, a.sq, at.seq, at.hk, r0 + r) : nullptr; });
+    stage_f32<DH, BM>(Gt, LM, nullptr, [&](int r) {
+        return r0 + r < a.rows ? (const float*)a.dout + qrow(a, a.sdo, at.seq, at.hk, r0 + r) : nullptr; });
+    __syncthreads();
+    for (int r = threadIdx.x; r < BM; r += 128) {
+        const bool in = r0 + r < a.rows;
+        float d = 0.f;
+        if (in) {
+            const float* o = (const float*)a.o + qrow(a, a.so, at.seq, at.hk, r0 + r);
+            for (int c = 0; c < DH; c++) d = fmaf(o[c], Gt[c * LM + r], d);
+            if (at.part == 0) a.delta[row0 + r0 + r] = d;
+        }
+        const float x = in ? a.lse[row0 + r0 + r] : -INFINITY;
+        s_lse[r] = x == -INFINITY ? INFINITY : x;
+        s_delta[r] = d;
+    }
+    float dq[RT][ND];
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < ND; j++) dq[i][j] = 0.f;
+    for (int k0 = kbeg; k0 < kend; k0 += BN) {
+        __syncthreads();
+        const bool in = threadIdx.x < BN && k0 + threadIdx.x < kend && kept(a, at.seq, k0 + threadIdx.x, len);
+        if (threadIdx.x < BN) ok[threadIdx.x] = in;
+        if (!__syncthreads_or(in)) continue;
+        stage_f32<DH, BN>(Kt, LB, Ks, [&](int r) {
+            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, k0 + r) : nullptr; });
+        stage_f32<DH, BN>(Vt, LB, nullptr, [&](int r) {
+            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, k0 + r) : nullptr; });
+        __syncthreads();
+        float s[RT][NC], p[RT][NC];
+        #pragma unroll
+        for (int i = 0; i < RT; i++)
+            #pragma unroll
+            for (int j = 0; j < NC; j++) s[i][j] = p[i][j] = 0.f;
+        tile_mm<RT, NC>(s, Qt, LM, Kt, LB, DH, ty, tx);
+        tile_mm<RT, NC>(p, Gt, LM, Vt, LB, DH, ty, tx);
+        #pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int r = ty * RT + i;
+            #pragma unroll
+            for (int j = 0; j < NC; j++) {
+                const float e = ok[tx * NC + j] ? expf(fmaf(s[i][j], a.scale, -s_lse[r])) : 0.f;
+                Ds[(tx * NC + j) * LM + r] = e * (p[i][j] - s_delta[r]);
+            }
+        }
+        __syncthreads();
+        tile_mm<RT, ND>(dq, Ds, LM, Ks, DH, BN, ty, tx);
+    }
+    #pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const int r = r0 + ty * RT + i;
+        if (r >= a.rows) continue;
+        float* p = a.nsplit > 1 ? a.part + ((row0 + r) * a.nsplit + at.part) * DH
+                                : (float*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r);
+        #pragma unroll
+        for (int j = 0; j < ND; j++) p[tx * ND + j] = dq[i][j] * a.scale;
+    }
+}
+
+template <int DH>
+__global__ void __launch_bounds__(128) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
+    constexpr int RT = 8, BK = 64, LM = BK + 4, BQ = F32<DH>::BN, LB = F32<DH>::LB, NC = BQ / 16, ND = DH / 16;
+    extern __shared__ __align__(16) float fs[];
+    __shared__ uint8_t ok[BK];
+    __shared__ float s_lse[BQ], s_delta[BQ];
+    float* Kt = fs;                  // [DH][LM]
+    float* Vt = Kt + DH * LM;        // [DH][LM]
+    float* Qt = Vt + DH * LM;        // [DH][LB]
+    float* Gt = Qt + DH * LB;        // [DH][LB]
+    float* Qs = Gt + DH * LB;        // [BQ][DH]
+    float* Gs = Qs + BQ * DH;        // [BQ][DH]
+    float* Ps = Gs + BQ * DH;        // [BQ][LM]
+    float* Ds = Ps + BQ * LM;        // [BQ][LM]
+    const Where at = where(a);
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int j0 = at.tile * BK, len = kept_len(a, at.seq);
+    const int qbeg = min(at.part * a.split, a.rows), qend = min(a.rows, qbeg + a.split);
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    const bool in = threadIdx.x < BK && kept(a, at.seq, j0 + threadIdx.x, len);
+    if (threadIdx.x < BK) ok[threadIdx.x] = in;
+    const bool any = __syncthreads_or(in);
+    float dk[RT][ND], dv[RT][ND];
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < ND; j++) dk[i][j] = dv[i][j] = 0.f;
+    if (any) {
+        stage_f32<DH, BK>(Kt, LM, nullptr, [&](int r) {
+            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, j0 + r) : nullptr; });
+        stage_f32<DH, BK>(Vt, LM, nullptr, [&](int r) {
+            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, j0 + r) : nullptr; });
+        for (int q0 = qbeg; q0 < qend; q0 += BQ) {
+            __syncthreads();
+            stage_f32<DH, BQ>(Qt, LB, Qs, [&](int r) {
+                return q0 + r < qend ? (const float*)a.q + qrow(a, a.sq, at.seq, at.hk, q0 + r) : nullptr; });
+            stage_f32<DH, BQ>(Gt, LB, Gs, [&](int r) {
+                return q0 + r < qend ? (const float*)a.dout + qrow(a, a.sdo, at.seq, at.hk, q0 + r) : nullptr; });
+            if (threadIdx.x < BQ) {
+                const bool have = q0 + threadIdx.x < qend;
+                const float x = have ? a.lse[row0 + q0 + threadIdx.x] : -INFINITY;
+                s_lse[threadIdx.x] = x == -INFINITY ? INFINITY : x;
+                s_delta[threadIdx.x] = have ? a.delta[row0 + q0 + threadIdx.x] : 0.f;
+            }
+            __syncthreads();
+            float s[RT][NC], p[RT][NC];
+            #pragma unroll
+            for (int i = 0; i < RT; i++)
+                #pragma unroll
+                for (int j = 0; j < NC; j++) s[i][j] = p[i][j] = 0.f;
+            tile_mm<RT, NC>(s, Kt, LM, Qt, LB, DH, ty, tx);
+            tile_mm<RT, NC>(p, Vt, LM, Gt, LB, DH, ty, tx);
+            #pragma unroll
+            for (int i = 0; i < RT; i++) {
+                const int key = ty * RT + i;
+                #pragma unroll
+                for (int j = 0; j < NC; j++) {
+                    const int c = tx * NC + j;
+                    const float e = ok[key] ? expf(fmaf(s[i][j], a.scale, -s_lse[c])) : 0.f;
+                    Ps[c * LM + key] = e;
+                    Ds[c * LM + key] = e * (p[i][j] - s_delta[c]);
+                }
+            }
+            __syncthreads();
+            tile_mm<RT, ND>(dv, Ps, LM, Gs, DH, BQ, ty, tx);
+            tile_mm<RT, ND>(dk, Ds, LM, Qs, DH, BQ, ty, tx);
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const int j = j0 + ty * RT + i;
+        if (j >= a.lk) continue;
+        const long part = ((((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part) * DH;
+        float* pk = a.nsplit > 1 ? a.part + part : (float*)a.dk + krow(a.sdk, at.seq, at.hk, j);
+        float* pv = a.nsplit > 1 ? a.part2 + part : (float*)a.dv + krow(a.sdv, at.seq, at.hk, j);
+        #pragma unroll
+        for (int d = 0; d < ND; d++) {
+            pk[tx * ND + d] = dk[i][d] * a.scale;
+            pv[tx * ND + d] = dv[i][d];
+        }
+    }
+}
+
+// ------------------------------------------------------------- host side
+// A problem whose tiles leave processors idle is split along its other axis:
+// about four blocks a processor, at least 256 rows of that axis to a part.
+struct Split { int n, len; };
+Split split_of(long tiles, int axis) {
+    Split s = {1, axis > 0 ? axis : 1};
+    if (tiles >= 148 * 2 || axis <= 256 || tiles == 0) return s;
+    long want = (148 * 4 + tiles - 1) / tiles;
+    want = std::min(want, (long)(axis + 255) / 256);
+    s.len = (int)((((axis + want - 1) / want) + 63) / 64 * 64);
+    s.n = (int)cdiv(axis, s.len);
+    return s;
+}
+struct FwdPlan { bool few; int bm; long tiles, blocks; Split sp; long o_ml, bytes; };
+FwdPlan fwd_plan(const PtcgCross& c) {
+    FwdPlan p;
+    const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
+    p.few = rows <= 16;
+    p.bm = p.few ? 16 : 64;
+    p.tiles = (rows + p.bm - 1) / p.bm;
+    p.sp = split_of(p.tiles * probs, c.lk);
+    p.blocks = p.tiles * probs * p.sp.n;
+    const long parts = p.sp.n > 1 ? rows * probs * p.sp.n : 0;
+    p.o_ml = (4 * parts * c.dh + 255) / 256 * 256;
+    p.bytes = p.sp.n > 1 ? p.o_ml + 8 * parts : 0;
+    return p;
+}
+struct BwdPlan { bool few; int bm; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
+BwdPlan bwd_plan(const PtcgCross& c) {
+    BwdPlan p;
+    const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
+    p.few = rows <= 16;
+    p.bm = p.few && c.dtype == PTCG_FP32 ? 16 : 64;
+    p.qtiles = (rows + p.bm - 1) / p.bm;
+    p.ktiles = (c.lk + 63) / 64;
+    p.qs = split_of(p.qtiles * probs, c.lk);               // dq: split over keys
+    p.ks = split_of(p.ktiles * probs, (int)rows);          // dk, dv: split over rows
+    p.qblocks = p.qtiles * probs * p.qs.n;
+    p.kblocks = p.ktiles * probs * p.ks.n;
+    p.o_part = (4 * rows * probs + 255) / 256 * 256;       // delta first
+    const long q = p.qs.n > 1 ? 4 * rows * probs * p.qs.n * c.dh : 0;
+    const long k = p.ks.n > 1 ? 4 * (long)c.lk * probs * p.ks.n * c.dh : 0;
+    p.o_part2 = p.o_part + k;
+    p.bytes = p.o_part + std::max(q, 2 * k);               // one after the other
+    return p;
+}
+
+// kernels with more than 48 KB of shared memory, their static arrays (under
+// 4 KB here) included, need the limit raised on the current device; a cheap
+// call, repeated so that no state is kept
+template <typename F>
+cudaError_t smem_limit(F f, int bytes) {
+    return bytes > 44 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)
+                             : cudaSuccess;
+}
+
+template <int DH, int WM, int WN, int NST>
+cudaError_t launch_fwd(const CrossArgs& a, long blocks, cudaStream_t s) {
+    int bytes = WM * 16 * DH * 2 + 2 * NST * 64 * DH * 2;
+    if (WN > 1) bytes = std::max(bytes, (WN * 32 + WN * 16 * DH) * 4);
+    const cudaError_t e = smem_limit(k_cross_fwd<DH, WM, WN, NST>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_fwd<DH, WM, WN, NST><<<(unsigned)blocks, WM * WN * 32, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH, int RT>
+cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
+    constexpr int LM = RT * 8 + 4, BN = F32<DH>::BN;
+    const int bytes = 4 * (DH * LM + DH * F32<DH>::LB + BN * DH + BN * LM);
+    const cudaError_t e = smem_limit(k_cross_fwd_f32<DH, RT>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_fwd_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH, int RT>
+cudaError_t launch_dq_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
+    constexpr int LM = RT * 8 + 4, BN = F32<DH>::BN;
+    const int bytes = 4 * (2 * DH * LM + 2 * DH * F32<DH>::LB + BN * DH + BN * LM);
+    const cudaError_t e = smem_limit(k_cross_dq_f32<DH, RT>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dq_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream_t s) {
+    cudaError_t e;
+    if (c.dtype == PTCG_BF16)
+        e = p.few ? launch_fwd<DH, 1, 4, 3>(a, p.blocks, s) : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
+    else
+        e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
+    if (e != cudaSuccess || p.sp.n == 1) return e;
+    const long nrows = (long)c.nseq * c.kv_heads * a.rows;
+    ++g_ptcg_launches;
+    if (c.dtype == PTCG_BF16) k_cross_join<bf16, DH><<<cdiv(nrows, 4), 128, 0, s>>>(a, nrows);
+    else k_cross_join<float, DH><<<cdiv(nrows, 4), 128, 0, s>>>(a, nrows);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream_t s) {
+    cudaError_t e = cudaSuccess;
+    const bool bf = c.dtype == PTCG_BF16;
+    const long probs = (long)c.nseq * c.kv_heads, nrows = probs * a.rows, nkeys = probs * a.lk;
+    if (p.qblocks) {
+        a.tiles = (int)p.qtiles; a.nsplit = p.qs.n; a.split = p.qs.len;
+        if (bf) {
+            constexpr int BN = DH == 128 ? 32 : 64;
+            const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2;
+            if ((e = smem_limit(k_cross_dq<DH>, bytes)) != cudaSuccess) return e;
+            ++g_ptcg_launches, k_cross_dq<DH><<<(unsigned)p.qblocks, 128, bytes, s>>>(a);
+        } else {
+            e = p.few ? launch_dq_f32<DH, 2>(a, p.qblocks, s) : launch_dq_f32<DH, 8>(a, p.qblocks, s);
+            if (e != cudaSuccess) return e;
+        }
+        if (p.qs.n > 1) {
+            ++g_ptcg_launches;
+            const unsigned grid = cdiv(nrows * (DH / 4), 256);
+            if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
+            else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
+        }
+    }
+    if (p.kblocks) {
+        a.tiles = (int)p.ktiles; a.nsplit = p.ks.n; a.split = p.ks.len;
+        ++g_ptcg_launches;
+        if (bf) {
+            constexpr int BQ = DH == 128 ? 32 : 64;
+            const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2;
+            if ((e = smem_limit(k_cross_dkv<DH>, bytes)) != cudaSuccess) return e;
+            k_cross_dkv<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
+        } else {
+            constexpr int BQ = F32<DH>::BN, LB = F32<DH>::LB;
+            const int bytes = 4 * (2 * DH * 68 + 2 * DH * LB + 2 * BQ * DH + 2 * BQ * 68);
+            if ((e = smem_limit(k_cross_dkv_f32<DH>, bytes)) != cudaSuccess) return e;
+            k_cross_dkv_f32<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
+        }
+        if (p.ks.n > 1) {
+            ++g_ptcg_launches;
+            const unsigned grid = cdiv(nkeys * (DH / 4), 256);
+            if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nkeys, 1);
+            else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nkeys, 1);
+        }
+    }
+    return e;
+}
+
+bool heads_ok(const PtcgHeads& s, const void* p, int dtype) {
+    const long sz = dt_size(dtype);
+    return (uintptr_t)p % 16 == 0 && (s.seq * sz) % 16 == 0 && (s.row * sz) % 16 == 0 && (s.head * sz) % 16 == 0;
+}
+// a written tensor: no two of its rows may share elements along one axis
+bool apart(const PtcgHeads& s, long nseq, long n, long nh, int dh) {
+    if (nseq == 0 || n == 0 || nh == 0) return true;
+    return (nseq <= 1 || s.seq >= dh) && (n <= 1 || s.row >= dh) && (nh <= 1 || s.head >= dh);
+}
+// 0, or an error code with its message set
+int check(const PtcgCross* c) {
+    OP_REQ(c, PTCG_EINVAL, "cross attention: null description");
+    OP_REQ(dt_ok(c->dtype), PTCG_EINVAL, "cross attention: unknown dtype %d", c->dtype);
+    OP_REQ(c->nseq >= 0 && c->lq >= 0 && c->lk >= 0 && c->heads > 0 && c->kv_heads > 0 &&
+           c->heads % c->kv_heads == 0, PTCG_EINVAL,
+           "cross attention: bad sizes (nseq %d, lq %d, lk %d, heads %d, kv_heads %d)", c->nseq, c->lq,
+           c->lk, c->heads, c->kv_heads);
+    OP_REQ(c->dh == 32 || c->dh == 64 || c->dh == 128, PTCG_EINVAL,
+           "cross attention: head width %d is not 32, 64 or 128", c->dh);
+    OP_REQ(c->scale > 0.f && c->scale < INFINITY, PTCG_EINVAL, "cross attention: scale must be positive and finite");
+    const long rows = (long)c->heads / c->kv_heads * c->lq;
+    OP_REQ(rows <= (1L << 30) && c->lk <= (1 << 30), PTCG_EINVAL, "cross attention: more than 2^30 rows");
+    return PTCG_OK;
+}
+CrossArgs args(const PtcgCross& c) {
+    CrossArgs a = {};
+    a.sq = c.q; a.sk = c.k; a.sv = c.v; a.so = c.out;
+    a.sdo = c.dout; a.sdq = c.dq; a.sdk = c.dk; a.sdv = c.dv;
+    a.lq = c.lq; a.lk = c.lk; a.heads = c.heads; a.kv_heads = c.kv_heads;
+    a.group = c.heads / c.kv_heads;
+    a.rows = a.group * c.lq;
+    a.scale = c.scale;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+long ptcg_cross_attention_fwd_scratch(const PtcgCross* c) {
+    return check(c) ? -1 : fwd_plan(*c).bytes;
+}
+
+int ptcg_cross_attention_fwd(const PtcgCross* c, const void* q, const void* k, const void* v,
+                             const unsigned char* keep, const int* kv_len, void* out, float* lse,
+                             void* scratch, long scratch_bytes, void* stream) {
+    const int rc = check(c);
+    if (rc) return rc;
+    if (c->nseq == 0 || c->lq == 0) return PTCG_OK;
+    OP_REQ(q && out && (c->lk == 0 || (k && v)), PTCG_EINVAL, "cross attention: null pointer");
+    OP_REQ(heads_ok(c->q, q, c->dtype) && heads_ok(c->k, k, c->dtype) && heads_ok(c->v, v, c->dtype) &&
+           heads_ok(c->out, out, c->dtype) && (uintptr_t)lse % 4 == 0 && (uintptr_t)kv_len % 4 == 0, PTCG_EINVAL,
+           "cross attention: rows must start on 16-byte boundaries");
+    OP_REQ(apart(c->out, c->nseq, c->lq, c->heads, c->dh), PTCG_EINVAL, "cross attention: out rows overlap");
+    const FwdPlan p = fwd_plan(*c);
+    OP_REQ(p.bytes == 0 || ((uintptr_t)scratch % 16 == 0 && scratch && scratch_bytes >= p.bytes), PTCG_ERANGE,
+           "cross attention: scratch of %ld bytes, %ld needed (16-byte aligned)", scratch ? scratch_bytes : 0L, p.bytes);
+    OP_REQ(p.blocks <= 0x7fffffffL, PTCG_EINVAL, "cross attention: too many tiles");
+    CrossArgs a = args(*c);
+    a.q = q; a.k = k; a.v = v; a.keep = keep; a.kv_len = kv_len; a.out = out; a.lse = lse;
+    a.part = (float*)scratch;
+    a.part_ml = (float2*)((uint8_t*)scratch + p.o_ml);
+    a.tiles = (int)p.tiles; a.nsplit = p.sp.n; a.split = p.sp.len;
+    cudaStream_t s = (cudaStream_t)stream;
+    OP_CK(c->dh == 32 ? fwd_dh<32>(a, *c, p, s) : c->dh == 64 ? fwd_dh<64>(a, *c, p, s) : fwd_dh<128>(a, *c, p, s));
+    OP_CKL();
+    return PTCG_OK;
+}
+
+long ptcg_cross_attention_bwd_scratch(const PtcgCross* c) {
+    return check(c) ? -1 : bwd_plan(*c).bytes;
+}
+
+int ptcg_cross_attention_bwd(const PtcgCross* c, const void* q, const void* k, const void* v,
+                             const unsigned char* keep, const int* kv_len, const void* out,
+                             const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                             void* scratch, long scratch_bytes, void* stream) {
+    const int rc = check(c);
+    if (rc) return rc;
+    if (c->nseq == 0 || (c->lq == 0 && c->lk == 0)) return PTCG_OK;
+    OP_REQ((c->lq == 0 || (q && out && lse && dout && dq)) && (c->lk == 0 || (k && v && dk && dv)),
+           PTCG_EINVAL, "cross attention gradient: null pointer");
+    OP_REQ(heads_ok(c->q, q, c->dtype) && heads_ok(c->k, k, c->dtype) && heads_ok(c->v, v, c->dtype) &&
+           heads_ok(c->out, out, c->dtype) && heads_ok(c->dout, dout, c->dtype) &&
+           heads_ok(c->dq, dq, c->dtype) && heads_ok(c->dk, dk, c->dtype) && heads_ok(c->dv, dv, c->dtype) &&
+           (uintptr_t)lse % 4 == 0 && (uintptr_t)kv_len % 4 == 0, PTCG_EINVAL,
+           "cross attention gradient: rows must start on 16-byte boundaries");
+    OP_REQ(apart(c->dq, c->nseq, c->lq, c->heads, c->dh) && apart(c->dk, c->nseq, c->lk, c->kv_heads, c->dh) &&
+           apart(c->dv, c->nseq, c->lk, c->kv_heads, c->dh), PTCG_EINVAL,
+           "cross attention gradient: rows of a gradient overlap");
+    const BwdPlan p = bwd_plan(*c);
+    OP_REQ(p.bytes == 0 || ((uintptr_t)scratch % 16 == 0 && scratch && scratch_bytes >= p.bytes), PTCG_ERANGE,
+           "cross attention gradient: scratch of %ld bytes, %ld needed (16-byte aligned)",
+           scratch ? scratch_bytes : 0L, p.bytes);
+    OP_REQ(p.qblocks <= 0x7fffffffL && p.kblocks <= 0x7fffffffL, PTCG_EINVAL, "cross attention gradient: too many tiles");
+    CrossArgs a = args(*c);
+    a.q = q; a.k = k; a.v = v; a.keep = keep; a.kv_len = kv_len; a.o = out; a.lse = (float*)lse;
+    a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.delta = (float*)scratch;
+    a.part = (float*)((uint8_t*)scratch + p.o_part);
+    a.part2 = (float*)((uint8_t*)scratch + p.o_part2);
+    cudaStream_t s = (cudaStream_t)stream;
+    OP_CK(c->dh == 32 ? bwd_dh<32>(a, *c, p, s) : c->dh == 64 ? bwd_dh<64>(a, *c, p, s) : bwd_dh<128>(a, *c, p, s));
+    OP_CKL();
+    return PTCG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,586 @@
+// Embedding lookup with scaling, and its gradient by sorted ids.
+//   forward    out[i, :] = scale * table[id_i, :]      (0 where id_i is the padding id)
+//   gradient   dtable[v, :] (+)= scale * sum over the i with id_i = v of dout[i, :]
+// The reference's embedding gradients are atomic adds from every token
+// (k_tok_cat_bwd, native/model/ptcg_model2.cu:36-64).  Here the places are
+// sorted by id first, so each table row is summed in the order of its places
+// (the result does not depend on scheduling) and written once, and an id
+// that half of the batch holds costs no contention.
+#include <algorithm>
+
+#include "vec.cuh"
+
+namespace {
+
+// -------------------------------------------------------------- forward
+// Bound: HBM (ids and output once; the table's touched rows once, from L2
+// after that).  LX lanes take a row's V-element pieces, 256 / LX rows to a
+// block pass, four rows in flight per thread.
+template <typename TT, typename TO, int V>
+__global__ void __launch_bounds__(256) k_embed_fwd(
+        TO* __restrict__ out, long ldo, const TT* __restrict__ table, long ldt,
+        const int* __restrict__ ids, long n, int vocab, int pieces, int lx_log2, float scale,
+        int pad_id, int has_pad) {
+    const int tx = threadIdx.x & ((1 << lx_log2) - 1), ty = threadIdx.x >> lx_log2;
+    const int ry = 256 >> lx_log2;
+    constexpr int U = 4;
+    for (long r0 = (long)blockIdx.x * ry * U; r0 < n; r0 += (long)gridDim.x * ry * U) {
+        int id[U];
+        #pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long r = r0 + u * ry + ty;
+            id[u] = r < n ? ids[r] : 0;
+        }
+        for (int c = tx; c < pieces; c += 1 << lx_log2) {
+            float v[U][V];
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int row = min(max(id[u], 0), vocab - 1);
+                VecIO<TT, V>::ld(v[u], table + (long)row * ldt + (long)c * V);
+            }
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                const long r = r0 + u * ry + ty;
+                if (r >= n) break;
+                const bool pad = has_pad && id[u] == pad_id;
+                #pragma unroll
+                for (int e = 0; e < V; e++) v[u][e] = pad ? 0.f : v[u][e] * scale;
+                VecIO<TO, V>::st(out + r * ldo + (long)c * V, v[u]);
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------- sort
+// Stable least-digit-first radix sort of (id, place), 8 bits a pass, two
+// launches a pass: the digit counts of each tile, then a scatter whose
+// blocks derive their own bases from all tiles' counts (a block reads
+// tiles x 256 counters from L2, which is cheaper here than a third launch
+// for the scan).  Bound: latency; it moves 16 bytes per place and pass.
+constexpr int SORT_T = 1024;
+
+// the sort key of a place: its clamped id, or `vocab` for a padding place,
+// which sorts behind every row
+PTCG_DEV uint32_t key_of(int id, int vocab, int pad_id, int has_pad) {
+    if (has_pad && id == pad_id) return (uint32_t)vocab;
+    return (uint32_t)min(max(id, 0), vocab - 1);
+}
+
+template <int ITEMS, bool FIRST>
+__global__ void __launch_bounds__(SORT_T) k_sort_count(
+        uint32_t* __restrict__ counts, const uint32_t* __restrict__ keys,
+        const int* __restrict__ ids, long n, int shift, int vocab, int pad_id, int has_pad,
+        uint8_t* __restrict__ present) {
+    __shared__ uint32_t hist[256];
+    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+    __syncthreads();
+    const long base = (long)blockIdx.x * SORT_T * ITEMS;
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const long i = base + k * SORT_T + threadIdx.x;
+        const bool in = i < n;
+        uint32_t key = 0;
+        if (in) {
+            key = FIRST ? key_of(ids[i], vocab, pad_id, has_pad) : keys[i];
+            // every writer stores the same 1
+            if (FIRST && key < (uint32_t)vocab) present[key] = 1;
+        }
+        // one shared atomic per distinct digit of the warp: hot ids would
+        // serialise 32 of them
+        const uint32_t d = in ? (key >> shift) & 255u : 256u;
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        if (in && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) counts[(long)blockIdx.x * 256 + threadIdx.x] = hist[threadIdx.x];
+}
+
+template <int ITEMS, bool FIRST>
+__global__ void __launch_bounds__(SORT_T) k_sort_scatter(
+        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out,
+        const uint32_t* __restrict__ counts, const uint32_t* __restrict__ keys,
+        const uint32_t* __restrict__ pos, const int* __restrict__ ids, long n, int shift,
+        int vocab, int pad_id, int has_pad) {
+    constexpr int NW = SORT_T / 32;
+    __shared__ uint32_t wcnt[NW][256];
+    __shared__ uint32_t tot[4][256], pre[4][256];
+    __shared__ uint32_t wsum[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tiles = gridDim.x, tile = blockIdx.x;
+    // counts of each digit over all tiles, and over the tiles before this one
+    {
+        const int d = tid & 255, part = tid >> 8;
+        uint32_t t = 0, p = 0;
+        #pragma unroll 4
+        for (int j = part; j < tiles; j += 4) {
+            const uint32_t c = counts[(long)j * 256 + d];
+            t += c;
+            p += j < tile ? c : 0u;
+        }
+        tot[part][d] = t;
+        pre[part][d] = p;
+        for (int i = tid; i < NW * 256; i += SORT_T) (&wcnt[0][0])[i] = 0;
+    }
+    __syncthreads();
+    // ranks inside the warp's run of 32 * ITEMS consecutive places: lanes of
+    // one digit in place order, after the warp's earlier ones
+    uint32_t key[ITEMS], ps[ITEMS];
+    uint16_t rank[ITEMS];
+    const long base = (long)tile * SORT_T * ITEMS + (long)warp * 32 * ITEMS;
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const long i = base + k * 32 + lane;
+        key[k] = 0;
+        ps[k] = (uint32_t)i;
+        if (i < n) {
+            if (FIRST) {
+                key[k] = key_of(ids[i], vocab, pad_id, has_pad);
+            } else {
+                key[k] = keys[i];
+                ps[k] = pos[i];
+            }
+        }
+    }
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const bool in = base + k * 32 + lane < n;
+        const uint32_t d = in ? (key[k] >> shift) & 255u : 256u;
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        uint32_t before = 0;
+        if (in) before = wcnt[warp][d];
+        __syncwarp();
+        rank[k] = (uint16_t)(before + __popc(same & ((1u << lane) - 1u)));
+        if (in && lane == __ffs(same) - 1) wcnt[warp][d] = before + __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    // first place of each digit for this tile, then for each of its warps
+    uint32_t all = 0, mine = 0;
+    if (tid < 256) {
+        all = tot[0][tid] + tot[1][tid] + tot[2][tid] + tot[3][tid];
+        mine = pre[0][tid] + pre[1][tid] + pre[2][tid] + pre[3][tid];
+        uint32_t x = all;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) wsum[warp] = x;
+        mine += x - all;
+    }
+    __syncthreads();
+    if (tid < 256) {
+        for (int w = 0; w < warp; w++) mine += wsum[w];
+        for (int w = 0; w < NW; w++) {
+            const uint32_t c = wcnt[w][tid];
+            wcnt[w][tid] = mine;
+            mine += c;
+        }
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        if (base + k * 32 + lane < n) {
+            const uint32_t to = wcnt[warp][(key[k] >> shift) & 255u] + rank[k];
+            keys_out[to] = key[k];
+            pos_out[to] = ps[k];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ sums
+// Segmented sum over the sorted places.  A block owns `chunk` consecutive
+// sorted places and a slice of G * V columns; each of its 256 / G lane groups
+// walks a run of them with the row sum in registers.  A segment (the places
+// of one id) inside one run is written straight to its table row.  A run
+// whose first segment began earlier, or whose last goes on, leaves that sum
+// as a partial: the block joins its groups' partials in order through shared
+// memory, and k_embed_join joins the blocks'.  Rows without a place are
+// zeroed by extra blocks.  Bound: HBM, dout read once as gathered rows.
+enum { SEG_HEAD = 1, SEG_THROUGH = 2, SEG_TAIL = 4 };
+
+struct SumArgs {
+    const void* dout; long lddo;
+    const uint32_t* keys; const uint32_t* pos;
+    long n;
+    float* dtab; long lddt;
+    float* head; float* tail;        // [chunks][width] partials of each block
+    uint32_t* flags; uint32_t* tail_id;
+    const uint8_t* present;
+    int vocab, width, pieces, accumulate;
+    int chunk, run, nchunks, zero_blocks;
+    float scale;
+};
+
+template <int V>
+PTCG_DEV void put_row(const SumArgs& a, uint32_t id, int piece, const float (&s)[V]) {
+    float* p = a.dtab + (long)id * a.lddt + (long)piece * V;
+    float v[V];
+    #pragma unroll
+    for (int e = 0; e < V; e++) v[e] = s[e] * a.scale;
+    if (a.accumulate) {
+        float o[V];
+        VecIO<float, V>::ld(o, p);
+        #pragma unroll
+        for (int e = 0; e < V; e++) v[e] += o[e];
+    }
+    VecIO<float, V>::st(p, v);
+}
+
+template <typename T, int V, int G>
+__global__ void __launch_bounds__(256) k_embed_sum(const __grid_constant__ SumArgs a) {
+    constexpr int NG = 256 / G, S = G * V, U = V == 8 ? 4 : 8;
+    __shared__ float s_head[NG][S], s_tail[NG][S];
+    __shared__ uint32_t s_flag[NG], s_hid[NG], s_tid[NG];
+    const int lane = threadIdx.x % G, grp = threadIdx.x / G;
+    const int piece = blockIdx.y * G + lane;
+    const bool col = piece < a.pieces;
+    if (blockIdx.x >= (unsigned)a.nchunks) {               // rows nothing refers to
+        const float z[V] = {};
+        for (long r = (long)(blockIdx.x - a.nchunks) * NG + grp; r < a.vocab;
+             r += (long)a.zero_blocks * NG)
+            if (col && !a.present[r])
+                VecIO<float, V>::st(a.dtab + r * a.lddt + (long)piece * V, z);
+        return;
+    }
+    const T* dout = (const T*)a.dout;
+    const uint32_t none = 0xffffffffu, vocab = (uint32_t)a.vocab;
+    const long c0 = (long)blockIdx.x * a.chunk, c1 = min(a.n, c0 + a.chunk);
+    const long r0 = min(c1, c0 + (long)grp * a.run), r1 = min(c1, r0 + a.run);
+    uint32_t flag = 0, hid = none, tid = none;
+    float acc[V];
+    #pragma unroll
+    for (int e = 0; e < V; e++) acc[e] = 0.f;
+    if (r0 < r1) {
+        uint32_t cur = a.keys[r0];
+        bool began = r0 > 0 && a.keys[r0 - 1] == cur;      // the open segment's start is earlier
+        const uint32_t after = r1 < a.n ? a.keys[r1] : none;
+        for (long i = r0; i < r1; i += U) {
+            uint32_t k[U];
+            float v[U][V];
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                const bool in = i + u < r1;
+                k[u] = in ? a.keys[i + u] : none;
+                // padding places (key vocab) carry no gradient: not read
+                const bool take = in && k[u] < vocab && col;
+                const long p = take ? (long)a.pos[i + u] : 0;
+                if (take) {
+                    VecIO<T, V>::ld(v[u], dout + p * a.lddo + (long)piece * V);
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < V; e++) v[u][e] = 0.f;
+                }
+            }
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (i + u >= r1) break;
+                if (k[u] != cur) {
+                    if (began) {
+                        flag |= SEG_HEAD;
+                        hid = cur;
+                        #pragma unroll
+                        for (int e = 0; e < V; e++) s_head[grp][lane * V + e] = acc[e];
+                    } else if (cur < vocab && col) {
+                        put_row<V>(a, cur, piece, acc);
+                    }
+                    began = false;
+                    cur = k[u];
+                    #pragma unroll
+                    for (int e = 0; e < V; e++) acc[e] = 0.f;
+                }
+                #pragma unroll
+                for (int e = 0; e < V; e++) acc[e] += v[u][e];
+            }
+        }
+        const bool on = after == cur;
+        if (began) {
+            flag |= SEG_HEAD | (on ? SEG_THROUGH : 0);
+            hid = cur;
+            #pragma unroll
+            for (int e = 0; e < V; e++) s_head[grp][lane * V + e] = acc[e];
+        } else if (on) {
+            flag |= SEG_TAIL;
+            tid = cur;
+            #pragma unroll
+            for (int e = 0; e < V; e++) s_tail[grp][lane * V + e] = acc[e];
+        } else if (cur < vocab && col) {
+            put_row<V>(a, cur, piece, acc);
+        }
+    }
+    if (lane == 0) { s_flag[grp] = flag; s_hid[grp] = hid; s_tid[grp] = tid; }
+    __syncthreads();
+    if (threadIdx.x >= G) return;
+    // one group's lanes join the runs in order; `open`: a sum is being carried,
+    // `early`: it began before this block
+    uint32_t out = 0, out_id = none;
+    bool open = false, early = false;
+    uint32_t id = none;
+    #pragma unroll
+    for (int e = 0; e < V; e++) acc[e] = 0.f;
+    for (int g = 0; g < NG; g++) {
+        const uint32_t f = s_flag[g];
+        if (f & SEG_HEAD) {
+            if (!open) { open = true; early = true; id = s_hid[g]; }
+            #pragma unroll
+            for (int e = 0; e < V; e++) acc[e] += s_head[g][lane * V + e];
+            if (!(f & SEG_THROUGH)) {
+                if (early) {
+                    out |= SEG_HEAD;
+                    if (col) VecIO<float, V>::st(a.head + (long)blockIdx.x * a.width + (long)piece * V, acc);
+                } else if (id < vocab && col) {
+                    put_row<V>(a, id, piece, acc);
+                }
+                open = false;
+            }
+        }
+        if (f & SEG_TAIL) {
+            open = true;
+            early = false;
+            id = s_tid[g];
+            #pragma unroll
+            for (int e = 0; e < V; e++) acc[e] = s_tail[g][lane * V + e];
+        }
+        if (!open) {
+            #pragma unroll
+            for (int e = 0; e < V; e++) acc[e] = 0.f;
+        }
+    }
+    if (open) {
+        out |= early ? SEG_HEAD | SEG_THROUGH : SEG_TAIL;
+        if (!early) out_id = id;
+        float* p = (early ? a.head : a.tail) + (long)blockIdx.x * a.width + (long)piece * V;
+        if (col) VecIO<float, V>::st(p, acc);
+    }
+    // every slice's block computes the same flags from the keys alone
+    if (threadIdx.x == 0 && blockIdx.y == 0) {
+        a.flags[blockIdx.x] = out;
+        a.tail_id[blockIdx.x] = out_id;
+    }
+}
+
+// Joins the segments that cross blocks: the block of chunk c whose tail goes
+// on adds the heads of the chunks after it, up to and including the first
+// that the segment does not pass through.  32 columns a block column, 8
+// threads over the partials of each, combined in a fixed order.
+__global__ void __launch_bounds__(256) k_embed_join(const __grid_constant__ SumArgs a) {
+    const int c = blockIdx.x;
+    if (!(a.flags[c] & SEG_TAIL)) return;
+    const uint32_t id = a.tail_id[c];
+    if (id >= (uint32_t)a.vocab) return;                    // the padding id's places
+    __shared__ float part[8][32];
+    __shared__ int s_end;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    // chunks c + 1 .. end hold the rest
+    if (threadIdx.x == 0) s_end = a.nchunks - 1;
+    for (int j0 = c + 1; j0 < a.nchunks; j0 += 256) {
+        __syncthreads();
+        const int j = j0 + threadIdx.x;
+        const bool stop = j < a.nchunks && !(a.flags[j] & SEG_THROUGH);
+        if (stop) atomicMin(&s_end, j);
+        if (__syncthreads_or(stop)) break;
+    }
+    __syncthreads();
+    const int end = s_end, len = end - c;                   // partial rows: tail + len heads
+    const int per = (len + 7) / 8;
+    for (int col = blockIdx.y * 32; col < a.width; col += gridDim.y * 32) {
+        const int x = col + tx;
+        float s = 0.f;
+        if (x < a.width) {
+            if (ty == 0) s = a.tail[(long)c * a.width + x];
+            const int j1 = min(len, (ty + 1) * per);
+            #pragma unroll 4
+            for (int j = ty * per; j < j1; j++) s += a.head[(long)(c + 1 + j) * a.width + x];
+        }
+        part[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && x < a.width) {
+            #pragma unroll
+            for (int k = 1; k < 8; k++) s += part[k][tx];
+            const float v[1] = {s};
+            put_row<1>(a, id, x, v);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------ host side
+struct Plan {
+    int items, tiles, passes;        // sort
+    int chunk, nchunks;              // sums (run and slices follow from the variant)
+    long o_keys[2], o_pos[2], o_counts, o_head, o_tail, o_flags, o_tid, o_present, bytes;
+};
+
+long up256(long x) { return (x + 255) / 256 * 256; }
+
+// Everything follows from n, vocab and width, so that the size can be asked
+// for before the call; the alignment-dependent choices do not change it.
+Plan plan(long n, int vocab, int width) {
+    Plan p;
+    // 16 places a thread fill the SMs from 2.4 M places on; below, 4 give
+    // four times the blocks
+    p.items = n > 148L * SORT_T * 4 ? 16 : 4;
+    p.tiles = (int)cdiv(n, (long)SORT_T * p.items);
+    int bits = 1;
+    while (bits < 31 && (1L << bits) <= vocab) bits++;      // keys 0 .. vocab
+    p.passes = (bits + 7) / 8;
+    // about eight blocks a processor over all column slices, at least 8
+    // places a lane group
+    const int slices = (int)cdiv(width, 256);
+    long want = (n * slices + 148 * 8 - 1) / (148 * 8);
+    p.chunk = (int)((want < 64 ? 64 : want) + 31) / 32 * 32;
+    p.nchunks = (int)cdiv(n, p.chunk);
+    long o = 0;
+    for (int i = 0; i < 2; i++) {
+        p.o_keys[i] = o; o = up256(o + 4 * n);
+        p.o_pos[i] = o; o = up256(o + 4 * n);
+    }
+    p.o_counts = o; o = up256(o + 4L * 256 * p.tiles);
+    p.o_head = o; o = up256(o + 4L * width * p.nchunks);
+    p.o_tail = o; o = up256(o + 4L * width * p.nchunks);
+    p.o_flags = o; o = up256(o + 4L * p.nchunks);
+    p.o_tid = o; o = up256(o + 4L * p.nchunks);
+    p.o_present = o; o = up256(o + vocab);
+    p.bytes = o;
+    return p;
+}
+
+template <typename TT, typename TO>
+void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids, long n,
+               int vocab, int width, float scale, int pad_id, int V, cudaStream_t s) {
+    const int pieces = width / V;
+    int lx = 0;
+    while (lx < 8 && (1 << lx) < pieces) lx++;
+    const long rows = (256 >> lx) * 4L;
+    const long blocks = (n + rows - 1) / rows;
+    const unsigned grid = (unsigned)(blocks < 148L * 32 ? blocks : 148L * 32);
+    ++g_ptcg_launches;
+    #define EF(V) k_embed_fwd<TT, TO, V><<<grid, 256, 0, s>>>((TO*)out, ldo, (const TT*)table, ldt, \
+        ids, n, vocab, pieces, lx, scale, pad_id, pad_id >= 0)
+    if (V == 8) EF(8); else EF(1);
+    #undef EF
+}
+
+template <int ITEMS>
+void sort_pass(int first, uint32_t* ko, uint32_t* po, const uint32_t* ki, const uint32_t* pi,
+               uint32_t* counts, const int* ids, long n, int shift, int vocab, int pad_id,
+               uint8_t* present, int tiles, cudaStream_t s) {
+    const int hp = pad_id >= 0;
+    g_ptcg_launches += 2;
+    if (first) {
+        k_sort_count<ITEMS, true><<<tiles, SORT_T, 0, s>>>(counts, ki, ids, n, shift, vocab, pad_id, hp, present);
+        k_sort_scatter<ITEMS, true><<<tiles, SORT_T, 0, s>>>(ko, po, counts, ki, pi, ids, n, shift, vocab, pad_id, hp);
+    } else {
+        k_sort_count<ITEMS, false><<<tiles, SORT_T, 0, s>>>(counts, ki, ids, n, shift, vocab, pad_id, hp, present);
+        k_sort_scatter<ITEMS, false><<<tiles, SORT_T, 0, s>>>(ko, po, counts, ki, pi, ids, n, shift, vocab, pad_id, hp);
+    }
+}
+
+template <typename T, int V, int G>
+void embed_sum(SumArgs a, cudaStream_t s) {
+    a.pieces = a.width / V;
+    a.run = (int)cdiv(a.chunk, 256 / G);
+    a.zero_blocks = a.accumulate ? 0 : (int)std::min<long>(148 * 4, cdiv(a.vocab, 256 / G));
+    const dim3 grid(a.nchunks + a.zero_blocks, cdiv(a.pieces, G));
+    ++g_ptcg_launches, k_embed_sum<T, V, G><<<grid, 256, 0, s>>>(a);
+}
+template <typename T>
+void embed_sum(const SumArgs& a, int V, cudaStream_t s) {
+    // a lane group as wide as the row needs: 8, 16 or 32 lanes
+    const int lanes = a.width / V;
+    if (V == 8) {
+        if (lanes <= 8) embed_sum<T, 8, 8>(a, s);
+        else if (lanes <= 16) embed_sum<T, 8, 16>(a, s);
+        else embed_sum<T, 8, 32>(a, s);
+    } else {
+        embed_sum<T, 1, 32>(a, s);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int ptcg_embedding_fwd(const void* table, int table_dtype, long ldt, int vocab, int width,
+                       const int* ids, long n, float scale, int pad_id, void* out, int out_dtype,
+                       long ldo, void* stream) {
+    OP_REQ(dt_ok(table_dtype) && dt_ok(out_dtype), PTCG_EINVAL, "embedding: unknown dtype");
+    OP_REQ(vocab > 0 && width > 0 && n >= 0 && ldt >= width && ldo >= width, PTCG_EINVAL,
+           "embedding: bad sizes (vocab %d, width %d, n %ld, ldt %ld, ldo %ld)", vocab, width, n,
+           ldt, ldo);
+    if (n == 0) return PTCG_OK;
+    OP_REQ(table && ids && out, PTCG_EINVAL, "embedding: null pointer");
+    OP_REQ(el_ok(table, table_dtype) && el_ok(out, out_dtype) && (uintptr_t)ids % 4 == 0,
+           PTCG_EINVAL, "embedding: pointer not aligned to its element");
+    cudaStream_t s = (cudaStream_t)stream;
+    const int V = width % 8 == 0 && vec_ok(table, table_dtype, ldt, 8) && vec_ok(out, out_dtype, ldo, 8) ? 8 : 1;
+    #define EF(TT, TO) embed_fwd<TT, TO>(out, ldo, table, ldt, ids, n, vocab, width, scale, pad_id, V, s)
+    if (table_dtype == PTCG_BF16) { if (out_dtype == PTCG_BF16) EF(bf16, bf16); else EF(bf16, float); }
+    else { if (out_dtype == PTCG_BF16) EF(float, bf16); else EF(float, float); }
+    #undef EF
+    OP_CKL();
+    return PTCG_OK;
+}
+
+long ptcg_embedding_bwd_scratch(long n, int vocab, int width) {
+    OP_REQ(n >= 0 && n <= 0x7fffffffL && vocab > 0 && width > 0, -1,
+           "embedding gradient: bad sizes (n %ld, vocab %d, width %d)", n, vocab, width);
+    return n == 0 ? 0 : plan(n, vocab, width).bytes;
+}
+
+int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* ids, long n,
+                       float scale, int pad_id, float* dtable, long lddt, int vocab, int width,
+                       int accumulate, void* scratch, long scratch_bytes, void* stream) {
+    OP_REQ(dt_ok(dout_dtype), PTCG_EINVAL, "embedding gradient: unknown dtype");
+    OP_REQ(vocab > 0 && width > 0 && n >= 0 && lddo >= width && lddt >= width && dtable, PTCG_EINVAL,
+           "embedding gradient: bad arguments (vocab %d, width %d, n %ld, lddo %ld, lddt %ld)",
+           vocab, width, n, lddo, lddt);
+    OP_REQ(n <= 0x7fffffffL, PTCG_EINVAL, "embedding gradient: more than 2^31 - 1 places");
+    OP_REQ((uintptr_t)dtable % 4 == 0, PTCG_EINVAL, "embedding gradient: dtable not aligned to its element");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (n == 0) {
+        if (!accumulate)
+            OP_CK(cudaMemset2DAsync(dtable, lddt * 4, 0, (size_t)width * 4, vocab, s));
+        return PTCG_OK;
+    }
+    OP_REQ(dout && ids && scratch, PTCG_EINVAL, "embedding gradient: null pointer");
+    OP_REQ(el_ok(dout, dout_dtype) && (uintptr_t)ids % 4 == 0 && (uintptr_t)scratch % 16 == 0,
+           PTCG_EINVAL, "embedding gradient: misaligned pointer (scratch: 16 bytes)");
+    const Plan p = plan(n, vocab, width);
+    OP_REQ(scratch_bytes >= p.bytes, PTCG_ERANGE, "embedding gradient: scratch of %ld bytes, %ld needed",
+           scratch_bytes, p.bytes);
+    uint8_t* base = (uint8_t*)scratch;
+    uint32_t* keys[2] = {(uint32_t*)(base + p.o_keys[0]), (uint32_t*)(base + p.o_keys[1])};
+    uint32_t* pos[2] = {(uint32_t*)(base + p.o_pos[0]), (uint32_t*)(base + p.o_pos[1])};
+    uint32_t* counts = (uint32_t*)(base + p.o_counts);
+    uint8_t* present = base + p.o_present;
+    OP_CK(cudaMemsetAsync(present, 0, vocab, s));
+    for (int i = 0; i < p.passes; i++) {
+        uint32_t *ko = keys[i & 1], *po = pos[i & 1], *ki = keys[(i & 1) ^ 1], *pi = pos[(i & 1) ^ 1];
+        if (p.items == 16)
+            sort_pass<16>(i == 0, ko, po, ki, pi, counts, ids, n, 8 * i, vocab, pad_id, present, p.tiles, s);
+        else
+            sort_pass<4>(i == 0, ko, po, ki, pi, counts, ids, n, 8 * i, vocab, pad_id, present, p.tiles, s);
+    }
+    SumArgs a;
+    a.dout = dout; a.lddo = lddo;
+    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1];
+    a.n = n;
+    a.dtab = dtable; a.lddt = lddt;
+    a.head = (float*)(base + p.o_head); a.tail = (float*)(base + p.o_tail);
+    a.flags = (uint32_t*)(base + p.o_flags); a.tail_id = (uint32_t*)(base + p.o_tid);
+    a.present = present;
+    a.vocab = vocab; a.width = width; a.pieces = 0; a.accumulate = accumulate != 0;
+    a.chunk = p.chunk; a.run = 0; a.nchunks = p.nchunks; a.zero_blocks = 0;
+    a.scale = scale;
+    const int V = width % 8 == 0 && vec_ok(dout, dout_dtype, lddo, 8) && vec_ok(dtable, PTCG_FP32, lddt, 8) ? 8 : 1;
+    if (dout_dtype == PTCG_BF16) embed_sum<bf16>(a, V, s); else embed_sum<float>(a, V, s);
+    if (p.nchunks > 1) {
+        const int cols = (int)cdiv(width, 32);
+        ++g_ptcg_launches, k_embed_join<<<dim3(p.nchunks, cols < 32 ? cols : 32), 256, 0, s>>>(a);
+    }
+    OP_CKL();
+    return PTCG_OK;
+}
+
+}  // extern "C"

@@ -10,6 +10,8 @@ enum { DT_F32 = 0, DT_BF16 = 1 };
 
 // number of kernels this library has launched (every launch site increments it)
 extern std::atomic<long long> g_ptcg_launches;
+// records the message ptcg_last_error() returns on this thread
+void set_err(const char* fmt, ...);
 enum { ACT_NONE = 0, ACT_GELU = 1, ACT_GELU_BWD = 2 };
 
 // C[m, n] = epilogue( alpha * sum_k A(m, k) * B(n, k) )

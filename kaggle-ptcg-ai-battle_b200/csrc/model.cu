@@ -37,7 +37,7 @@ static std::atomic<int> g_fused_mlp{0};
 
 // ------------------------------------------------------------------ errors
 static thread_local char g_err[1024];
-static void set_err(const char* fmt, ...) {
+void set_err(const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof g_err, fmt, ap);

@@ -32,6 +32,16 @@ class PtcgShape(C.Structure):
                    s.n_cards, s.n_attacks, s.n_skills)
 
 
+class PtcgHeads(C.Structure):
+    _fields_ = [("seq", L), ("row", L), ("head", L)]
+
+
+class PtcgCross(C.Structure):
+    _fields_ = ([(n, I) for n in ("dtype", "nseq", "lq", "lk", "heads", "kv_heads", "dh")]
+                + [("scale", F)]
+                + [(n, PtcgHeads) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")])
+
+
 GRAD_HOOK = C.CFUNCTYPE(None, C.c_void_p, C.c_long, C.c_long, C.c_void_p)
 
 _SIGS = {
@@ -98,6 +108,17 @@ _SIGS = {
     "ptcg_eval_gelu": (I, [P, P, P, I, P]),
     "ptcg_attention_fwd": (I, [I, P, L, P, P, L, P, I, I, I, P]),
     "ptcg_attention_bwd": (I, [I, P, L, P, P, L, P, L, P, P, L, P, I, I, I, P]),
+    "ptcg_embedding_fwd": (I, [P, I, L, I, I, P, L, F, I, P, I, L, P]),
+    "ptcg_embedding_bwd_scratch": (L, [L, I, I]),
+    "ptcg_embedding_bwd": (I, [P, I, L, P, L, F, I, P, L, I, I, I, P, L, P]),
+    "ptcg_layer_norm_fwd": (I, [P, I, L, P, P, F, P, I, L, P, P, L, I, P]),
+    "ptcg_layer_norm_bwd_scratch": (L, [L, I]),
+    "ptcg_layer_norm_bwd": (I, [P, I, L, P, I, L, P, P, P, P, L, P, L, P, P, I, L, I, P, L, P]),
+    "ptcg_cross_attention_fwd_scratch": (L, [C.POINTER(PtcgCross)]),
+    "ptcg_cross_attention_fwd": (I, [C.POINTER(PtcgCross), P, P, P, P, P, P, P, P, L, P]),
+    "ptcg_cross_attention_bwd_scratch": (L, [C.POINTER(PtcgCross)]),
+    "ptcg_cross_attention_bwd": (I, [C.POINTER(PtcgCross), P, P, P, P, P, P, P, P, P, P, P, P, L,
+                                     P]),
     "ptcg_device_error": (I, []),
     "ptcg_set_attention_impl": (I, [I]),
     "ptcg_get_attention_impl": (I, []),

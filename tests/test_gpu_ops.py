@@ -1,0 +1,477 @@
+"""The decoder operators on the GPU against their formulas in 64 bits, inside
+bounds that count the roundings (ops_reference.py), at the sizes, masks,
+strides and calls where they can go wrong."""
+import itertools
+import math
+
+import pytest
+import torch
+
+import ops_reference as ref
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    import ptcg_b200.ops
+    return ptcg_b200.ops
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+# -------------------------------------------------------------- embedding
+@pytest.mark.parametrize("td,od", list(itertools.product([F32, BF16], repeat=2)))
+@pytest.mark.parametrize("n,vocab,width", [(1, 1, 1), (3, 7, 8), (64, 4096, 128), (1000, 17, 33),
+                                           (257, 50, 1032), (5, 9, 2049)])
+def test_embedding_forward(ops, td, od, n, vocab, width):
+    g = gen(n + width)
+    table = rand(g, vocab, width, dtype=td)
+    ids = torch.randint(-3, vocab + 3, (n,), generator=g, device="cuda", dtype=torch.int32)
+    for pad in (None, 0):
+        got = ops.embedding(table, ids, scale=1.7, pad_id=pad, out_dtype=od)
+        scale = float(torch.tensor(1.7, dtype=F32))
+        want, bound = ref.embedding(table, ids, scale, pad, od)
+        assert got.dtype == od and got.shape == (n, width)
+        ref.within(got, want, bound)
+
+
+def test_embedding_forward_views(ops):
+    g = gen(1)
+    ids = torch.randint(0, 20, (2, 3, 5), generator=g, device="cuda", dtype=torch.int32)
+    for table in (rand(g, 20, 72)[:, 8:40], rand(g, 20, 41)[:, 3:36], rand(g, 33, 20).t(),
+                  rand(g, 20, 40, dtype=BF16)[:, 1:33]):
+        got = ops.embedding(table, ids, scale=0.5)
+        want, bound = ref.embedding(table, ids, 0.5, None, table.dtype)
+        ref.within(got, want, bound)
+    assert ops.embedding(rand(g, 4, 8), ids[:0]).shape == (0, 3, 5, 8)
+
+
+GRADS = [  # n, vocab, width, how the ids fall
+    (1, 1, 1, "one"), (1, 300, 8, "any"), (7, 3, 33, "any"), (64, 4096, 128, "any"),
+    (31, 5, 40, "one"), (4095, 257, 8, "any"), (4097, 255, 64, "skew"), (8192, 256, 16, "one"),
+    (5000, 65537, 24, "any"), (3000, 70000, 9, "skew"), (20000, 40, 136, "skew"),
+    (12289, 11, 7, "skew"), (2500, 4000, 520, "any"), (700001, 1000, 8, "skew"),
+    (611000, 3, 1, "any")]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,vocab,width,how", GRADS)
+def test_embedding_gradient(ops, dtype, n, vocab, width, how):
+    g = gen(n + vocab)
+    if how == "one":
+        ids = torch.full((n,), vocab // 2, device="cuda", dtype=torch.int32)
+    elif how == "any":
+        ids = torch.randint(-2, vocab + 2, (n,), generator=g, device="cuda", dtype=torch.int32)
+    else:
+        u = torch.rand(n, generator=g, device="cuda")
+        ids = (torch.exp(u * math.log(vocab)).int() - 1).clamp(0, vocab - 1)
+    dout = rand(g, n, width, dtype=dtype)
+    for pad in (None, vocab // 2):
+        want, bound = ref.embedding_grad(dout, ids, vocab, 1.5, pad)
+        got = ops.embedding_backward(dout, ids, vocab, scale=1.5, pad_id=pad)
+        ref.within(got, want, bound, f"pad {pad}")
+        again = ops.embedding_backward(dout, ids, vocab, scale=1.5, pad_id=pad)
+        assert torch.equal(got, again)                     # no order that depends on scheduling
+        base = rand(g, vocab, width)
+        acc = ops.embedding_backward(dout, ids, vocab, scale=1.5, pad_id=pad, dtable=base.clone(),
+                                     accumulate=True)
+        ref.within(acc, base.double() + want, bound + 2 * ref.U * (base.double().abs() + want.abs()))
+        rows = torch.unique(ids[ids != pad] if pad is not None else ids).long().clamp(0, vocab - 1)
+        still = torch.ones(vocab, dtype=torch.bool, device="cuda")
+        still[rows] = False
+        assert torch.equal(acc[still], base[still])
+
+
+def test_embedding_gradient_views(ops):
+    g = gen(3)
+    ids = torch.randint(0, 50, (6, 100), generator=g, device="cuda", dtype=torch.int32)
+    big = rand(g, 6, 100, 80, dtype=BF16)
+    for dout in (big[..., 8:72], big[..., 3:68], big[:, :, :64].transpose(0, 1).transpose(0, 1),
+                 big[:1, :1, :32].expand(6, 100, 32)):
+        width = dout.shape[-1]
+        want, bound = ref.embedding_grad(dout, ids, 50, 1.0, None)
+        ref.within(ops.embedding_backward(dout, ids, 50), want, bound)
+        frame = torch.full((50, width + 8), 7.0, device="cuda")
+        got = ops.embedding_backward(dout, ids, 50, dtable=frame[:, 4:width + 4])
+        ref.within(got, want, bound)
+        assert (frame[:, :4] == 7).all() and (frame[:, width + 4:] == 7).all()
+    none = ops.embedding_backward(big[:0], ids[:0], 50)
+    assert none.shape == (50, 80) and (none == 0).all()
+    keep = torch.ones(50, 80, device="cuda")
+    assert (ops.embedding_backward(big[:0], ids[:0], 50, dtable=keep, accumulate=True) == 1).all()
+
+
+def test_embedding_padding_may_hold_anything(ops):
+    g = gen(4)
+    ids = torch.randint(0, 6, (500,), generator=g, device="cuda", dtype=torch.int32)
+    dout = rand(g, 500, 24)
+    want, bound = ref.embedding_grad(dout, ids, 6, 1.0, 5)
+    dout[ids == 5] = math.nan
+    table = rand(g, 6, 24)
+    table[5] = math.inf
+    ref.within(ops.embedding_backward(dout, ids, 6, pad_id=5), want, bound)
+    assert (ops.embedding(table, ids, pad_id=5)[ids == 5] == 0).all()
+
+
+# ------------------------------------------------------------- layer norm
+ROWS_WIDTHS = [(1, 1), (3, 2), (1, 256), (9, 31), (17, 32), (8, 33), (5, 100), (300, 128),
+               (1000, 256), (33, 634), (7, 768), (10, 1023), (10, 1024), (4, 1025), (300, 1028),
+               (5, 2050), (40, 5001), (160, 8192), (6000, 36), (5000, 61)]
+
+
+@pytest.mark.parametrize("xd,yd", list(itertools.product([F32, BF16], repeat=2)))
+@pytest.mark.parametrize("rows,width", ROWS_WIDTHS)
+def test_layer_norm(ops, xd, yd, rows, width):
+    g = gen(rows + width)
+    x = (rand(g, rows, width) * (0.2 + 3 * torch.rand(rows, 1, generator=g, device="cuda"))
+         + 5 * rand(g, rows, 1)).to(xd)
+    gamma, beta = 1 + 0.3 * rand(g, width), rand(g, width)
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    f = ref.norm(x, gamma, beta, eps)
+    y, mean, rstd = ops.layer_norm(x, gamma, beta, out_dtype=yd)
+    assert y.dtype == yd
+    ref.within(y, f["y"], f["e_y"] + ref.HALF[yd] * (f["y"].abs() + f["e_y"]), "y")
+    ref.within(mean, f["mean"][:, 0], f["e_mean"][:, 0], "mean")
+    ref.within(rstd, f["rstd"][:, 0], f["e_rstd"][:, 0], "rstd")
+    y2, none, _ = ops.layer_norm(x, gamma, beta, out_dtype=yd, stats=False)
+    assert none is None and torch.equal(y, y2)
+    dy = rand(g, rows, width, dtype=yd)
+    for dres in (None, rand(g, rows, width, dtype=xd)):
+        dx, e_dx, dg, e_dg, db, e_db = ref.norm_grad(f, dy, dres, xd)
+        got = ops.layer_norm_backward(dy, x, gamma, mean, rstd, dres=dres)
+        assert got[0].dtype == xd
+        # the stored statistics the backward reads are the ones bounded above
+        ref.within(got[0], dx, 2 * e_dx, "dx")
+        ref.within(got[1], dg, 2 * e_dg, "dgamma")
+        ref.within(got[2], db, e_db, "dbeta")
+        again = ops.layer_norm_backward(dy, x, gamma, mean, rstd, dres=dres)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    base = rand(g, 2, width)
+    acc = ops.layer_norm_backward(dy, x, gamma, mean, rstd, dgamma=base[0].clone(),
+                                  dbeta=base[1].clone(), accumulate=True)
+    ref.within(acc[1], base[0].double() + dg, 2 * e_dg + 2 * ref.U * (base[0].abs() + dg.abs()))
+    ref.within(acc[2], base[1].double() + db, e_db + 2 * ref.U * (base[1].abs() + db.abs()))
+    only = ops.layer_norm_backward(dy, x, gamma, mean, rstd, weight_grads=False)
+    assert only[1] is None and only[2] is None
+    ref.within(only[0], ref.norm_grad(f, dy, None, xd)[0], 2 * ref.norm_grad(f, dy, None, xd)[1], "dx alone")
+
+
+def test_layer_norm_plain_views_and_empty(ops):
+    g = gen(9)
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    big = rand(g, 4, 6, 300)
+    for x in (big, big[..., 20:120], big[..., 1:98], big[:, ::2], big.transpose(0, 1),
+              big[:1].expand(4, 6, 300)):
+        f = ref.norm(x, None, None, eps)
+        y, mean, rstd = ops.layer_norm(x)
+        ref.within(y, f["y"], f["e_y"] + ref.U * f["y"].abs())
+        dy = rand(g, *x.shape)
+        dx, e_dx, dg, e_dg, db, e_db = ref.norm_grad(f, dy, None, F32)
+        got = ops.layer_norm_backward(dy, x, None, mean, rstd)
+        ref.within(got[0], dx, 2 * e_dx)
+        ref.within(got[1], dg, 2 * e_dg)
+        ref.within(got[2], db, e_db)
+    e = torch.zeros(0, 300, device="cuda")
+    y, mean, rstd = ops.layer_norm(e)
+    assert y.shape == (0, 300) and mean.shape == (0,)
+    dx, dg, db = ops.layer_norm_backward(e, e, None, mean, rstd)
+    assert dx.shape == (0, 300) and (dg == 0).all() and (db == 0).all()
+
+
+def test_layer_norm_in_place(pkg, ops):
+    """y over x, dx over dres and dx over dy through the C entry."""
+    import ptcg_b200.native as n
+    lib, g = n.lib(), gen(11)
+    s = torch.cuda.current_stream().cuda_stream
+    for rows, width in ((37, 256), (21, 2600), (13, 77)):
+        x = rand(g, rows, width)
+        gamma, beta = rand(g, width), rand(g, width)
+        y, mean, rstd = ops.layer_norm(x, gamma, beta)
+        z = x.clone()
+        p = lambda t: t.data_ptr()                                     # noqa: E731
+        assert lib.ptcg_layer_norm_fwd(p(z), 0, width, p(gamma), p(beta), 1e-5, p(z), 0, width,
+                                       None, None, rows, width, s) == 0
+        assert torch.equal(z, y)
+        dy, dres = rand(g, rows, width), rand(g, rows, width)
+        dx, dg, db = ops.layer_norm_backward(dy, x, gamma, mean, rstd, dres=dres)
+        need = lib.ptcg_layer_norm_bwd_scratch(rows, width)
+        scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+        for over in (dres.clone(), dy.clone()):
+            src = {"dy": dy, "dres": dres}
+            src["dres" if torch.equal(over, dres) else "dy"] = over
+            w = torch.empty(2, width, device="cuda")
+            assert lib.ptcg_layer_norm_bwd(
+                p(src["dy"]), 0, width, p(x), 0, width, p(gamma), p(mean), p(rstd), p(src["dres"]),
+                width, p(over), width, p(w[0]), p(w[1]), 0, rows, width, p(scratch), need, s) == 0
+            assert torch.equal(over, dx) and torch.equal(w[0], dg) and torch.equal(w[1], db)
+
+
+def test_layer_norm_constant_and_far_rows(ops):
+    """A constant row has variance 0 (y = beta); a row far from 0 keeps its
+    digits, since the variance is taken about the mean."""
+    x = torch.full((3, 640), 12345.0, device="cuda")
+    y, mean, rstd = ops.layer_norm(x, None, torch.full((640,), 0.5, device="cuda"))
+    assert (mean == 12345).all() and (y == 0.5).all()
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    assert torch.allclose(rstd.double(), torch.full((3,), eps ** -0.5, device="cuda", dtype=torch.float64),
+                          rtol=2 ** -20)
+
+
+# -------------------------------------------------------- cross attention
+def problem(seed, nseq, lq, lk, heads, kvh, dh, dtype, mask, layout="rows"):
+    g = gen(seed)
+    q = rand(g, nseq, lq, heads, dh, dtype=dtype)
+    if layout == "heads":
+        k, v = (rand(g, nseq, kvh, lk, dh, dtype=dtype).transpose(1, 2) for _ in range(2))
+    elif layout == "packed":                     # q as a slice, k and v interleaved
+        q = rand(g, nseq, lq, heads, 3 * dh, dtype=dtype)[..., dh:2 * dh]
+        k, v = rand(g, nseq, lk, 2, kvh, dh, dtype=dtype).unbind(2)
+    else:
+        k, v = (rand(g, nseq, lk, kvh, dh, dtype=dtype) for _ in range(2))
+    keep = kv_len = None
+    if "keep" in mask:
+        keep = torch.rand(nseq, lk, generator=g, device="cuda") < 0.6
+        keep[nseq // 2] = False                  # a sequence without a key
+        keep[0, : lk // 2] = False               # leading holes, tiles with no key
+    if "len" in mask:
+        kv_len = torch.randint(-2, lk + 4, (nseq,), generator=g, device="cuda", dtype=torch.int32)
+        kv_len[0], kv_len[-1] = lk, 0
+    return q, k, v, {"keep": keep, "kv_len": kv_len}
+
+
+def run_cross(ops, q, k, v, mask, scale=None, seed=5):
+    dout = rand(gen(seed), *q.shape, dtype=q.dtype)
+    out, lse = ops.cross_attention(q, k, v, scale=scale, **mask)
+    grads = ops.cross_attention_backward(dout, q, k, v, out, lse, scale=scale, **mask)
+    return dout, (out, lse, *grads)
+
+
+def check_cross(ops, q, k, v, mask, scale=None):
+    dout, got = run_cross(ops, q, k, v, mask, scale)
+    r = ref.cross(q, k, v, scale=scale, dout=dout, **mask)
+    for name, t in zip(("out", "lse", "dq", "dk", "dv"), got):
+        assert t.dtype == (F32 if name == "lse" else q.dtype)
+        ref.within(t, r[name], r["e_" + name], name)
+    live = ref.live_keys(k.shape[0], k.shape[1], mask["keep"], mask["kv_len"], "cuda")
+    assert (got[3][~live] == 0).all() and (got[4][~live] == 0).all()
+    empty = ~live.any(-1)
+    assert (got[0][empty] == 0).all() and (got[2][empty] == 0).all()
+    assert (got[1][empty] == -math.inf).all()
+    return dout, got
+
+
+CROSS = [  # nseq, lq, lk, heads, kv_heads, dh
+    (1, 1, 1, 1, 1, 32), (4, 1, 129, 8, 8, 32), (3, 1, 700, 8, 2, 64), (2, 1, 3000, 8, 1, 128),
+    (5, 64, 129, 8, 8, 32), (3, 17, 63, 4, 2, 64), (2, 65, 64, 2, 2, 128), (2, 130, 65, 4, 1, 32),
+    (1, 63, 1000, 2, 1, 128), (1, 700, 33, 3, 3, 64), (1, 1500, 70, 2, 1, 32), (7, 5, 8, 6, 3, 32),
+    (2, 16, 257, 1, 1, 128), (1, 300, 520, 4, 4, 128), (300, 9, 31, 2, 1, 32)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask", ["none", "keep", "len", "keep len"])
+@pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", CROSS)
+def test_cross_attention(ops, dtype, mask, nseq, lq, lk, heads, kvh, dh):
+    q, k, v, m = problem(nseq * lq + lk, nseq, lq, lk, heads, kvh, dh, dtype, mask)
+    dout, got = check_cross(ops, q, k, v, m)
+    again = run_cross(ops, q, k, v, m)[1]
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("layout", ["heads", "packed"])
+@pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", [(3, 40, 75, 4, 2, 32), (2, 1, 900, 4, 4, 64),
+                                                     (2, 90, 40, 2, 2, 128)])
+def test_cross_attention_layouts(ops, dtype, layout, nseq, lq, lk, heads, kvh, dh):
+    q, k, v, m = problem(7, nseq, lq, lk, heads, kvh, dh, dtype, "keep len", layout)
+    check_cross(ops, q, k, v, m, scale=0.37)
+    # one encoder's states for every sequence: their gradients come per sequence
+    check_cross(ops, q, k[:1].expand_as(k), v[:1].expand_as(v), m)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lq", [1, 40])
+def test_cross_attention_masked_keys_may_hold_anything(ops, dtype, lq):
+    q, k, v, m = problem(13, 4, lq, 600, 4, 2, 64, dtype, "keep len")
+    dout, want = run_cross(ops, q, k, v, m)
+    live = ref.live_keys(4, 600, m["keep"], m["kv_len"], "cuda")
+    for junk in (math.nan, math.inf, -math.inf, torch.finfo(dtype).min):
+        kj, vj = k.clone(), v.clone()
+        kj[~live] = junk
+        vj[~live] = junk
+        got = run_cross(ops, q, kj, vj, m)[1]
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), junk
+    # keep as bytes other than 0 / 1
+    m8 = {"keep": m["keep"].to(torch.uint8) * 255, "kv_len": m["kv_len"]}
+    assert all(torch.equal(a, b) for a, b in zip(run_cross(ops, q, k, v, m8)[1], want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_cross_attention_no_lengths(ops, dtype):
+    z = lambda *s: torch.zeros(*s, device="cuda", dtype=dtype)     # noqa: E731
+    out, lse = ops.cross_attention(z(2, 3, 4, 32), z(2, 0, 2, 32), z(2, 0, 2, 32))
+    assert (out == 0).all() and (lse == -math.inf).all()
+    dq, dk, dv = ops.cross_attention_backward(out, z(2, 3, 4, 32), z(2, 0, 2, 32), z(2, 0, 2, 32), out, lse)
+    assert (dq == 0).all() and dk.shape == (2, 0, 2, 32)
+    q, k = z(2, 0, 4, 32), z(2, 70, 2, 32) + 1
+    out, lse = ops.cross_attention(q, k, k)
+    assert out.shape == (2, 0, 4, 32) and lse.shape == (2, 4, 0)
+    dq, dk, dv = ops.cross_attention_backward(out, q, k, k, out, lse)
+    assert (dk == 0).all() and (dv == 0).all()
+    out, lse = ops.cross_attention(z(0, 3, 4, 32), z(0, 70, 2, 32), z(0, 70, 2, 32))
+    assert out.shape == (0, 3, 4, 32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_cross_attention_large_scores(ops, dtype):
+    """Scores of hundreds: the running maximum keeps every exponential in
+    range, and rows whose maximum comes last are rescaled."""
+    q, k, v, m = problem(17, 2, 33, 300, 2, 2, 32, dtype, "none")
+    k = k * torch.linspace(0.1, 12, 300, device="cuda", dtype=dtype).view(1, 300, 1, 1)
+    q = q * 4
+    check_cross(ops, q, k, v, m)
+    check_cross(ops, q, k.flip(1), v, m)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_cross_attention_offsets_past_32_bits(ops, dtype):
+    """Sequences of one cache that lie more than 2^31 elements apart."""
+    far = (1 << 31) + 64
+    buf = torch.empty(far + 70 * 2 * 64, device="cuda", dtype=dtype)
+    k = buf.as_strided((2, 70, 2, 32), (far, 128, 32, 1))
+    v = buf.as_strided((2, 70, 2, 32), (far, 128, 32, 1), 64)
+    q, k0, v0, m = problem(19, 2, 21, 70, 4, 2, 32, dtype, "none")
+    k.copy_(k0)
+    v.copy_(v0)
+    check_cross(ops, q, k, v, m)
+
+
+def test_cross_attention_gradient_against_differences(ops):
+    """The fp32 gradients along a direction against central differences of the
+    formula in 64 bits (step 1e-5: the difference itself is good to 1e-9 of
+    the sums involved, below the gradient's own bound)."""
+    q, k, v, m = problem(23, 3, 19, 45, 4, 2, 32, F32, "keep len")
+    dout, got = run_cross(ops, q, k, v, m)
+    r = ref.cross(q, k, v, dout=dout, **m)
+    loss = lambda a, b, c: (ref.cross(a, b, c, **m)["out"] * dout.double()).sum()   # noqa: E731
+    base = [t.double() for t in (q, k, v)]
+    for i, name in enumerate(("dq", "dk", "dv")):
+        d = rand(gen(i), *base[i].shape).double()
+        plus, minus = list(base), list(base)
+        plus[i], minus[i] = base[i] + 1e-5 * d, base[i] - 1e-5 * d
+        diff = (loss(*plus) - loss(*minus)) / 2e-5
+        along = (got[2 + i].double() * d).sum()
+        bound = (r["e_" + name] * d.abs()).sum() + 1e-8 * (r[name] * d).abs().sum()
+        assert (diff - along).abs() <= bound, name
+
+
+# ------------------------------------------------------------ all together
+def decoder(ops, w, ids, enc, mask, dy=None):
+    """One pre-norm decoder sublayer: embedded options, norm, cross attention
+    to the encoder's rows, residual; with dy also the gradients of the table,
+    the norm and the encoder's keys and values."""
+    n, lq = ids.shape
+    x = ops.embedding(w["table"], ids, scale=2.0, pad_id=0)
+    h, mean, rstd = ops.layer_norm(x, w["gamma"], w["beta"], out_dtype=BF16)
+    q = h.view(n, lq, 4, 32)
+    k, v = enc[..., :64].unflatten(-1, (2, 32)), enc[..., 64:].unflatten(-1, (2, 32))
+    out, lse = ops.cross_attention(q, k, v, **mask)
+    y = x + out.reshape(n, lq, 128).float()
+    if dy is None:
+        return (y,)
+    dq, dk, dv = ops.cross_attention_backward(dy.to(BF16).view_as(q), q, k, v, out, lse, **mask)
+    dx, dg, db = ops.layer_norm_backward(dq.view(n, lq, 128), x, w["gamma"], mean, rstd, dres=dy)
+    return y, ops.embedding_backward(dx, ids, w["table"].shape[0], scale=2.0, pad_id=0), dg, db, dk, dv
+
+
+def decoder_inputs(seed):
+    g = gen(seed)
+    w = {"table": rand(g, 50, 128), "gamma": 1 + 0.1 * rand(g, 128), "beta": 0.1 * rand(g, 128)}
+    ids = torch.randint(0, 50, (6, 13), generator=g, device="cuda", dtype=torch.int32)
+    enc = rand(g, 6, 37, 128, dtype=BF16)
+    keep = torch.rand(6, 37, generator=g, device="cuda") < 0.7
+    return w, ids, enc, {"keep": keep, "kv_len": None}, rand(g, 6, 13, 128)
+
+
+def test_decoder_sublayer_against_autograd(ops):
+    """The chain against 64-bit autograd of the same formulas.  Every value
+    passes two or three bf16 roundings (2^-8 each: h, out, dq and the operands
+    P and dS), so each result is within 4 * 2^-8 in 2-norm."""
+    w, ids, enc, mask, dy = decoder_inputs(31)
+    got = decoder(ops, w, ids, enc, mask, dy)
+    t, ga, be, en = (a.double().requires_grad_() for a in (w["table"], w["gamma"], w["beta"], enc))
+    x = t[ids.long()] * 2.0 * (ids != 0)[..., None]
+    h = torch.nn.functional.layer_norm(x, (128,), ga, be)
+    q = h.view(6, 13, 4, 32)
+    k, v = (en[..., i:i + 64].unflatten(-1, (2, 32)).repeat_interleave(2, 2) for i in (0, 64))
+    s = torch.einsum("nihd,njhd->nhij", q, k) / math.sqrt(32)
+    p = torch.softmax(s.masked_fill(~mask["keep"][:, None, None, :], -math.inf), -1)
+    y = x + torch.einsum("nhij,njhd->nihd", p, v).reshape(6, 13, 128)
+    y.backward(dy.double())
+    want = (y, t.grad, ga.grad, be.grad, en.grad[..., :64].unflatten(-1, (2, 32)),
+            en.grad[..., 64:].unflatten(-1, (2, 32)))
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert (a.double() - b).norm() <= 4 * 2.0 ** -8 * b.norm(), i
+
+
+def test_graph_capture_and_replay(ops):
+    """Two captured graphs, replayed in turn on new inputs beside eager calls,
+    give the eager results bit for bit."""
+    sets = [decoder_inputs(s) for s in (41, 42)]
+    eager = [decoder(ops, *s) for s in sets]
+    graphs = []
+    for _ in range(2):
+        w, ids, enc, mask, dy = decoder_inputs(43)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            decoder(ops, w, ids, enc, mask, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs = decoder(ops, w, ids, enc, mask, dy)
+        graphs.append((gr, (w, ids, enc, mask, dy), outs))
+    for turn in range(4):
+        gr, (w, ids, enc, mask, dy), outs = graphs[turn % 2]
+        nw, nids, nenc, nmask, ndy = sets[turn // 2]
+        for k in w:
+            w[k].copy_(nw[k])
+        ids.copy_(nids), enc.copy_(nenc), mask["keep"].copy_(nmask["keep"]), dy.copy_(ndy)
+        gr.replay()
+        beside = decoder(ops, *sets[turn // 2])
+        torch.cuda.synchronize()
+        for a, b, c in zip(outs, eager[turn // 2], beside):
+            assert torch.equal(a, b) and torch.equal(c, b)
+
+
+def test_two_streams_at_once(ops):
+    """Calls that overlap on two streams share nothing."""
+    sets = [decoder_inputs(s) for s in (51, 52)]
+    want = [decoder(ops, *s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(decoder(ops, *sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_launches_are_counted(pkg, ops):
+    import ptcg_b200.native as n
+    lib = n.lib()
+    before = lib.ptcg_launch_count()
+    decoder(ops, *decoder_inputs(61))
+    # forward 3, attention backward 2, norm backward 2, embedding sort 2 and sums 1 at least
+    assert lib.ptcg_launch_count() - before >= 10
