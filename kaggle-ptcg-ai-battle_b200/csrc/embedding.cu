@@ -15,7 +15,8 @@ namespace {
 // -------------------------------------------------------------- forward
 // Bound: HBM (ids and output once; the table's touched rows once, from L2
 // after that).  LX lanes take a row's V-element pieces, 256 / LX rows to a
-// block pass, four rows in flight per thread.
+// block pass, four rows in flight per thread and the next rows' ids ahead of
+// them.
 template <typename TT, typename TO, int V>
 __global__ void __launch_bounds__(256) k_embed_fwd(
         TO* __restrict__ out, long ldo, const TT* __restrict__ table, long ldt,
@@ -24,13 +25,21 @@ __global__ void __launch_bounds__(256) k_embed_fwd(
     const int tx = threadIdx.x & ((1 << lx_log2) - 1), ty = threadIdx.x >> lx_log2;
     const int ry = 256 >> lx_log2;
     constexpr int U = 4;
-    for (long r0 = (long)blockIdx.x * ry * U; r0 < n; r0 += (long)gridDim.x * ry * U) {
-        int id[U];
+    const long step = (long)gridDim.x * ry * U;
+    int next[U];
+    auto fetch = [&](long r0) {
         #pragma unroll
         for (int u = 0; u < U; u++) {
             const long r = r0 + u * ry + ty;
-            id[u] = r < n ? ids[r] : 0;
+            next[u] = r < n ? ids[r] : 0;
         }
+    };
+    fetch((long)blockIdx.x * ry * U);
+    for (long r0 = (long)blockIdx.x * ry * U; r0 < n; r0 += step) {
+        int id[U];
+        #pragma unroll
+        for (int u = 0; u < U; u++) id[u] = next[u];
+        fetch(r0 + step);
         for (int c = tx; c < pieces; c += 1 << lx_log2) {
             float v[U][V];
             #pragma unroll
@@ -52,12 +61,14 @@ __global__ void __launch_bounds__(256) k_embed_fwd(
 }
 
 // ----------------------------------------------------------------- sort
-// Stable least-digit-first radix sort of (id, place), 8 bits a pass, two
-// launches a pass: the digit counts of each tile, then a scatter whose
-// blocks derive their own bases from all tiles' counts (a block reads
-// tiles x 256 counters from L2, which is cheaper here than a third launch
-// for the scan).  Bound: latency; it moves 16 bytes per place and pass.
-constexpr int SORT_T = 1024;
+// Stable least-digit-first radix sort of (id, place), up to 9 bits a pass, two
+// launches a pass: the digit counts of each tile, then a scatter whose blocks
+// derive their own bases from all tiles' counts (a block reads tiles x bins
+// counters from L2, which is cheaper here than a third launch for the scan).
+// Lanes with equal digits find each other by one ballot per digit bit; the
+// match instruction took 166 us where this takes 20 (first count of 2 M places).
+// Bound: latency and the scattered 8-byte writes; 16 bytes per place and pass.
+constexpr int SORT_T = 1024, MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 
 // the sort key of a place: its clamped id, or `vocab` for a padding place,
 // which sorts behind every row
@@ -65,125 +76,138 @@ PTCG_DEV uint32_t key_of(int id, int vocab, int pad_id, int has_pad) {
     if (has_pad && id == pad_id) return (uint32_t)vocab;
     return (uint32_t)min(max(id, 0), vocab - 1);
 }
+// the lanes with the same digit among those with `in`
+PTCG_DEV uint32_t same_digit(uint32_t d, bool in, int bits) {
+    uint32_t m = __ballot_sync(0xffffffffu, in);
+    for (int b = 0; b < bits; b++) {
+        const bool one = (d >> b) & 1;
+        const uint32_t v = __ballot_sync(0xffffffffu, one);
+        m &= one ? v : ~v;
+    }
+    return m;
+}
+
+struct SortArgs {
+    uint32_t *counts, *keys_out, *pos_out;
+    const uint32_t *keys, *pos;
+    const int* ids;
+    long n;
+    int shift, bits, vocab, pad_id, has_pad;
+};
 
 template <int ITEMS, bool FIRST>
-__global__ void __launch_bounds__(SORT_T) k_sort_count(
-        uint32_t* __restrict__ counts, const uint32_t* __restrict__ keys,
-        const int* __restrict__ ids, long n, int shift, int vocab, int pad_id, int has_pad,
-        uint8_t* __restrict__ present) {
-    __shared__ uint32_t hist[256];
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+__global__ void __launch_bounds__(SORT_T) k_sort_count(const __grid_constant__ SortArgs a) {
+    __shared__ uint32_t hist[MAX_BINS];
+    const int bins = 1 << a.bits, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < bins; i += SORT_T) hist[i] = 0;
     __syncthreads();
     const long base = (long)blockIdx.x * SORT_T * ITEMS;
+    uint32_t key[ITEMS];
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
         const long i = base + k * SORT_T + threadIdx.x;
-        const bool in = i < n;
-        uint32_t key = 0;
-        if (in) {
-            key = FIRST ? key_of(ids[i], vocab, pad_id, has_pad) : keys[i];
-            // every writer stores the same 1
-            if (FIRST && key < (uint32_t)vocab) present[key] = 1;
-        }
-        // one shared atomic per distinct digit of the warp: hot ids would
-        // serialise 32 of them
-        const uint32_t d = in ? (key >> shift) & 255u : 256u;
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
-        if (in && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
+        key[k] = 0;
+        if (i < a.n) key[k] = FIRST ? key_of(a.ids[i], a.vocab, a.pad_id, a.has_pad) : a.keys[i];
+    }
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const bool in = base + k * SORT_T + threadIdx.x < a.n;
+        const uint32_t d = (key[k] >> a.shift) & (bins - 1);
+        const uint32_t same = same_digit(d, in, a.bits);
+        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
     }
     __syncthreads();
-    if (threadIdx.x < 256) counts[(long)blockIdx.x * 256 + threadIdx.x] = hist[threadIdx.x];
+    for (int i = threadIdx.x; i < bins; i += SORT_T) a.counts[(long)blockIdx.x * bins + i] = hist[i];
 }
 
 template <int ITEMS, bool FIRST>
-__global__ void __launch_bounds__(SORT_T) k_sort_scatter(
-        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out,
-        const uint32_t* __restrict__ counts, const uint32_t* __restrict__ keys,
-        const uint32_t* __restrict__ pos, const int* __restrict__ ids, long n, int shift,
-        int vocab, int pad_id, int has_pad) {
+__global__ void __launch_bounds__(SORT_T) k_sort_scatter(const __grid_constant__ SortArgs a) {
     constexpr int NW = SORT_T / 32;
-    __shared__ uint32_t wcnt[NW][256];
-    __shared__ uint32_t tot[4][256], pre[4][256];
-    __shared__ uint32_t wsum[8];
+    // per warp and digit: its count, then its first place relative to the tile's
+    __shared__ uint16_t wcnt[NW][MAX_BINS];
+    __shared__ uint32_t tot[SORT_T], pre[SORT_T];
+    __shared__ uint32_t first[MAX_BINS], wsum[MAX_BINS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int tiles = gridDim.x, tile = blockIdx.x;
-    // counts of each digit over all tiles, and over the tiles before this one
-    {
-        const int d = tid & 255, part = tid >> 8;
-        uint32_t t = 0, p = 0;
-        #pragma unroll 4
-        for (int j = part; j < tiles; j += 4) {
-            const uint32_t c = counts[(long)j * 256 + d];
-            t += c;
-            p += j < tile ? c : 0u;
-        }
-        tot[part][d] = t;
-        pre[part][d] = p;
-        for (int i = tid; i < NW * 256; i += SORT_T) (&wcnt[0][0])[i] = 0;
-    }
-    __syncthreads();
-    // ranks inside the warp's run of 32 * ITEMS consecutive places: lanes of
-    // one digit in place order, after the warp's earlier ones
+    const int bins = 1 << a.bits, tiles = gridDim.x, tile = blockIdx.x;
     uint32_t key[ITEMS], ps[ITEMS];
-    uint16_t rank[ITEMS];
     const long base = (long)tile * SORT_T * ITEMS + (long)warp * 32 * ITEMS;
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
         const long i = base + k * 32 + lane;
         key[k] = 0;
         ps[k] = (uint32_t)i;
-        if (i < n) {
+        if (i < a.n) {
             if (FIRST) {
-                key[k] = key_of(ids[i], vocab, pad_id, has_pad);
+                key[k] = key_of(a.ids[i], a.vocab, a.pad_id, a.has_pad);
             } else {
-                key[k] = keys[i];
-                ps[k] = pos[i];
+                key[k] = a.keys[i];
+                ps[k] = a.pos[i];
             }
         }
     }
+    {   // counts of each digit over all tiles, and over the tiles before this one
+        const int d = tid & (bins - 1), part = tid >> a.bits, parts = SORT_T >> a.bits;
+        uint32_t t = 0, p = 0;
+        #pragma unroll 4
+        for (int j = part; j < tiles; j += parts) {
+            const uint32_t c = a.counts[(long)j * bins + d];
+            t += c;
+            p += j < tile ? c : 0u;
+        }
+        tot[tid] = t;
+        pre[tid] = p;
+        for (int i = tid; i < NW * MAX_BINS / 2; i += SORT_T) ((uint32_t*)wcnt)[i] = 0;
+    }
+    __syncthreads();
+    // ranks inside the warp's run of 32 * ITEMS consecutive places: lanes of
+    // one digit in place order, after the warp's earlier ones
+    uint16_t rank[ITEMS];
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
-        const bool in = base + k * 32 + lane < n;
-        const uint32_t d = in ? (key[k] >> shift) & 255u : 256u;
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        const bool in = base + k * 32 + lane < a.n;
+        const uint32_t d = (key[k] >> a.shift) & (bins - 1);
+        const uint32_t same = same_digit(d, in, a.bits);
         uint32_t before = 0;
         if (in) before = wcnt[warp][d];
         __syncwarp();
         rank[k] = (uint16_t)(before + __popc(same & ((1u << lane) - 1u)));
-        if (in && lane == __ffs(same) - 1) wcnt[warp][d] = before + __popc(same);
+        if (in && lane == __ffs(same) - 1) wcnt[warp][d] = (uint16_t)(before + __popc(same));
         __syncwarp();
     }
     __syncthreads();
     // first place of each digit for this tile, then for each of its warps
     uint32_t all = 0, mine = 0;
-    if (tid < 256) {
-        all = tot[0][tid] + tot[1][tid] + tot[2][tid] + tot[3][tid];
-        mine = pre[0][tid] + pre[1][tid] + pre[2][tid] + pre[3][tid];
+    if (tid < bins) {
+        for (int j = tid; j < SORT_T; j += bins) { all += tot[j]; mine += pre[j]; }
         uint32_t x = all;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            const uint32_t y = __shfl_up_sync(__activemask(), x, o);
             if (lane >= o) x += y;
         }
-        if (lane == 31) wsum[warp] = x;
+        if (lane == 31 || tid == bins - 1) wsum[warp] = x;
         mine += x - all;
+        uint32_t c = 0;
+        #pragma unroll 8
+        for (int w = 0; w < NW; w++) {
+            const uint32_t v = wcnt[w][tid];
+            wcnt[w][tid] = (uint16_t)c;                    // below the tile's 16384 places
+            c += v;
+        }
     }
     __syncthreads();
-    if (tid < 256) {
+    if (tid < bins) {
         for (int w = 0; w < warp; w++) mine += wsum[w];
-        for (int w = 0; w < NW; w++) {
-            const uint32_t c = wcnt[w][tid];
-            wcnt[w][tid] = mine;
-            mine += c;
-        }
+        first[tid] = mine;
     }
     __syncthreads();
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
-        if (base + k * 32 + lane < n) {
-            const uint32_t to = wcnt[warp][(key[k] >> shift) & 255u] + rank[k];
-            keys_out[to] = key[k];
-            pos_out[to] = ps[k];
+        if (base + k * 32 + lane < a.n) {
+            const uint32_t d = (key[k] >> a.shift) & (bins - 1);
+            const uint32_t to = first[d] + wcnt[warp][d] + rank[k];
+            a.keys_out[to] = key[k];
+            a.pos_out[to] = ps[k];
         }
     }
 }
@@ -197,6 +221,7 @@ __global__ void __launch_bounds__(SORT_T) k_sort_scatter(
 // as a partial: the block joins its groups' partials in order through shared
 // memory, and k_embed_join joins the blocks'.  Rows without a place are
 // zeroed by extra blocks.  Bound: HBM, dout read once as gathered rows.
+constexpr int MAX_CHUNK = 2048;
 enum { SEG_HEAD = 1, SEG_THROUGH = 2, SEG_TAIL = 4 };
 
 struct SumArgs {
@@ -206,7 +231,6 @@ struct SumArgs {
     float* dtab; long lddt;
     float* head; float* tail;        // [chunks][width] partials of each block
     uint32_t* flags; uint32_t* tail_id;
-    const uint8_t* present;
     int vocab, width, pieces, accumulate;
     int chunk, run, nchunks, zero_blocks;
     float scale;
@@ -229,53 +253,67 @@ PTCG_DEV void put_row(const SumArgs& a, uint32_t id, int piece, const float (&s)
 
 template <typename T, int V, int G>
 __global__ void __launch_bounds__(256) k_embed_sum(const __grid_constant__ SumArgs a) {
-    constexpr int NG = 256 / G, S = G * V, U = V == 8 ? 4 : 8;
+    constexpr int NG = 256 / G, S = G * V, U = 8;
     __shared__ float s_head[NG][S], s_tail[NG][S];
+    __shared__ uint32_t s_key[MAX_CHUNK + 2], s_pos[MAX_CHUNK];
     __shared__ uint32_t s_flag[NG], s_hid[NG], s_tid[NG];
     const int lane = threadIdx.x % G, grp = threadIdx.x / G;
     const int piece = blockIdx.y * G + lane;
     const bool col = piece < a.pieces;
     if (blockIdx.x >= (unsigned)a.nchunks) {               // rows nothing refers to
+        // 256 rows at a time, a search in the sorted ids for each
         const float z[V] = {};
-        for (long r = (long)(blockIdx.x - a.nchunks) * NG + grp; r < a.vocab;
-             r += (long)a.zero_blocks * NG)
-            if (col && !a.present[r])
-                VecIO<float, V>::st(a.dtab + r * a.lddt + (long)piece * V, z);
+        for (long b = blockIdx.x - a.nchunks; b * 256 < a.vocab; b += a.zero_blocks) {
+            const long row = b * 256 + threadIdx.x;
+            long lo = 0, hi = a.n;                         // first place with a key >= row
+            while (lo < hi) {
+                const long mid = (lo + hi) >> 1;
+                if (a.keys[mid] < (uint32_t)row) lo = mid + 1; else hi = mid;
+            }
+            __syncthreads();
+            s_key[threadIdx.x] = row < a.vocab && !(lo < a.n && a.keys[lo] == (uint32_t)row);
+            __syncthreads();
+            for (int i = grp; i < 256; i += NG)
+                if (col && s_key[i])
+                    VecIO<float, V>::st(a.dtab + (b * 256 + i) * a.lddt + (long)piece * V, z);
+        }
         return;
     }
-    const T* dout = (const T*)a.dout;
     const uint32_t none = 0xffffffffu, vocab = (uint32_t)a.vocab;
-    const long c0 = (long)blockIdx.x * a.chunk, c1 = min(a.n, c0 + a.chunk);
-    const long r0 = min(c1, c0 + (long)grp * a.run), r1 = min(c1, r0 + a.run);
+    const long c0 = (long)blockIdx.x * a.chunk;
+    const int len = (int)min((long)a.chunk, a.n - c0);
+    // the chunk's keys with one neighbour on either side, and its places
+    for (int i = threadIdx.x; i < len + 2; i += 256) {
+        const long at = c0 - 1 + i;
+        s_key[i] = at >= 0 && at < a.n ? a.keys[at] : none;
+        if (i < len) s_pos[i] = a.pos[c0 + i];
+    }
+    __syncthreads();
+    const uint32_t* key = s_key + 1;
+    const T* dout = (const T*)a.dout + (long)piece * V;
+    const int r0 = min(len, grp * a.run), r1 = min(len, r0 + a.run);
     uint32_t flag = 0, hid = none, tid = none;
     float acc[V];
     #pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.f;
     if (r0 < r1) {
-        uint32_t cur = a.keys[r0];
-        bool began = r0 > 0 && a.keys[r0 - 1] == cur;      // the open segment's start is earlier
-        const uint32_t after = r1 < a.n ? a.keys[r1] : none;
-        for (long i = r0; i < r1; i += U) {
-            uint32_t k[U];
-            float v[U][V];
+        uint32_t cur = key[r0];
+        bool began = key[r0 - 1] == cur;                   // the open segment's start is earlier
+        const uint32_t after = key[r1];
+        for (int i = r0; i < r1; i += U) {
+            Raw<T, V> raw[U];
             #pragma unroll
             for (int u = 0; u < U; u++) {
-                const bool in = i + u < r1;
-                k[u] = in ? a.keys[i + u] : none;
                 // padding places (key vocab) carry no gradient: not read
-                const bool take = in && k[u] < vocab && col;
-                const long p = take ? (long)a.pos[i + u] : 0;
-                if (take) {
-                    VecIO<T, V>::ld(v[u], dout + p * a.lddo + (long)piece * V);
-                } else {
-                    #pragma unroll
-                    for (int e = 0; e < V; e++) v[u][e] = 0.f;
-                }
+                const bool take = i + u < r1 && key[min(i + u, r1 - 1)] < vocab && col;
+                if (take) raw[u].ld(dout + (long)s_pos[i + u] * a.lddo);
+                else raw[u].zero();
             }
             #pragma unroll
             for (int u = 0; u < U; u++) {
                 if (i + u >= r1) break;
-                if (k[u] != cur) {
+                const uint32_t k = key[i + u];
+                if (k != cur) {
                     if (began) {
                         flag |= SEG_HEAD;
                         hid = cur;
@@ -285,12 +323,14 @@ __global__ void __launch_bounds__(256) k_embed_sum(const __grid_constant__ SumAr
                         put_row<V>(a, cur, piece, acc);
                     }
                     began = false;
-                    cur = k[u];
+                    cur = k;
                     #pragma unroll
                     for (int e = 0; e < V; e++) acc[e] = 0.f;
                 }
+                float v[V];
+                raw[u].get(v);
                 #pragma unroll
-                for (int e = 0; e < V; e++) acc[e] += v[u][e];
+                for (int e = 0; e < V; e++) acc[e] += v[e];
             }
         }
         const bool on = after == cur;
@@ -406,9 +446,9 @@ __global__ void __launch_bounds__(256) k_embed_join(const __grid_constant__ SumA
 
 // ------------------------------------------------------------ host side
 struct Plan {
-    int items, tiles, passes;        // sort
+    int items, tiles, passes, bits;  // sort: bits of a digit
     int chunk, nchunks;              // sums (run and slices follow from the variant)
-    long o_keys[2], o_pos[2], o_counts, o_head, o_tail, o_flags, o_tid, o_present, bytes;
+    long o_keys[2], o_pos[2], o_counts, o_head, o_tail, o_flags, o_tid, bytes;
 };
 
 long up256(long x) { return (x + 255) / 256 * 256; }
@@ -423,24 +463,24 @@ Plan plan(long n, int vocab, int width) {
     p.tiles = (int)cdiv(n, (long)SORT_T * p.items);
     int bits = 1;
     while (bits < 31 && (1L << bits) <= vocab) bits++;      // keys 0 .. vocab
-    p.passes = (bits + 7) / 8;
+    p.passes = (bits + MAX_BITS - 1) / MAX_BITS;
+    p.bits = (bits + p.passes - 1) / p.passes;
     // about eight blocks a processor over all column slices, at least 8
     // places a lane group
     const int slices = (int)cdiv(width, 256);
     long want = (n * slices + 148 * 8 - 1) / (148 * 8);
-    p.chunk = (int)((want < 64 ? 64 : want) + 31) / 32 * 32;
+    p.chunk = (int)(std::min(std::max(want, 64L), (long)MAX_CHUNK) + 31) / 32 * 32;
     p.nchunks = (int)cdiv(n, p.chunk);
     long o = 0;
     for (int i = 0; i < 2; i++) {
         p.o_keys[i] = o; o = up256(o + 4 * n);
         p.o_pos[i] = o; o = up256(o + 4 * n);
     }
-    p.o_counts = o; o = up256(o + 4L * 256 * p.tiles);
+    p.o_counts = o; o = up256(o + (4L << p.bits) * p.tiles);
     p.o_head = o; o = up256(o + 4L * width * p.nchunks);
     p.o_tail = o; o = up256(o + 4L * width * p.nchunks);
     p.o_flags = o; o = up256(o + 4L * p.nchunks);
     p.o_tid = o; o = up256(o + 4L * p.nchunks);
-    p.o_present = o; o = up256(o + vocab);
     p.bytes = o;
     return p;
 }
@@ -462,17 +502,14 @@ void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids,
 }
 
 template <int ITEMS>
-void sort_pass(int first, uint32_t* ko, uint32_t* po, const uint32_t* ki, const uint32_t* pi,
-               uint32_t* counts, const int* ids, long n, int shift, int vocab, int pad_id,
-               uint8_t* present, int tiles, cudaStream_t s) {
-    const int hp = pad_id >= 0;
+void sort_pass(const SortArgs& a, bool first, int tiles, cudaStream_t s) {
     g_ptcg_launches += 2;
     if (first) {
-        k_sort_count<ITEMS, true><<<tiles, SORT_T, 0, s>>>(counts, ki, ids, n, shift, vocab, pad_id, hp, present);
-        k_sort_scatter<ITEMS, true><<<tiles, SORT_T, 0, s>>>(ko, po, counts, ki, pi, ids, n, shift, vocab, pad_id, hp);
+        k_sort_count<ITEMS, true><<<tiles, SORT_T, 0, s>>>(a);
+        k_sort_scatter<ITEMS, true><<<tiles, SORT_T, 0, s>>>(a);
     } else {
-        k_sort_count<ITEMS, false><<<tiles, SORT_T, 0, s>>>(counts, ki, ids, n, shift, vocab, pad_id, hp, present);
-        k_sort_scatter<ITEMS, false><<<tiles, SORT_T, 0, s>>>(ko, po, counts, ki, pi, ids, n, shift, vocab, pad_id, hp);
+        k_sort_count<ITEMS, false><<<tiles, SORT_T, 0, s>>>(a);
+        k_sort_scatter<ITEMS, false><<<tiles, SORT_T, 0, s>>>(a);
     }
 }
 
@@ -480,18 +517,19 @@ template <typename T, int V, int G>
 void embed_sum(SumArgs a, cudaStream_t s) {
     a.pieces = a.width / V;
     a.run = (int)cdiv(a.chunk, 256 / G);
-    a.zero_blocks = a.accumulate ? 0 : (int)std::min<long>(148 * 4, cdiv(a.vocab, 256 / G));
+    a.zero_blocks = a.accumulate ? 0 : (int)std::min<long>(148 * 4, cdiv(a.vocab, 256));
     const dim3 grid(a.nchunks + a.zero_blocks, cdiv(a.pieces, G));
     ++g_ptcg_launches, k_embed_sum<T, V, G><<<grid, 256, 0, s>>>(a);
 }
 template <typename T>
 void embed_sum(const SumArgs& a, int V, cudaStream_t s) {
     // a lane group as wide as the row needs: 8, 16 or 32 lanes
+    constexpr int VV = sizeof(T) == 2 ? 8 : 4;
     const int lanes = a.width / V;
-    if (V == 8) {
-        if (lanes <= 8) embed_sum<T, 8, 8>(a, s);
-        else if (lanes <= 16) embed_sum<T, 8, 16>(a, s);
-        else embed_sum<T, 8, 32>(a, s);
+    if (V == VV) {
+        if (lanes <= 8) embed_sum<T, VV, 8>(a, s);
+        else if (lanes <= 16) embed_sum<T, VV, 16>(a, s);
+        else embed_sum<T, VV, 32>(a, s);
     } else {
         embed_sum<T, 1, 32>(a, s);
     }
@@ -552,15 +590,12 @@ int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* i
     uint8_t* base = (uint8_t*)scratch;
     uint32_t* keys[2] = {(uint32_t*)(base + p.o_keys[0]), (uint32_t*)(base + p.o_keys[1])};
     uint32_t* pos[2] = {(uint32_t*)(base + p.o_pos[0]), (uint32_t*)(base + p.o_pos[1])};
-    uint32_t* counts = (uint32_t*)(base + p.o_counts);
-    uint8_t* present = base + p.o_present;
-    OP_CK(cudaMemsetAsync(present, 0, vocab, s));
     for (int i = 0; i < p.passes; i++) {
-        uint32_t *ko = keys[i & 1], *po = pos[i & 1], *ki = keys[(i & 1) ^ 1], *pi = pos[(i & 1) ^ 1];
-        if (p.items == 16)
-            sort_pass<16>(i == 0, ko, po, ki, pi, counts, ids, n, 8 * i, vocab, pad_id, present, p.tiles, s);
-        else
-            sort_pass<4>(i == 0, ko, po, ki, pi, counts, ids, n, 8 * i, vocab, pad_id, present, p.tiles, s);
+        const int to = i & 1;
+        const SortArgs sa = {(uint32_t*)(base + p.o_counts), keys[to], pos[to], keys[to ^ 1], pos[to ^ 1],
+                             ids, n, i * p.bits, p.bits, vocab, pad_id, pad_id >= 0};
+        if (p.items == 16) sort_pass<16>(sa, i == 0, p.tiles, s);
+        else sort_pass<4>(sa, i == 0, p.tiles, s);
     }
     SumArgs a;
     a.dout = dout; a.lddo = lddo;
@@ -569,15 +604,15 @@ int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* i
     a.dtab = dtable; a.lddt = lddt;
     a.head = (float*)(base + p.o_head); a.tail = (float*)(base + p.o_tail);
     a.flags = (uint32_t*)(base + p.o_flags); a.tail_id = (uint32_t*)(base + p.o_tid);
-    a.present = present;
     a.vocab = vocab; a.width = width; a.pieces = 0; a.accumulate = accumulate != 0;
     a.chunk = p.chunk; a.run = 0; a.nchunks = p.nchunks; a.zero_blocks = 0;
     a.scale = scale;
-    const int V = width % 8 == 0 && vec_ok(dout, dout_dtype, lddo, 8) && vec_ok(dtable, PTCG_FP32, lddt, 8) ? 8 : 1;
+    const int v = dout_dtype == PTCG_BF16 ? 8 : 4;
+    const int V = width % v == 0 && vec_ok(dout, dout_dtype, lddo, v) && vec_ok(dtable, PTCG_FP32, lddt, v) ? v : 1;
     if (dout_dtype == PTCG_BF16) embed_sum<bf16>(a, V, s); else embed_sum<float>(a, V, s);
     if (p.nchunks > 1) {
         const int cols = (int)cdiv(width, 32);
-        ++g_ptcg_launches, k_embed_join<<<dim3(p.nchunks, cols < 32 ? cols : 32), 256, 0, s>>>(a);
+        ++g_ptcg_launches, k_embed_join<<<dim3(p.nchunks, cols < 4 ? cols : 4), 256, 0, s>>>(a);
     }
     OP_CKL();
     return PTCG_OK;

@@ -74,6 +74,42 @@ template <> struct VecIO<bf16, 8> {
     }
 };
 
+// one 16-byte piece (or one element) as it lies in memory, converted later:
+// half the registers of converted bf16 while many loads are in flight
+template <typename T, int V> struct Raw;
+template <> struct Raw<bf16, 8> {
+    uint4 r;
+    PTCG_DEV void ld(const bf16* p) { r = *reinterpret_cast<const uint4*>(p); }
+    PTCG_DEV void zero() { r = make_uint4(0u, 0u, 0u, 0u); }
+    PTCG_DEV void get(float (&v)[8]) const {
+        unpack_bf2(r.x, v[0], v[1]);
+        unpack_bf2(r.y, v[2], v[3]);
+        unpack_bf2(r.z, v[4], v[5]);
+        unpack_bf2(r.w, v[6], v[7]);
+    }
+};
+template <> struct Raw<bf16, 4> {
+    uint2 r;
+    PTCG_DEV void ld(const bf16* p) { r = *reinterpret_cast<const uint2*>(p); }
+    PTCG_DEV void zero() { r = make_uint2(0u, 0u); }
+    PTCG_DEV void get(float (&v)[4]) const {
+        unpack_bf2(r.x, v[0], v[1]);
+        unpack_bf2(r.y, v[2], v[3]);
+    }
+};
+template <> struct Raw<float, 4> {
+    float4 r;
+    PTCG_DEV void ld(const float* p) { r = *reinterpret_cast<const float4*>(p); }
+    PTCG_DEV void zero() { r = make_float4(0.f, 0.f, 0.f, 0.f); }
+    PTCG_DEV void get(float (&v)[4]) const { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
+};
+template <typename T> struct Raw<T, 1> {
+    T r;
+    PTCG_DEV void ld(const T* p) { r = *p; }
+    PTCG_DEV void zero() { r = from_f<T>(0.f); }
+    PTCG_DEV void get(float (&v)[1]) const { v[0] = to_f<T>(r); }
+};
+
 static inline int dt_size(int dtype) { return dtype == PTCG_BF16 ? 2 : 4; }
 static inline bool dt_ok(int dtype) { return dtype == PTCG_FP32 || dtype == PTCG_BF16; }
 // rows of `ld` elements from p can be read V elements at a time (16-byte
