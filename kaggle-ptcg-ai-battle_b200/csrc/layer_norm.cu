@@ -16,9 +16,9 @@ namespace {
 
 constexpr int MAXW = PTCG_LN_MAX_WIDTH;
 // one warp holds rows of up to 1024 columns, NV pieces of V columns per lane;
-// wider rows are shared by the warps of a block, 512 columns each, so that the
-// backward's six registers per column still fit 512 threads
-constexpr int WARP_COLS = 1024, SHARED_COLS = 512, MAX_THREADS = MAXW / SHARED_COLS * 32;
+// wider rows are shared by the warps of a block, 256 columns each, so that the
+// backward's registers per column still fit 1024 threads
+constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MAX_THREADS = MAXW / SHARED_COLS * 32;
 
 // Bound: HBM.  A row belongs to one warp (width <= 1024, eight rows to a
 // block) or to the W warps of a block (MULTI).  Lane l of warp w owns pieces
@@ -34,9 +34,7 @@ PTCG_DEV float row_sum(float v, float (*red)[32], int slot, int w, int lane, int
     if (!MULTI) return v;
     if (lane == 0) red[slot][w] = v;
     __syncthreads();
-    float t = 0.f;
-    for (int i = 0; i < W; i++) t += red[slot][i];
-    return t;
+    return warp_sum(lane < W ? red[slot][lane] : 0.f);
 }
 
 template <typename TX, typename TY, int V, int NV, bool MULTI>
@@ -63,20 +61,28 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         }
     }
     const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
-    int slot = 0;
-    for (long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp; r < rows; r += step) {
-        float v[NV][V];
-        float s = 0.f;
+    // the next row's loads are in flight while this one is reduced, where the
+    // registers allow it
+    constexpr bool AHEAD = NV * V <= 8;
+    Raw<TX, V> row[NV];
+    auto fetch = [&](long r) {
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int p = piece_at<V, NV>(w, lane, k);
-            if (p < pieces) {
-                VecIO<TX, V>::ld(v[k], x + r * ldx + (long)p * V);
-            } else {
-                #pragma unroll
-                for (int e = 0; e < V; e++) v[k][e] = 0.f;
-            }
+            row[k].zero();
+            if (r < rows && p < pieces) row[k].ld(x + r * ldx + (long)p * V);
         }
+    };
+    int slot = 0;
+    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
+    if (AHEAD) fetch(r);
+    for (; r < rows; r += step) {
+        float v[NV][V];
+        float s = 0.f;
+        if (!AHEAD) fetch(r);
+        #pragma unroll
+        for (int k = 0; k < NV; k++) row[k].get(v[k]);
+        if (AHEAD) fetch(r + step);
         #pragma unroll
         for (int k = 0; k < NV; k++)
             #pragma unroll
@@ -86,10 +92,9 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         float q = 0.f;
         #pragma unroll
         for (int k = 0; k < NV; k++) {
-            if (piece_at<V, NV>(w, lane, k) < pieces) {
-                #pragma unroll
-                for (int e = 0; e < V; e++) { const float d = v[k][e] - mu; q = fmaf(d, d, q); }
-            }
+            const float in = piece_at<V, NV>(w, lane, k) < pieces ? 1.f : 0.f;
+            #pragma unroll
+            for (int e = 0; e < V; e++) { const float d = (v[k][e] - mu) * in; q = fmaf(d, d, q); }
         }
         const float rs = rsqrtf(fmaf(row_sum<MULTI>(q, red, slot + 1, w, lane, W), inv, eps));
         slot ^= 2;
@@ -137,21 +142,37 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
     }
     const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
     int slot = 0;
-    for (long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp; r < rows; r += step) {
-        float h[NV][V], g[NV][V], d[NV][V];
-        const float mu = mean[r], rs = rstd[r];
+    // the next row's loads are in flight while this one is reduced, where the
+    // registers allow it
+    constexpr bool AHEAD = !MULTI && NV * V <= 8;
+    struct Row { Raw<TX, V> x[NV], r[NV]; Raw<TY, V> g[NV]; float mu, rs; } row;
+    auto fetch = [&](long r) {
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int p = piece_at<V, NV>(w, lane, k);
-            if (p < pieces) {
-                VecIO<TX, V>::ld(h[k], x + r * ldx + (long)p * V);
-                VecIO<TY, V>::ld(g[k], dy + r * lddy + (long)p * V);
-                if (dres) VecIO<TX, V>::ld(d[k], dres + r * lddres + (long)p * V);
-            } else {
-                #pragma unroll
-                for (int e = 0; e < V; e++) { h[k][e] = mu; g[k][e] = 0.f; }
+            row.x[k].zero(); row.g[k].zero(); row.r[k].zero();
+            if (r < rows && p < pieces) {
+                row.x[k].ld(x + r * ldx + (long)p * V);
+                row.g[k].ld(dy + r * lddy + (long)p * V);
+                if (dres) row.r[k].ld(dres + r * lddres + (long)p * V);
             }
         }
+        row.mu = r < rows ? mean[r] : 0.f;
+        row.rs = r < rows ? rstd[r] : 0.f;
+    };
+    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
+    if (AHEAD) fetch(r);
+    for (; r < rows; r += step) {
+        float h[NV][V], g[NV][V], d[NV][V];
+        if (!AHEAD) fetch(r);
+        const float mu = row.mu, rs = row.rs;
+        #pragma unroll
+        for (int k = 0; k < NV; k++) {
+            row.x[k].get(h[k]);
+            row.g[k].get(g[k]);
+            row.r[k].get(d[k]);
+        }
+        if (AHEAD) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
         #pragma unroll
         for (int k = 0; k < NV; k++) {
@@ -171,8 +192,8 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
             s2 = warp_sum(s2);
             if (lane == 0) { red[slot][w] = s1; red[slot + 1][w] = s2; }
             __syncthreads();
-            s1 = s2 = 0.f;
-            for (int i = 0; i < W; i++) { s1 += red[slot][i]; s2 += red[slot + 1][i]; }
+            s1 = warp_sum(lane < W ? red[slot][lane] : 0.f);
+            s2 = warp_sum(lane < W ? red[slot + 1][lane] : 0.f);
             slot ^= 2;
         } else {
             s1 = warp_sum(s1);
@@ -290,13 +311,13 @@ void fwd(const Cfg& c, void* y, long ldy, float* mean, float* rstd, const void* 
          const float* gamma, const float* beta, long rows, int width, float eps, cudaStream_t s) {
     #define LN(V, NV, M) fwd<TX, TY, V, NV, M>(y, ldy, mean, rstd, x, ldx, gamma, beta, rows, width, eps, c.W, s)
     if (c.V == 4) {
-        if (c.W) LN(4, 4, true);
+        if (c.W) LN(4, 2, true);
         else if (c.NV == 1) LN(4, 1, false);
         else if (c.NV == 2) LN(4, 2, false);
         else if (c.NV == 4) LN(4, 4, false);
         else LN(4, 8, false);
     } else {
-        if (c.W) LN(1, 16, true);
+        if (c.W) LN(1, 8, true);
         else if (c.NV == 4) LN(1, 4, false);
         else if (c.NV == 8) LN(1, 8, false);
         else if (c.NV == 16) LN(1, 16, false);
@@ -321,13 +342,13 @@ template <typename TX, typename TY>
 void bwd(const Cfg& c, const BwdArgs& a, int blocks, cudaStream_t s) {
     #define LN(V, NV, M) bwd<TX, TY, V, NV, M>(a, blocks, c.W, s)
     if (c.V == 4) {
-        if (c.W) LN(4, 4, true);
+        if (c.W) LN(4, 2, true);
         else if (c.NV == 1) LN(4, 1, false);
         else if (c.NV == 2) LN(4, 2, false);
         else if (c.NV == 4) LN(4, 4, false);
         else LN(4, 8, false);
     } else {
-        if (c.W) LN(1, 16, true);
+        if (c.W) LN(1, 8, true);
         else if (c.NV == 4) LN(1, 4, false);
         else if (c.NV == 8) LN(1, 8, false);
         else if (c.NV == 16) LN(1, 16, false);
