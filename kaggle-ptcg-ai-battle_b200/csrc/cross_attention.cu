@@ -146,7 +146,7 @@ PTCG_DEV float quad_sum(float v) {
 // rounding).  WN = 4 is the form for at most 16 rows (single tokens): the four
 // warps take 16 keys each of every tile and are joined at the end.
 template <int DH, int WM, int WN, int NST>
-__global__ void __launch_bounds__(WM * WN * 32) k_cross_fwd(const __grid_constant__ CrossArgs a) {
+__global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_cross_fwd(const __grid_constant__ CrossArgs a) {
     constexpr int THREADS = WM * WN * 32, BM = WM * 16, BN = 64, KW = BN / WN, NT = KW / 8;
     constexpr int KS = DH / 16, TILE = BN * DH * 2;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(WM * WN * 32) k_cross_fwd(const __grid_constan
     uint32_t qf[KS][4];
     const float sc = a.scale * LOG2E;
     const int t = lane & 3;
+    const bool mine = r0 + wm * 16 < a.rows;        // this warp has rows
     for (int j = 0; j < nt; j++) {
         const bool next = mask_byte(j + NST);
         cp_wait<NST - 2>();
@@ -202,22 +203,25 @@ __global__ void __launch_bounds__(WM * WN * 32) k_cross_fwd(const __grid_constan
         // this warp's keys: all 64, or its 16
         const uint32_t v0 = WN == 1 ? w0 : ((wn & 2 ? w1 : w0) >> ((wn & 1) * 16)) & 0xffffu;
         const uint32_t v1 = WN == 1 ? w1 : 0u;
-        if (v0 | v1) {
+        if ((v0 | v1) && mine) {
             const uint32_t kt = sK + (j % NST) * TILE, vt = sV + (j % NST) * TILE;
+            // 16 keys at a time; groups that are masked whole are skipped
+            auto group = [&](int i) { return ((i < 2 ? v0 : v1) >> ((i & 1) * 16)) & 0xffffu; };
             float s[NT][4];
             #pragma unroll
-            for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-            #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int i = 0; i < NT / 2; i++) {
                 #pragma unroll
-                for (int i = 0; i < NT / 2; i++) {
+                for (int e = 0; e < 4; e++) s[2 * i][e] = s[2 * i + 1][e] = 0.f;
+                if (!group(i)) continue;
+                #pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
                     uint32_t b[4];
                     frag_bn<DH>(b, kt, wn * KW + i * 16, ks, lane);
                     mma(s[2 * i], qf[ks], b[0], b[1]);
                     mma(s[2 * i + 1], qf[ks], b[2], b[3]);
                 }
             }
-            if ((v0 & v1) != 0xffffffffu) {
+            if ((v0 & (WN == 1 ? v1 : 0xffffffffu)) != (WN == 1 ? 0xffffffffu : 0xffffu)) {
                 #pragma unroll
                 for (int i = 0; i < NT; i++) {
                     const uint32_t w = (i < 4 ? v0 : v1) >> ((i & 3) * 8 + 2 * t);
@@ -244,16 +248,17 @@ __global__ void __launch_bounds__(WM * WN * 32) k_cross_fwd(const __grid_constan
             m0 = n0;
             m1 = n1;
             #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                s[i][0] = ex2_approx(fmaf(s[i][0], sc, -u0));
-                s[i][1] = ex2_approx(fmaf(s[i][1], sc, -u0));
-                s[i][2] = ex2_approx(fmaf(s[i][2], sc, -u1));
-                s[i][3] = ex2_approx(fmaf(s[i][3], sc, -u1));
-                l0 += s[i][0] + s[i][1];
-                l1 += s[i][2] + s[i][3];
-            }
-            #pragma unroll
             for (int i = 0; i < NT / 2; i++) {
+                if (!group(i)) continue;
+                #pragma unroll
+                for (int n = 2 * i; n < 2 * i + 2; n++) {
+                    s[n][0] = ex2_approx(fmaf(s[n][0], sc, -u0));
+                    s[n][1] = ex2_approx(fmaf(s[n][1], sc, -u0));
+                    s[n][2] = ex2_approx(fmaf(s[n][2], sc, -u1));
+                    s[n][3] = ex2_approx(fmaf(s[n][3], sc, -u1));
+                    l0 += s[n][0] + s[n][1];
+                    l1 += s[n][2] + s[n][3];
+                }
                 const uint32_t p[4] = {pack_bf2(s[2 * i][0], s[2 * i][1]), pack_bf2(s[2 * i][2], s[2 * i][3]),
                                        pack_bf2(s[2 * i + 1][0], s[2 * i + 1][1]),
                                        pack_bf2(s[2 * i + 1][2], s[2 * i + 1][3])};
@@ -686,6 +691,214 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
     }
 }
 
+// Backward of problems of at most 64 stacked rows in one kernel: the rows stay
+// in shared memory while a block walks the keys 64 at a time, so S, P and dS
+// are computed once (five products instead of the seven of the pair above) and
+// a key tile's dk and dv are finished at once.  S^T and dP^T have keys as rows
+// (16 a warp); dS^T goes through shared memory, from where the warps take it
+// transposed as the left operand of dq += dS k (16 rows and a share of the
+// columns each), which stays in registers over all keys.
+template <int DH, int NR>                    // 16 NR rows
+__global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const __grid_constant__ CrossArgs a) {
+    constexpr int THREADS = 128, BM = NR * 16, BN = 64, KS = DH / 16, TILE = BN * DH * 2;
+    constexpr int NT = BM / 8;               // 8-row tiles of the stacked rows
+    constexpr int DR = 4 / NR > 0 ? 4 / NR : 1;             // warps that share a group of 16 rows
+    constexpr int ND = (KS + DR - 1) / DR;   // 16-column pieces of dq a warp owns
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t bits[3][2];
+    __shared__ float s_lse[BM], s_delta[BM];
+    const uint32_t sQ = s_addr(sm), sG = sQ + BM * DH * 2, sK = sG + BM * DH * 2, sV = sK + 2 * TILE;
+    const uint32_t sD = sV + 2 * TILE;       // dS^T [64 keys][BM rows], rows of 16 bytes permuted
+    const Where at = where(a);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int len = kept_len(a, at.seq);
+    // parts tile [0, lk), so that the masked tail's dk and dv are written too
+    const int kbeg = at.part * a.split, kend = min(a.lk, kbeg + a.split);
+    const int nt = (kend - kbeg + BN - 1) / BN;
+    const bf16 *K = (const bf16*)a.k, *V = (const bf16*)a.v;
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    auto mask_byte = [&](int j) {
+        const int key = kbeg + j * BN + warp * 32 + lane;
+        return warp < 2 && key < kend && kept(a, at.seq, key, len);
+    };
+    auto put_bits = [&](int j, bool b) {
+        const uint32_t m = __ballot_sync(0xffffffffu, b);
+        if (warp < 2 && lane == 0) bits[j % 3][warp] = m;
+    };
+    auto load = [&](int j) {
+        if (j < nt) {
+            stage_k<DH, BN, THREADS>(sK + (j & 1) * TILE, K, a.sk, at.seq, at.hk, kbeg + j * BN, bits[j % 3]);
+            stage_k<DH, BN, THREADS>(sV + (j & 1) * TILE, V, a.sv, at.seq, at.hk, kbeg + j * BN, bits[j % 3]);
+        }
+        cp_commit();
+    };
+    put_bits(0, mask_byte(0));
+    put_bits(1, mask_byte(1));
+    stage_q<DH, BM, THREADS>(sQ, (const bf16*)a.q, a.sq, a, at.seq, at.hk, 0);
+    stage_q<DH, BM, THREADS>(sG, (const bf16*)a.dout, a.sdo, a, at.seq, at.hk, 0);
+    __syncthreads();
+    load(0);
+    {   // delta = dout . out, THREADS / BM threads a row, and the log2-domain lse
+        // (+inf makes the probabilities of rows without keys and past the end zero)
+        constexpr int TR = THREADS / BM, PC = DH / 8;       // threads a row, 16-byte pieces
+        const int r = threadIdx.x / TR, h = threadIdx.x % TR;
+        float d = 0.f;
+        if (r < a.rows) {
+            const bf16* og = (const bf16*)a.o + qrow(a, a.so, at.seq, at.hk, r);
+            const bf16* gg = (const bf16*)a.dout + qrow(a, a.sdo, at.seq, at.hk, r);
+            for (int c = h; c < PC; c += TR) {
+                float x[8], y[8];
+                VecIO<bf16, 8>::ld(x, og + c * 8);
+                VecIO<bf16, 8>::ld(y, gg + c * 8);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) d = fmaf(x[e], y[e], d);
+            }
+        }
+        #pragma unroll
+        for (int o = 1; o < TR; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (h == 0) {
+            const float x = r < a.rows ? a.lse[row0 + r] : -INFINITY;
+            s_lse[r] = x == -INFINITY ? INFINITY : x * LOG2E;
+            s_delta[r] = d;
+        }
+    }
+    const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
+    const float sc = a.scale * LOG2E;
+    const int qr = NR == 1 ? 0 : warp % NR, qd = NR == 1 ? warp : warp / NR;   // dq rows, first column piece
+    float dq[ND][2][4];
+    #pragma unroll
+    for (int i = 0; i < ND; i++)
+        #pragma unroll
+        for (int e = 0; e < 4; e++) dq[i][0][e] = dq[i][1][e] = 0.f;
+    // 16-byte piece c (8 rows) of key row k of the dS^T tile
+    auto ds_off = [&](int k, int c) {
+        return sD + (uint32_t)(k * BM * 2 + ((c ^ (NT == 8 ? k & 7 : NT == 4 ? (k >> 1) & 3 : (k >> 2) & 1)) << 4));
+    };
+    for (int j = 0; j < nt; j++) {
+        const bool next = mask_byte(j + 2);
+        cp_wait<0>();
+        __syncthreads();
+        load(j + 1);
+        const uint32_t w0 = bits[j % 3][0], w1 = bits[j % 3][1];
+        const uint32_t wk = ((warp & 2 ? w1 : w0) >> ((warp & 1) * 16)) & 0xffffu;
+        const uint32_t kt = sK + (j & 1) * TILE, vt = sV + (j & 1) * TILE;
+        const int ja = kbeg + j * BN + warp * 16 + g;
+        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja) + 2 * t;
+        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja) + 2 * t;
+        const bool ina = ja < kend, inb = ja + 8 < kend;
+        if (wk) {
+            float s[NT][4], p[NT][4];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+                p[i][0] = p[i][1] = p[i][2] = p[i][3] = 0.f;
+            }
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                uint32_t kf[4], vf[4];
+                frag_a<DH>(kf, kt, warp * 16, ks, lane);
+                frag_a<DH>(vf, vt, warp * 16, ks, lane);
+                #pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    uint32_t b[4];
+                    frag_bn<DH>(b, sQ, i * 16, ks, lane);
+                    mma(s[2 * i], kf, b[0], b[1]);
+                    mma(s[2 * i + 1], kf, b[2], b[3]);
+                    frag_bn<DH>(b, sG, i * 16, ks, lane);
+                    mma(p[2 * i], vf, b[0], b[1]);
+                    mma(p[2 * i + 1], vf, b[2], b[3]);
+                }
+            }
+            const bool ka = (wk >> g) & 1, kb = (wk >> (g + 8)) & 1;
+            uint32_t pf[NT / 2][4], df[NT / 2][4];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const int c = i * 8 + 2 * t;
+                const float x0 = s_lse[c], x1 = s_lse[c + 1], d0 = s_delta[c], d1 = s_delta[c + 1];
+                const float e0 = ka ? ex2_approx(fmaf(s[i][0], sc, -x0)) : 0.f;
+                const float e1 = ka ? ex2_approx(fmaf(s[i][1], sc, -x1)) : 0.f;
+                const float e2 = kb ? ex2_approx(fmaf(s[i][2], sc, -x0)) : 0.f;
+                const float e3 = kb ? ex2_approx(fmaf(s[i][3], sc, -x1)) : 0.f;
+                pf[i >> 1][(i & 1) * 2] = pack_bf2(e0, e1);
+                pf[i >> 1][(i & 1) * 2 + 1] = pack_bf2(e2, e3);
+                const uint32_t da = pack_bf2(e0 * (p[i][0] - d0), e1 * (p[i][1] - d1));
+                const uint32_t db = pack_bf2(e2 * (p[i][2] - d0), e3 * (p[i][3] - d1));
+                df[i >> 1][(i & 1) * 2] = da;
+                df[i >> 1][(i & 1) * 2 + 1] = db;
+                asm volatile("st.shared.b32 [%0], %1;" :: "r"(ds_off(warp * 16 + g, i) + 4 * t), "r"(da) : "memory");
+                asm volatile("st.shared.b32 [%0], %1;" :: "r"(ds_off(warp * 16 + g + 8, i) + 4 * t), "r"(db) : "memory");
+            }
+            #pragma unroll
+            for (int which = 0; which < 2; which++) {
+                float acc[DH / 8][4];
+                #pragma unroll
+                for (int i = 0; i < DH / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+                #pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    #pragma unroll
+                    for (int d = 0; d < KS; d++) {
+                        uint32_t b[4];
+                        frag_bk<DH>(b, which ? sQ : sG, i * 16, d, lane);
+                        mma(acc[2 * d], which ? df[i] : pf[i], b[0], b[1]);
+                        mma(acc[2 * d + 1], which ? df[i] : pf[i], b[2], b[3]);
+                    }
+                }
+                const float f = which ? a.scale : 1.f;
+                bf16* out = which ? pk : pv;
+                const long down = 8 * (which ? a.sdk.row : a.sdv.row);
+                #pragma unroll
+                for (int i = 0; i < DH / 8; i++) {
+                    if (ina) *(uint32_t*)(out + i * 8) = pack_bf2(acc[i][0] * f, acc[i][1] * f);
+                    if (inb) *(uint32_t*)(out + down + i * 8) = pack_bf2(acc[i][2] * f, acc[i][3] * f);
+                }
+            }
+        } else {                                 // masked keys: no gradient
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) {
+                if (ina) { *(uint32_t*)(pk + i * 8) = 0u; *(uint32_t*)(pv + i * 8) = 0u; }
+                if (inb) { *(uint32_t*)(pk + 8 * a.sdk.row + i * 8) = 0u; *(uint32_t*)(pv + 8 * a.sdv.row + i * 8) = 0u; }
+            }
+        }
+        put_bits(j + 2, next);
+        if (w0 | w1) {                           // the same for every warp
+            __syncthreads();
+            #pragma unroll
+            for (int k = 0; k < BN / 16; k++) {
+                if (!(((k & 2 ? w1 : w0) >> ((k & 1) * 16)) & 0xffffu)) continue;
+                uint32_t f[4];                   // dS rows 16 qr .., keys 16 k ..
+                ldsm4t(f, ds_off(k * 16 + (mi >> 1) * 8 + (lane & 7), qr * 2 + (mi & 1)));
+                #pragma unroll
+                for (int i = 0; i < ND; i++) {
+                    const int d = qd + i * DR;
+                    if (d >= KS) break;
+                    uint32_t b[4];
+                    frag_bk<DH>(b, kt, k * 16, d, lane);
+                    mma(dq[i][0], f, b[0], b[1]);
+                    mma(dq[i][1], f, b[2], b[3]);
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int r = qr * 16 + g + half * 8;
+        if (r >= a.rows) continue;
+        #pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const int d = qd + i * DR;
+            if (d >= KS) break;
+            #pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float x = dq[i][n][2 * half] * a.scale, y = dq[i][n][2 * half + 1] * a.scale;
+                const int c = d * 16 + n * 8 + 2 * t;
+                if (a.nsplit > 1) *(float2*)(a.part + ((row0 + r) * a.nsplit + at.part) * DH + c) = make_float2(x, y);
+                else *(uint32_t*)((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r) + c) = pack_bf2(x, y);
+            }
+        }
+    }
+}
+
 // sums the parts of a split gradient in order: one 4-column piece a thread.
 // keys: the rows are key rows of a.dk (from part) and a.dv (from part2),
 // else stacked rows of a.dq
@@ -1061,11 +1274,12 @@ FwdPlan fwd_plan(const PtcgCross& c) {
     p.bytes = p.sp.n > 1 ? p.o_ml + 8 * parts : 0;
     return p;
 }
-struct BwdPlan { bool few; int bm; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
+struct BwdPlan { bool few, rows; int bm; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
 BwdPlan bwd_plan(const PtcgCross& c) {
     BwdPlan p;
     const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
     p.few = rows <= 16;
+    p.rows = c.dtype == PTCG_BF16 && rows > 0 && rows <= 64;
     p.bm = p.few && c.dtype == PTCG_FP32 ? 16 : 64;
     p.qtiles = (rows + p.bm - 1) / p.bm;
     p.ktiles = (c.lk + 63) / 64;
@@ -1131,11 +1345,27 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
     else k_cross_join<float, DH><<<cdiv(nrows, 4), 128, 0, s>>>(a, nrows);
     return cudaSuccess;
 }
+template <int DH, int NR>
+cudaError_t launch_bwd_rows(const CrossArgs& a, long blocks, cudaStream_t s) {
+    const int bytes = 2 * NR * 16 * DH * 2 + 4 * 64 * DH * 2 + 64 * NR * 16 * 2;
+    const cudaError_t e = smem_limit(k_cross_bwd_rows<DH, NR>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_bwd_rows<DH, NR><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
 template <int DH>
 cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
     const bool bf = c.dtype == PTCG_BF16;
     const long probs = (long)c.nseq * c.kv_heads, nrows = probs * a.rows, nkeys = probs * a.lk;
+    if (p.rows && p.qblocks) {
+        a.tiles = 1; a.nsplit = p.qs.n; a.split = p.qs.len;
+        e = a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, p.qblocks, s)
+            : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, p.qblocks, s) : launch_bwd_rows<DH, 4>(a, p.qblocks, s);
+        if (e == cudaSuccess && p.qs.n > 1)
+            ++g_ptcg_launches, k_cross_sum<bf16, DH><<<cdiv(nrows * (DH / 4), 256), 256, 0, s>>>(a, nrows, 0);
+        return e;
+    }
     if (p.qblocks) {
         a.tiles = (int)p.qtiles; a.nsplit = p.qs.n; a.split = p.qs.len;
         if (bf) {
