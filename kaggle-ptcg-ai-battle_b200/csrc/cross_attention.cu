@@ -20,6 +20,21 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// n / d for 0 <= n < 2^31 as a multiply-high, an add and a shift: with
+// 2^(l-1) < d <= 2^l and mul = floor(2^32 (2^l - d) / d) + 1, the quotient is
+// (mulhi(n, mul) + n) >> l (the divisions by sizes known only at the launch
+// were a sixth of the short problems' instructions)
+struct FastDiv {
+    unsigned mul, shift, d;
+    PTCG_DEV unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+FastDiv fast_div(unsigned d) {
+    FastDiv f = {0, 0, d};
+    while ((1ull << f.shift) < d) f.shift++;
+    f.mul = (unsigned)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    return f;
+}
+
 struct CrossArgs {
     const void *q, *k, *v, *o, *dout;
     const uint8_t* keep;
@@ -32,12 +47,13 @@ struct CrossArgs {
     PtcgHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
     int lq, lk, heads, kv_heads, group, rows;      // rows = group * lq
     int tiles, nsplit, split;                      // `split` rows of the split axis per part
+    FastDiv by_lq, by_tiles, by_nsplit, by_kv;
     float scale;
 };
 
 // element offset of stacked row r of key head hk in a query-like tensor
 PTCG_DEV long qrow(const CrossArgs& a, const PtcgHeads& s, int seq, int hk, int r) {
-    const int g = r / a.lq;
+    const int g = a.by_lq.div(r);
     return seq * s.seq + (r - g * a.lq) * s.row + (long)(hk * a.group + g) * s.head;
 }
 PTCG_DEV long krow(const PtcgHeads& s, int seq, int hk, int j) {
@@ -53,11 +69,11 @@ PTCG_DEV bool kept(const CrossArgs& a, int seq, int j, int len) {
 struct Where { int tile, part, hk, seq; };
 PTCG_DEV Where where(const CrossArgs& a) {
     Where w;
-    unsigned b = blockIdx.x;
-    w.tile = b % a.tiles; b /= a.tiles;
-    w.part = b % a.nsplit; b /= a.nsplit;
-    w.hk = b % a.kv_heads;
-    w.seq = b / a.kv_heads;
+    const unsigned b = blockIdx.x, c = a.by_tiles.div(b), d = a.by_nsplit.div(c), e = a.by_kv.div(d);
+    w.tile = b - c * a.by_tiles.d;
+    w.part = c - d * a.by_nsplit.d;
+    w.hk = d - e * a.by_kv.d;
+    w.seq = e;
     return w;
 }
 
@@ -107,26 +123,42 @@ template <int DH> PTCG_DEV void frag_bk(uint32_t (&f)[4], uint32_t base, int k0,
     const int mi = lane >> 3;
     ldsm4t(f, base + tile_off<DH>(k0 + (mi & 1) * 8 + (lane & 7), nd * 2 + (mi >> 1)));
 }
+// Staging: a thread takes piece tid % P of rows tid / P, + THREADS / P, ..; that
+// step is a multiple of 8 rows, so the permutation, and with it the offset in
+// the tile, moves by a constant.
+template <int DH, int THREADS> struct Lanes {
+    static constexpr int P = DH / 8, STEP = THREADS / P;
+    static_assert(STEP % 8 == 0, "the tile's permutation repeats every 8 rows");
+    int r, c;
+    uint32_t off;
+    PTCG_DEV Lanes() : r(threadIdx.x / P), c(threadIdx.x % P), off(tile_off<DH>(r, c)) {}
+};
 // stacked query rows r0 .. +N into a tile; rows past R are zeros
 template <int DH, int N, int THREADS>
 PTCG_DEV void stage_q(uint32_t dst, const bf16* src, const PtcgHeads& s, const CrossArgs& a,
                       int seq, int hk, int r0) {
-    constexpr int P = DH / 8;
-    for (int i = threadIdx.x; i < N * P; i += THREADS) {
-        const int r = i / P, c = i % P;
-        const bool in = r0 + r < a.rows;
-        cp16(dst + tile_off<DH>(r, c), src + (in ? qrow(a, s, seq, hk, r0 + r) + c * 8 : 0), in);
+    const Lanes<DH, THREADS> l;
+    const bf16* base = src + seq * s.seq + (long)(hk * a.group) * s.head + l.c * 8;
+    #pragma unroll
+    for (int n = 0; n < N; n += l.STEP) {
+        if (N % l.STEP && l.r + n >= N) break;
+        const int r = r0 + l.r + n;
+        const bool in = r < a.rows;
+        const int g = a.by_lq.div(in ? r : 0), i = (in ? r : 0) - g * a.lq;
+        cp16(dst + l.off + n * DH * 2, base + i * s.row + g * s.head, in);
     }
 }
-// key rows j0 .. +N into a tile; rows whose bit is clear are zeros
+// key rows j0 .. +N into a tile; rows whose bit is clear are zeros and are not read
 template <int DH, int N, int THREADS>
 PTCG_DEV void stage_k(uint32_t dst, const bf16* src, const PtcgHeads& s, int seq, int hk, int j0,
                       const uint32_t* bits) {
-    constexpr int P = DH / 8;
-    for (int i = threadIdx.x; i < N * P; i += THREADS) {
-        const int r = i / P, c = i % P;
+    const Lanes<DH, THREADS> l;
+    const bf16* base = src + krow(s, seq, hk, j0 + l.r) + l.c * 8;
+    #pragma unroll
+    for (int n = 0; n < N; n += l.STEP) {
+        const int r = l.r + n;
         const bool in = (bits[r >> 5] >> (r & 31)) & 1;
-        cp16(dst + tile_off<DH>(r, c), src + (in ? krow(s, seq, hk, j0 + r) + c * 8 : 0), in);
+        cp16(dst + l.off + n * DH * 2, in ? base + n * s.row : src, in);
     }
 }
 PTCG_DEV float quad_max(float v) {
@@ -1260,6 +1292,13 @@ Split split_of(long tiles, int axis) {
     s.n = (int)cdiv(axis, s.len);
     return s;
 }
+void set_tiles(CrossArgs& a, long tiles, const Split& s) {
+    a.tiles = (int)tiles;
+    a.nsplit = s.n;
+    a.split = s.len;
+    a.by_tiles = fast_div((unsigned)tiles);
+    a.by_nsplit = fast_div(s.n);
+}
 struct FwdPlan { bool few; int bm; long tiles, blocks; Split sp; long o_ml, bytes; };
 FwdPlan fwd_plan(const PtcgCross& c) {
     FwdPlan p;
@@ -1359,7 +1398,7 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
     const bool bf = c.dtype == PTCG_BF16;
     const long probs = (long)c.nseq * c.kv_heads, nrows = probs * a.rows, nkeys = probs * a.lk;
     if (p.rows && p.qblocks) {
-        a.tiles = 1; a.nsplit = p.qs.n; a.split = p.qs.len;
+        set_tiles(a, 1, p.qs);
         e = a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, p.qblocks, s)
             : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, p.qblocks, s) : launch_bwd_rows<DH, 4>(a, p.qblocks, s);
         if (e == cudaSuccess && p.qs.n > 1)
@@ -1367,7 +1406,7 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
         return e;
     }
     if (p.qblocks) {
-        a.tiles = (int)p.qtiles; a.nsplit = p.qs.n; a.split = p.qs.len;
+        set_tiles(a, p.qtiles, p.qs);
         if (bf) {
             constexpr int BN = DH == 128 ? 32 : 64;
             const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2;
@@ -1385,7 +1424,7 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
         }
     }
     if (p.kblocks) {
-        a.tiles = (int)p.ktiles; a.nsplit = p.ks.n; a.split = p.ks.len;
+        set_tiles(a, p.ktiles, p.ks);
         ++g_ptcg_launches;
         if (bf) {
             constexpr int BQ = DH == 128 ? 32 : 64;
@@ -1440,6 +1479,8 @@ CrossArgs args(const PtcgCross& c) {
     a.group = c.heads / c.kv_heads;
     a.rows = a.group * c.lq;
     a.scale = c.scale;
+    a.by_lq = fast_div(c.lq > 0 ? c.lq : 1);
+    a.by_kv = fast_div(c.kv_heads);
     return a;
 }
 
@@ -1470,7 +1511,7 @@ int ptcg_cross_attention_fwd(const PtcgCross* c, const void* q, const void* k, c
     a.q = q; a.k = k; a.v = v; a.keep = keep; a.kv_len = kv_len; a.out = out; a.lse = lse;
     a.part = (float*)scratch;
     a.part_ml = (float2*)((uint8_t*)scratch + p.o_ml);
-    a.tiles = (int)p.tiles; a.nsplit = p.sp.n; a.split = p.sp.len;
+    set_tiles(a, p.tiles, p.sp);
     cudaStream_t s = (cudaStream_t)stream;
     OP_CK(c->dh == 32 ? fwd_dh<32>(a, *c, p, s) : c->dh == 64 ? fwd_dh<64>(a, *c, p, s) : fwd_dh<128>(a, *c, p, s));
     OP_CKL();
