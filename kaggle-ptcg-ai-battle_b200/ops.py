@@ -20,6 +20,7 @@ from . import native
 from .native import PtcgCross, PtcgError, PtcgHeads, check
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
+_BYTES = (torch.bool, torch.uint8)
 
 
 def _bad(msg):
@@ -43,7 +44,7 @@ def _f32(dev, shape, **tensors):
     for name, t in tensors.items():
         if t is None:
             continue
-        if t.dtype != torch.float32 or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.device != dev or t.shape != shape or not t.is_contiguous():
             _bad(f"{name} must be a contiguous float32 tensor of shape {shape} on {dev}")
 
 
@@ -52,22 +53,29 @@ def _ptr(t):
 
 
 def _call(dev, fn, *args):
-    """fn(*args, stream) with `dev` current."""
+    """fn(*args, stream) with `dev` current, on its current stream (the raw
+    handle: a Stream object costs as much as the launch)."""
     if dev.type != "cuda":
         _bad("the operators run on CUDA tensors")
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        check(rc)
 
 
 def _rows(t, width, what):
     """(tensor as rows of `width` contiguous elements, rows, pitch); a copy only
     where the leading dimensions have no common pitch."""
-    if t.dim() == 0 or t.shape[-1] != width:
-        _bad(f"{what}: last dimension must be {width}, got shape {tuple(t.shape)}")
-    if t.dim() != 2:
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        _bad(f"{what}: last dimension must be {width}, got shape {tuple(shape)}")
+    if t.is_contiguous():
+        return t, t.numel() // width if width else 0, width
+    if len(shape) != 2:
         t = t.reshape(-1, width)
     if width > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < width:
         t = t.contiguous()
@@ -147,7 +155,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out_dtype=None, stats=True):
     dev, width = x.device, x.shape[-1] if x.dim() else 0
     xr, n, ldx = _rows(x, width, "x")
     _f32(dev, (width,), gamma=gamma, beta=beta)
-    y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=dev)
+    y = torch.empty(*x.shape, dtype=out_dtype or x.dtype, device=dev)
     mean = torch.empty(x.shape[:-1], device=dev) if stats else None
     rstd = torch.empty(x.shape[:-1], device=dev) if stats else None
     _call(dev, native.lib().ptcg_layer_norm_fwd, xr.data_ptr(), _dt(x, "x"), ldx, _ptr(gamma),
@@ -169,7 +177,7 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dres=None, dgamma=None, dbeta=
     gr, _, ldg = _rows(dy, width, "dy")
     rr, _, ldr = _rows(dres, width, "dres") if dres is not None else (None, 0, 0)
     _f32(dev, (width,), gamma=gamma, dgamma=dgamma, dbeta=dbeta)
-    _f32(dev, tuple(x.shape[:-1]), mean=mean, rstd=rstd)
+    _f32(dev, x.shape[:-1], mean=mean, rstd=rstd)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if not weight_grads:
         if dgamma is not None or dbeta is not None:
@@ -190,19 +198,28 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dres=None, dgamma=None, dbeta=
 
 # -------------------------------------------------------- cross attention
 @functools.lru_cache(maxsize=256)
-def _cross(dtype, dims, scale, strides):
-    """The C description of a problem: plain sizes and strides, no addresses."""
-    return PtcgCross(dtype, *dims, scale, *[PtcgHeads(*s) for s in strides])
+def _cross(dtype, dims, scale, strides, backward):
+    """The C description of a problem (plain sizes and strides, no addresses)
+    and the bytes of scratch it needs."""
+    c = PtcgCross(dtype, *dims, scale, *[PtcgHeads(*s) for s in strides])
+    lib = native.lib()
+    nbytes = (lib.ptcg_cross_attention_bwd_scratch if backward
+              else lib.ptcg_cross_attention_fwd_scratch)(c)
+    if nbytes < 0:
+        _bad(lib.ptcg_last_error().decode())
+    return c, nbytes
 
 
 _ZERO = (0, 0, 0)
 
 
 def _head_strides(t, what):
-    if t.shape[3] > 1 and t.stride(3) != 1:
+    a, b, c, d = t.stride()
+    n, r, h, w = t.shape
+    if d != 1 and w > 1:
         _bad(f"{what}: the head's elements must be contiguous, got strides {t.stride()}")
     # a dimension of one element has no stride that matters
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+    return a if n > 1 else 0, b if r > 1 else 0, c if h > 1 else 0
 
 
 def _cross_args(q, k, v, keep, kv_len, scale):
@@ -211,18 +228,19 @@ def _cross_args(q, k, v, keep, kv_len, scale):
     dev, dt = q.device, _dt(q, "q")
     nseq, lq, heads, dh = q.shape
     lk, kvh = k.shape[1], k.shape[2]
-    if k.shape != (nseq, lk, kvh, dh) or v.shape != k.shape:
+    if k.shape[0] != nseq or k.shape[3] != dh or v.shape != k.shape:
         _bad(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         _bad("q, k and v must have one type")
-    _on(dev, k=k, v=v, keep=keep, kv_len=kv_len)
+    if k.device != dev or v.device != dev:
+        _on(dev, k=k, v=v)
     if keep is not None:
-        if keep.shape != (nseq, lk) or keep.dtype not in (torch.bool, torch.uint8):
-            _bad(f"keep must be a bool or uint8 tensor of shape {(nseq, lk)}")
+        if keep.shape != (nseq, lk) or keep.dtype not in _BYTES or keep.device != dev:
+            _bad(f"keep must be a bool or uint8 tensor of shape {(nseq, lk)} on {dev}")
         keep = keep.contiguous()
     if kv_len is not None:
-        if kv_len.shape != (nseq,) or kv_len.dtype != torch.int32:
-            _bad(f"kv_len must be an int32 tensor of shape {(nseq,)}")
+        if kv_len.shape != (nseq,) or kv_len.dtype != torch.int32 or kv_len.device != dev:
+            _bad(f"kv_len must be an int32 tensor of shape {(nseq,)} on {dev}")
         kv_len = kv_len.contiguous()
     scale = dh ** -0.5 if scale is None else float(scale)
     return dev, dt, (nseq, lq, lk, heads, kvh, dh), keep, kv_len, scale
@@ -238,13 +256,11 @@ def cross_attention(q, k, v, keep=None, kv_len=None, scale=None):
     nseq, lq, lk, heads, kvh, dh = dims
     out = torch.empty(nseq, lq, heads, dh, dtype=q.dtype, device=dev)
     lse = torch.empty(nseq, heads, lq, device=dev)
-    c = _cross(dt, dims, scale, (_head_strides(q, "q"), _head_strides(k, "k"),
-                                 _head_strides(v, "v"), (lq * heads * dh, heads * dh, dh),
-                                 _ZERO, _ZERO, _ZERO, _ZERO))
-    lib = native.lib()
-    nbytes = lib.ptcg_cross_attention_fwd_scratch(c)
+    c, nbytes = _cross(dt, dims, scale, (_head_strides(q, "q"), _head_strides(k, "k"),
+                                         _head_strides(v, "v"), (lq * heads * dh, heads * dh, dh),
+                                         _ZERO, _ZERO, _ZERO, _ZERO), False)
     scratch = _scratch(nbytes, dev)
-    _call(dev, lib.ptcg_cross_attention_fwd, c, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    _call(dev, native.lib().ptcg_cross_attention_fwd, c, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _ptr(keep), _ptr(kv_len), out.data_ptr(), lse.data_ptr(), _ptr(scratch), nbytes)
     return out, lse
 
@@ -263,13 +279,11 @@ def cross_attention_backward(dout, q, k, v, out, lse, keep=None, kv_len=None, sc
     dk = torch.empty(nseq, lk, kvh, dh, dtype=q.dtype, device=dev)
     dv = torch.empty(nseq, lk, kvh, dh, dtype=q.dtype, device=dev)
     sq, sk = (lq * heads * dh, heads * dh, dh), (lk * kvh * dh, kvh * dh, dh)
-    c = _cross(dt, dims, scale, (_head_strides(q, "q"), _head_strides(k, "k"),
-                                 _head_strides(v, "v"), _head_strides(out, "out"),
-                                 _head_strides(dout, "dout"), sq, sk, sk))
-    lib = native.lib()
-    nbytes = lib.ptcg_cross_attention_bwd_scratch(c)
+    c, nbytes = _cross(dt, dims, scale, (_head_strides(q, "q"), _head_strides(k, "k"),
+                                         _head_strides(v, "v"), _head_strides(out, "out"),
+                                         _head_strides(dout, "dout"), sq, sk, sk), True)
     scratch = _scratch(nbytes, dev)
-    _call(dev, lib.ptcg_cross_attention_bwd, c, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    _call(dev, native.lib().ptcg_cross_attention_bwd, c, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _ptr(keep), _ptr(kv_len), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(scratch), nbytes)
     return dq, dk, dv
