@@ -958,43 +958,84 @@ __global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ Cross
 }
 
 // ------------------------------------------------------------------ fp32
-// Exact fp32 on the SIMT cores.  128 threads as 8 x 16: thread (ty, tx) owns
-// RT rows x NC columns of every product, all of which are
-//   acc[i][j] += sum_k A[k][ty RT + i] B[k][tx NC + j]
-// over tiles in shared memory, two rows at a time on the packed f32x2 path.
-template <int RT, int NC>
-PTCG_DEV void tile_mm(float (&acc)[RT][NC], const float* A, int lda, const float* B, int ldb, int K,
-                      int ty, int tx) {
+// Exact fp32 on the SIMT cores.  128 threads as 8 x 16: thread (ty, tx) owns RT
+// rows (rows_of) and NC columns of every product, computed two multiply-adds
+// at a time on the packed f32x2 path.  All tiles are row-major copies of the
+// tensors (cp.async, pitch DH + 4 floats, so that the rows a quarter warp
+// touches fall into different banks); two forms of product serve them:
+//   mm_rows   acc[i][j] = sum_d A[row i][d] B[row tx + 16 j][d], pairs along d
+//   mm_outer  acc[i][j] += sum_k A[k][row i] B[k][col j], pairs along the rows,
+//             A a probability tile that the threads wrote with k as its row
+template <int RT> PTCG_DEV int row_of(int ty, int i) {
+    return RT == 8 ? (i >> 2) * 32 + ty * 4 + (i & 3) : ty * RT + i;
+}
+template <int NC> PTCG_DEV int col_of(int tx, int j) {
+    return NC == 8 ? (j >> 2) * 64 + tx * 4 + (j & 3) : tx * NC + j;
+}
+// keys (or stacked rows) per tile of the fp32 kernels, and their pitch
+template <int DH> struct F32 { static constexpr int BN = DH == 128 ? 32 : 64, LD = DH + 4; };
+
+template <int RT, int NC, int DH>
+PTCG_DEV void mm_rows(float (&acc)[RT][NC], const float* A, const float* B, int ty, int tx) {
+    constexpr int LD = F32<DH>::LD;
+    unsigned long long c[RT][NC];
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) c[i][j] = 0ull;
+    #pragma unroll 2
+    for (int d = 0; d < DH; d += 4) {
+        ulonglong2 b[NC];
+        #pragma unroll
+        for (int j = 0; j < NC; j++) b[j] = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * j) * LD + d);
+        #pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(A + row_of<RT>(ty, i) * LD + d);
+            #pragma unroll
+            for (int j = 0; j < NC; j++) c[i][j] = fma2(x.y, b[j].y, fma2(x.x, b[j].x, c[i][j]));
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) {
+            float lo, hi;
+            upk2(c[i][j], lo, hi);
+            acc[i][j] = lo + hi;
+        }
+}
+template <int RT, int NC, int K>
+PTCG_DEV void mm_outer(float (&acc)[RT][NC], const float* A, int lda, const float* B, int ldb, int ty, int tx) {
     unsigned long long c[RT / 2][NC];
     #pragma unroll
     for (int i = 0; i < RT / 2; i++)
         #pragma unroll
         for (int j = 0; j < NC; j++) c[i][j] = pk2(acc[2 * i][j], acc[2 * i + 1][j]);
-    const float* pa = A + ty * RT;
-    const float* pb = B + tx * NC;
     #pragma unroll 4
-    for (int k = 0; k < K; k++, pa += lda, pb += ldb) {
+    for (int k = 0; k < K; k++) {
         unsigned long long x[RT / 2];
-        float y[NC];
-        if (RT >= 4) {
-            #pragma unroll
-            for (int i = 0; i < RT / 4; i++) {
-                const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(pa + 4 * i);
-                x[2 * i] = u.x;
-                x[RT >= 4 ? 2 * i + 1 : 0] = u.y;
+        #pragma unroll
+        for (int i = 0; i < RT; i += 4) {
+            const float* p = A + k * lda + row_of<RT>(ty, i);
+            if constexpr (RT >= 4) {
+                const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p);
+                x[i / 2] = u.x;
+                x[i / 2 + 1] = u.y;
+            } else {
+                x[0] = *reinterpret_cast<const unsigned long long*>(p);
             }
-        } else {
-            x[0] = *reinterpret_cast<const unsigned long long*>(pa);
         }
-        if (NC >= 4) {
-            #pragma unroll
-            for (int j = 0; j < NC / 4; j++) {
-                const float4 v = *reinterpret_cast<const float4*>(pb + 4 * j);
-                y[4 * j] = v.x; y[(4 * j + 1) % NC] = v.y; y[(4 * j + 2) % NC] = v.z; y[(4 * j + 3) % NC] = v.w;
+        float y[NC];
+        #pragma unroll
+        for (int j = 0; j < NC; j += 4) {
+            const float* p = B + k * ldb + col_of<NC>(tx, j);
+            if constexpr (NC >= 4) {
+                const float4 v = *reinterpret_cast<const float4*>(p);
+                y[j] = v.x; y[j + 1] = v.y; y[j + 2] = v.z; y[j + 3] = v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(p);
+                y[0] = v.x; y[1] = v.y;
             }
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(pb);
-            y[0] = v.x; y[1] = v.y;
         }
         #pragma unroll
         for (int j = 0; j < NC; j++) {
@@ -1008,16 +1049,41 @@ PTCG_DEV void tile_mm(float (&acc)[RT][NC], const float* A, int lda, const float
         #pragma unroll
         for (int j = 0; j < NC; j++) upk2(c[i][j], acc[2 * i][j], acc[2 * i + 1][j]);
 }
-// N rows of DH floats: transposed to T[d][row] (pitch ldt) and / or as they
-// are to X[row][d]; row(r) gives the source or null (zeros)
+template <int RT, int NC> PTCG_DEV void clear(float (&acc)[RT][NC]) {
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) acc[i][j] = 0.f;
+}
+// the thread's RT values of column k into row k of a [k][row] tile
+template <int RT> PTCG_DEV void put_rows(float* T, int ld, int k, int ty, const float (&v)[RT]) {
+    #pragma unroll
+    for (int i = 0; i < RT; i += 4) {
+        float* p = T + k * ld + row_of<RT>(ty, i);
+        if constexpr (RT >= 4) *reinterpret_cast<float4*>(p) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    }
+}
+// one thread's columns of a result row
+template <int NC> PTCG_DEV void put_cols(float* p, int tx, const float (&v)[NC], float f) {
+    #pragma unroll
+    for (int j = 0; j < NC; j += 4) {
+        float* q = p + col_of<NC>(tx, j);
+        if constexpr (NC >= 4) *reinterpret_cast<float4*>(q) = make_float4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
+        else *reinterpret_cast<float2*>(q) = make_float2(v[0] * f, v[1] * f);
+    }
+}
+// N rows of DH floats, asynchronously; row(r) gives the source or null (zeros)
 template <int DH, int N, typename F>
-PTCG_DEV void stage_f32(float* T, int ldt, float* X, F row) {
-    for (int i = threadIdx.x; i < N * (DH / 4); i += 128) {
-        const int r = i % N, c = i / N * 4;
-        const float* p = row(r);
-        const float4 v = p ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (T) { T[c * ldt + r] = v.x; T[(c + 1) * ldt + r] = v.y; T[(c + 2) * ldt + r] = v.z; T[(c + 3) * ldt + r] = v.w; }
-        if (X) *reinterpret_cast<float4*>(X + r * DH + c) = v;
+PTCG_DEV void stage_f32(float* dst, const float* any, F row) {
+    constexpr int P = DH / 4, STEP = 128 / P;
+    const int r0 = threadIdx.x / P, c = threadIdx.x % P * 4;
+    const uint32_t to = s_addr(dst + r0 * F32<DH>::LD + c);
+    #pragma unroll
+    for (int n = 0; n < N; n += STEP) {
+        if (N % STEP && r0 + n >= N) break;
+        const float* p = row(r0 + n);
+        cp16(to + n * F32<DH>::LD * 4, p ? p + c : any, p != nullptr);
     }
 }
 PTCG_DEV float row16_max(float v) {
@@ -1030,85 +1096,108 @@ PTCG_DEV float row16_sum(float v) {
     for (int o = 1; o < 16; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// keys per tile of the fp32 kernels, and shared-memory pitches
-template <int DH> struct F32 { static constexpr int BN = DH == 128 ? 32 : 64, LB = BN + 4; };
+PTCG_DEV const float* q_ptr(const CrossArgs& a, const void* p, const PtcgHeads& s, const Where& at, int r, int end) {
+    return r < end ? (const float*)p + qrow(a, s, at.seq, at.hk, r) : nullptr;
+}
+PTCG_DEV const float* k_ptr(const void* p, const PtcgHeads& s, const Where& at, int j, bool ok) {
+    return ok ? (const float*)p + krow(s, at.seq, at.hk, j) : nullptr;
+}
+// lse as the backward uses it: +inf makes the probabilities of rows without
+// keys and of rows past the end zero
+PTCG_DEV float lse_or_inf(const CrossArgs& a, long row, bool in) {
+    const float x = in ? a.lse[row] : -INFINITY;
+    return x == -INFINITY ? INFINITY : x;
+}
+// delta = dout . out of row r, whose dout lies in shared memory
+template <int DH> PTCG_DEV float delta_f32(const CrossArgs& a, const Where& at, int r, const float* g) {
+    const float* o = (const float*)a.o + qrow(a, a.so, at.seq, at.hk, r);
+    float d = 0.f;
+    #pragma unroll 4
+    for (int c = 0; c < DH; c += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(o + c), y = *reinterpret_cast<const float4*>(g + c);
+        d = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, d))));
+    }
+    return d;
+}
 
 template <int DH, int RT>
 __global__ void __launch_bounds__(128) k_cross_fwd_f32(const __grid_constant__ CrossArgs a) {
-    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LB = F32<DH>::LB, NC = BN / 16, ND = DH / 16;
+    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LD = F32<DH>::LD, NC = BN / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
-    __shared__ uint8_t ok[64];
-    float* Qt = fs;                  // [DH][LM]
-    float* Kt = Qt + DH * LM;        // [DH][LB]
-    float* Vs = Kt + DH * LB;        // [BN][DH]
-    float* Ps = Vs + BN * DH;        // [BN][LM]
+    __shared__ uint8_t ok[BN];
+    float* Qs = fs;                  // [BM][LD]
+    float* Ks = Qs + BM * LD;        // [BN][LD]
+    float* Vs = Ks + BN * LD;        // [BN][LD]
+    float* Ps = Vs + BN * LD;        // [BN][LM]
     const Where at = where(a);
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
     const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
-    const float* q = (const float*)a.q;
-    stage_f32<DH, BM>(Qt, LM, nullptr, [&](int r) {
-        return r0 + r < a.rows ? q + qrow(a, a.sq, at.seq, at.hk, r0 + r) : nullptr; });
+    stage_f32<DH, BM>(Qs, (const float*)a.q, [&](int r) { return q_ptr(a, a.q, a.sq, at, r0 + r, a.rows); });
     float o[RT][ND], m[RT], l[RT];
+    clear(o);
     #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
-        #pragma unroll
-        for (int j = 0; j < ND; j++) o[i][j] = 0.f;
-    }
+    for (int i = 0; i < RT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
     for (int k0 = kbeg; k0 < kend; k0 += BN) {
-        __syncthreads();
-        const bool in = threadIdx.x < BN && k0 + threadIdx.x < kend && kept(a, at.seq, k0 + threadIdx.x, len);
+        const int key = k0 + threadIdx.x;
+        const bool in = threadIdx.x < BN && key < kend && kept(a, at.seq, key, len);
+        __syncthreads();                             // the last tile is done with
         if (threadIdx.x < BN) ok[threadIdx.x] = in;
         if (!__syncthreads_or(in)) continue;
-        stage_f32<DH, BN>(Kt, LB, nullptr, [&](int r) {
-            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, k0 + r) : nullptr; });
-        stage_f32<DH, BN>(nullptr, 0, Vs, [&](int r) {
-            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, k0 + r) : nullptr; });
+        stage_f32<DH, BN>(Ks, (const float*)a.k, [&](int r) { return k_ptr(a.k, a.sk, at, k0 + r, ok[r]); });
+        cp_commit();
+        stage_f32<DH, BN>(Vs, (const float*)a.v, [&](int r) { return k_ptr(a.v, a.sv, at, k0 + r, ok[r]); });
+        cp_commit();
+        cp_wait<1>();
         __syncthreads();
         float s[RT][NC];
+        mm_rows<RT, NC, DH>(s, Qs, Ks, ty, tx);
         #pragma unroll
-        for (int i = 0; i < RT; i++)
+        for (int j = 0; j < NC; j++) {
+            const bool live = ok[tx + 16 * j];
             #pragma unroll
-            for (int j = 0; j < NC; j++) s[i][j] = 0.f;
-        tile_mm<RT, NC>(s, Qt, LM, Kt, LB, DH, ty, tx);
+            for (int i = 0; i < RT; i++) s[i][j] = live ? s[i][j] * a.scale : -INFINITY;
+        }
         #pragma unroll
         for (int i = 0; i < RT; i++) {
-            float x = -INFINITY;
+            float x = s[i][0];
             #pragma unroll
-            for (int j = 0; j < NC; j++) {
-                s[i][j] = ok[tx * NC + j] ? s[i][j] * a.scale : -INFINITY;
-                x = fmaxf(x, s[i][j]);
-            }
+            for (int j = 1; j < NC; j++) x = fmaxf(x, s[i][j]);
             const float n = fmaxf(m[i], row16_max(x)), u = n == -INFINITY ? 0.f : n;
-            const float c = expf(m[i] - u);
+            const float c = __expf(m[i] - u);
             m[i] = n;
             float t = 0.f;
             #pragma unroll
             for (int j = 0; j < NC; j++) {
-                s[i][j] = expf(s[i][j] - u);
+                s[i][j] = __expf(s[i][j] - u);
                 t += s[i][j];
-                Ps[(tx * NC + j) * LM + ty * RT + i] = s[i][j];
             }
             l[i] = fmaf(l[i], c, t);
             #pragma unroll
             for (int j = 0; j < ND; j++) o[i][j] *= c;
         }
+        #pragma unroll
+        for (int j = 0; j < NC; j++) {
+            float v[RT];
+            #pragma unroll
+            for (int i = 0; i < RT; i++) v[i] = s[i][j];
+            put_rows<RT>(Ps, LM, tx + 16 * j, ty, v);
+        }
+        cp_wait<0>();
         __syncthreads();
-        tile_mm<RT, ND>(o, Ps, LM, Vs, DH, BN, ty, tx);
+        mm_outer<RT, ND, BN>(o, Ps, LM, Vs, LD, ty, tx);
     }
+    cp_wait<0>();
     #pragma unroll
     for (int i = 0; i < RT; i++) {
         const float t = row16_sum(l[i]);
-        const int r = r0 + ty * RT + i;
+        const int r = r0 + row_of<RT>(ty, i);
         if (r >= a.rows) continue;
         const long row = ((long)at.seq * a.kv_heads + at.hk) * a.rows + r;
         const float inv = a.nsplit > 1 ? 1.f : t == 0.f ? 0.f : 1.f / t;
         float* p = a.nsplit > 1 ? a.part + (row * a.nsplit + at.part) * DH
                                 : (float*)a.out + qrow(a, a.so, at.seq, at.hk, r);
-        #pragma unroll
-        for (int j = 0; j < ND; j++) p[tx * ND + j] = o[i][j] * inv;
+        put_cols<ND>(p, tx, o[i], inv);
         if (tx == 0) {
             // the parts carry their maximum in the log2 domain, as the bf16 kernel's do
             if (a.nsplit > 1) a.part_ml[row * a.nsplit + at.part] = make_float2(m[i] * LOG2E, t);
@@ -1119,162 +1208,200 @@ __global__ void __launch_bounds__(128) k_cross_fwd_f32(const __grid_constant__ C
 
 template <int DH, int RT>
 __global__ void __launch_bounds__(128) k_cross_dq_f32(const __grid_constant__ CrossArgs a) {
-    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LB = F32<DH>::LB, NC = BN / 16, ND = DH / 16;
+    constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LD = F32<DH>::LD, NC = BN / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
-    __shared__ uint8_t ok[64];
+    __shared__ uint8_t ok[BN];
     __shared__ float s_lse[BM], s_delta[BM];
-    float* Qt = fs;                  // [DH][LM]
-    float* Gt = Qt + DH * LM;        // [DH][LM]
-    float* Kt = Gt + DH * LM;        // [DH][LB]
-    float* Vt = Kt + DH * LB;        // [DH][LB]
-    float* Ks = Vt + DH * LB;        // [BN][DH]
-    float* Ds = Ks + BN * DH;        // [BN][LM]
+    float* Qs = fs;                  // [BM][LD]
+    float* Gs = Qs + BM * LD;        // [BM][LD]
+    float* Ks = Gs + BM * LD;        // [BN][LD]
+    float* Vs = Ks + BN * LD;        // [BN][LD]
+    float* Ds = Vs + BN * LD;        // [BN][LM]
     const Where at = where(a);
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
     const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
     const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
-    stage_f32<DH, BM>(Qt, LM, nullptr, [&](int r) {
-        return r0 + r < a.rows ? (const float*)a.q + qrow(a, a.sq, at.seq, at.hk, r0 + r) : nullptr; });
-    stage_f32<DH, BM>(Gt, LM, nullptr, [&](int r) {
-        return r0 + r < a.rows ? (const float*)a.dout + qrow(a, a.sdo, at.seq, at.hk, r0 + r) : nullptr; });
+    stage_f32<DH, BM>(Qs, (const float*)a.q, [&](int r) { return q_ptr(a, a.q, a.sq, at, r0 + r, a.rows); });
+    stage_f32<DH, BM>(Gs, (const float*)a.dout, [&](int r) { return q_ptr(a, a.dout, a.sdo, at, r0 + r, a.rows); });
+    cp_commit();
+    cp_wait<0>();
     __syncthreads();
     for (int r = threadIdx.x; r < BM; r += 128) {
         const bool in = r0 + r < a.rows;
-        float d = 0.f;
-        if (in) {
-            const float* o = (const float*)a.o + qrow(a, a.so, at.seq, at.hk, r0 + r);
-            for (int c = 0; c < DH; c++) d = fmaf(o[c], Gt[c * LM + r], d);
-            if (at.part == 0) a.delta[row0 + r0 + r] = d;
-        }
-        const float x = in ? a.lse[row0 + r0 + r] : -INFINITY;
-        s_lse[r] = x == -INFINITY ? INFINITY : x;
+        const float d = in ? delta_f32<DH>(a, at, r0 + r, Gs + r * LD) : 0.f;
+        if (in && at.part == 0) a.delta[row0 + r0 + r] = d;
+        s_lse[r] = lse_or_inf(a, row0 + r0 + r, in);
         s_delta[r] = d;
     }
     float dq[RT][ND];
-    #pragma unroll
-    for (int i = 0; i < RT; i++)
-        #pragma unroll
-        for (int j = 0; j < ND; j++) dq[i][j] = 0.f;
+    clear(dq);
     for (int k0 = kbeg; k0 < kend; k0 += BN) {
+        const int key = k0 + threadIdx.x;
+        const bool in = threadIdx.x < BN && key < kend && kept(a, at.seq, key, len);
         __syncthreads();
-        const bool in = threadIdx.x < BN && k0 + threadIdx.x < kend && kept(a, at.seq, k0 + threadIdx.x, len);
         if (threadIdx.x < BN) ok[threadIdx.x] = in;
         if (!__syncthreads_or(in)) continue;
-        stage_f32<DH, BN>(Kt, LB, Ks, [&](int r) {
-            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, k0 + r) : nullptr; });
-        stage_f32<DH, BN>(Vt, LB, nullptr, [&](int r) {
-            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, k0 + r) : nullptr; });
+        stage_f32<DH, BN>(Ks, (const float*)a.k, [&](int r) { return k_ptr(a.k, a.sk, at, k0 + r, ok[r]); });
+        cp_commit();
+        stage_f32<DH, BN>(Vs, (const float*)a.v, [&](int r) { return k_ptr(a.v, a.sv, at, k0 + r, ok[r]); });
+        cp_commit();
+        cp_wait<1>();
         __syncthreads();
         float s[RT][NC], p[RT][NC];
+        mm_rows<RT, NC, DH>(s, Qs, Ks, ty, tx);
+        cp_wait<0>();
+        __syncthreads();
+        mm_rows<RT, NC, DH>(p, Gs, Vs, ty, tx);
         #pragma unroll
-        for (int i = 0; i < RT; i++)
+        for (int j = 0; j < NC; j++) {
+            const bool live = ok[tx + 16 * j];
+            float v[RT];
             #pragma unroll
-            for (int j = 0; j < NC; j++) s[i][j] = p[i][j] = 0.f;
-        tile_mm<RT, NC>(s, Qt, LM, Kt, LB, DH, ty, tx);
-        tile_mm<RT, NC>(p, Gt, LM, Vt, LB, DH, ty, tx);
-        #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int r = ty * RT + i;
-            #pragma unroll
-            for (int j = 0; j < NC; j++) {
-                const float e = ok[tx * NC + j] ? expf(fmaf(s[i][j], a.scale, -s_lse[r])) : 0.f;
-                Ds[(tx * NC + j) * LM + r] = e * (p[i][j] - s_delta[r]);
+            for (int i = 0; i < RT; i++) {
+                const int r = row_of<RT>(ty, i);
+                const float e = live ? __expf(fmaf(s[i][j], a.scale, -s_lse[r])) : 0.f;
+                v[i] = e * (p[i][j] - s_delta[r]);
             }
+            put_rows<RT>(Ds, LM, tx + 16 * j, ty, v);
         }
         __syncthreads();
-        tile_mm<RT, ND>(dq, Ds, LM, Ks, DH, BN, ty, tx);
+        mm_outer<RT, ND, BN>(dq, Ds, LM, Ks, LD, ty, tx);
     }
     #pragma unroll
     for (int i = 0; i < RT; i++) {
-        const int r = r0 + ty * RT + i;
+        const int r = r0 + row_of<RT>(ty, i);
         if (r >= a.rows) continue;
-        float* p = a.nsplit > 1 ? a.part + ((row0 + r) * a.nsplit + at.part) * DH
-                                : (float*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r);
-        #pragma unroll
-        for (int j = 0; j < ND; j++) p[tx * ND + j] = dq[i][j] * a.scale;
+        put_cols<ND>(a.nsplit > 1 ? a.part + ((row0 + r) * a.nsplit + at.part) * DH
+                                  : (float*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), tx, dq[i], a.scale);
     }
 }
 
-template <int DH>
+// dk and dv of a key tile over the stacked rows (ROWS: at most 64 of them, all
+// in one tile, and dq as well: each block then walks the key tiles and S is
+// computed once, as in k_cross_bwd_rows)
+template <int DH, bool ROWS>
 __global__ void __launch_bounds__(128) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
-    constexpr int RT = 8, BK = 64, LM = BK + 4, BQ = F32<DH>::BN, LB = F32<DH>::LB, NC = BQ / 16, ND = DH / 16;
+    constexpr int RT = 8, BK = 64, LM = BK + 4, BQ = ROWS ? 64 : F32<DH>::BN, LQ = BQ + 4, LD = F32<DH>::LD;
+    constexpr int NC = BQ / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
     __shared__ uint8_t ok[BK];
     __shared__ float s_lse[BQ], s_delta[BQ];
-    float* Kt = fs;                  // [DH][LM]
-    float* Vt = Kt + DH * LM;        // [DH][LM]
-    float* Qt = Vt + DH * LM;        // [DH][LB]
-    float* Gt = Qt + DH * LB;        // [DH][LB]
-    float* Qs = Gt + DH * LB;        // [BQ][DH]
-    float* Gs = Qs + BQ * DH;        // [BQ][DH]
-    float* Ps = Gs + BQ * DH;        // [BQ][LM]
-    float* Ds = Ps + BQ * LM;        // [BQ][LM]
+    float* Ks = fs;                  // [BK][LD]
+    float* Vs = Ks + BK * LD;        // [BK][LD]
+    float* Qs = Vs + BK * LD;        // [BQ][LD]
+    float* Gs = Qs + BQ * LD;        // [BQ][LD]
+    float* Ps = Gs + BQ * LD;        // [BQ][LM] P, then dS
+    float* Ds = Ps + BQ * LM;        // ROWS: [BK][LQ] dS with the keys as rows, else [BQ][LM]
     const Where at = where(a);
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int j0 = at.tile * BK, len = kept_len(a, at.seq);
-    const int qbeg = min(at.part * a.split, a.rows), qend = min(a.rows, qbeg + a.split);
+    const int len = kept_len(a, at.seq);
     const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
-    const bool in = threadIdx.x < BK && kept(a, at.seq, j0 + threadIdx.x, len);
-    if (threadIdx.x < BK) ok[threadIdx.x] = in;
-    const bool any = __syncthreads_or(in);
-    float dk[RT][ND], dv[RT][ND];
-    #pragma unroll
-    for (int i = 0; i < RT; i++)
-        #pragma unroll
-        for (int j = 0; j < ND; j++) dk[i][j] = dv[i][j] = 0.f;
-    if (any) {
-        stage_f32<DH, BK>(Kt, LM, nullptr, [&](int r) {
-            return ok[r] ? (const float*)a.k + krow(a.sk, at.seq, at.hk, j0 + r) : nullptr; });
-        stage_f32<DH, BK>(Vt, LM, nullptr, [&](int r) {
-            return ok[r] ? (const float*)a.v + krow(a.sv, at.seq, at.hk, j0 + r) : nullptr; });
-        for (int q0 = qbeg; q0 < qend; q0 += BQ) {
-            __syncthreads();
-            stage_f32<DH, BQ>(Qt, LB, Qs, [&](int r) {
-                return q0 + r < qend ? (const float*)a.q + qrow(a, a.sq, at.seq, at.hk, q0 + r) : nullptr; });
-            stage_f32<DH, BQ>(Gt, LB, Gs, [&](int r) {
-                return q0 + r < qend ? (const float*)a.dout + qrow(a, a.sdo, at.seq, at.hk, q0 + r) : nullptr; });
-            if (threadIdx.x < BQ) {
-                const bool have = q0 + threadIdx.x < qend;
-                const float x = have ? a.lse[row0 + q0 + threadIdx.x] : -INFINITY;
-                s_lse[threadIdx.x] = x == -INFINITY ? INFINITY : x;
-                s_delta[threadIdx.x] = have ? a.delta[row0 + q0 + threadIdx.x] : 0.f;
-            }
-            __syncthreads();
-            float s[RT][NC], p[RT][NC];
-            #pragma unroll
-            for (int i = 0; i < RT; i++)
-                #pragma unroll
-                for (int j = 0; j < NC; j++) s[i][j] = p[i][j] = 0.f;
-            tile_mm<RT, NC>(s, Kt, LM, Qt, LB, DH, ty, tx);
-            tile_mm<RT, NC>(p, Vt, LM, Gt, LB, DH, ty, tx);
-            #pragma unroll
-            for (int i = 0; i < RT; i++) {
-                const int key = ty * RT + i;
-                #pragma unroll
-                for (int j = 0; j < NC; j++) {
-                    const int c = tx * NC + j;
-                    const float e = ok[key] ? expf(fmaf(s[i][j], a.scale, -s_lse[c])) : 0.f;
-                    Ps[c * LM + key] = e;
-                    Ds[c * LM + key] = e * (p[i][j] - s_delta[c]);
-                }
-            }
-            __syncthreads();
-            tile_mm<RT, ND>(dv, Ps, LM, Gs, DH, BQ, ty, tx);
-            tile_mm<RT, ND>(dk, Ds, LM, Qs, DH, BQ, ty, tx);
+    // ROWS: the key tiles of this part; else one key tile and this part's rows
+    const int kfrom = ROWS ? at.part * a.split : at.tile * BK;
+    const int kto = ROWS ? min(a.lk, kfrom + a.split) : min(a.lk, kfrom + BK);
+    const int qbeg = ROWS ? 0 : min(at.part * a.split, a.rows), qend = ROWS ? a.rows : min(a.rows, qbeg + a.split);
+    float dq[ROWS ? RT : 1][ROWS ? ND : 1];
+    clear(dq);
+    auto stage_rows = [&](int q0) {
+        stage_f32<DH, BQ>(Qs, (const float*)a.q, [&](int r) { return q_ptr(a, a.q, a.sq, at, q0 + r, qend); });
+        stage_f32<DH, BQ>(Gs, (const float*)a.dout, [&](int r) { return q_ptr(a, a.dout, a.sdo, at, q0 + r, qend); });
+        cp_commit();
+    };
+    if (ROWS) {
+        stage_rows(0);
+        cp_wait<0>();
+        __syncthreads();
+        if (threadIdx.x < BQ) {
+            const int r = threadIdx.x;
+            s_lse[r] = lse_or_inf(a, row0 + r, r < a.rows);
+            s_delta[r] = r < a.rows ? delta_f32<DH>(a, at, r, Gs + r * LD) : 0.f;
         }
     }
-    #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const int j = j0 + ty * RT + i;
-        if (j >= a.lk) continue;
-        const long part = ((((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part) * DH;
-        float* pk = a.nsplit > 1 ? a.part + part : (float*)a.dk + krow(a.sdk, at.seq, at.hk, j);
-        float* pv = a.nsplit > 1 ? a.part2 + part : (float*)a.dv + krow(a.sdv, at.seq, at.hk, j);
+    for (int j0 = kfrom; j0 < kto; j0 += BK) {
+        const bool in = threadIdx.x < BK && j0 + threadIdx.x < kto && kept(a, at.seq, j0 + threadIdx.x, len);
+        __syncthreads();
+        if (threadIdx.x < BK) ok[threadIdx.x] = in;
+        const bool any = __syncthreads_or(in);
+        float dk[RT][ND], dv[RT][ND];
+        clear(dk);
+        clear(dv);
+        if (any) {
+            stage_f32<DH, BK>(Ks, (const float*)a.k, [&](int r) { return k_ptr(a.k, a.sk, at, j0 + r, ok[r]); });
+            stage_f32<DH, BK>(Vs, (const float*)a.v, [&](int r) { return k_ptr(a.v, a.sv, at, j0 + r, ok[r]); });
+            cp_commit();
+            for (int q0 = qbeg; q0 < qend; q0 += BQ) {
+                if (!ROWS) {
+                    __syncthreads();
+                    stage_rows(q0);
+                    if (threadIdx.x < BQ) {
+                        const int r = q0 + threadIdx.x;
+                        s_lse[threadIdx.x] = lse_or_inf(a, row0 + r, r < qend);
+                        s_delta[threadIdx.x] = r < qend ? a.delta[row0 + r] : 0.f;
+                    }
+                }
+                cp_wait<0>();
+                __syncthreads();
+                float s[RT][NC], p[RT][NC];
+                mm_rows<RT, NC, DH>(s, Ks, Qs, ty, tx);
+                mm_rows<RT, NC, DH>(p, Vs, Gs, ty, tx);
+                #pragma unroll
+                for (int j = 0; j < NC; j++) {
+                    const int c = tx + 16 * j;
+                    const float x = s_lse[c], d = s_delta[c];
+                    float v[RT];
+                    #pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        v[i] = ok[row_of<RT>(ty, i)] ? __expf(fmaf(s[i][j], a.scale, -x)) : 0.f;
+                        p[i][j] = v[i] * (p[i][j] - d);
+                    }
+                    put_rows<RT>(Ps, LM, c, ty, v);
+                    #pragma unroll
+                    for (int i = 0; i < RT; i++) v[i] = p[i][j];
+                    if (ROWS) {
+                        #pragma unroll
+                        for (int i = 0; i < RT; i++) Ds[row_of<RT>(ty, i) * LQ + c] = v[i];
+                    } else {
+                        put_rows<RT>(Ds, LM, c, ty, v);
+                    }
+                }
+                __syncthreads();
+                mm_outer<RT, ND, BQ>(dv, Ps, LM, Gs, LD, ty, tx);
+                if constexpr (ROWS) {
+                    mm_outer<RT, ND, BK>(dq, Ds, LQ, Ks, LD, ty, tx);
+                    __syncthreads();
+                    #pragma unroll
+                    for (int j = 0; j < NC; j++) {
+                        float v[RT];
+                        #pragma unroll
+                        for (int i = 0; i < RT; i++) v[i] = p[i][j];
+                        put_rows<RT>(Ps, LM, tx + 16 * j, ty, v);
+                    }
+                    __syncthreads();
+                    mm_outer<RT, ND, BQ>(dk, Ps, LM, Qs, LD, ty, tx);
+                } else {
+                    mm_outer<RT, ND, BQ>(dk, Ds, LM, Qs, LD, ty, tx);
+                }
+            }
+            cp_wait<0>();
+        }
         #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            pk[tx * ND + d] = dk[i][d] * a.scale;
-            pv[tx * ND + d] = dv[i][d];
+        for (int i = 0; i < RT; i++) {
+            const int j = j0 + row_of<RT>(ty, i);
+            if (j >= kto) continue;
+            const bool parts = !ROWS && a.nsplit > 1;
+            const long part = ((((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part) * DH;
+            put_cols<ND>(parts ? a.part + part : (float*)a.dk + krow(a.sdk, at.seq, at.hk, j), tx, dk[i], a.scale);
+            put_cols<ND>(parts ? a.part2 + part : (float*)a.dv + krow(a.sdv, at.seq, at.hk, j), tx, dv[i], 1.f);
+        }
+    }
+    if constexpr (ROWS) {
+        #pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int r = row_of<RT>(ty, i);
+            if (r >= a.rows) continue;
+            put_cols<ND>(a.nsplit > 1 ? a.part + ((row0 + r) * a.nsplit + at.part) * DH
+                                      : (float*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), tx, dq[i], a.scale);
         }
     }
 }
@@ -1318,8 +1445,8 @@ BwdPlan bwd_plan(const PtcgCross& c) {
     BwdPlan p;
     const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
     p.few = rows <= 16;
-    p.rows = c.dtype == PTCG_BF16 && rows > 0 && rows <= 64;
-    p.bm = p.few && c.dtype == PTCG_FP32 ? 16 : 64;
+    p.rows = rows > 0 && rows <= 64;
+    p.bm = 64;
     p.qtiles = (rows + p.bm - 1) / p.bm;
     p.ktiles = (c.lk + 63) / 64;
     p.qs = split_of(p.qtiles * probs, c.lk);               // dq: split over keys
@@ -1354,8 +1481,8 @@ cudaError_t launch_fwd(const CrossArgs& a, long blocks, cudaStream_t s) {
 }
 template <int DH, int RT>
 cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
-    constexpr int LM = RT * 8 + 4, BN = F32<DH>::BN;
-    const int bytes = 4 * (DH * LM + DH * F32<DH>::LB + BN * DH + BN * LM);
+    constexpr int BM = RT * 8, BN = F32<DH>::BN;
+    const int bytes = 4 * ((BM + 2 * BN) * F32<DH>::LD + BN * (BM + 4));
     const cudaError_t e = smem_limit(k_cross_fwd_f32<DH, RT>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_fwd_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
@@ -1363,11 +1490,20 @@ cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
 }
 template <int DH, int RT>
 cudaError_t launch_dq_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
-    constexpr int LM = RT * 8 + 4, BN = F32<DH>::BN;
-    const int bytes = 4 * (2 * DH * LM + 2 * DH * F32<DH>::LB + BN * DH + BN * LM);
+    constexpr int BM = RT * 8, BN = F32<DH>::BN;
+    const int bytes = 4 * (2 * (BM + BN) * F32<DH>::LD + BN * (BM + 4));
     const cudaError_t e = smem_limit(k_cross_dq_f32<DH, RT>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_dq_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH, bool ROWS>
+cudaError_t launch_dkv_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
+    constexpr int BQ = ROWS ? 64 : F32<DH>::BN;
+    const int bytes = 4 * (2 * (64 + BQ) * F32<DH>::LD + 2 * BQ * 68);
+    const cudaError_t e = smem_limit(k_cross_dkv_f32<DH, ROWS>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dkv_f32<DH, ROWS><<<(unsigned)blocks, 128, bytes, s>>>(a);
     return cudaSuccess;
 }
 template <int DH>
@@ -1399,10 +1535,14 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
     const long probs = (long)c.nseq * c.kv_heads, nrows = probs * a.rows, nkeys = probs * a.lk;
     if (p.rows && p.qblocks) {
         set_tiles(a, 1, p.qs);
-        e = a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, p.qblocks, s)
+        e = !bf ? launch_dkv_f32<DH, true>(a, p.qblocks, s)
+            : a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, p.qblocks, s)
             : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, p.qblocks, s) : launch_bwd_rows<DH, 4>(a, p.qblocks, s);
-        if (e == cudaSuccess && p.qs.n > 1)
-            ++g_ptcg_launches, k_cross_sum<bf16, DH><<<cdiv(nrows * (DH / 4), 256), 256, 0, s>>>(a, nrows, 0);
+        if (e != cudaSuccess || p.qs.n == 1) return e;
+        ++g_ptcg_launches;
+        const unsigned grid = cdiv(nrows * (DH / 4), 256);
+        if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
+        else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
         return e;
     }
     if (p.qblocks) {
@@ -1413,8 +1553,7 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
             if ((e = smem_limit(k_cross_dq<DH>, bytes)) != cudaSuccess) return e;
             ++g_ptcg_launches, k_cross_dq<DH><<<(unsigned)p.qblocks, 128, bytes, s>>>(a);
         } else {
-            e = p.few ? launch_dq_f32<DH, 2>(a, p.qblocks, s) : launch_dq_f32<DH, 8>(a, p.qblocks, s);
-            if (e != cudaSuccess) return e;
+            if ((e = launch_dq_f32<DH, 8>(a, p.qblocks, s)) != cudaSuccess) return e;
         }
         if (p.qs.n > 1) {
             ++g_ptcg_launches;
@@ -1425,17 +1564,13 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream
     }
     if (p.kblocks) {
         set_tiles(a, p.ktiles, p.ks);
-        ++g_ptcg_launches;
         if (bf) {
             constexpr int BQ = DH == 128 ? 32 : 64;
             const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2;
             if ((e = smem_limit(k_cross_dkv<DH>, bytes)) != cudaSuccess) return e;
-            k_cross_dkv<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
-        } else {
-            constexpr int BQ = F32<DH>::BN, LB = F32<DH>::LB;
-            const int bytes = 4 * (2 * DH * 68 + 2 * DH * LB + 2 * BQ * DH + 2 * BQ * 68);
-            if ((e = smem_limit(k_cross_dkv_f32<DH>, bytes)) != cudaSuccess) return e;
-            k_cross_dkv_f32<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
+            ++g_ptcg_launches, k_cross_dkv<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
+        } else if ((e = launch_dkv_f32<DH, false>(a, p.kblocks, s)) != cudaSuccess) {
+            return e;
         }
         if (p.ks.n > 1) {
             ++g_ptcg_launches;
