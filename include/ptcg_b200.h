@@ -560,7 +560,8 @@ int ptcg_gemm_ex(int M, int N, int K, const void* A, long lda, int a_kmajor, con
 int ptcg_tensor_cores(void);
 /* First error code a bounded device-side wait recorded since the last call
  * (0 = none; the kernel that timed out returned early; 100 + code for the
- * tcgen05 attention, 200 + code for the fused rollout MLP).  Resets the flag. */
+ * tcgen05 attention, 200 + code for the fused rollout MLP, 300 + code for the
+ * tcgen05 cross attention).  Resets the flag. */
 int ptcg_device_error(void);
 
 /* Kernels of the bf16 attention (no counterpart in the reference, whose

@@ -20,7 +20,7 @@ FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxe
          "-I" + INCLUDE, "-I" + CSRC]
 SOURCES = ["model.cu", "gemm_simt.cu", "gemm_tc.cu", "attention.cu", "attention_tc.cu",
            "puffer_plugin.cu", "dp_nccl.cu", "mlp_tc.cu", "embedding.cu", "layer_norm.cu",
-           "cross_attention.cu"]
+           "cross_attention.cu", "cross_attention_tc.cu"]
 
 
 def _needs(obj, deps):

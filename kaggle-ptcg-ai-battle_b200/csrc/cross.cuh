@@ -1,0 +1,80 @@
+// What the cross-attention kernels share: the launch arguments, the addresses
+// of stacked query rows and key rows, the key masks and asynchronous copies.
+#pragma once
+#include "vec.cuh"
+
+namespace cross {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// n / d for 0 <= n < 2^31 as a multiply-high, an add and a shift: with
+// 2^(l-1) < d <= 2^l and mul = floor(2^32 (2^l - d) / d) + 1, the quotient is
+// (mulhi(n, mul) + n) >> l (the divisions by sizes known only at the launch
+// were a sixth of the short problems' instructions)
+struct FastDiv {
+    unsigned mul, shift, d;
+    PTCG_DEV unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+inline FastDiv fast_div(unsigned d) {
+    FastDiv f = {0, 0, d};
+    while ((1ull << f.shift) < d) f.shift++;
+    f.mul = (unsigned)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    return f;
+}
+
+struct CrossArgs {
+    const void *q, *k, *v, *o, *dout;
+    const uint8_t* keep;
+    const int* kv_len;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;
+    // split work: fp32 partial rows and, in the forward, their (max, sum)
+    float *part, *part2;
+    float2* part_ml;
+    PtcgHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    int nseq, lq, lk, heads, kv_heads, group, rows;      // rows = group * lq
+    int tiles, nsplit, split;                      // `split` rows of the split axis per part
+    FastDiv by_lq, by_tiles, by_nsplit, by_kv;
+    float scale;
+};
+
+// element offset of stacked row r of key head hk in a query-like tensor
+PTCG_DEV long qrow(const CrossArgs& a, const PtcgHeads& s, int seq, int hk, int r) {
+    const int g = a.by_lq.div(r);
+    return seq * s.seq + (r - g * a.lq) * s.row + (long)(hk * a.group + g) * s.head;
+}
+PTCG_DEV long krow(const PtcgHeads& s, int seq, int hk, int j) {
+    return seq * s.seq + j * s.row + hk * s.head;
+}
+PTCG_DEV int kept_len(const CrossArgs& a, int seq) {
+    return a.kv_len ? min(max(a.kv_len[seq], 0), a.lk) : a.lk;
+}
+PTCG_DEV bool kept(const CrossArgs& a, int seq, int j, int len) {
+    return j < len && (!a.keep || a.keep[(long)seq * a.lk + j] != 0);
+}
+// block index -> (tile of the problem, part of the split axis, key head, sequence)
+struct Where { int tile, part, hk, seq; };
+PTCG_DEV Where where(const CrossArgs& a) {
+    Where w;
+    const unsigned b = blockIdx.x, c = a.by_tiles.div(b), d = a.by_nsplit.div(c), e = a.by_kv.div(d);
+    w.tile = b - c * a.by_tiles.d;
+    w.part = c - d * a.by_nsplit.d;
+    w.hk = d - e * a.by_kv.d;
+    w.seq = e;
+    return w;
+}
+
+PTCG_DEV uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+PTCG_DEV void cp16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 :: "r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+PTCG_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> PTCG_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// tcgen05 kernels (cross_attention_tc.cu), bf16: the rows of a forward block
+constexpr int TC_ROWS = 256;
+// (*taken = false: K or V has strides that TMA does not address; nothing ran)
+cudaError_t fwd_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken);
+
+}  // namespace cross

@@ -14,71 +14,13 @@
 // they hold (NaN, infinities, rows never written) has no effect.
 #include <algorithm>
 
-#include "vec.cuh"
+#include "cross.cuh"
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-// n / d for 0 <= n < 2^31 as a multiply-high, an add and a shift: with
-// 2^(l-1) < d <= 2^l and mul = floor(2^32 (2^l - d) / d) + 1, the quotient is
-// (mulhi(n, mul) + n) >> l (the divisions by sizes known only at the launch
-// were a sixth of the short problems' instructions)
-struct FastDiv {
-    unsigned mul, shift, d;
-    PTCG_DEV unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-FastDiv fast_div(unsigned d) {
-    FastDiv f = {0, 0, d};
-    while ((1ull << f.shift) < d) f.shift++;
-    f.mul = (unsigned)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
-    return f;
-}
-
-struct CrossArgs {
-    const void *q, *k, *v, *o, *dout;
-    const uint8_t* keep;
-    const int* kv_len;
-    void *out, *dq, *dk, *dv;
-    float *lse, *delta;
-    // split work: fp32 partial rows and, in the forward, their (max, sum)
-    float *part, *part2;
-    float2* part_ml;
-    PtcgHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
-    int lq, lk, heads, kv_heads, group, rows;      // rows = group * lq
-    int tiles, nsplit, split;                      // `split` rows of the split axis per part
-    FastDiv by_lq, by_tiles, by_nsplit, by_kv;
-    float scale;
-};
-
-// element offset of stacked row r of key head hk in a query-like tensor
-PTCG_DEV long qrow(const CrossArgs& a, const PtcgHeads& s, int seq, int hk, int r) {
-    const int g = a.by_lq.div(r);
-    return seq * s.seq + (r - g * a.lq) * s.row + (long)(hk * a.group + g) * s.head;
-}
-PTCG_DEV long krow(const PtcgHeads& s, int seq, int hk, int j) {
-    return seq * s.seq + j * s.row + hk * s.head;
-}
-PTCG_DEV int kept_len(const CrossArgs& a, int seq) {
-    return a.kv_len ? min(max(a.kv_len[seq], 0), a.lk) : a.lk;
-}
-PTCG_DEV bool kept(const CrossArgs& a, int seq, int j, int len) {
-    return j < len && (!a.keep || a.keep[(long)seq * a.lk + j] != 0);
-}
-// block index -> (tile of the problem, part of the split axis, key head, sequence)
-struct Where { int tile, part, hk, seq; };
-PTCG_DEV Where where(const CrossArgs& a) {
-    Where w;
-    const unsigned b = blockIdx.x, c = a.by_tiles.div(b), d = a.by_nsplit.div(c), e = a.by_kv.div(d);
-    w.tile = b - c * a.by_tiles.d;
-    w.part = c - d * a.by_nsplit.d;
-    w.hk = d - e * a.by_kv.d;
-    w.seq = e;
-    return w;
-}
+using namespace cross;
 
 // ------------------------------------------------------- mma.sync pieces
-PTCG_DEV uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 PTCG_DEV void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
@@ -93,13 +35,6 @@ PTCG_DEV void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-PTCG_DEV void cp16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                 :: "r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-PTCG_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> PTCG_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
-
 // bf16 tiles of DH columns without padding: the 16-byte pieces of a row are
 // permuted by the row so that the eight rows an ldmatrix phase touches fall
 // into different banks (a 64-byte row shares its 128-byte line with its
@@ -1121,7 +1056,7 @@ template <int DH> PTCG_DEV float delta_f32(const CrossArgs& a, const Where& at, 
 }
 
 template <int DH, int RT>
-__global__ void __launch_bounds__(128) k_cross_fwd_f32(const __grid_constant__ CrossArgs a) {
+__global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_f32(const __grid_constant__ CrossArgs a) {
     constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LD = F32<DH>::LD, NC = BN / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
     __shared__ uint8_t ok[BN];
@@ -1207,7 +1142,7 @@ __global__ void __launch_bounds__(128) k_cross_fwd_f32(const __grid_constant__ C
 }
 
 template <int DH, int RT>
-__global__ void __launch_bounds__(128) k_cross_dq_f32(const __grid_constant__ CrossArgs a) {
+__global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dq_f32(const __grid_constant__ CrossArgs a) {
     constexpr int BM = RT * 8, LM = BM + 4, BN = F32<DH>::BN, LD = F32<DH>::LD, NC = BN / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
     __shared__ uint8_t ok[BN];
@@ -1281,7 +1216,7 @@ __global__ void __launch_bounds__(128) k_cross_dq_f32(const __grid_constant__ Cr
 // in one tile, and dq as well: each block then walks the key tiles and S is
 // computed once, as in k_cross_bwd_rows)
 template <int DH, bool ROWS>
-__global__ void __launch_bounds__(128) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
+__global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
     constexpr int RT = 8, BK = 64, LM = BK + 4, BQ = ROWS ? 64 : F32<DH>::BN, LQ = BQ + 4, LD = F32<DH>::LD;
     constexpr int NC = BQ / 16, ND = DH / 16;
     extern __shared__ __align__(16) float fs[];
@@ -1407,13 +1342,14 @@ __global__ void __launch_bounds__(128) k_cross_dkv_f32(const __grid_constant__ C
 }
 
 // ------------------------------------------------------------- host side
-// A problem whose tiles leave processors idle is split along its other axis:
-// about four blocks a processor, at least 256 rows of that axis to a part.
+// A problem whose tiles leave processors idle is split along its other axis,
+// at least 256 rows of it to a part: into about four blocks a processor, or
+// (tcgen05: one block fills a processor) as many as run at once.
 struct Split { int n, len; };
-Split split_of(long tiles, int axis) {
+Split split_of(long tiles, int axis, bool tc = false) {
     Split s = {1, axis > 0 ? axis : 1};
-    if (tiles >= 148 * 2 || axis <= 256 || tiles == 0) return s;
-    long want = (148 * 4 + tiles - 1) / tiles;
+    if (tiles >= (tc ? 75 : 148 * 2) || axis <= 256 || tiles == 0) return s;
+    long want = tc ? 148 / tiles : (148 * 4 + tiles - 1) / tiles;
     want = std::min(want, (long)(axis + 255) / 256);
     s.len = (int)((((axis + want - 1) / want) + 63) / 64 * 64);
     s.n = (int)cdiv(axis, s.len);
@@ -1426,14 +1362,26 @@ void set_tiles(CrossArgs& a, long tiles, const Split& s) {
     a.by_tiles = fast_div((unsigned)tiles);
     a.by_nsplit = fast_div(s.n);
 }
-struct FwdPlan { bool few; int bm; long tiles, blocks; Split sp; long o_ml, bytes; };
+// Which bf16 forwards run on tcgen05 (256-row blocks, one to a processor) and
+// which on mma.sync (64-row blocks, several to a processor).  Measured, us,
+// mma.sync / tcgen05: width 128: 4 x 4101 rows on 8191 keys 2260 / 508, 130 on
+// 257 153 / 94, 1024 on 100 109 / 68, but 130 on 64 54 / 57; width 64: 4 x 4101
+// on 8191 1410 / 450, 130 on 257 99 / 73; width 32, where a tile's products are
+// short and half-empty tiles cost most: 512 on 512 54 / 43, 256 on 256 30 / 29,
+// 130 on 257 47 / 63.
+bool use_tc(const PtcgCross& c, long rows) {
+    if (c.dtype != PTCG_BF16 || !gemm_tc_available()) return false;
+    return c.dh == 32 ? rows >= 384 && c.lk >= 256 : rows > 64 && c.lk > 64;
+}
+struct FwdPlan { bool few, tc; int bm; long tiles, blocks; Split sp; long o_ml, bytes; };
 FwdPlan fwd_plan(const PtcgCross& c) {
     FwdPlan p;
     const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
     p.few = rows <= 16;
-    p.bm = p.few ? 16 : 64;
+    p.tc = use_tc(c, rows);
+    p.bm = p.few ? 16 : p.tc ? TC_ROWS : 64;
     p.tiles = (rows + p.bm - 1) / p.bm;
-    p.sp = split_of(p.tiles * probs, c.lk);
+    p.sp = split_of(p.tiles * probs, c.lk, p.tc);
     p.blocks = p.tiles * probs * p.sp.n;
     const long parts = p.sp.n > 1 ? rows * probs * p.sp.n : 0;
     p.o_ml = (4 * parts * c.dh + 255) / 256 * 256;
@@ -1509,9 +1457,18 @@ cudaError_t launch_dkv_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
 template <int DH>
 cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream_t s) {
     cudaError_t e;
-    if (c.dtype == PTCG_BF16)
+    bool taken = false;
+    if (p.tc) {
+        e = fwd_tc(DH, a, p.blocks, s, &taken);
+        if (e != cudaSuccess) return e;
+    }
+    if (p.tc && !taken) {                          // the same parts, in 64-row tiles
+        const long tiles = (a.rows + 63) / 64;
+        set_tiles(a, tiles, p.sp);
+        e = launch_fwd<DH, 4, 1, 2>(a, tiles * c.nseq * c.kv_heads * p.sp.n, s);
+    } else if (!p.tc && c.dtype == PTCG_BF16)
         e = p.few ? launch_fwd<DH, 1, 4, 3>(a, p.blocks, s) : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
-    else
+    else if (!p.tc)
         e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
     if (e != cudaSuccess || p.sp.n == 1) return e;
     const long nrows = (long)c.nseq * c.kv_heads * a.rows;
@@ -1610,7 +1567,7 @@ CrossArgs args(const PtcgCross& c) {
     CrossArgs a = {};
     a.sq = c.q; a.sk = c.k; a.sv = c.v; a.so = c.out;
     a.sdo = c.dout; a.sdq = c.dq; a.sdk = c.dk; a.sdv = c.dv;
-    a.lq = c.lq; a.lk = c.lk; a.heads = c.heads; a.kv_heads = c.kv_heads;
+    a.nseq = c.nseq; a.lq = c.lq; a.lk = c.lk; a.heads = c.heads; a.kv_heads = c.kv_heads;
     a.group = c.heads / c.kv_heads;
     a.rows = a.group * c.lq;
     a.scale = c.scale;

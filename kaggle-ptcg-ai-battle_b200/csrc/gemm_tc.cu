@@ -911,6 +911,26 @@ bool gemm_tc_available() {
     return g_ok;
 }
 
+bool tc_make_map_4d(CUtensorMap* m, const void* ptr, const long (&dims)[4], const long (&strides)[3],
+                    int box_in, int box_rows, int swizzle_bytes) {
+    if (!gemm_tc_available()) return false;
+    cuuint64_t d[4], st[3];
+    for (int i = 0; i < 4; i++) {
+        if (dims[i] < 1 || dims[i] > 0xffffffffL) return false;
+        d[i] = (cuuint64_t)dims[i];
+    }
+    for (int i = 0; i < 3; i++) {
+        if (strides[i] < 1 || strides[i] * 2 >= 1L << 40 || strides[i] * 2 % 16) return false;
+        st[i] = (cuuint64_t)strides[i] * 2;
+    }
+    cuuint32_t box[4] = {(cuuint32_t)box_in, (cuuint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), d, st, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tc_make_map_2d(CUtensorMap* m, const void* ptr, int dtype, long inner, long outer, long ld,
                     int box_in, int box_out, int swizzle_bytes) {
     if (!gemm_tc_available()) return false;

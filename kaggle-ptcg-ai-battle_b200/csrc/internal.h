@@ -55,6 +55,10 @@ bool gemm_tc_available();
 // box_in x box_out, swizzle 0 / 32 / 64 / 128 bytes); false if unavailable
 bool tc_make_map_2d(CUtensorMap* m, const void* ptr, int dtype, long inner, long outer, long ld,
                     int box_in, int box_out, int swizzle_bytes);
+// 4-D map of bf16 (innermost contiguous, the outer strides in elements), box
+// {box_in, box_rows, 1, 1}, swizzle 64 or 128 bytes; false if not addressable
+bool tc_make_map_4d(CUtensorMap* m, const void* ptr, const long (&dims)[4], const long (&strides)[3],
+                    int box_in, int box_rows, int swizzle_bytes);
 int tc_num_sms();
 // first error code recorded by a tcgen05 kernel since the last call (0 = none)
 int ptcg_tc_error_read_reset();
@@ -140,3 +144,5 @@ bool mlp_fwd_tc(const void* a, long lda, const void* w1, long ldw1, const float*
                 const void* w2, long ldw2, const float* b2, const float* res, long ld_res,
                 float* out, long ld_out, int rows, int D, int F, cudaStream_t s);
 int mlp_tc_error_read_reset();
+// the same for the tcgen05 cross attention (cross_attention_tc.cu)
+int cross_tc_error_read_reset();

@@ -2510,8 +2510,8 @@ int ptcg_set_fused_mlp(int on) {
 
 int ptcg_device_error(void) {
     const int g = ptcg_tc_error_read_reset(), a = attn_tc_error_read_reset(),
-              m = mlp_tc_error_read_reset();
-    return g ? g : (a ? 100 + a : (m ? 200 + m : 0));
+              m = mlp_tc_error_read_reset(), c = cross_tc_error_read_reset();
+    return g ? g : (a ? 100 + a : (m ? 200 + m : (c ? 300 + c : 0)));
 }
 
 int ptcg_gemm(int M, int N, int K, const void* A, long lda, int a_kmajor, const void* B, long ldb,

@@ -285,6 +285,45 @@ def test_cross_attention(ops, dtype, mask, nseq, lq, lk, heads, kvh, dh):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+LONG = [  # the shapes of the long-problem kernels: nseq, lq, lk, heads, kv_heads, dh
+    (1, 65, 129, 1, 1, 64), (1, 128, 256, 2, 2, 128), (2, 300, 520, 2, 1, 128), (2, 400, 300, 2, 2, 32),
+    (1, 1100, 700, 2, 1, 64), (3, 70, 2000, 2, 2, 128), (2, 129, 385, 3, 1, 32), (1, 1500, 1025, 1, 1, 32),
+    (40, 80, 100, 4, 4, 64), (1, 257, 65, 1, 1, 128)]
+
+
+@pytest.mark.parametrize("mask", ["none", "keep", "len", "keep len"])
+@pytest.mark.parametrize("layout", ["rows", "heads", "packed"])
+@pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", LONG)
+def test_cross_attention_long(pkg, ops, mask, layout, nseq, lq, lk, heads, kvh, dh):
+    import ptcg_b200.native as n
+    q, k, v, m = problem(lq + lk, nseq, lq, lk, heads, kvh, dh, BF16, mask, layout)
+    dout, got = check_cross(ops, q, k, v, m)
+    assert n.lib().ptcg_device_error() == 0
+    for _ in range(3):
+        again = run_cross(ops, q, k, v, m)[1]
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    live = ref.live_keys(nseq, lk, m["keep"], m["kv_len"], "cuda")
+    if not live.all():                              # masked rows may hold anything
+        kj, vj = k.clone(), v.clone()
+        kj[~live] = math.nan
+        vj[~live] = math.nan
+        assert all(torch.equal(a, b) for a, b in zip(run_cross(ops, q, kj, vj, m)[1], got))
+    # one encoder's states for every sequence, and one key head's for all heads
+    check_cross(ops, q, k[:1].expand_as(k), v[:1].expand_as(v), m)
+    check_cross(ops, q, k[:, :, :1].expand_as(k), v[:, :, :1].expand_as(v), m)
+
+
+def test_cross_attention_long_growing_scores(ops):
+    """Maxima that rise by small and large steps along the keys: the shift of
+    a row lags behind its maximum by up to 2^8, then its output is rescaled."""
+    for dh in (32, 64, 128):
+        for top in (2.0, 14.0):
+            q, k, v, m = problem(29, 1, 400, 900, 1, 1, dh, BF16, "none")
+            k = k * torch.linspace(0.1, top, 900, device="cuda", dtype=BF16).view(1, 900, 1, 1)
+            check_cross(ops, q * 2, k, v, m)
+            check_cross(ops, q * 2, k.flip(1), v, m)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("layout", ["heads", "packed"])
 @pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", [(3, 40, 75, 4, 2, 32), (2, 1, 900, 4, 4, 64),
