@@ -510,7 +510,7 @@ int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, 
  *   lse[s, head, i] = log sum exp S (natural log).
  * Key j of sequence s is kept when j < kv_len[s] (int32 per sequence, clamped
  * to [0, lk]; NULL: lk) and keep[s * lk + j] != 0 (NULL: all).  Masked keys
- * are not read: they may hold anything.  A query row with no kept key gets
+ * have no effect whatever they hold, NaN included.  A query row with no kept key gets
  * out = 0, lse = -inf and takes no gradient.  Backward (out and lse from the
  * forward): dq, dk, dv; dk / dv are summed over a group's query heads and are
  * zero for masked keys.  Each tensor has its own strides in elements:

@@ -72,9 +72,13 @@ PTCG_DEV void cp16(uint32_t dst, const void* src, bool take) {
 PTCG_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> PTCG_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
-// tcgen05 kernels (cross_attention_tc.cu), bf16: the rows of a forward block
-constexpr int TC_ROWS = 256;
-// (*taken = false: K or V has strides that TMA does not address; nothing ran)
+// tcgen05 kernels (cross_attention_tc.cu), bf16, over `blocks` blocks: the
+// forward in tiles of 256 stacked rows, dq in tiles of 128 stacked rows (and
+// delta), dk and dv in tiles of 128 keys, whose split is in 64-row blocks of
+// one query head.  *taken = false: strides that TMA does not address; nothing ran
+constexpr int TC_ROWS = 256, TC_TILE = 128, TC_BLOCK = 64;
 cudaError_t fwd_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken);
+cudaError_t dq_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken);
+cudaError_t dkv_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken);
 
 }  // namespace cross

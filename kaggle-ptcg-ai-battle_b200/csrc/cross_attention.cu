@@ -1388,17 +1388,17 @@ FwdPlan fwd_plan(const PtcgCross& c) {
     p.bytes = p.sp.n > 1 ? p.o_ml + 8 * parts : 0;
     return p;
 }
-struct BwdPlan { bool few, rows; int bm; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
-BwdPlan bwd_plan(const PtcgCross& c) {
+struct BwdPlan { bool rows; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
+BwdPlan bwd_plan(const PtcgCross& c, bool tc) {
     BwdPlan p;
-    const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
-    p.few = rows <= 16;
+    const long group = c.heads / c.kv_heads, rows = group * c.lq, probs = (long)c.nseq * c.kv_heads;
+    const long tile = tc ? TC_TILE : 64;
     p.rows = rows > 0 && rows <= 64;
-    p.bm = 64;
-    p.qtiles = (rows + p.bm - 1) / p.bm;
-    p.ktiles = (c.lk + 63) / 64;
-    p.qs = split_of(p.qtiles * probs, c.lk);               // dq: split over keys
-    p.ks = split_of(p.ktiles * probs, (int)rows);          // dk, dv: split over rows
+    p.qtiles = (rows + tile - 1) / tile;
+    p.ktiles = (c.lk + tile - 1) / tile;
+    // dq: split over keys; dk and dv: over rows (tcgen05: in whole blocks of a head)
+    p.qs = split_of(p.qtiles * probs, c.lk, tc);
+    p.ks = split_of(p.ktiles * probs, (int)(tc ? group * cdiv(c.lq, TC_BLOCK) * TC_BLOCK : rows), tc);
     p.qblocks = p.qtiles * probs * p.qs.n;
     p.kblocks = p.ktiles * probs * p.ks.n;
     p.o_part = (4 * rows * probs + 255) / 256 * 256;       // delta first
@@ -1407,6 +1407,30 @@ BwdPlan bwd_plan(const PtcgCross& c) {
     p.o_part2 = p.o_part + k;
     p.bytes = p.o_part + std::max(q, 2 * k);               // one after the other
     return p;
+}
+// Which bf16 backwards run on tcgen05.  Measured, us, mma.sync / tcgen05 (rows
+// x keys).  dq, width 128: 4 x 4101 x 8191 2690 / 757, 256 x 256 126 / 98,
+// 130 x 257 194 / 175, but 130 x 70 101 / 140; width 64: 1354 / 549, but
+// 130 x 257 100 / 118; width 32: 776 / 470, 512 x 512 61 / 59, but 256 x 256
+// 37 / 45.  dk and dv, width 128: 3361 / 1068, 130 x 70 92 / 61; width 64:
+// 1620 / 820, 130 x 257 134 / 136, 130 x 70 55 / 45; width 32: 922 / 794,
+// 1024 x 100 40 / 33, but 512 x 512 68 / 69 and 256 x 256 40 / 46.
+bool use_tc_dq(const PtcgCross& c) {
+    if (c.dtype != PTCG_BF16 || !gemm_tc_available()) return false;
+    const long rows = (long)c.heads / c.kv_heads * c.lq;
+    return c.dh == 128 ? rows > 64 && c.lk >= 256
+           : c.dh == 64 ? rows > 64 && c.lk >= 384 : rows >= 384 && c.lk >= 512;
+}
+// dk and dv take their row blocks per query head: not where short heads would
+// leave them half empty
+bool use_tc_dkv(const PtcgCross& c) {
+    if (c.dtype != PTCG_BF16 || !gemm_tc_available()) return false;
+    const long rows = (long)c.heads / c.kv_heads * c.lq;
+    return 2L * cdiv(c.lq, TC_BLOCK) * TC_BLOCK <= 3L * c.lq && c.lk > 64 && rows > (c.dh == 32 ? 768 : 64);
+}
+long bwd_bytes(const PtcgCross& c) {
+    const long b = bwd_plan(c, false).bytes;
+    return use_tc_dq(c) || use_tc_dkv(c) ? std::max(b, bwd_plan(c, true).bytes) : b;
 }
 
 // kernels with more than 48 KB of shared memory, their static arrays (under
@@ -1434,6 +1458,24 @@ cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
     const cudaError_t e = smem_limit(k_cross_fwd_f32<DH, RT>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_fwd_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t launch_dq(const CrossArgs& a, long blocks, cudaStream_t s) {
+    constexpr int BN = DH == 128 ? 32 : 64;
+    const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2;
+    const cudaError_t e = smem_limit(k_cross_dq<DH>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dq<DH><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t launch_dkv(const CrossArgs& a, long blocks, cudaStream_t s) {
+    constexpr int BQ = DH == 128 ? 32 : 64;
+    const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2;
+    const cudaError_t e = smem_limit(k_cross_dkv<DH>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dkv<DH><<<(unsigned)blocks, 128, bytes, s>>>(a);
     return cudaSuccess;
 }
 template <int DH, int RT>
@@ -1486,55 +1528,61 @@ cudaError_t launch_bwd_rows(const CrossArgs& a, long blocks, cudaStream_t s) {
     return cudaSuccess;
 }
 template <int DH>
-cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, const BwdPlan& p, cudaStream_t s) {
+void sum_parts(const CrossArgs& a, bool bf, long nrows, int keys, cudaStream_t s) {
+    const unsigned grid = cdiv(nrows * (DH / 4), 256);
+    ++g_ptcg_launches;
+    if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nrows, keys);
+    else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nrows, keys);
+}
+template <int DH>
+cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, uint8_t* scratch, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
     const bool bf = c.dtype == PTCG_BF16;
     const long probs = (long)c.nseq * c.kv_heads, nrows = probs * a.rows, nkeys = probs * a.lk;
-    if (p.rows && p.qblocks) {
-        set_tiles(a, 1, p.qs);
-        e = !bf ? launch_dkv_f32<DH, true>(a, p.qblocks, s)
-            : a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, p.qblocks, s)
-            : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, p.qblocks, s) : launch_bwd_rows<DH, 4>(a, p.qblocks, s);
-        if (e != cudaSuccess || p.qs.n == 1) return e;
-        ++g_ptcg_launches;
-        const unsigned grid = cdiv(nrows * (DH / 4), 256);
-        if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
-        else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
+    const BwdPlan plain = bwd_plan(c, false);
+    auto parts = [&](const BwdPlan& p) {
+        a.part = (float*)(scratch + p.o_part);
+        a.part2 = (float*)(scratch + p.o_part2);
+    };
+    a.delta = (float*)scratch;
+    parts(plain);
+    if (plain.rows && plain.qblocks) {
+        set_tiles(a, 1, plain.qs);
+        e = !bf ? launch_dkv_f32<DH, true>(a, plain.qblocks, s)
+            : a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, plain.qblocks, s)
+            : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, plain.qblocks, s) : launch_bwd_rows<DH, 4>(a, plain.qblocks, s);
+        if (e == cudaSuccess && a.nsplit > 1) sum_parts<DH>(a, bf, nrows, 0, s);
         return e;
     }
-    if (p.qblocks) {
-        set_tiles(a, p.qtiles, p.qs);
-        if (bf) {
-            constexpr int BN = DH == 128 ? 32 : 64;
-            const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2;
-            if ((e = smem_limit(k_cross_dq<DH>, bytes)) != cudaSuccess) return e;
-            ++g_ptcg_launches, k_cross_dq<DH><<<(unsigned)p.qblocks, 128, bytes, s>>>(a);
-        } else {
-            if ((e = launch_dq_f32<DH, 8>(a, p.qblocks, s)) != cudaSuccess) return e;
+    const BwdPlan tc = bwd_plan(c, true);
+    if (plain.qblocks) {
+        bool taken = false;
+        if (use_tc_dq(c)) {
+            parts(tc);
+            set_tiles(a, tc.qtiles, tc.qs);
+            e = dq_tc(DH, a, tc.qblocks, s, &taken);
         }
-        if (p.qs.n > 1) {
-            ++g_ptcg_launches;
-            const unsigned grid = cdiv(nrows * (DH / 4), 256);
-            if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
-            else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nrows, 0);
+        if (e == cudaSuccess && !taken) {
+            parts(plain);
+            set_tiles(a, plain.qtiles, plain.qs);
+            e = bf ? launch_dq<DH>(a, plain.qblocks, s) : launch_dq_f32<DH, 8>(a, plain.qblocks, s);
         }
+        if (e != cudaSuccess) return e;
+        if (a.nsplit > 1) sum_parts<DH>(a, bf, nrows, 0, s);
     }
-    if (p.kblocks) {
-        set_tiles(a, p.ktiles, p.ks);
-        if (bf) {
-            constexpr int BQ = DH == 128 ? 32 : 64;
-            const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2;
-            if ((e = smem_limit(k_cross_dkv<DH>, bytes)) != cudaSuccess) return e;
-            ++g_ptcg_launches, k_cross_dkv<DH><<<(unsigned)p.kblocks, 128, bytes, s>>>(a);
-        } else if ((e = launch_dkv_f32<DH, false>(a, p.kblocks, s)) != cudaSuccess) {
-            return e;
+    if (plain.kblocks) {
+        bool taken = false;
+        if (use_tc_dkv(c)) {
+            parts(tc);
+            set_tiles(a, tc.ktiles, tc.ks);
+            e = dkv_tc(DH, a, tc.kblocks, s, &taken);
         }
-        if (p.ks.n > 1) {
-            ++g_ptcg_launches;
-            const unsigned grid = cdiv(nkeys * (DH / 4), 256);
-            if (bf) k_cross_sum<bf16, DH><<<grid, 256, 0, s>>>(a, nkeys, 1);
-            else k_cross_sum<float, DH><<<grid, 256, 0, s>>>(a, nkeys, 1);
+        if (e == cudaSuccess && !taken) {
+            parts(plain);
+            set_tiles(a, plain.ktiles, plain.ks);
+            e = bf ? launch_dkv<DH>(a, plain.kblocks, s) : launch_dkv_f32<DH, false>(a, plain.kblocks, s);
         }
+        if (e == cudaSuccess && a.nsplit > 1) sum_parts<DH>(a, bf, nkeys, 1, s);
     }
     return e;
 }
@@ -1611,7 +1659,7 @@ int ptcg_cross_attention_fwd(const PtcgCross* c, const void* q, const void* k, c
 }
 
 long ptcg_cross_attention_bwd_scratch(const PtcgCross* c) {
-    return check(c) ? -1 : bwd_plan(*c).bytes;
+    return check(c) ? -1 : bwd_bytes(*c);
 }
 
 int ptcg_cross_attention_bwd(const PtcgCross* c, const void* q, const void* k, const void* v,
@@ -1631,19 +1679,18 @@ int ptcg_cross_attention_bwd(const PtcgCross* c, const void* q, const void* k, c
     OP_REQ(apart(c->dq, c->nseq, c->lq, c->heads, c->dh) && apart(c->dk, c->nseq, c->lk, c->kv_heads, c->dh) &&
            apart(c->dv, c->nseq, c->lk, c->kv_heads, c->dh), PTCG_EINVAL,
            "cross attention gradient: rows of a gradient overlap");
-    const BwdPlan p = bwd_plan(*c);
-    OP_REQ(p.bytes == 0 || ((uintptr_t)scratch % 16 == 0 && scratch && scratch_bytes >= p.bytes), PTCG_ERANGE,
+    const BwdPlan p = bwd_plan(*c, false);
+    const long need = bwd_bytes(*c);
+    OP_REQ(need == 0 || ((uintptr_t)scratch % 16 == 0 && scratch && scratch_bytes >= need), PTCG_ERANGE,
            "cross attention gradient: scratch of %ld bytes, %ld needed (16-byte aligned)",
-           scratch ? scratch_bytes : 0L, p.bytes);
+           scratch ? scratch_bytes : 0L, need);
     OP_REQ(p.qblocks <= 0x7fffffffL && p.kblocks <= 0x7fffffffL, PTCG_EINVAL, "cross attention gradient: too many tiles");
     CrossArgs a = args(*c);
     a.q = q; a.k = k; a.v = v; a.keep = keep; a.kv_len = kv_len; a.o = out; a.lse = (float*)lse;
     a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
-    a.delta = (float*)scratch;
-    a.part = (float*)((uint8_t*)scratch + p.o_part);
-    a.part2 = (float*)((uint8_t*)scratch + p.o_part2);
+    uint8_t* base = (uint8_t*)scratch;
     cudaStream_t s = (cudaStream_t)stream;
-    OP_CK(c->dh == 32 ? bwd_dh<32>(a, *c, p, s) : c->dh == 64 ? bwd_dh<64>(a, *c, p, s) : bwd_dh<128>(a, *c, p, s));
+    OP_CK(c->dh == 32 ? bwd_dh<32>(a, *c, base, s) : c->dh == 64 ? bwd_dh<64>(a, *c, base, s) : bwd_dh<128>(a, *c, base, s));
     OP_CKL();
     return PTCG_OK;
 }

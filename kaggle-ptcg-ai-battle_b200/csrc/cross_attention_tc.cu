@@ -120,6 +120,17 @@ template <int W> struct KeyBits {
     }
 };
 
+// zeros in the rows of a tile whose bit is clear
+template <int DH, int N>
+PTCG_DEV void clear_rows(uint8_t* tile, const uint32_t (&w)[N / 32], int lane) {
+    #pragma unroll
+    for (int c = 0; c < N / 32; c++) {
+        if ((w[c] >> lane) & 1) continue;
+        #pragma unroll
+        for (int q = 0; q < DH / 8; q++)
+            *(uint4*)(tile + Tile<DH, N>::off(c * 32 + lane, q)) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
 // 128 stacked query rows from r0 by the 128 threads of a warpgroup; rows past
 // the end are zeros.  Returns when this thread's pieces are there
 template <int DH>
@@ -169,21 +180,21 @@ PTCG_DEV void tma_4d(uint32_t dst, const CUtensorMap* map, uint32_t b, int x, in
                  " [%0], [%1, {%3, %4, %5, %6}], [%2];"
                  :: "r"(dst), "l"((uint64_t)map), "r"(b), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// a tensor of key rows for TMA: dimensions (column, row, head, sequence); a
+// a tensor of rows for TMA: dimensions (column, row, head, sequence); a
 // dimension that the tensor repeats (stride 0) has one entry and coordinate 0
-struct KeyMap { CUtensorMap map; int heads, seqs; };
+struct RowMap { CUtensorMap map; int heads, seqs; };
+// rows row .. + N - 1 of one head into a tile; the barrier has been told the bytes
 template <int DH, int N>
-PTCG_DEV void load_keys(uint32_t dst, const KeyMap& m, uint32_t b, int row, const Where& at) {
+PTCG_DEV void load_rows(uint32_t dst, const RowMap& m, uint32_t b, int row, int head, int seq) {
     using T = Tile<DH, N>;
-    bar_expect_tx(b, T::BYTES);
     #pragma unroll
     for (int c = 0; c < DH * 2 / T::ROWB; c++)
-        tma_4d(dst + c * T::BLOCK, &m.map, b, c * (T::ROWB / 2), row, at.hk * m.heads, at.seq * m.seqs);
+        tma_4d(dst + c * T::BLOCK, &m.map, b, c * (T::ROWB / 2), row, head * m.heads, seq * m.seqs);
 }
 
 template <int DH>
 __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
-        const __grid_constant__ CrossArgs a, const __grid_constant__ KeyMap kmap, const __grid_constant__ KeyMap vmap) {
+        const __grid_constant__ CrossArgs a, const __grid_constant__ RowMap kmap, const __grid_constant__ RowMap vmap) {
     using F = Fwd<DH>;
     using T = Tile<DH, 128>;
     constexpr int NS = F::NS, KS = DH / 16, BN = 128;
@@ -233,9 +244,11 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
                 const int s = j % NS;
                 const uint32_t parity = (uint32_t)(((j / NS) & 1) ^ 1);
                 if (!wait_bar(kfree + 8 * s, parity, abort_flag, 1)) break;
-                load_keys<DH, BN>(sK + s * T::BYTES, kmap, kfull + 8 * s, kbeg + j * BN, at);
+                bar_expect_tx(kfull + 8 * s, T::BYTES);
+                load_rows<DH, BN>(sK + s * T::BYTES, kmap, kfull + 8 * s, kbeg + j * BN, at.hk, at.seq);
                 if (!wait_bar(vfree + 8 * s, parity, abort_flag, 2)) { j++; break; }
-                load_keys<DH, BN>(sV + s * T::BYTES, vmap, vfull + 8 * s, kbeg + j * BN, at);
+                bar_expect_tx(vfull + 8 * s, T::BYTES);
+                load_rows<DH, BN>(sV + s * T::BYTES, vmap, vfull + 8 * s, kbeg + j * BN, at.hk, at.seq);
             }
             // on an abort, let the copies still in flight land before exiting
             if (*abort_flag)
@@ -256,14 +269,7 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
             const int s = j % NS;
             if (!wait_warp(vfull + 8 * s, (j / NS) & 1, abort_flag, 3)) break;
             if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-                #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if ((w[c] >> lane) & 1) continue;
-                    uint8_t* row = smem + (2 + NS + s) * T::BYTES;
-                    #pragma unroll
-                    for (int q = 0; q < DH / 8; q++)        // all pieces: their order does not matter
-                        *(uint4*)(row + T::off(c * 32 + lane, q)) = make_uint4(0u, 0u, 0u, 0u);
-                }
+                clear_rows<DH, BN>(smem + (2 + NS + s) * T::BYTES, w, lane);
                 fence_async();
                 __syncwarp();
             }
@@ -448,27 +454,591 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
+// ----------------------------------------------------------------- backward
+// Two kernels, so that every gradient is written by one block in a fixed
+// order: dk and dv of a key tile over all rows, and dq of a row tile over all
+// keys (S and dP are computed in both: 7 products instead of 5, but no sums
+// across blocks).  In both, blocks of 64 of the walked axis alternate between
+// two TMEM buffers, each with its own warpgroup, so that one block's products
+// run while the other's probabilities are computed; P and dS go to TMEM as
+// bf16 over the scores and are the A operands of the products after them.
+// Warps 0-3 and 4-7 compute (a TMEM lane per thread), a lane of warp 8 loads
+// by TMA, warp 9 prepares, warp 10 issues the MMAs.
+// Bound: the tensor core; a block of 128 x 64 scores takes 1024 clocks of
+// products in the first kernel and 768 in the second, 512 of exponentials.
+constexpr int BB = 64;                       // rows or keys of a block
+constexpr int ONE_PER_SM = 120 * 1024;       // shared memory that keeps a second block off the processor
+
+// 64 fp32 values of this lane, 32 columns at a time
+PTCG_DEV void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+    tmem_ld32(taddr, v);
+    tmem_ld32(taddr + 32, v + 32);
+    tmem_wait_ld();
+}
+// x[i] y[i] as bf16, ANDed with `mask`, over 32 columns
+template <typename F>
+PTCG_DEV void tmem_put64(uint32_t taddr, uint32_t mask, F pair) {
+    #pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint32_t p[16];
+        #pragma unroll
+        for (int i = 0; i < 16; i++) p[i] = pair(32 * h + 2 * i) & mask;
+        tmem_st16(taddr + 16 * h, p);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+}
+// 32 columns of an accumulator row to a bf16 (or fp32 part) row, times f; rows
+// that are not `live` get zeros
+PTCG_DEV void write32(uint32_t taddr, float f, bool live, bool in, bf16* out, float* part) {
+    float o[32];
+    tmem_ld32(taddr, o);
+    tmem_wait_ld();
+    #pragma unroll
+    for (int i = 0; i < 32; i++) o[i] = live ? o[i] * f : 0.f;
+    if (!in) return;
+    if (part) {
+        #pragma unroll
+        for (int i = 0; i < 8; i++) ((float4*)part)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            ((uint4*)out)[i] = make_uint4(pack_bf2(o[8 * i], o[8 * i + 1]), pack_bf2(o[8 * i + 2], o[8 * i + 3]),
+                                          pack_bf2(o[8 * i + 4], o[8 * i + 5]), pack_bf2(o[8 * i + 6], o[8 * i + 7]));
+    }
+}
+// start and end of a block's life with TMEM; warp 10 allocates and frees
+PTCG_DEV void tmem_alloc(uint32_t* slot) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(s_addr(slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+PTCG_DEV void tmem_free(uint32_t tmem) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
+}
+
+// dk, dv of 128 keys (M, a TMEM lane each).  Row blocks are taken per query
+// head (TMA fills rows past lq with zeros; their log-sum-exp counts as +inf).
+//   S^T = K Q^T, dP^T = V dO^T (N = 64 rows);  dV += P^T dO, dK += dS^T Q
+// TMEM: buffer b: S^T at 128 b, dP^T at 128 b + 64; dV at 256, dK at 256 + DH.
+template <int DH> struct Dkv {
+    using T = Tile<DH, 128>;
+    using R = Tile<DH, BB>;
+    static constexpr int NS = DH == 128 ? 4 : DH == 64 ? 6 : 8;     // row stages (dout and q)
+    // barriers: kvfull full[NS] stat[NS] free[NS] sfull[2] dpfull[2] pready[2] dsready[2] ofull drain
+    static constexpr int BARS = 3 * NS + 11;
+    static constexpr int BYTES = 1024 + 2 * T::BYTES + 2 * NS * R::BYTES + NS * 2 * BB * 4 + BARS * 8 + 16;
+    static constexpr int SMEM = BYTES > ONE_PER_SM ? BYTES : ONE_PER_SM;
+    static constexpr int THREADS = 384;
+};
+
 template <int DH>
-bool key_map(KeyMap* m, const void* p, const PtcgHeads& s, const CrossArgs& a, int box_rows) {
+__global__ void __launch_bounds__(Dkv<DH>::THREADS, 1) k_cross_dkv_tc(
+        const __grid_constant__ CrossArgs a, const __grid_constant__ RowMap kmap,
+        const __grid_constant__ RowMap vmap, const __grid_constant__ RowMap qmap,
+        const __grid_constant__ RowMap gmap, FastDiv by_blocks) {
+    using F = Dkv<DH>;
+    using T = typename F::T;
+    using R = typename F::R;
+    constexpr int NS = F::NS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t sK = s_addr(smem), sV = sK + T::BYTES, sQ = sV + T::BYTES, sG = sQ + NS * R::BYTES;
+    float* stats = (float*)(smem + 2 * T::BYTES + 2 * NS * R::BYTES);  // [NS][-lse2 | -delta][64]
+    uint64_t* bars = (uint64_t*)(stats + NS * 2 * BB);
+    const uint32_t kvfull = s_addr(bars), full = kvfull + 8, stat = full + 8 * NS, free_ = stat + 8 * NS,
+                   sfull = free_ + 8 * NS, dpfull = sfull + 16, pready = dpfull + 16,
+                   dsready = pready + 16, ofull = dsready + 16, drain = ofull + 8;
+    uint32_t* tmem_slot = (uint32_t*)(bars + F::BARS);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Where at = where(a);
+    const int j0 = at.tile * 128, len = kept_len(a, at.seq);
+    // the row blocks of this part: block n is rows 64 (n % per head) .. of head n / per head
+    const int n0 = at.part * (a.split / BB), n1 = min((int)by_blocks.d * a.group, n0 + a.split / BB);
+    KeyBits<4> kb;
+    kb.fetch(a, at.seq, j0, a.lk, len, lane);
+    uint32_t w[4];
+    kb.words(w);
+    const int nb = (w[0] | w[1] | w[2] | w[3]) ? n1 - n0 : 0;           // nothing to add for masked keys
+    if (threadIdx.x == 0) {
+        bar_init(kvfull, 1);
+        for (int i = 0; i < NS; i++) { bar_init(full + 8 * i, 1); bar_init(stat + 8 * i, 1); bar_init(free_ + 8 * i, 1); }
+        for (int b = 0; b < 2; b++) {
+            bar_init(sfull + 8 * b, 1); bar_init(dpfull + 8 * b, 1);
+            bar_init(pready + 8 * b, 128); bar_init(dsready + 8 * b, 128);
+        }
+        bar_init(ofull, 1);
+        bar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async();
+    }
+    if (warp == 10) tmem_alloc(tmem_slot);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (warp == 8) {
+        // ------------------------------------------------- TMA lane
+        if (lane == 0 && nb > 0) {
+            bar_expect_tx(kvfull, 2 * T::BYTES);
+            load_rows<DH, 128>(sK, kmap, kvfull, j0, at.hk, at.seq);
+            load_rows<DH, 128>(sV, vmap, kvfull, j0, at.hk, at.seq);
+            int n = 0;
+            for (; n < nb; n++) {
+                const int s = n % NS, g = by_blocks.div(n0 + n), i0 = (n0 + n - g * by_blocks.d) * BB;
+                if (!wait_bar(free_ + 8 * s, (uint32_t)(((n / NS) & 1) ^ 1), abort_flag, 11)) break;
+                bar_expect_tx(full + 8 * s, 2 * R::BYTES);
+                load_rows<DH, BB>(sQ + s * R::BYTES, qmap, full + 8 * s, i0, at.hk * a.group + g, at.seq);
+                load_rows<DH, BB>(sG + s * R::BYTES, gmap, full + 8 * s, i0, at.hk * a.group + g, at.seq);
+            }
+            if (*abort_flag) {                       // copies still in flight land before the exit
+                bar_drain(kvfull, 0);
+                for (int i = max(0, n - NS); i < n; i++) bar_drain(full + 8 * (i % NS), (i / NS) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // -------------------------------- log-sum-exp and delta of each block
+        for (int n = 0; n < nb; n++) {
+            const int s = n % NS, g = by_blocks.div(n0 + n), i0 = (n0 + n - g * by_blocks.d) * BB;
+            const long base = ((long)at.seq * a.heads + at.hk * a.group + g) * a.lq;
+            float x[2], d[2];
+            #pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int i = i0 + 32 * e + lane;
+                const float v = i < a.lq ? a.lse[base + i] : -INFINITY;
+                x[e] = v == -INFINITY ? -INFINITY : -v * LOG2E;
+                d[e] = i < a.lq ? -a.delta[base + i] : 0.f;
+            }
+            if (!wait_warp(free_ + 8 * s, (uint32_t)(((n / NS) & 1) ^ 1), abort_flag, 12)) break;
+            #pragma unroll
+            for (int e = 0; e < 2; e++) {
+                stats[s * 2 * BB + 32 * e + lane] = x[e];
+                stats[s * 2 * BB + BB + 32 * e + lane] = d[e];
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(stat + 8 * s);
+        }
+    } else if (warp >= 10) {
+        // ---------------------------------------------------- MMA warp
+        if (warp == 10 && nb > 0) {
+            const uint32_t ids = idesc_bf16(BB, 0, 0), ido = idesc_bf16(DH, 0, 1);
+            const uint32_t klo = T::lo_k(sK), vlo = T::lo_k(sV);
+            const uint32_t qk = R::lo_k(sQ), gk = R::lo_k(sG), qm = R::lo_mn(sQ), gm = R::lo_mn(sG);
+            bool ok = wait_warp(kvfull, 0, abort_flag, 13);
+            int s_in = 0, s_out = 0;                 // stages of the next scores and of the next sums
+            uint32_t p_in = 0;
+            for (int n = -2; ok && n < nb; n++) {
+                const int b = n & 1;                 // buffer of blocks n and n + 2
+                const bool more = n + 2 < nb;
+                if (more) ok = wait_warp(full + 8 * s_in, p_in, abort_flag, 14);
+                const uint32_t off_in = (s_in * R::BYTES) >> 4, off_out = (s_out * R::BYTES) >> 4;
+                if (n >= 0) {
+                    ok = ok && wait_warp(pready + 8 * b, (n >> 1) & 1, abort_flag, 15);
+                    tc_fence_after();
+                    if (ok && elect_one()) {
+                        #pragma unroll
+                        for (int s = 0; s < BB / 16; s++)
+                            mma_bf16_ts(tmem + 256, tmem + 128 * b + 8 * s, R::mnmajor(gm + off_out, s), ido, s > 0 ? 1u : n > 0);
+                    }
+                    __syncwarp();
+                    ok = ok && wait_warp(dsready + 8 * b, (n >> 1) & 1, abort_flag, 16);
+                }
+                tc_fence_after();
+                if (ok && elect_one()) {
+                    if (n >= 0) {
+                        #pragma unroll
+                        for (int s = 0; s < BB / 16; s++)
+                            mma_bf16_ts(tmem + 256 + DH, tmem + 128 * b + 64 + 8 * s, R::mnmajor(qm + off_out, s), ido, s > 0 ? 1u : n > 0);
+                        mma_commit_to(free_ + 8 * s_out);
+                        if (n == nb - 1) mma_commit_to(ofull);
+                    }
+                    if (more) {
+                        #pragma unroll
+                        for (int s = 0; s < DH / 16; s++)
+                            mma_bf16(tmem + 128 * b, T::kmajor(klo, s), R::kmajor(qk + off_in, s), ids, s > 0);
+                        mma_commit_to(sfull + 8 * b);
+                        #pragma unroll
+                        for (int s = 0; s < DH / 16; s++)
+                            mma_bf16(tmem + 128 * b + 64, T::kmajor(vlo, s), R::kmajor(gk + off_in, s), ids, s > 0);
+                        mma_commit_to(dpfull + 8 * b);
+                    }
+                }
+                __syncwarp();
+                if (more && ++s_in == NS) { s_in = 0; p_in ^= 1; }
+                if (n >= 0 && ++s_out == NS) s_out = 0;
+            }
+            // no MMA may still be in flight when TMEM is released
+            if (elect_one()) {
+                mma_commit_to(drain);
+                bar_drain(drain, 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------ P^T and dS^T
+        const int b = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(quad * 32) << 16, tb = tmem + lane_off + 128 * b;
+        const bool live = ((quad < 2 ? (quad ? w[1] : w[0]) : (quad == 2 ? w[2] : w[3])) >> lane) & 1;
+        const uint32_t mask = live ? 0xffffffffu : 0u;
+        const unsigned long long sc2 = splat2(a.scale * LOG2E);
+        bool ok = true;
+        for (int n = b; ok && n < nb; n += 2) {
+            const uint32_t ph = (n >> 1) & 1;
+            const float* nl = stats + (n % NS) * 2 * BB;
+            const float* nd = nl + BB;
+            ok = wait_warp(stat + 8 * (n % NS), (n / NS) & 1, abort_flag, 17) && wait_warp(sfull + 8 * b, ph, abort_flag, 18);
+            if (!ok) break;
+            tc_fence_after();
+            float v[64];
+            tmem_ld64(tb, v);
+            #pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+                const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(nl + i);
+                upk2(fma2(pk2(v[i], v[i + 1]), sc2, l.x), v[i], v[i + 1]);
+                upk2(fma2(pk2(v[i + 2], v[i + 3]), sc2, l.y), v[i + 2], v[i + 3]);
+                #pragma unroll
+                for (int e = 0; e < 4; e++) v[i + e] = ex2_approx(v[i + e]);
+            }
+            tmem_put64(tb, mask, [&](int i) { return pack_bf2(v[i], v[i + 1]); });
+            bar_arrive(pready + 8 * b);
+            ok = wait_warp(dpfull + 8 * b, ph, abort_flag, 19);
+            if (!ok) break;
+            tc_fence_after();
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float d[32];
+                tmem_ld32(tb + 64 + 32 * h, d);
+                tmem_wait_ld();
+                #pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(nd + 32 * h + i);
+                    float* e = v + 32 * h + i;
+                    upk2(mul2(pk2(e[0], e[1]), add2(pk2(d[i], d[i + 1]), x.x)), e[0], e[1]);
+                    upk2(mul2(pk2(e[2], e[3]), add2(pk2(d[i + 2], d[i + 3]), x.y)), e[2], e[3]);
+                }
+            }
+            tmem_put64(tb + 64, mask, [&](int i) { return pack_bf2(v[i], v[i + 1]); });
+            bar_arrive(dsready + 8 * b);
+        }
+        if (ok && nb > 0) ok = wait_warp(ofull, 0, abort_flag, 20);
+        if (ok) {
+            tc_fence_after();
+            // warpgroup 0 writes dv, warpgroup 1 dk
+            const int j = j0 + row;
+            const bool in = j < a.lk;
+            const long prow = (((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part;
+            const long orow = in ? krow(b ? a.sdk : a.sdv, at.seq, at.hk, j) : 0;
+            bf16* out = (bf16*)(b ? a.dk : a.dv) + orow;
+            float* part = a.nsplit > 1 ? (b ? a.part : a.part2) + prow * DH : nullptr;
+            #pragma unroll
+            for (int c = 0; c < DH / 32; c++)
+                write32(tmem + lane_off + 256 + b * DH + 32 * c, b ? a.scale : 1.f, live && nb > 0, in,
+                        out + 32 * c, part ? part + 32 * c : nullptr);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 10) tmem_free(tmem);
+}
+
+// dq of 128 stacked rows (M, a TMEM lane each), which hold q and dout in TMEM:
+//   S = Q K^T, dP = dO V^T (A from TMEM, N = 64 keys);  dQ += dS K
+// also delta = dout . out, for the kernel above.  K rows of masked keys are
+// zeroed in shared memory (dS = 0 there, but 0 * NaN is NaN).
+// TMEM: dQ at 0, buffer b: S at 128 + 128 b, dP 64 on; q at 384, dout at 448.
+template <int DH> struct Dq {
+    using R = Tile<DH, BB>;
+    static constexpr int NS = DH == 128 ? 5 : 8;                    // key stages (K and V)
+    // barriers: qfull kfull[NS] kready[NS] vfull[NS] free[NS] sfull[2] dpfull[2] dsready[2] ofull drain
+    static constexpr int BARS = 4 * NS + 9;
+    static constexpr int BYTES = 1024 + 2 * NS * R::BYTES + 2 * 128 * 4 + BARS * 8 + 16;
+    static constexpr int SMEM = BYTES > ONE_PER_SM ? BYTES : ONE_PER_SM;
+    static constexpr int THREADS = 384;
+};
+
+template <int DH>
+__global__ void __launch_bounds__(Dq<DH>::THREADS, 1) k_cross_dq_tc(
+        const __grid_constant__ CrossArgs a, const __grid_constant__ RowMap kmap,
+        const __grid_constant__ RowMap vmap) {
+    using F = Dq<DH>;
+    using R = typename F::R;
+    constexpr int NS = F::NS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t sK = s_addr(smem), sV = sK + NS * R::BYTES;
+    float* s_lse = (float*)(smem + 2 * NS * R::BYTES);               // [128] -lse2, [128] -delta
+    float* s_delta = s_lse + 128;
+    uint64_t* bars = (uint64_t*)(s_delta + 128);
+    const uint32_t qfull = s_addr(bars), kfull = qfull + 8, kready = kfull + 8 * NS, vfull = kready + 8 * NS,
+                   free_ = vfull + 8 * NS, sfull = free_ + 8 * NS, dpfull = sfull + 16,
+                   dsready = dpfull + 16, ofull = dsready + 16, drain = ofull + 8;
+    uint32_t* tmem_slot = (uint32_t*)(bars + F::BARS);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Where at = where(a);
+    const int r0 = at.tile * 128, len = kept_len(a, at.seq);
+    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    const int nb = (kend - kbeg + BB - 1) / BB;
+    if (threadIdx.x == 0) {
+        bar_init(qfull, 256);
+        for (int i = 0; i < NS; i++) {
+            bar_init(kfull + 8 * i, 1); bar_init(kready + 8 * i, 1);
+            bar_init(vfull + 8 * i, 1); bar_init(free_ + 8 * i, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            bar_init(sfull + 8 * b, 1); bar_init(dpfull + 8 * b, 1); bar_init(dsready + 8 * b, 128);
+        }
+        bar_init(ofull, 1);
+        bar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async();
+    }
+    if (warp == 10) tmem_alloc(tmem_slot);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (warp == 8) {
+        // ------------------------------------------------- TMA lane
+        if (lane == 0) {
+            int n = 0;
+            for (; n < nb; n++) {
+                const int s = n % NS;
+                if (!wait_bar(free_ + 8 * s, (uint32_t)(((n / NS) & 1) ^ 1), abort_flag, 31)) break;
+                bar_expect_tx(kfull + 8 * s, R::BYTES);
+                load_rows<DH, BB>(sK + s * R::BYTES, kmap, kfull + 8 * s, kbeg + n * BB, at.hk, at.seq);
+                bar_expect_tx(vfull + 8 * s, R::BYTES);
+                load_rows<DH, BB>(sV + s * R::BYTES, vmap, vfull + 8 * s, kbeg + n * BB, at.hk, at.seq);
+            }
+            if (*abort_flag)                         // copies still in flight land before the exit
+                for (int i = max(0, n - NS); i < n; i++) {
+                    bar_drain(kfull + 8 * (i % NS), (i / NS) & 1);
+                    bar_drain(vfull + 8 * (i % NS), (i / NS) & 1);
+                }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ------------------------------------ masked rows of K become zeros
+        KeyBits<2> kb;
+        kb.fetch(a, at.seq, kbeg, kend, len, lane);
+        for (int n = 0; n < nb; n++) {
+            uint32_t w[2];
+            kb.words(w);
+            kb.fetch(a, at.seq, kbeg + (n + 1) * BB, kend, len, lane);
+            const int s = n % NS;
+            if (!wait_warp(kfull + 8 * s, (n / NS) & 1, abort_flag, 32)) break;
+            if ((w[0] & w[1]) != 0xffffffffu) {
+                clear_rows<DH, BB>(smem + s * R::BYTES, w, lane);
+                fence_async();
+                __syncwarp();
+            }
+            if (lane == 0) bar_arrive(kready + 8 * s);
+        }
+    } else if (warp >= 10) {
+        // ---------------------------------------------------- MMA warp
+        if (warp == 10 && nb > 0) {
+            const uint32_t ids = idesc_bf16(BB, 0, 0), ido = idesc_bf16(DH, 0, 1);
+            const uint32_t kk = R::lo_k(sK), vk = R::lo_k(sV), km = R::lo_mn(sK);
+            bool ok = wait_warp(qfull, 0, abort_flag, 33);
+            int s_in = 0, s_out = 0;
+            uint32_t p_in = 0;
+            for (int n = -2; ok && n < nb; n++) {
+                const int b = n & 1;
+                const bool more = n + 2 < nb;
+                if (more) ok = wait_warp(kready + 8 * s_in, p_in, abort_flag, 34) && wait_warp(vfull + 8 * s_in, p_in, abort_flag, 35);
+                const uint32_t off_in = (s_in * R::BYTES) >> 4, off_out = (s_out * R::BYTES) >> 4;
+                const uint32_t tb = tmem + 128 + 128 * b;
+                if (n >= 0) ok = ok && wait_warp(dsready + 8 * b, (n >> 1) & 1, abort_flag, 36);
+                tc_fence_after();
+                if (ok && elect_one()) {
+                    if (n >= 0) {
+                        #pragma unroll
+                        for (int s = 0; s < BB / 16; s++)
+                            mma_bf16_ts(tmem, tb + 8 * s, R::mnmajor(km + off_out, s), ido, s > 0 ? 1u : n > 0);
+                        mma_commit_to(free_ + 8 * s_out);
+                        if (n == nb - 1) mma_commit_to(ofull);
+                    }
+                    if (more) {
+                        #pragma unroll
+                        for (int s = 0; s < DH / 16; s++)
+                            mma_bf16_ts(tb, tmem + 384 + 8 * s, R::kmajor(kk + off_in, s), ids, s > 0);
+                        mma_commit_to(sfull + 8 * b);
+                        #pragma unroll
+                        for (int s = 0; s < DH / 16; s++)
+                            mma_bf16_ts(tb + 64, tmem + 448 + 8 * s, R::kmajor(vk + off_in, s), ids, s > 0);
+                        mma_commit_to(dpfull + 8 * b);
+                    }
+                }
+                __syncwarp();
+                if (more && ++s_in == NS) { s_in = 0; p_in ^= 1; }
+                if (n >= 0 && ++s_out == NS) s_out = 0;
+            }
+            if (elect_one()) {
+                mma_commit_to(drain);
+                bar_drain(drain, 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------------------ dS
+        const int b = warp >> 2, quad = warp & 3, row = quad * 32 + lane, r = r0 + row;
+        const uint32_t lane_off = (uint32_t)(quad * 32) << 16, tb = tmem + lane_off + 128 + 128 * b;
+        const bool in = r < a.rows;
+        const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows + r;
+        {   // warpgroup 0 brings q to TMEM, warpgroup 1 dout, and both make the row's numbers
+            const uint4* src = (const uint4*)((const bf16*)(b ? a.dout : a.q) + (in ? qrow(a, b ? a.sdo : a.sq, at.seq, at.hk, r) : 0));
+            const uint4* og = (const uint4*)((const bf16*)a.o + (in ? qrow(a, a.so, at.seq, at.hk, r) : 0));
+            float d = 0.f;
+            #pragma unroll
+            for (int c = 0; c < DH / 32; c++) {
+                uint32_t p[16];
+                #pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint4 x = in ? src[4 * c + q] : make_uint4(0u, 0u, 0u, 0u);
+                    p[4 * q] = x.x; p[4 * q + 1] = x.y; p[4 * q + 2] = x.z; p[4 * q + 3] = x.w;
+                    if (b == 1 && in) {
+                        const uint4 y = og[4 * c + q];
+                        const uint32_t u[4] = {y.x, y.y, y.z, y.w};
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float x0, x1, y0, y1;
+                            unpack_bf2(p[4 * q + e], x0, x1);
+                            unpack_bf2(u[e], y0, y1);
+                            d = fmaf(x0, y0, fmaf(x1, y1, d));
+                        }
+                    }
+                }
+                tmem_st16(tmem + lane_off + (b ? 448 : 384) + 16 * c, p);
+            }
+            if (b == 1) {
+                s_delta[row] = -d;
+                if (in && at.part == 0) a.delta[row0] = d;
+            } else {
+                const float x = in ? a.lse[row0] : -INFINITY;
+                s_lse[row] = x == -INFINITY ? -INFINITY : -x * LOG2E;
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            bar_arrive(qfull);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        const unsigned long long sc2 = splat2(a.scale * LOG2E), nl2 = splat2(s_lse[row]), nd2 = splat2(s_delta[row]);
+        bool ok = true;
+        KeyBits<2> kb;
+        kb.fetch(a, at.seq, kbeg + b * BB, kend, len, lane);
+        for (int n = b; ok && n < nb; n += 2) {
+            const uint32_t ph = (n >> 1) & 1;
+            uint32_t w[2];
+            kb.words(w);
+            kb.fetch(a, at.seq, kbeg + (n + 2) * BB, kend, len, lane);
+            ok = wait_warp(sfull + 8 * b, ph, abort_flag, 37);
+            if (!ok) break;
+            tc_fence_after();
+            float v[64];
+            tmem_ld64(tb, v);
+            #pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+                upk2(fma2(pk2(v[i], v[i + 1]), sc2, nl2), v[i], v[i + 1]);
+                v[i] = ex2_approx(v[i]);
+                v[i + 1] = ex2_approx(v[i + 1]);
+            }
+            ok = wait_warp(dpfull + 8 * b, ph, abort_flag, 38);
+            if (!ok) break;
+            tc_fence_after();
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float d[32];
+                tmem_ld32(tb + 64 + 32 * h, d);
+                tmem_wait_ld();
+                #pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float* e = v + 32 * h + i;
+                    upk2(mul2(pk2(e[0], e[1]), add2(pk2(d[i], d[i + 1]), nd2)), e[0], e[1]);
+                }
+                if (w[h] != 0xffffffffu) {
+                    #pragma unroll
+                    for (int i = 0; i < 32; i++) if (!((w[h] >> i) & 1)) v[32 * h + i] = 0.f;
+                }
+            }
+            tmem_put64(tb, 0xffffffffu, [&](int i) { return pack_bf2(v[i], v[i + 1]); });
+            bar_arrive(dsready + 8 * b);
+        }
+        if (ok && nb > 0) ok = wait_warp(ofull, 0, abort_flag, 39);
+        if (ok) {
+            tc_fence_after();
+            // 32-column pieces of dq, in turn to the two warpgroups
+            bf16* out = (bf16*)a.dq + (in ? qrow(a, a.sdq, at.seq, at.hk, r) : 0);
+            float* part = a.nsplit > 1 ? a.part + (row0 * a.nsplit + at.part) * DH : nullptr;
+            #pragma unroll
+            for (int c = 0; c < DH / 32; c++)
+                if ((c & 1) == b)
+                    write32(tmem + lane_off + 32 * c, a.scale, nb > 0, in, out + 32 * c, part ? part + 32 * c : nullptr);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 10) tmem_free(tmem);
+}
+
+// ------------------------------------------------------------------- host
+// the map of a tensor with `rows` rows and `heads` heads, or false
+template <int DH>
+bool row_map(RowMap* m, const void* p, const PtcgHeads& s, long rows, int heads, int nseq, int box_rows) {
     m->seqs = s.seq != 0;
     m->heads = s.head != 0;
-    const long dims[4] = {DH, a.lk, m->heads ? a.kv_heads : 1, m->seqs ? a.nseq : 1};
+    const long dims[4] = {DH, rows, m->heads ? heads : 1, m->seqs ? nseq : 1};
     // a dimension of one entry may have any stride
-    const long strides[3] = {a.lk > 1 ? s.row : DH, dims[2] > 1 ? s.head : DH, dims[3] > 1 ? s.seq : DH};
+    const long strides[3] = {rows > 1 ? s.row : DH, dims[2] > 1 ? s.head : DH, dims[3] > 1 ? s.seq : DH};
     for (long x : strides)
         if (x <= 0) return false;
     const int rowb = Tile<DH, 128>::ROWB;
     return tc_make_map_4d(&m->map, p, dims, strides, rowb / 2, box_rows, rowb);
 }
+template <typename F>
+cudaError_t smem_limit(F f, int bytes) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
 
 template <int DH>
-cudaError_t launch(const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) {
-    KeyMap km, vm;
-    *taken = key_map<DH>(&km, a.k, a.sk, a, 128) && key_map<DH>(&vm, a.v, a.sv, a, 128);
+cudaError_t launch_fwd(const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) {
+    RowMap km, vm;
+    *taken = row_map<DH>(&km, a.k, a.sk, a.lk, a.kv_heads, a.nseq, 128) &&
+             row_map<DH>(&vm, a.v, a.sv, a.lk, a.kv_heads, a.nseq, 128);
     if (!*taken) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(k_cross_fwd_tc<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fwd<DH>::SMEM);
+    const cudaError_t e = smem_limit(k_cross_fwd_tc<DH>, Fwd<DH>::SMEM);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_fwd_tc<DH><<<(unsigned)blocks, Fwd<DH>::THREADS, Fwd<DH>::SMEM, s>>>(a, km, vm);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t launch_dq(const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) {
+    RowMap km, vm;
+    *taken = row_map<DH>(&km, a.k, a.sk, a.lk, a.kv_heads, a.nseq, BB) &&
+             row_map<DH>(&vm, a.v, a.sv, a.lk, a.kv_heads, a.nseq, BB);
+    if (!*taken) return cudaSuccess;
+    const cudaError_t e = smem_limit(k_cross_dq_tc<DH>, Dq<DH>::SMEM);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dq_tc<DH><<<(unsigned)blocks, Dq<DH>::THREADS, Dq<DH>::SMEM, s>>>(a, km, vm);
+    return cudaSuccess;
+}
+template <int DH>
+cudaError_t launch_dkv(const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) {
+    RowMap km, vm, qm, gm;
+    *taken = row_map<DH>(&km, a.k, a.sk, a.lk, a.kv_heads, a.nseq, 128) &&
+             row_map<DH>(&vm, a.v, a.sv, a.lk, a.kv_heads, a.nseq, 128) &&
+             row_map<DH>(&qm, a.q, a.sq, a.lq, a.heads, a.nseq, BB) &&
+             row_map<DH>(&gm, a.dout, a.sdo, a.lq, a.heads, a.nseq, BB);
+    if (!*taken) return cudaSuccess;
+    const cudaError_t e = smem_limit(k_cross_dkv_tc<DH>, Dkv<DH>::SMEM);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_dkv_tc<DH><<<(unsigned)blocks, Dkv<DH>::THREADS, Dkv<DH>::SMEM, s>>>(
+        a, km, vm, qm, gm, fast_div((a.lq + BB - 1) / BB));
     return cudaSuccess;
 }
 
@@ -476,10 +1046,11 @@ cudaError_t launch(const CrossArgs& a, long blocks, cudaStream_t s, bool* taken)
 
 namespace cross {
 
-cudaError_t fwd_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) {
-    return dh == 32 ? launch<32>(a, blocks, s, taken)
-           : dh == 64 ? launch<64>(a, blocks, s, taken) : launch<128>(a, blocks, s, taken);
-}
+#define BY_DH(F) (dh == 32 ? F<32>(a, blocks, s, taken) : dh == 64 ? F<64>(a, blocks, s, taken) : F<128>(a, blocks, s, taken))
+cudaError_t fwd_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) { return BY_DH(launch_fwd); }
+cudaError_t dq_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) { return BY_DH(launch_dq); }
+cudaError_t dkv_tc(int dh, const CrossArgs& a, long blocks, cudaStream_t s, bool* taken) { return BY_DH(launch_dkv); }
+#undef BY_DH
 
 }  // namespace cross
 
