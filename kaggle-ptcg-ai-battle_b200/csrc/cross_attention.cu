@@ -43,20 +43,22 @@ template <int DH> PTCG_DEV uint32_t tile_off(int row, int piece) {
     const int x = DH == 32 ? (row >> 1) & 3 : row & 7;
     return (uint32_t)(row * DH * 2 + ((piece ^ x) << 4));
 }
-// A fragment of rows r0 .. +15, columns 16 ks ..
-template <int DH> PTCG_DEV void frag_a(uint32_t (&f)[4], uint32_t base, int r0, int ks, int lane) {
-    const int mi = lane >> 3;
-    ldsm4(f, base + tile_off<DH>(r0 + (mi & 1) * 8 + (lane & 7), ks * 2 + (mi >> 1)));
+// This lane's part of an ldmatrix address: for A fragments of rows r0 .. +15 and
+// for B fragments of B[k][n] = X[k][n] (rows k0 .. +15), or for B fragments of
+// B[k][n] = X[n][k] (rows n0 .. +15).  Added to a tile's address (a multiple of
+// 256 bytes), the 16-column step ks is an exclusive or of the piece bits and the
+// row step a constant, so one address serves all fragments of a tile.
+template <int DH> PTCG_DEV uint32_t lane_rows(int lane) {
+    return tile_off<DH>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
 }
-// B fragments of B[k][n] = X[n][k]: rows n0 .. +15 of X, columns 16 ks ..
-template <int DH> PTCG_DEV void frag_bn(uint32_t (&f)[4], uint32_t base, int n0, int ks, int lane) {
-    const int mi = lane >> 3;
-    ldsm4(f, base + tile_off<DH>(n0 + (mi >> 1) * 8 + (lane & 7), ks * 2 + (mi & 1)));
+template <int DH> PTCG_DEV uint32_t lane_cols(int lane) {
+    return tile_off<DH>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
 }
-// B fragments of B[k][n] = X[k][n]: rows k0 .. +15 of X, columns 16 nd ..
-template <int DH> PTCG_DEV void frag_bk(uint32_t (&f)[4], uint32_t base, int k0, int nd, int lane) {
-    const int mi = lane >> 3;
-    ldsm4t(f, base + tile_off<DH>(k0 + (mi & 1) * 8 + (lane & 7), nd * 2 + (mi >> 1)));
+template <int DH> PTCG_DEV void frag(uint32_t (&f)[4], uint32_t at, int r0, int ks) {
+    ldsm4(f, (at ^ (uint32_t)(ks * 32)) + r0 * DH * 2);
+}
+template <int DH> PTCG_DEV void frag_t(uint32_t (&f)[4], uint32_t at, int r0, int ks) {
+    ldsm4t(f, (at ^ (uint32_t)(ks * 32)) + r0 * DH * 2);
 }
 // Staging: a thread takes piece tid % P of rows tid / P, + THREADS / P, ..; that
 // step is a multiple of 8 rows, so the permutation, and with it the offset in
@@ -113,14 +115,18 @@ PTCG_DEV float quad_sum(float v) {
 // rounding).  WN = 4 is the form for at most 16 rows (single tokens): the four
 // warps take 16 keys each of every tile and are joined at the end.
 template <int DH, int WM, int WN, int NST>
-__global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_cross_fwd(const __grid_constant__ CrossArgs a) {
+__global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 5 : 1) k_cross_fwd(const __grid_constant__ CrossArgs a) {
     constexpr int THREADS = WM * WN * 32, BM = WM * 16, BN = 64, KW = BN / WN, NT = KW / 8;
     constexpr int KS = DH / 16, TILE = BN * DH * 2;
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
     __shared__ uint32_t bits[NST + 1][2];
+    // 0 for a kept key, -inf for a masked one: where the scores start from
+    __shared__ __align__(8) float bias[NST + 1][BN];
     const uint32_t sQ = s_addr(sm), sK = sQ + BM * DH * 2, sV = sK + NST * TILE;
     const Where at = where(a);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
     const int wm = WN == 1 ? warp : 0, wn = WN == 1 ? 0 : warp;
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
     const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
@@ -133,7 +139,10 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_c
     };
     auto put_bits = [&](int j, bool b) {
         const uint32_t m = __ballot_sync(0xffffffffu, b);
-        if (warp < 2 && lane == 0) bits[j % (NST + 1)][warp] = m;
+        if (warp < 2) {
+            bias[j % (NST + 1)][warp * 32 + lane] = b ? 0.f : -INFINITY;
+            if (lane == 0) bits[j % (NST + 1)][warp] = m;
+        }
     };
     auto load = [&](int j) {
         if (j < nt) {
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_c
         load(j + NST - 1);
         if (j == 0) {
             #pragma unroll
-            for (int ks = 0; ks < KS; ks++) frag_a<DH>(qf[ks], sQ, wm * 16, ks, lane);
+            for (int ks = 0; ks < KS; ks++) frag<DH>(qf[ks], sQ + fr, wm * 16, ks);
         }
         const uint32_t w0 = bits[j % (NST + 1)][0], w1 = bits[j % (NST + 1)][1];
         // this warp's keys: all 64, or its 16
@@ -173,27 +182,24 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_c
         if ((v0 | v1) && mine) {
             const uint32_t kt = sK + (j % NST) * TILE, vt = sV + (j % NST) * TILE;
             // 16 keys at a time; groups that are masked whole are skipped
+            const float* bj = bias[j % (NST + 1)] + wn * KW + 2 * t;
             auto group = [&](int i) { return ((i < 2 ? v0 : v1) >> ((i & 1) * 16)) & 0xffffu; };
             float s[NT][4];
             #pragma unroll
             for (int i = 0; i < NT / 2; i++) {
                 #pragma unroll
-                for (int e = 0; e < 4; e++) s[2 * i][e] = s[2 * i + 1][e] = 0.f;
+                for (int n = 2 * i; n < 2 * i + 2; n++) {
+                    const float2 b = *(const float2*)(bj + n * 8);
+                    s[n][0] = s[n][2] = b.x;
+                    s[n][1] = s[n][3] = b.y;
+                }
                 if (!group(i)) continue;
                 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t b[4];
-                    frag_bn<DH>(b, kt, wn * KW + i * 16, ks, lane);
+                    frag<DH>(b, kt + fc, wn * KW + i * 16, ks);
                     mma(s[2 * i], qf[ks], b[0], b[1]);
                     mma(s[2 * i + 1], qf[ks], b[2], b[3]);
-                }
-            }
-            if ((v0 & (WN == 1 ? v1 : 0xffffffffu)) != (WN == 1 ? 0xffffffffu : 0xffffu)) {
-                #pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const uint32_t w = (i < 4 ? v0 : v1) >> ((i & 3) * 8 + 2 * t);
-                    if (!(w & 1)) s[i][0] = s[i][2] = -INFINITY;
-                    if (!(w & 2)) s[i][1] = s[i][3] = -INFINITY;
                 }
             }
             float x0 = -INFINITY, x1 = -INFINITY;
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 6 : 1) k_c
                 #pragma unroll
                 for (int d = 0; d < KS; d++) {
                     uint32_t b[4];
-                    frag_bk<DH>(b, vt, wn * KW + i * 16, d, lane);
+                    frag_t<DH>(b, vt + fr, wn * KW + i * 16, d);
                     mma(o[2 * d], p, b[0], b[1]);
                     mma(o[2 * d + 1], p, b[2], b[3]);
                 }
@@ -353,12 +359,14 @@ template <int DH>
 __global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossArgs a) {
     constexpr int THREADS = 128, BM = 64, BN = DH == 128 ? 32 : 64, NT = BN / 8, KS = DH / 16;
     constexpr int TILE = BN * DH * 2;
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
     __shared__ uint32_t bits[3][2];
     __shared__ float s_delta[BM];
     const uint32_t sK = s_addr(sm), sV = sK + 2 * TILE, sQ = sV + 2 * TILE, sG = sQ + BM * DH * 2;
     const Where at = where(a);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
     const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
     const int nt = (kend - kbeg + BN - 1) / BN;
@@ -427,8 +435,8 @@ __global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossA
         if (j == 0) {
             #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                frag_a<DH>(qf[ks], sQ, warp * 16, ks, lane);
-                frag_a<DH>(gf[ks], sG, warp * 16, ks, lane);
+                frag<DH>(qf[ks], sQ + fr, warp * 16, ks);
+                frag<DH>(gf[ks], sG + fr, warp * 16, ks);
             }
             da = s_delta[warp * 16 + g];
             db = s_delta[warp * 16 + g + 8];
@@ -447,10 +455,10 @@ __global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossA
                 #pragma unroll
                 for (int i = 0; i < NT / 2; i++) {
                     uint32_t b[4];
-                    frag_bn<DH>(b, kt, i * 16, ks, lane);
+                    frag<DH>(b, kt + fc, i * 16, ks);
                     mma(s[2 * i], qf[ks], b[0], b[1]);
                     mma(s[2 * i + 1], qf[ks], b[2], b[3]);
-                    frag_bn<DH>(b, vt, i * 16, ks, lane);
+                    frag<DH>(b, vt + fc, i * 16, ks);
                     mma(p[2 * i], gf[ks], b[0], b[1]);
                     mma(p[2 * i + 1], gf[ks], b[2], b[3]);
                 }
@@ -475,7 +483,7 @@ __global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossA
                 #pragma unroll
                 for (int d = 0; d < KS; d++) {
                     uint32_t b[4];
-                    frag_bk<DH>(b, kt, i * 16, d, lane);
+                    frag_t<DH>(b, kt + fr, i * 16, d);
                     mma(dq[2 * d], f, b[0], b[1]);
                     mma(dq[2 * d + 1], f, b[2], b[3]);
                 }
@@ -510,12 +518,14 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
     constexpr int THREADS = 128, BK = 64, BQ = DH == 128 ? 32 : 64, NT = BQ / 8, KS = DH / 16;
     constexpr int QT = BQ * DH * 2;
     constexpr bool REGS = DH < 128;              // k and v fragments stay in registers
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
     __shared__ uint32_t bits[2];
     __shared__ float s_lse[2][BQ], s_delta[2][BQ];
     const uint32_t sK = s_addr(sm), sV = sK + BK * DH * 2, sQ = sV + BK * DH * 2, sG = sQ + 2 * QT;
     const Where at = where(a);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
     const int j0 = at.tile * BK, len = kept_len(a, at.seq);
     const int qbeg = min(at.part * a.split, a.rows), qend = min(a.rows, qbeg + a.split);
     const int nt = (qend - qbeg + BQ - 1) / BQ;
@@ -571,8 +581,8 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
             if (REGS && j == 0) {
                 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    frag_a<DH>(kf[REGS ? ks : 0], sK, warp * 16, ks, lane);
-                    frag_a<DH>(vf[REGS ? ks : 0], sV, warp * 16, ks, lane);
+                    frag<DH>(kf[REGS ? ks : 0], sK + fr, warp * 16, ks);
+                    frag<DH>(vf[REGS ? ks : 0], sV + fr, warp * 16, ks);
                 }
             }
             const uint32_t qt = sQ + (j & 1) * QT, gt = sG + (j & 1) * QT;
@@ -585,16 +595,16 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
             #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 if (!REGS) {
-                    frag_a<DH>(kf[0], sK, warp * 16, ks, lane);
-                    frag_a<DH>(vf[0], sV, warp * 16, ks, lane);
+                    frag<DH>(kf[0], sK + fr, warp * 16, ks);
+                    frag<DH>(vf[0], sV + fr, warp * 16, ks);
                 }
                 #pragma unroll
                 for (int i = 0; i < NT / 2; i++) {
                     uint32_t b[4];
-                    frag_bn<DH>(b, qt, i * 16, ks, lane);
+                    frag<DH>(b, qt + fc, i * 16, ks);
                     mma(s[2 * i], kf[REGS ? ks : 0], b[0], b[1]);
                     mma(s[2 * i + 1], kf[REGS ? ks : 0], b[2], b[3]);
-                    frag_bn<DH>(b, gt, i * 16, ks, lane);
+                    frag<DH>(b, gt + fc, i * 16, ks);
                     mma(p[2 * i], vf[REGS ? ks : 0], b[0], b[1]);
                     mma(p[2 * i + 1], vf[REGS ? ks : 0], b[2], b[3]);
                 }
@@ -624,10 +634,10 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
                 #pragma unroll
                 for (int d = 0; d < KS; d++) {
                     uint32_t b[4];
-                    frag_bk<DH>(b, gt, i * 16, d, lane);
+                    frag_t<DH>(b, gt + fr, i * 16, d);
                     mma(dv[2 * d], pf, b[0], b[1]);
                     mma(dv[2 * d + 1], pf, b[2], b[3]);
-                    frag_bk<DH>(b, qt, i * 16, d, lane);
+                    frag_t<DH>(b, qt + fr, i * 16, d);
                     mma(dk[2 * d], df, b[0], b[1]);
                     mma(dk[2 * d + 1], df, b[2], b[3]);
                 }
@@ -671,13 +681,15 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
     constexpr int NT = BM / 8;               // 8-row tiles of the stacked rows
     constexpr int DR = 4 / NR > 0 ? 4 / NR : 1;             // warps that share a group of 16 rows
     constexpr int ND = (KS + DR - 1) / DR;   // 16-column pieces of dq a warp owns
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
     __shared__ uint32_t bits[3][2];
     __shared__ float s_lse[BM], s_delta[BM];
     const uint32_t sQ = s_addr(sm), sG = sQ + BM * DH * 2, sK = sG + BM * DH * 2, sV = sK + 2 * TILE;
     const uint32_t sD = sV + 2 * TILE;       // dS^T [64 keys][BM rows], rows of 16 bytes permuted
     const Where at = where(a);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
     const int len = kept_len(a, at.seq);
     // parts tile [0, lk), so that the masked tail's dk and dv are written too
     const int kbeg = at.part * a.split, kend = min(a.lk, kbeg + a.split);
@@ -755,37 +767,37 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
         const bool ina = ja < kend, inb = ja + 8 < kend;
         if (wk) {
             float s[NT][4], p[NT][4];
+            // the scores of a masked key start, and stay, at -inf
+            const float ma = (wk >> g) & 1 ? 0.f : -INFINITY, mb = (wk >> (g + 8)) & 1 ? 0.f : -INFINITY;
             #pragma unroll
             for (int i = 0; i < NT; i++) {
-                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+                s[i][0] = s[i][1] = ma;
+                s[i][2] = s[i][3] = mb;
                 p[i][0] = p[i][1] = p[i][2] = p[i][3] = 0.f;
             }
             #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 uint32_t kf[4], vf[4];
-                frag_a<DH>(kf, kt, warp * 16, ks, lane);
-                frag_a<DH>(vf, vt, warp * 16, ks, lane);
+                frag<DH>(kf, kt + fr, warp * 16, ks);
+                frag<DH>(vf, vt + fr, warp * 16, ks);
                 #pragma unroll
                 for (int i = 0; i < NT / 2; i++) {
                     uint32_t b[4];
-                    frag_bn<DH>(b, sQ, i * 16, ks, lane);
+                    frag<DH>(b, sQ + fc, i * 16, ks);
                     mma(s[2 * i], kf, b[0], b[1]);
                     mma(s[2 * i + 1], kf, b[2], b[3]);
-                    frag_bn<DH>(b, sG, i * 16, ks, lane);
+                    frag<DH>(b, sG + fc, i * 16, ks);
                     mma(p[2 * i], vf, b[0], b[1]);
                     mma(p[2 * i + 1], vf, b[2], b[3]);
                 }
             }
-            const bool ka = (wk >> g) & 1, kb = (wk >> (g + 8)) & 1;
             uint32_t pf[NT / 2][4], df[NT / 2][4];
             #pragma unroll
             for (int i = 0; i < NT; i++) {
                 const int c = i * 8 + 2 * t;
                 const float x0 = s_lse[c], x1 = s_lse[c + 1], d0 = s_delta[c], d1 = s_delta[c + 1];
-                const float e0 = ka ? ex2_approx(fmaf(s[i][0], sc, -x0)) : 0.f;
-                const float e1 = ka ? ex2_approx(fmaf(s[i][1], sc, -x1)) : 0.f;
-                const float e2 = kb ? ex2_approx(fmaf(s[i][2], sc, -x0)) : 0.f;
-                const float e3 = kb ? ex2_approx(fmaf(s[i][3], sc, -x1)) : 0.f;
+                const float e0 = ex2_approx(fmaf(s[i][0], sc, -x0)), e1 = ex2_approx(fmaf(s[i][1], sc, -x1));
+                const float e2 = ex2_approx(fmaf(s[i][2], sc, -x0)), e3 = ex2_approx(fmaf(s[i][3], sc, -x1));
                 pf[i >> 1][(i & 1) * 2] = pack_bf2(e0, e1);
                 pf[i >> 1][(i & 1) * 2 + 1] = pack_bf2(e2, e3);
                 const uint32_t da = pack_bf2(e0 * (p[i][0] - d0), e1 * (p[i][1] - d1));
@@ -805,7 +817,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                     #pragma unroll
                     for (int d = 0; d < KS; d++) {
                         uint32_t b[4];
-                        frag_bk<DH>(b, which ? sQ : sG, i * 16, d, lane);
+                        frag_t<DH>(b, (which ? sQ : sG) + fr, i * 16, d);
                         mma(acc[2 * d], which ? df[i] : pf[i], b[0], b[1]);
                         mma(acc[2 * d + 1], which ? df[i] : pf[i], b[2], b[3]);
                     }
@@ -839,7 +851,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                     const int d = qd + i * DR;
                     if (d >= KS) break;
                     uint32_t b[4];
-                    frag_bk<DH>(b, kt, k * 16, d, lane);
+                    frag_t<DH>(b, kt + fr, k * 16, d);
                     mma(dq[i][0], f, b[0], b[1]);
                     mma(dq[i][1], f, b[2], b[3]);
                 }
@@ -1444,8 +1456,8 @@ cudaError_t smem_limit(F f, int bytes) {
 
 template <int DH, int WM, int WN, int NST>
 cudaError_t launch_fwd(const CrossArgs& a, long blocks, cudaStream_t s) {
-    int bytes = WM * 16 * DH * 2 + 2 * NST * 64 * DH * 2;
-    if (WN > 1) bytes = std::max(bytes, (WN * 32 + WN * 16 * DH) * 4);
+    int bytes = WM * 16 * DH * 2 + 2 * NST * 64 * DH * 2 + 256;
+    if (WN > 1) bytes = std::max(bytes, (WN * 32 + WN * 16 * DH) * 4 + 256);
     const cudaError_t e = smem_limit(k_cross_fwd<DH, WM, WN, NST>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_fwd<DH, WM, WN, NST><<<(unsigned)blocks, WM * WN * 32, bytes, s>>>(a);
@@ -1463,7 +1475,7 @@ cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
 template <int DH>
 cudaError_t launch_dq(const CrossArgs& a, long blocks, cudaStream_t s) {
     constexpr int BN = DH == 128 ? 32 : 64;
-    const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2;
+    const int bytes = 4 * BN * DH * 2 + 2 * 64 * DH * 2 + 256;
     const cudaError_t e = smem_limit(k_cross_dq<DH>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_dq<DH><<<(unsigned)blocks, 128, bytes, s>>>(a);
@@ -1472,7 +1484,7 @@ cudaError_t launch_dq(const CrossArgs& a, long blocks, cudaStream_t s) {
 template <int DH>
 cudaError_t launch_dkv(const CrossArgs& a, long blocks, cudaStream_t s) {
     constexpr int BQ = DH == 128 ? 32 : 64;
-    const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2;
+    const int bytes = 2 * 64 * DH * 2 + 4 * BQ * DH * 2 + 256;
     const cudaError_t e = smem_limit(k_cross_dkv<DH>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_dkv<DH><<<(unsigned)blocks, 128, bytes, s>>>(a);
@@ -1521,7 +1533,7 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
 }
 template <int DH, int NR>
 cudaError_t launch_bwd_rows(const CrossArgs& a, long blocks, cudaStream_t s) {
-    const int bytes = 2 * NR * 16 * DH * 2 + 4 * 64 * DH * 2 + 64 * NR * 16 * 2;
+    const int bytes = 2 * NR * 16 * DH * 2 + 4 * 64 * DH * 2 + 64 * NR * 16 * 2 + 256;
     const cudaError_t e = smem_limit(k_cross_bwd_rows<DH, NR>, bytes);
     if (e != cudaSuccess) return e;
     ++g_ptcg_launches, k_cross_bwd_rows<DH, NR><<<(unsigned)blocks, 128, bytes, s>>>(a);
