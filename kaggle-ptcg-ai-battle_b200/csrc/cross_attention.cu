@@ -318,6 +318,167 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 5 : 1) k_c
     }
 }
 
+// The form for keys that fit a block's shared memory whole (a board's rows, a
+// short context): nothing is pipelined, the masks are read once, and each warp
+// walks the 16-key groups that have a kept key two at a time.  The tiled kernel
+// spends some 390 instructions a warp on every 64 keys besides the groups' own
+// 45 (staging, barriers, stages, masked groups' maxima); here that is paid once.
+constexpr int SHORT_KEYS = 256;
+
+// mask words and score offsets of all keys (a multiple of 32 of them, up to
+// SHORT_KEYS), by the block's four warps
+PTCG_DEV void short_masks(const CrossArgs& a, int seq, int len, uint32_t* words, float* bias) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (a.lk + 31) / 32;
+    const uint8_t* keep = a.keep ? a.keep + (long)seq * a.lk : nullptr;
+    #pragma unroll
+    for (int i = 0; i < SHORT_KEYS / 128; i++) {
+        const int w = warp + 4 * i, key = w * 32 + lane;
+        if (w >= n) break;
+        const bool in = key < len && (!keep || keep[key] != 0);
+        const uint32_t m = __ballot_sync(0xffffffffu, in);
+        bias[key] = in ? 0.f : -INFINITY;
+        if (lane == 0) words[w] = m;
+    }
+}
+// bit i: 16-key group i has a kept key
+PTCG_DEV uint32_t short_groups(const CrossArgs& a, const uint32_t* words, int lane) {
+    const bool in = lane * 16 < a.lk && ((words[lane >> 1] >> ((lane & 1) * 16)) & 0xffffu);
+    return __ballot_sync(0xffffffffu, in);
+}
+// all kept rows of K and V (zeros for masked ones)
+template <int DH>
+PTCG_DEV void short_stage(const CrossArgs& a, const Where& at, uint32_t sK, uint32_t sV, int rows, const uint32_t* words) {
+    const Lanes<DH, 128> l;
+    const bf16* k = (const bf16*)a.k + krow(a.sk, at.seq, at.hk, l.r) + l.c * 8;
+    const bf16* v = (const bf16*)a.v + krow(a.sv, at.seq, at.hk, l.r) + l.c * 8;
+    const long dk = l.STEP * a.sk.row, dv = l.STEP * a.sv.row;
+    uint32_t off = l.off;
+    for (int r = l.r; r < rows; r += l.STEP) {
+        const bool in = (words[r >> 5] >> (r & 31)) & 1;
+        cp16(sK + off, in ? k : (const bf16*)a.k, in);
+        cp16(sV + off, in ? v : (const bf16*)a.v, in);
+        k += dk;
+        v += dv;
+        off += l.STEP * DH * 2;
+    }
+}
+
+template <int DH>
+__global__ void __launch_bounds__(128, DH == 32 ? 6 : DH == 64 ? 3 : 2) k_cross_fwd_short(const __grid_constant__ CrossArgs a) {
+    constexpr int BM = 64, KS = DH / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
+    __shared__ uint32_t words[SHORT_KEYS / 32];
+    __shared__ __align__(8) float bias[SHORT_KEYS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, keys = (a.lk + 15) & ~15;
+    const uint32_t sQ = s_addr(sm), sK = sQ + BM * DH * 2, sV = sK + keys * DH * 2;
+    const Where at = where(a);
+    const int r0 = at.tile * BM, len = kept_len(a, at.seq);
+    stage_q<DH, BM, 128>(sQ, (const bf16*)a.q, a.sq, a, at.seq, at.hk, r0);
+    short_masks(a, at.seq, len, words, bias);
+    __syncthreads();
+    short_stage<DH>(a, at, sK, sV, keys, words);
+    uint32_t rem = short_groups(a, words, lane);
+    cp_commit();
+    cp_wait<0>();
+    __syncthreads();
+    if (r0 + warp * 16 >= a.rows) return;
+    const uint32_t fr = lane_rows<DH>(lane), kt = sK + lane_cols<DH>(lane), vt = sV + fr;
+    uint32_t qf[KS][4];
+    #pragma unroll
+    for (int ks = 0; ks < KS; ks++) frag<DH>(qf[ks], sQ + fr, warp * 16, ks);
+    float o[DH / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    #pragma unroll
+    for (int i = 0; i < DH / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    const float sc = a.scale * LOG2E;
+    const int g = lane >> 2, t = lane & 3;
+    while (rem) {
+        const int ka = __ffs(rem) - 1;
+        rem &= rem - 1;
+        const bool two = rem != 0;
+        const int kb = two ? __ffs(rem) - 1 : ka;
+        rem &= rem - 1;                             // 0 stays 0
+        float s[4][4];
+        #pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const float2 b = *(const float2*)(bias + (n < 2 ? ka : kb) * 16 + (n & 1) * 8 + 2 * t);
+            s[n][0] = s[n][2] = n < 2 || two ? b.x : -INFINITY;
+            s[n][1] = s[n][3] = n < 2 || two ? b.y : -INFINITY;
+        }
+        #pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            uint32_t b[4];
+            frag<DH>(b, kt, ka * 16, ks);
+            mma(s[0], qf[ks], b[0], b[1]);
+            mma(s[1], qf[ks], b[2], b[3]);
+        }
+        if (two) {
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                uint32_t b[4];
+                frag<DH>(b, kt, kb * 16, ks);
+                mma(s[2], qf[ks], b[0], b[1]);
+                mma(s[3], qf[ks], b[2], b[3]);
+            }
+        }
+        float x0 = fmaxf(s[0][0], s[0][1]), x1 = fmaxf(s[0][2], s[0][3]);
+        #pragma unroll
+        for (int n = 1; n < 4; n++) {
+            x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
+            x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
+        }
+        // a kept key among these: the maxima are finite unless the scores are not
+        const float n0 = fmaxf(m0, quad_max(x0) * sc), n1 = fmaxf(m1, quad_max(x1) * sc);
+        const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
+        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+            const float c0 = ex2_approx(m0 - u0), c1 = ex2_approx(m1 - u1);
+            l0 *= c0;
+            l1 *= c1;
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) { o[i][0] *= c0; o[i][1] *= c0; o[i][2] *= c1; o[i][3] *= c1; }
+            m0 = n0;
+            m1 = n1;
+        }
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (h == 1 && !two) break;
+            #pragma unroll
+            for (int n = 2 * h; n < 2 * h + 2; n++) {
+                s[n][0] = ex2_approx(fmaf(s[n][0], sc, -u0));
+                s[n][1] = ex2_approx(fmaf(s[n][1], sc, -u0));
+                s[n][2] = ex2_approx(fmaf(s[n][2], sc, -u1));
+                s[n][3] = ex2_approx(fmaf(s[n][3], sc, -u1));
+                l0 += s[n][0] + s[n][1];
+                l1 += s[n][2] + s[n][3];
+            }
+            const uint32_t p[4] = {pack_bf2(s[2 * h][0], s[2 * h][1]), pack_bf2(s[2 * h][2], s[2 * h][3]),
+                                   pack_bf2(s[2 * h + 1][0], s[2 * h + 1][1]),
+                                   pack_bf2(s[2 * h + 1][2], s[2 * h + 1][3])};
+            #pragma unroll
+            for (int d = 0; d < KS; d++) {
+                uint32_t b[4];
+                frag_t<DH>(b, vt, (h ? kb : ka) * 16, d);
+                mma(o[2 * d], p, b[0], b[1]);
+                mma(o[2 * d + 1], p, b[2], b[3]);
+            }
+        }
+    }
+    l0 = quad_sum(l0);
+    l1 = quad_sum(l1);
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int r = r0 + warp * 16 + g + half * 8;
+        if (r >= a.rows) continue;
+        const float m = half ? m1 : m0, l = half ? l1 : l0, inv = l == 0.f ? 0.f : 1.f / l;
+        bf16* p = (bf16*)a.out + qrow(a, a.so, at.seq, at.hk, r) + 2 * t;
+        #pragma unroll
+        for (int i = 0; i < DH / 8; i++)
+            *(uint32_t*)(p + i * 8) = pack_bf2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+        if (t == 0 && a.lse)
+            a.lse[((long)at.seq * a.kv_heads + at.hk) * a.rows + r] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    }
+}
+
 // joins the parts of a split forward: a warp per stacked row
 template <typename T, int DH>
 __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ CrossArgs a, long nrows) {
@@ -874,6 +1035,199 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                 if (a.nsplit > 1) *(float2*)(a.part + ((row0 + r) * a.nsplit + at.part) * DH + c) = make_float2(x, y);
                 else *(uint32_t*)((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r) + c) = pack_bf2(x, y);
             }
+        }
+    }
+}
+
+// The same for keys that fit shared memory whole: every warp takes each fourth
+// 16-key group that has a kept key, dS^T of all of them is kept, and dq is one
+// product at the end; three barriers in all.
+template <int DH, int NR>                    // 16 NR rows
+__global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_bwd_short(const __grid_constant__ CrossArgs a) {
+    constexpr int BM = NR * 16, KS = DH / 16, NT = BM / 8;
+    constexpr int DR = 4 / NR, ND = (KS + DR - 1) / DR;
+    constexpr int TR = 128 / BM, PC = DH / 8 / TR > 0 ? DH / 8 / TR : 1;   // threads a row, pieces each
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 255) & ~(uintptr_t)255);
+    __shared__ uint32_t words[SHORT_KEYS / 32];
+    __shared__ float bias[SHORT_KEYS];
+    __shared__ __align__(8) float s_lse[BM], s_delta[BM];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, keys = (a.lk + 15) & ~15;
+    const uint32_t sQ = s_addr(sm), sG = sQ + BM * DH * 2, sK = sG + BM * DH * 2, sV = sK + keys * DH * 2;
+    const uint32_t sD = sV + keys * DH * 2;  // dS^T [keys][BM rows], rows of 16 bytes permuted
+    const Where at = where(a);
+    const int len = kept_len(a, at.seq);
+    const long row0 = ((long)at.seq * a.kv_heads + at.hk) * a.rows;
+    stage_q<DH, BM, 128>(sQ, (const bf16*)a.q, a.sq, a, at.seq, at.hk, 0);
+    stage_q<DH, BM, 128>(sG, (const bf16*)a.dout, a.sdo, a, at.seq, at.hk, 0);
+    cp_commit();
+    // the row whose delta this thread shares in: out and the log-sum-exp come now
+    const int dr = threadIdx.x / TR, dp = threadIdx.x % TR;
+    uint4 og[PC];
+    float lr = -INFINITY;
+    if (dr < a.rows) {
+        const uint4* p = (const uint4*)((const bf16*)a.o + qrow(a, a.so, at.seq, at.hk, dr));
+        #pragma unroll
+        for (int c = 0; c < PC; c++) og[c] = dp + c * TR < DH / 8 ? p[dp + c * TR] : make_uint4(0u, 0u, 0u, 0u);
+        lr = a.lse[row0 + dr];
+    } else {
+        #pragma unroll
+        for (int c = 0; c < PC; c++) og[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    short_masks(a, at.seq, len, words, bias);
+    __syncthreads();
+    short_stage<DH>(a, at, sK, sV, keys, words);
+    const uint32_t active = short_groups(a, words, lane);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    {
+        float d = 0.f;
+        #pragma unroll
+        for (int c = 0; c < PC; c++) {
+            if (dp + c * TR >= DH / 8) break;
+            uint4 y;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(sG + tile_off<DH>(dr, dp + c * TR)));
+            const uint32_t u[4] = {og[c].x, og[c].y, og[c].z, og[c].w}, v[4] = {y.x, y.y, y.z, y.w};
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float u0, u1, v0, v1;
+                unpack_bf2(u[e], u0, u1);
+                unpack_bf2(v[e], v0, v1);
+                d = fmaf(u0, v0, fmaf(u1, v1, d));
+            }
+        }
+        #pragma unroll
+        for (int o = 1; o < TR; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (dp == 0) {
+            s_lse[dr] = lr == -INFINITY ? INFINITY : lr * LOG2E;
+            s_delta[dr] = d;
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();
+    const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
+    const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
+    const float sc = a.scale * LOG2E;
+    // 16-byte piece c (8 rows) of key row k of dS^T
+    auto ds_off = [&](int k, int c) {
+        return sD + (uint32_t)(k * BM * 2 + ((c ^ (NT == 8 ? k & 7 : NT == 4 ? (k >> 1) & 3 : (k >> 2) & 1)) << 4));
+    };
+    const int groups = keys / 16;
+    int turn = 0;
+    for (int k = 0; k < groups; k++) {
+        const bool on = (active >> k) & 1;
+        if (((on ? turn++ : k) & 3) != warp) continue;
+        const int ja = k * 16 + g;
+        const bool ina = ja < a.lk, inb = ja + 8 < a.lk;
+        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja) + 2 * t;
+        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja) + 2 * t;
+        if (!on) {                               // masked keys: no gradient
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) {
+                if (ina) { *(uint32_t*)(pk + i * 8) = 0u; *(uint32_t*)(pv + i * 8) = 0u; }
+                if (inb) { *(uint32_t*)(pk + 8 * a.sdk.row + i * 8) = 0u; *(uint32_t*)(pv + 8 * a.sdv.row + i * 8) = 0u; }
+            }
+            continue;
+        }
+        float s[NT][4], p[NT][4];
+        const float ma = bias[ja], mb = bias[ja + 8];
+        #pragma unroll
+        for (int i = 0; i < NT; i++) {
+            s[i][0] = s[i][1] = ma;
+            s[i][2] = s[i][3] = mb;
+            p[i][0] = p[i][1] = p[i][2] = p[i][3] = 0.f;
+        }
+        #pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            uint32_t kf[4], vf[4];
+            frag<DH>(kf, sK + fr, k * 16, ks);
+            frag<DH>(vf, sV + fr, k * 16, ks);
+            #pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                uint32_t b[4];
+                frag<DH>(b, sQ + fc, i * 16, ks);
+                mma(s[2 * i], kf, b[0], b[1]);
+                mma(s[2 * i + 1], kf, b[2], b[3]);
+                frag<DH>(b, sG + fc, i * 16, ks);
+                mma(p[2 * i], vf, b[0], b[1]);
+                mma(p[2 * i + 1], vf, b[2], b[3]);
+            }
+        }
+        uint32_t pf[NT / 2][4], df[NT / 2][4];
+        #pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const float2 x = *(const float2*)(s_lse + i * 8 + 2 * t), d = *(const float2*)(s_delta + i * 8 + 2 * t);
+            const float e0 = ex2_approx(fmaf(s[i][0], sc, -x.x)), e1 = ex2_approx(fmaf(s[i][1], sc, -x.y));
+            const float e2 = ex2_approx(fmaf(s[i][2], sc, -x.x)), e3 = ex2_approx(fmaf(s[i][3], sc, -x.y));
+            pf[i >> 1][(i & 1) * 2] = pack_bf2(e0, e1);
+            pf[i >> 1][(i & 1) * 2 + 1] = pack_bf2(e2, e3);
+            const uint32_t da = pack_bf2(e0 * (p[i][0] - d.x), e1 * (p[i][1] - d.y));
+            const uint32_t db = pack_bf2(e2 * (p[i][2] - d.x), e3 * (p[i][3] - d.y));
+            df[i >> 1][(i & 1) * 2] = da;
+            df[i >> 1][(i & 1) * 2 + 1] = db;
+            asm volatile("st.shared.b32 [%0], %1;" :: "r"(ds_off(ja, i) + 4 * t), "r"(da) : "memory");
+            asm volatile("st.shared.b32 [%0], %1;" :: "r"(ds_off(ja + 8, i) + 4 * t), "r"(db) : "memory");
+        }
+        #pragma unroll
+        for (int which = 0; which < 2; which++) {
+            float acc[DH / 8][4];
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            #pragma unroll
+            for (int i = 0; i < NT / 2; i++) {
+                #pragma unroll
+                for (int d = 0; d < KS; d++) {
+                    uint32_t b[4];
+                    frag_t<DH>(b, (which ? sQ : sG) + fr, i * 16, d);
+                    mma(acc[2 * d], which ? df[i] : pf[i], b[0], b[1]);
+                    mma(acc[2 * d + 1], which ? df[i] : pf[i], b[2], b[3]);
+                }
+            }
+            const float f = which ? a.scale : 1.f;
+            bf16* out = which ? pk : pv;
+            const long down = 8 * (which ? a.sdk.row : a.sdv.row);
+            #pragma unroll
+            for (int i = 0; i < DH / 8; i++) {
+                if (ina) *(uint32_t*)(out + i * 8) = pack_bf2(acc[i][0] * f, acc[i][1] * f);
+                if (inb) *(uint32_t*)(out + down + i * 8) = pack_bf2(acc[i][2] * f, acc[i][3] * f);
+            }
+        }
+    }
+    __syncthreads();
+    const int qr = NR == 1 ? 0 : warp % NR, qd = NR == 1 ? warp : warp / NR;   // dq rows, first column piece
+    float dq[ND][2][4];
+    #pragma unroll
+    for (int i = 0; i < ND; i++)
+        #pragma unroll
+        for (int e = 0; e < 4; e++) dq[i][0][e] = dq[i][1][e] = 0.f;
+    for (uint32_t rem = active; rem; rem &= rem - 1) {
+        const int k = __ffs(rem) - 1;
+        uint32_t f[4];                           // dS rows 16 qr .., keys 16 k ..
+        ldsm4t(f, ds_off(k * 16 + (mi >> 1) * 8 + (lane & 7), qr * 2 + (mi & 1)));
+        #pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const int d = qd + i * DR;
+            if (d >= KS) break;
+            uint32_t b[4];
+            frag_t<DH>(b, sK + fr, k * 16, d);
+            mma(dq[i][0], f, b[0], b[1]);
+            mma(dq[i][1], f, b[2], b[3]);
+        }
+    }
+    #pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const int r = qr * 16 + g + half * 8;
+        if (r >= a.rows) continue;
+        bf16* out = (bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r) + 2 * t;
+        #pragma unroll
+        for (int i = 0; i < ND; i++) {
+            const int d = qd + i * DR;
+            if (d >= KS) break;
+            #pragma unroll
+            for (int n = 0; n < 2; n++)
+                *(uint32_t*)(out + d * 16 + n * 8) = pack_bf2(dq[i][n][2 * half] * a.scale, dq[i][n][2 * half + 1] * a.scale);
         }
     }
 }
@@ -1463,6 +1817,22 @@ cudaError_t launch_fwd(const CrossArgs& a, long blocks, cudaStream_t s) {
     ++g_ptcg_launches, k_cross_fwd<DH, WM, WN, NST><<<(unsigned)blocks, WM * WN * 32, bytes, s>>>(a);
     return cudaSuccess;
 }
+// dynamic shared memory of the kernels for short keys; they take problems whose
+// keys leave room for two blocks on a processor
+int short_fwd_bytes(int dh, int lk) { return (64 + 2 * ((lk + 15) & ~15)) * dh * 2 + 256; }
+int short_bwd_bytes(int dh, int lk, int rows) {
+    const int keys = (lk + 15) & ~15;
+    return (2 * rows + 2 * keys) * dh * 2 + keys * rows * 2 + 256;
+}
+bool is_short(int lk, int bytes) { return lk <= SHORT_KEYS && bytes <= 108 * 1024; }
+template <int DH>
+cudaError_t launch_fwd_short(const CrossArgs& a, long blocks, cudaStream_t s) {
+    const int bytes = short_fwd_bytes(DH, a.lk);
+    const cudaError_t e = smem_limit(k_cross_fwd_short<DH>, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_cross_fwd_short<DH><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    return cudaSuccess;
+}
 template <int DH, int RT>
 cudaError_t launch_fwd_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
     constexpr int BM = RT * 8, BN = F32<DH>::BN;
@@ -1521,7 +1891,9 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
         set_tiles(a, tiles, p.sp);
         e = launch_fwd<DH, 4, 1, 2>(a, tiles * c.nseq * c.kv_heads * p.sp.n, s);
     } else if (!p.tc && c.dtype == PTCG_BF16)
-        e = p.few ? launch_fwd<DH, 1, 4, 3>(a, p.blocks, s) : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
+        e = p.few ? launch_fwd<DH, 1, 4, 3>(a, p.blocks, s)
+            : p.sp.n == 1 && is_short(c.lk, short_fwd_bytes(DH, c.lk)) ? launch_fwd_short<DH>(a, p.blocks, s)
+            : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
     else if (!p.tc)
         e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
     if (e != cudaSuccess || p.sp.n == 1) return e;
@@ -1533,6 +1905,13 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
 }
 template <int DH, int NR>
 cudaError_t launch_bwd_rows(const CrossArgs& a, long blocks, cudaStream_t s) {
+    const int whole = short_bwd_bytes(DH, a.lk, NR * 16);
+    if (a.nsplit == 1 && is_short(a.lk, whole)) {
+        const cudaError_t e = smem_limit(k_cross_bwd_short<DH, NR>, whole);
+        if (e != cudaSuccess) return e;
+        ++g_ptcg_launches, k_cross_bwd_short<DH, NR><<<(unsigned)blocks, 128, whole, s>>>(a);
+        return cudaSuccess;
+    }
     const int bytes = 2 * NR * 16 * DH * 2 + 4 * 64 * DH * 2 + 64 * NR * 16 * 2 + 256;
     const cudaError_t e = smem_limit(k_cross_bwd_rows<DH, NR>, bytes);
     if (e != cudaSuccess) return e;
