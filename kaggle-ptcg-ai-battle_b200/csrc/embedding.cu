@@ -120,94 +120,182 @@ __global__ void __launch_bounds__(SORT_T) k_sort_count(const __grid_constant__ S
     for (int i = threadIdx.x; i < bins; i += SORT_T) a.counts[(long)blockIdx.x * bins + i] = hist[i];
 }
 
-template <int ITEMS, bool FIRST>
-__global__ void __launch_bounds__(SORT_T) k_sort_scatter(const __grid_constant__ SortArgs a) {
+// Shared memory of a tile's sort: per warp and digit the count, then the first
+// place among the tile's places of that digit; the digits' first places.
+struct TileSort {
+    uint16_t wcnt[SORT_T / 32][MAX_BINS];
+    uint32_t start[MAX_BINS], total[MAX_BINS], wsum[MAX_BINS / 32];
+};
+// Where each of this thread's ITEMS places goes in its tile sorted by the digit
+// (stable: a warp holds 32 * ITEMS consecutive places, lane by lane).  Ends
+// with a barrier; t.start and t.total hold the digits' first places and counts.
+template <int ITEMS>
+PTCG_DEV void tile_places(TileSort& t, uint32_t (&to)[ITEMS], const uint32_t (&key)[ITEMS], int n, int shift, int bits) {
     constexpr int NW = SORT_T / 32;
-    // per warp and digit: its count, then its first place relative to the tile's
-    __shared__ uint16_t wcnt[NW][MAX_BINS];
-    __shared__ uint32_t tot[SORT_T], pre[SORT_T];
-    __shared__ uint32_t first[MAX_BINS], wsum[MAX_BINS / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int bins = 1 << a.bits, tiles = gridDim.x, tile = blockIdx.x;
-    uint32_t key[ITEMS], ps[ITEMS];
-    const long base = (long)tile * SORT_T * ITEMS + (long)warp * 32 * ITEMS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
+    const int base = warp * 32 * ITEMS;
+    for (int i = tid; i < NW * MAX_BINS / 2; i += SORT_T) ((uint32_t*)t.wcnt)[i] = 0;
+    __syncthreads();
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
-        const long i = base + k * 32 + lane;
+        const bool in = base + k * 32 + lane < n;
+        const uint32_t d = (key[k] >> shift) & (bins - 1);
+        const uint32_t same = same_digit(d, in, bits);
+        uint32_t before = 0;
+        if (in) before = t.wcnt[warp][d];
+        __syncwarp();
+        to[k] = before + __popc(same & ((1u << lane) - 1u));
+        if (in && lane == __ffs(same) - 1) t.wcnt[warp][d] = (uint16_t)(before + __popc(same));
+        __syncwarp();
+    }
+    __syncthreads();
+    uint32_t all = 0, x = 0;
+    if (tid < MAX_BINS) {
+        if (tid < bins) {
+            #pragma unroll 8
+            for (int w = 0; w < NW; w++) {
+                const uint32_t v = t.wcnt[w][tid];
+                t.wcnt[w][tid] = (uint16_t)all;            // below the tile's 16384 places
+                all += v;
+            }
+            t.total[tid] = all;
+        }
+        x = all;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) t.wsum[warp] = x;
+    }
+    __syncthreads();
+    if (tid < bins) {
+        uint32_t s = x - all;
+        for (int w = 0; w < warp; w++) s += t.wsum[w];
+        t.start[tid] = s;
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const uint32_t d = (key[k] >> shift) & (bins - 1);
+        to[k] += t.start[d] + t.wcnt[warp][d];
+    }
+}
+
+// A tile's places, brought into digit order in shared memory, so that they
+// leave as runs of neighbours (scattered 4-byte writes took twice as long)
+template <int ITEMS, bool FIRST>
+__global__ void __launch_bounds__(SORT_T) k_sort_scatter(const __grid_constant__ SortArgs a) {
+    constexpr int TILE = SORT_T * ITEMS;
+    extern __shared__ uint32_t sorted[];                   // [TILE] keys, [TILE] places
+    __shared__ TileSort t;
+    __shared__ uint32_t tot[SORT_T], pre[SORT_T], base[MAX_BINS], wsum[MAX_BINS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int bins = 1 << a.bits, tiles = gridDim.x, tile = blockIdx.x;
+    const long first = (long)tile * TILE;
+    const int n = (int)min((long)TILE, a.n - first);
+    uint32_t key[ITEMS], ps[ITEMS], to[ITEMS];
+    #pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const int i = warp * 32 * ITEMS + k * 32 + lane;
         key[k] = 0;
-        ps[k] = (uint32_t)i;
-        if (i < a.n) {
+        ps[k] = (uint32_t)(first + i);
+        if (i < n) {
             if (FIRST) {
-                key[k] = key_of(a.ids[i], a.vocab, a.pad_id, a.has_pad);
+                key[k] = key_of(a.ids[first + i], a.vocab, a.pad_id, a.has_pad);
             } else {
-                key[k] = a.keys[i];
-                ps[k] = a.pos[i];
+                key[k] = a.keys[first + i];
+                ps[k] = a.pos[first + i];
             }
         }
     }
     {   // counts of each digit over all tiles, and over the tiles before this one
         const int d = tid & (bins - 1), part = tid >> a.bits, parts = SORT_T >> a.bits;
-        uint32_t t = 0, p = 0;
+        uint32_t x = 0, p = 0;
         #pragma unroll 4
         for (int j = part; j < tiles; j += parts) {
             const uint32_t c = a.counts[(long)j * bins + d];
-            t += c;
+            x += c;
             p += j < tile ? c : 0u;
         }
-        tot[tid] = t;
+        tot[tid] = x;
         pre[tid] = p;
-        for (int i = tid; i < NW * MAX_BINS / 2; i += SORT_T) ((uint32_t*)wcnt)[i] = 0;
     }
-    __syncthreads();
-    // ranks inside the warp's run of 32 * ITEMS consecutive places: lanes of
-    // one digit in place order, after the warp's earlier ones
-    uint16_t rank[ITEMS];
+    tile_places<ITEMS>(t, to, key, n, a.shift, a.bits);
     #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
-        const bool in = base + k * 32 + lane < a.n;
-        const uint32_t d = (key[k] >> a.shift) & (bins - 1);
-        const uint32_t same = same_digit(d, in, a.bits);
-        uint32_t before = 0;
-        if (in) before = wcnt[warp][d];
-        __syncwarp();
-        rank[k] = (uint16_t)(before + __popc(same & ((1u << lane) - 1u)));
-        if (in && lane == __ffs(same) - 1) wcnt[warp][d] = (uint16_t)(before + __popc(same));
-        __syncwarp();
+        if (warp * 32 * ITEMS + k * 32 + lane < n) {
+            sorted[to[k]] = key[k];
+            sorted[TILE + to[k]] = ps[k];
+        }
     }
-    __syncthreads();
-    // first place of each digit for this tile, then for each of its warps
-    uint32_t all = 0, mine = 0;
-    if (tid < bins) {
-        for (int j = tid; j < SORT_T; j += bins) { all += tot[j]; mine += pre[j]; }
-        uint32_t x = all;
+    // the digits' first places for this tile, less their first places in it
+    uint32_t all = 0, mine = 0, x = 0;
+    if (tid < MAX_BINS) {
+        if (tid < bins)
+            for (int j = tid; j < SORT_T; j += bins) { all += tot[j]; mine += pre[j]; }
+        x = all;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(__activemask(), x, o);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        if (lane == 31 || tid == bins - 1) wsum[warp] = x;
-        mine += x - all;
-        uint32_t c = 0;
-        #pragma unroll 8
-        for (int w = 0; w < NW; w++) {
-            const uint32_t v = wcnt[w][tid];
-            wcnt[w][tid] = (uint16_t)c;                    // below the tile's 16384 places
-            c += v;
-        }
+        if (lane == 31) wsum[warp] = x;
     }
     __syncthreads();
     if (tid < bins) {
+        mine += x - all;
         for (int w = 0; w < warp; w++) mine += wsum[w];
-        first[tid] = mine;
+        base[tid] = mine - t.start[tid];
     }
     __syncthreads();
+    for (int i = tid; i < n; i += SORT_T) {
+        const uint32_t k = sorted[i], at = base[(k >> a.shift) & (bins - 1)] + i;
+        a.keys_out[at] = k;
+        a.pos_out[at] = sorted[TILE + i];
+    }
+}
+
+// All passes of a batch that one block holds, in one launch: for small batches
+// the launches would cost more than the sort
+constexpr int SMALL_ITEMS = 8, SMALL_N = SORT_T * SMALL_ITEMS;
+__global__ void __launch_bounds__(SORT_T) k_sort_small(const __grid_constant__ SortArgs a, int passes) {
+    extern __shared__ uint32_t sorted[];                   // [SMALL_N] keys, [SMALL_N] places
+    __shared__ TileSort t;
+    const int n = (int)a.n, base = (threadIdx.x >> 5) * 32 * SMALL_ITEMS + (threadIdx.x & 31);
+    uint32_t key[SMALL_ITEMS], ps[SMALL_ITEMS], to[SMALL_ITEMS];
     #pragma unroll
-    for (int k = 0; k < ITEMS; k++) {
-        if (base + k * 32 + lane < a.n) {
-            const uint32_t d = (key[k] >> a.shift) & (bins - 1);
-            const uint32_t to = first[d] + wcnt[warp][d] + rank[k];
-            a.keys_out[to] = key[k];
-            a.pos_out[to] = ps[k];
+    for (int k = 0; k < SMALL_ITEMS; k++) {
+        const int i = base + k * 32;
+        key[k] = i < n ? key_of(a.ids[i], a.vocab, a.pad_id, a.has_pad) : 0u;
+        ps[k] = (uint32_t)i;
+    }
+    for (int p = 0; p < passes; p++) {
+        tile_places<SMALL_ITEMS>(t, to, key, n, p * a.bits, a.bits);
+        #pragma unroll
+        for (int k = 0; k < SMALL_ITEMS; k++) {
+            if (base + k * 32 < n) {
+                sorted[to[k]] = key[k];
+                sorted[SMALL_N + to[k]] = ps[k];
+            }
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int k = 0; k < SMALL_ITEMS; k++) {
+            const int i = base + k * 32;
+            if (i < n) {
+                key[k] = sorted[i];
+                ps[k] = sorted[SMALL_N + i];
+            }
+        }
+        __syncthreads();
+    }
+    #pragma unroll
+    for (int k = 0; k < SMALL_ITEMS; k++) {
+        const int i = base + k * 32;
+        if (i < n) {
+            a.keys_out[i] = key[k];
+            a.pos_out[i] = ps[k];
         }
     }
 }
@@ -501,16 +589,22 @@ void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids,
     #undef EF
 }
 
-template <int ITEMS>
-void sort_pass(const SortArgs& a, bool first, int tiles, cudaStream_t s) {
+template <int ITEMS, bool FIRST>
+cudaError_t sort_pass(const SortArgs& a, int tiles, cudaStream_t s) {
+    constexpr int bytes = 8 * SORT_T * ITEMS;
+    const cudaError_t e = cudaFuncSetAttribute(k_sort_scatter<ITEMS, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
     g_ptcg_launches += 2;
-    if (first) {
-        k_sort_count<ITEMS, true><<<tiles, SORT_T, 0, s>>>(a);
-        k_sort_scatter<ITEMS, true><<<tiles, SORT_T, 0, s>>>(a);
-    } else {
-        k_sort_count<ITEMS, false><<<tiles, SORT_T, 0, s>>>(a);
-        k_sort_scatter<ITEMS, false><<<tiles, SORT_T, 0, s>>>(a);
-    }
+    k_sort_count<ITEMS, FIRST><<<tiles, SORT_T, 0, s>>>(a);
+    k_sort_scatter<ITEMS, FIRST><<<tiles, SORT_T, bytes, s>>>(a);
+    return cudaSuccess;
+}
+cudaError_t sort_small(const SortArgs& a, int passes, cudaStream_t s) {
+    constexpr int bytes = 8 * SMALL_N;
+    const cudaError_t e = cudaFuncSetAttribute(k_sort_small, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    ++g_ptcg_launches, k_sort_small<<<1, SORT_T, bytes, s>>>(a, passes);
+    return cudaSuccess;
 }
 
 template <typename T, int V, int G>
@@ -590,16 +684,19 @@ int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* i
     uint8_t* base = (uint8_t*)scratch;
     uint32_t* keys[2] = {(uint32_t*)(base + p.o_keys[0]), (uint32_t*)(base + p.o_keys[1])};
     uint32_t* pos[2] = {(uint32_t*)(base + p.o_pos[0]), (uint32_t*)(base + p.o_pos[1])};
-    for (int i = 0; i < p.passes; i++) {
+    const bool small = n <= SMALL_N;
+    for (int i = 0; i < (small ? 1 : p.passes); i++) {
         const int to = i & 1;
         const SortArgs sa = {(uint32_t*)(base + p.o_counts), keys[to], pos[to], keys[to ^ 1], pos[to ^ 1],
                              ids, n, i * p.bits, p.bits, vocab, pad_id, pad_id >= 0};
-        if (p.items == 16) sort_pass<16>(sa, i == 0, p.tiles, s);
-        else sort_pass<4>(sa, i == 0, p.tiles, s);
+        OP_CK(small ? sort_small(sa, p.passes, s)
+              : p.items == 16 ? (i == 0 ? sort_pass<16, true>(sa, p.tiles, s) : sort_pass<16, false>(sa, p.tiles, s))
+                              : (i == 0 ? sort_pass<4, true>(sa, p.tiles, s) : sort_pass<4, false>(sa, p.tiles, s)));
     }
+    const int last = small ? 0 : (p.passes - 1) & 1;
     SumArgs a;
     a.dout = dout; a.lddo = lddo;
-    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1];
+    a.keys = keys[last]; a.pos = pos[last];
     a.n = n;
     a.dtab = dtable; a.lddt = lddt;
     a.head = (float*)(base + p.o_head); a.tail = (float*)(base + p.o_tail);
