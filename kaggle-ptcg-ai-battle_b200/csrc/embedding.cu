@@ -489,8 +489,8 @@ __global__ void __launch_bounds__(256) k_embed_sum(const __grid_constant__ SumAr
 
 // Joins the segments that cross blocks: the block of chunk c whose tail goes
 // on adds the heads of the chunks after it, up to and including the first
-// that the segment does not pass through.  32 columns a block column, 8
-// threads over the partials of each, combined in a fixed order.
+// that the segment does not pass through: a thread a column, or, for an id that
+// many chunks hold, 8 threads over the partials of each, combined in order.
 __global__ void __launch_bounds__(256) k_embed_join(const __grid_constant__ SumArgs a) {
     const int c = blockIdx.x;
     if (!(a.flags[c] & SEG_TAIL)) return;
@@ -510,6 +510,16 @@ __global__ void __launch_bounds__(256) k_embed_join(const __grid_constant__ SumA
     }
     __syncthreads();
     const int end = s_end, len = end - c;                   // partial rows: tail + len heads
+    if (len <= 16) {                                        // a thread a column
+        for (int x = blockIdx.y * 256 + threadIdx.x; x < a.width; x += gridDim.y * 256) {
+            float s = a.tail[(long)c * a.width + x];
+            #pragma unroll 4
+            for (int j = 0; j < len; j++) s += a.head[(long)(c + 1 + j) * a.width + x];
+            const float v[1] = {s};
+            put_row<1>(a, id, x, v);
+        }
+        return;
+    }
     const int per = (len + 7) / 8;
     for (int col = blockIdx.y * 32; col < a.width; col += gridDim.y * 32) {
         const int x = col + tx;
