@@ -479,36 +479,43 @@ __global__ void __launch_bounds__(128, DH == 32 ? 6 : DH == 64 ? 3 : 2) k_cross_
     }
 }
 
-// joins the parts of a split forward: a warp per stacked row
+// joins the parts of a split forward: a block per stacked row, whose warps take
+// every fourth part and are added in order (single tokens over a long cache
+// have few rows, and each has many parts)
 template <typename T, int DH>
-__global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ CrossArgs a, long nrows) {
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= nrows) return;
+__global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ CrossArgs a) {
+    constexpr int C = DH / 32;                      // columns a lane
+    __shared__ float sy[4][DH], sl[4];
+    const long row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float2* ml = a.part_ml + row * a.nsplit;
     float m = -INFINITY;
     for (int i = lane; i < a.nsplit; i += 32) m = fmaxf(m, ml[i].x);
     m = warp_max(m);
     const float u = m == -INFINITY ? 0.f : m;
-    float l = 0.f, y[DH / 32];
+    float l = 0.f, y[C];
     #pragma unroll
-    for (int e = 0; e < DH / 32; e++) y[e] = 0.f;
+    for (int e = 0; e < C; e++) y[e] = 0.f;
     const float* p = a.part + row * a.nsplit * DH + lane;
-    #pragma unroll 4
-    for (int i = 0; i < a.nsplit; i++) {
+    #pragma unroll 8
+    for (int i = warp; i < a.nsplit; i += 4) {
         const float2 x = ml[i];
         const float c = ex2_approx(x.x - u);
         l = fmaf(x.y, c, l);
         #pragma unroll
-        for (int e = 0; e < DH / 32; e++) y[e] = fmaf(p[(long)i * DH + e * 32], c, y[e]);
+        for (int e = 0; e < C; e++) y[e] = fmaf(p[(long)i * DH + e * 32], c, y[e]);
     }
+    #pragma unroll
+    for (int e = 0; e < C; e++) sy[warp][e * 32 + lane] = y[e];
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    l = sl[0] + sl[1] + sl[2] + sl[3];
     const long b = row / a.rows;
     const int seq = (int)(b / a.kv_heads), hk = (int)(b % a.kv_heads), r = (int)(row - b * a.rows);
-    T* out = (T*)a.out + qrow(a, a.so, seq, hk, r) + lane;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    #pragma unroll
-    for (int e = 0; e < DH / 32; e++) out[e * 32] = from_f<T>(y[e] * inv);
-    if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    for (int d = threadIdx.x; d < DH; d += 128)
+        ((T*)a.out + qrow(a, a.so, seq, hk, r))[d] = from_f<T>((sy[0][d] + sy[1][d] + sy[2][d] + sy[3][d]) * inv);
+    if (threadIdx.x == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 // --------------------------------------------------------- bf16 backward
@@ -1899,8 +1906,8 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
     if (e != cudaSuccess || p.sp.n == 1) return e;
     const long nrows = (long)c.nseq * c.kv_heads * a.rows;
     ++g_ptcg_launches;
-    if (c.dtype == PTCG_BF16) k_cross_join<bf16, DH><<<cdiv(nrows, 4), 128, 0, s>>>(a, nrows);
-    else k_cross_join<float, DH><<<cdiv(nrows, 4), 128, 0, s>>>(a, nrows);
+    if (c.dtype == PTCG_BF16) k_cross_join<bf16, DH><<<(unsigned)nrows, 128, 0, s>>>(a);
+    else k_cross_join<float, DH><<<(unsigned)nrows, 128, 0, s>>>(a);
     return cudaSuccess;
 }
 template <int DH, int NR>
