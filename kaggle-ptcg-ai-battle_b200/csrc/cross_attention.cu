@@ -1587,11 +1587,11 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dq_f32(const __
 
 // dk and dv of a key tile over the stacked rows (ROWS: at most 64 of them, all
 // in one tile, and dq as well: each block then walks the key tiles and S is
-// computed once, as in k_cross_bwd_rows)
-template <int DH, bool ROWS>
+// computed once, as in k_cross_bwd_rows; BQ rows in a tile, 16 for single tokens)
+template <int DH, bool ROWS, int BQ>
 __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
-    constexpr int RT = 8, BK = 64, LM = BK + 4, BQ = ROWS ? 64 : F32<DH>::BN, LQ = BQ + 4, LD = F32<DH>::LD;
-    constexpr int NC = BQ / 16, ND = DH / 16;
+    constexpr int RT = 8, BK = 64, LM = BK + 4, LQ = BQ + 4, LD = F32<DH>::LD;
+    constexpr int NC = BQ / 16, ND = DH / 16, RQ = ROWS ? BQ / 8 : 1;
     extern __shared__ __align__(16) float fs[];
     __shared__ uint8_t ok[BK];
     __shared__ float s_lse[BQ], s_delta[BQ];
@@ -1609,7 +1609,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
     const int kfrom = ROWS ? at.part * a.split : at.tile * BK;
     const int kto = ROWS ? min(a.lk, kfrom + a.split) : min(a.lk, kfrom + BK);
     const int qbeg = ROWS ? 0 : min(at.part * a.split, a.rows), qend = ROWS ? a.rows : min(a.rows, qbeg + a.split);
-    float dq[ROWS ? RT : 1][ROWS ? ND : 1];
+    float dq[RQ][ROWS ? ND : 1];
     clear(dq);
     auto stage_rows = [&](int q0) {
         stage_f32<DH, BQ>(Qs, (const float*)a.q, [&](int r) { return q_ptr(a, a.q, a.sq, at, q0 + r, qend); });
@@ -1676,7 +1676,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
                 __syncthreads();
                 mm_outer<RT, ND, BQ>(dv, Ps, LM, Gs, LD, ty, tx);
                 if constexpr (ROWS) {
-                    mm_outer<RT, ND, BK>(dq, Ds, LQ, Ks, LD, ty, tx);
+                    mm_outer<RQ, ND, BK>(dq, Ds, LQ, Ks, LD, ty, tx);
                     __syncthreads();
                     #pragma unroll
                     for (int j = 0; j < NC; j++) {
@@ -1705,8 +1705,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
     }
     if constexpr (ROWS) {
         #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int r = row_of<RT>(ty, i);
+        for (int i = 0; i < RQ; i++) {
+            const int r = row_of<RQ>(ty, i);
             if (r >= a.rows) continue;
             put_cols<ND>(a.nsplit > 1 ? a.part + ((row0 + r) * a.nsplit + at.part) * DH
                                       : (float*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), tx, dq[i], a.scale);
@@ -1766,7 +1766,9 @@ BwdPlan bwd_plan(const PtcgCross& c, bool tc) {
     BwdPlan p;
     const long group = c.heads / c.kv_heads, rows = group * c.lq, probs = (long)c.nseq * c.kv_heads;
     const long tile = tc ? TC_TILE : 64;
-    p.rows = rows > 0 && rows <= 64;
+    // (fp32 rows of width 128 spill registers in the one-kernel form past 16
+    // rows: 61 x 93 of them 2070 us a 512 x 8 batch, some 1700 in two kernels)
+    p.rows = rows > 0 && rows <= (c.dtype == PTCG_FP32 && c.dh == 128 ? 16 : 64);
     p.qtiles = (rows + tile - 1) / tile;
     p.ktiles = (c.lk + tile - 1) / tile;
     // dq: split over keys; dk and dv: over rows (tcgen05: in whole blocks of a head)
@@ -1876,13 +1878,12 @@ cudaError_t launch_dq_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
     ++g_ptcg_launches, k_cross_dq_f32<DH, RT><<<(unsigned)blocks, 128, bytes, s>>>(a);
     return cudaSuccess;
 }
-template <int DH, bool ROWS>
+template <int DH, bool ROWS, int BQ>
 cudaError_t launch_dkv_f32(const CrossArgs& a, long blocks, cudaStream_t s) {
-    constexpr int BQ = ROWS ? 64 : F32<DH>::BN;
-    const int bytes = 4 * (2 * (64 + BQ) * F32<DH>::LD + 2 * BQ * 68);
-    const cudaError_t e = smem_limit(k_cross_dkv_f32<DH, ROWS>, bytes);
+    const int bytes = 4 * (2 * (64 + BQ) * F32<DH>::LD + BQ * 68 + std::max(BQ * 68, 64 * (BQ + 4)));
+    const cudaError_t e = smem_limit(k_cross_dkv_f32<DH, ROWS, BQ>, bytes);
     if (e != cudaSuccess) return e;
-    ++g_ptcg_launches, k_cross_dkv_f32<DH, ROWS><<<(unsigned)blocks, 128, bytes, s>>>(a);
+    ++g_ptcg_launches, k_cross_dkv_f32<DH, ROWS, BQ><<<(unsigned)blocks, 128, bytes, s>>>(a);
     return cudaSuccess;
 }
 template <int DH>
@@ -1946,7 +1947,8 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, uint8_t* scratch, cudaStream
     parts(plain);
     if (plain.rows && plain.qblocks) {
         set_tiles(a, 1, plain.qs);
-        e = !bf ? launch_dkv_f32<DH, true>(a, plain.qblocks, s)
+        e = !bf ? (a.rows <= 16 ? launch_dkv_f32<DH, true, 16>(a, plain.qblocks, s)
+                                   : launch_dkv_f32<DH, true, DH == 128 ? 16 : 64>(a, plain.qblocks, s))
             : a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, plain.qblocks, s)
             : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, plain.qblocks, s) : launch_bwd_rows<DH, 4>(a, plain.qblocks, s);
         if (e == cudaSuccess && a.nsplit > 1) sum_parts<DH>(a, bf, nrows, 0, s);
@@ -1978,7 +1980,7 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, uint8_t* scratch, cudaStream
         if (e == cudaSuccess && !taken) {
             parts(plain);
             set_tiles(a, plain.ktiles, plain.ks);
-            e = bf ? launch_dkv<DH>(a, plain.kblocks, s) : launch_dkv_f32<DH, false>(a, plain.kblocks, s);
+            e = bf ? launch_dkv<DH>(a, plain.kblocks, s) : launch_dkv_f32<DH, false, F32<DH>::BN>(a, plain.kblocks, s);
         }
         if (e == cudaSuccess && a.nsplit > 1) sum_parts<DH>(a, bf, nkeys, 1, s);
     }

@@ -9,6 +9,7 @@
 // row in registers, so no cancellation between sums of squares; everything
 // is fp32 until the one rounding to the output's type.
 #include <algorithm>
+#include <initializer_list>
 
 #include "vec.cuh"
 
@@ -37,44 +38,69 @@ PTCG_DEV float row_sum(float v, float (*red)[32], int slot, int w, int lane, int
     return warp_sum(lane < W ? red[slot][lane] : 0.f);
 }
 
-template <typename TX, typename TY, int V, int NV, bool MULTI>
+// Columns of a row: `body` pieces of V from `head` on, and up to 2 (V - 1) single
+// ones at its ends, one each to the first lanes of the row's first warp.  Rows
+// that start on V-element boundaries have none of those; other rows are taken
+// PHASED: every row of a warp (or block) starts at the same phase, so that its
+// pieces are aligned and its lanes keep their columns (row steps are multiples
+// of V for that).
+template <int V, bool PHASED> struct Columns {
+    int head, body, edge;                           // edge: this lane's single column, or -1
+    PTCG_DEV Columns(int phase, int width, bool first_warp, int lane) {
+        head = PHASED ? (V - phase) & (V - 1) : 0;
+        if (PHASED && head > width) head = width;
+        body = (width - head) / V;
+        const int tail = width - head - body * V;
+        edge = !PHASED || !first_warp ? -1 : lane < head ? lane : lane < head + tail ? width - tail + lane - head : -1;
+    }
+    PTCG_DEV bool has(int p) const { return p < body; }
+    PTCG_DEV int at(int p) const { return head + p * V; }
+};
+
+template <typename TX, typename TY, int V, int NV, bool MULTI, bool PHASED>
 __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         TY* y, long ldy, float* mean, float* rstd, const TX* x, long ldx,
         const float* __restrict__ gamma, const float* __restrict__ beta, long rows, int width,
         float eps) {
     __shared__ float red[4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-    const int w = MULTI ? warp : 0, pieces = width / V;
+    const int w = MULTI ? warp : 0;
     const float inv = 1.f / (float)width;
+    const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
+    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
+    const int phase = PHASED ? (int)(((uintptr_t)x / sizeof(TX) + r * ldx) & (V - 1)) : 0;
+    const Columns<V, PHASED> cols(phase, width, w == 0, lane);
+    const bool edge = PHASED && cols.edge >= 0;
     float gm[NV][V], bt[NV][V];
     #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int p = piece_at<V, NV>(w, lane, k);
         #pragma unroll
-        for (int e = 0; e < V; e++) { gm[k][e] = 1.f; bt[k][e] = 0.f; }
-        if (p < pieces) {
-            #pragma unroll
-            for (int e = 0; e < V; e++) {
-                if (gamma) gm[k][e] = gamma[p * V + e];
-                if (beta) bt[k][e] = beta[p * V + e];
-            }
+        for (int e = 0; e < V; e++) {
+            gm[k][e] = gamma && cols.has(p) ? gamma[cols.at(p) + e] : 1.f;
+            bt[k][e] = beta && cols.has(p) ? beta[cols.at(p) + e] : 0.f;
         }
     }
-    const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
+    const float ge = edge && gamma ? gamma[cols.edge] : 1.f, be = edge && beta ? beta[cols.edge] : 0.f;
     // the next row's loads are in flight while this one is reduced, where the
     // registers allow it
     constexpr bool AHEAD = NV * V <= 8;
     Raw<TX, V> row[NV];
-    auto fetch = [&](long r) {
+    Raw<TX, 1> single;
+    auto fetch = [&](long i) {
+        const TX* xr = x + i * ldx;
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int p = piece_at<V, NV>(w, lane, k);
             row[k].zero();
-            if (r < rows && p < pieces) row[k].ld(x + r * ldx + (long)p * V);
+            if (i < rows && cols.has(p)) row[k].ld(xr + cols.at(p));
+        }
+        if (PHASED) {
+            single.zero();
+            if (i < rows && edge) single.ld(xr + cols.edge);
         }
     };
     int slot = 0;
-    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
     if (AHEAD) fetch(r);
     for (; r < rows; r += step) {
         float v[NV][V];
@@ -82,6 +108,11 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         if (!AHEAD) fetch(r);
         #pragma unroll
         for (int k = 0; k < NV; k++) row[k].get(v[k]);
+        float se[1] = {0.f};
+        if (PHASED) {
+            single.get(se);
+            s = se[0];
+        }
         if (AHEAD) fetch(r + step);
         #pragma unroll
         for (int k = 0; k < NV; k++)
@@ -92,10 +123,14 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         float q = 0.f;
         #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const float in = piece_at<V, NV>(w, lane, k) < pieces ? 1.f : 0.f;
+            const float in = cols.has(piece_at<V, NV>(w, lane, k)) ? 1.f : 0.f;
             #pragma unroll
-            for (int e = 0; e < V; e++) { const float d = (v[k][e] - mu) * in; q = fmaf(d, d, q); }
+            for (int e = 0; e < V; e++) {
+                const float d = (v[k][e] - mu) * in;
+                q = fmaf(d, d, q);
+            }
         }
+        if (edge) q = fmaf(se[0] - mu, se[0] - mu, q);
         const float rs = rsqrtf(fmaf(row_sum<MULTI>(q, red, slot + 1, w, lane, W), inv, eps));
         slot ^= 2;
         if (lane == 0 && w == 0) {
@@ -104,13 +139,12 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         }
         #pragma unroll
         for (int k = 0; k < NV; k++) {
+            #pragma unroll
+            for (int e = 0; e < V; e++) v[k][e] = fmaf((v[k][e] - mu) * rs, gm[k][e], bt[k][e]);
             const int p = piece_at<V, NV>(w, lane, k);
-            if (p < pieces) {
-                #pragma unroll
-                for (int e = 0; e < V; e++) v[k][e] = fmaf((v[k][e] - mu) * rs, gm[k][e], bt[k][e]);
-                VecIO<TY, V>::st(y + r * ldy + (long)p * V, v[k]);
-            }
+            if (cols.has(p)) VecIO<TY, V>::st(y + r * ldy + cols.at(p), v[k]);
         }
+        if (edge) y[r * ldy + cols.edge] = from_f<TY>(fmaf((se[0] - mu) * rs, ge, be));
     }
 }
 
@@ -119,48 +153,61 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
 // warp order through shared memory, as one partial row of dgamma and dbeta;
 // k_layer_norm_wgrad adds the blocks' partials in a fixed order.  No atomics,
 // so equal inputs give equal bits.
-template <typename TX, typename TY, int V, int NV, bool MULTI>
+template <typename TX, typename TY, int V, int NV, bool MULTI, bool PHASED>
 __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
         TX* dx, long lddx, const TY* dy, long lddy, const TX* x, long ldx,
         const TX* dres, long lddres, const float* __restrict__ gamma,
         const float* __restrict__ mean, const float* __restrict__ rstd, long rows, int width,
         float* __restrict__ partial) {
     __shared__ float red[4][32];
-    extern __shared__ float cols[];                 // [2][width] of a one-warp-per-row block
+    extern __shared__ float wsum[];                 // [2][width] of a one-warp-per-row block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-    const int w = MULTI ? warp : 0, pieces = width / V;
+    const int w = MULTI ? warp : 0;
     const float inv = 1.f / (float)width;
+    const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
+    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
+    const int phase = PHASED ? (int)(((uintptr_t)x / sizeof(TX) + r * ldx) & (V - 1)) : 0;
+    const Columns<V, PHASED> cols(phase, width, w == 0, lane);
+    const bool edge = PHASED && cols.edge >= 0;
     float gm[NV][V], ag[NV][V], ab[NV][V];
     #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int p = piece_at<V, NV>(w, lane, k);
         #pragma unroll
         for (int e = 0; e < V; e++) {
-            gm[k][e] = gamma && p < pieces ? gamma[p * V + e] : 1.f;
+            gm[k][e] = gamma && cols.has(p) ? gamma[cols.at(p) + e] : 1.f;
             ag[k][e] = ab[k][e] = 0.f;
         }
     }
-    const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
+    const float ge = edge && gamma ? gamma[cols.edge] : 1.f;
+    float age = 0.f, abe = 0.f;
     int slot = 0;
     // the next row's loads are in flight while this one is reduced, where the
     // registers allow it
     constexpr bool AHEAD = !MULTI && NV * V <= 8;
-    struct Row { Raw<TX, V> x[NV], r[NV]; Raw<TY, V> g[NV]; float mu, rs; } row;
-    auto fetch = [&](long r) {
+    struct Row { Raw<TX, V> x[NV], r[NV]; Raw<TY, V> g[NV]; Raw<TX, 1> xe, re; Raw<TY, 1> ge; float mu, rs; } row;
+    auto fetch = [&](long i) {
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int p = piece_at<V, NV>(w, lane, k);
             row.x[k].zero(); row.g[k].zero(); row.r[k].zero();
-            if (r < rows && p < pieces) {
-                row.x[k].ld(x + r * ldx + (long)p * V);
-                row.g[k].ld(dy + r * lddy + (long)p * V);
-                if (dres) row.r[k].ld(dres + r * lddres + (long)p * V);
+            if (i < rows && cols.has(p)) {
+                row.x[k].ld(x + i * ldx + cols.at(p));
+                row.g[k].ld(dy + i * lddy + cols.at(p));
+                if (dres) row.r[k].ld(dres + i * lddres + cols.at(p));
             }
         }
-        row.mu = r < rows ? mean[r] : 0.f;
-        row.rs = r < rows ? rstd[r] : 0.f;
+        if (PHASED) {
+            row.xe.zero(); row.ge.zero(); row.re.zero();
+            if (i < rows && edge) {
+                row.xe.ld(x + i * ldx + cols.edge);
+                row.ge.ld(dy + i * lddy + cols.edge);
+                if (dres) row.re.ld(dres + i * lddres + cols.edge);
+            }
+        }
+        row.mu = i < rows ? mean[i] : 0.f;
+        row.rs = i < rows ? rstd[i] : 0.f;
     };
-    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
     if (AHEAD) fetch(r);
     for (; r < rows; r += step) {
         float h[NV][V], g[NV][V], d[NV][V];
@@ -172,8 +219,22 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
             row.g[k].get(g[k]);
             row.r[k].get(d[k]);
         }
+        float xe[1] = {0.f}, gy[1] = {0.f}, re[1] = {0.f};
+        if (PHASED) {
+            row.xe.get(xe);
+            row.ge.get(gy);
+            row.re.get(re);
+        }
         if (AHEAD) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
+        if (PHASED) {                               // 0 gradient where there is no edge column
+            xe[0] = (xe[0] - mu) * rs;
+            age = fmaf(gy[0], xe[0], age);
+            abe += gy[0];
+            gy[0] *= ge;
+            s1 = gy[0];
+            s2 = gy[0] * xe[0];
+        }
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             #pragma unroll
@@ -202,15 +263,17 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
         const float m1 = __fmul_rn(s1, inv), m2 = __fmul_rn(s2, inv);
         #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int p = piece_at<V, NV>(w, lane, k);
-            if (p < pieces) {
-                #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float t = (g[k][e] - m1 - h[k][e] * m2) * rs;
-                    h[k][e] = dres ? t + d[k][e] : t;
-                }
-                VecIO<TX, V>::st(dx + r * lddx + (long)p * V, h[k]);
+            #pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float t = (g[k][e] - m1 - h[k][e] * m2) * rs;
+                h[k][e] = dres ? t + d[k][e] : t;
             }
+            const int p = piece_at<V, NV>(w, lane, k);
+            if (cols.has(p)) VecIO<TX, V>::st(dx + r * lddx + cols.at(p), h[k]);
+        }
+        if (edge) {
+            const float t = (gy[0] - m1 - xe[0] * m2) * rs;
+            dx[r * lddx + cols.edge] = from_f<TX>(dres ? t + re[0] : t);
         }
     }
     if (!partial) return;
@@ -219,33 +282,36 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int p = piece_at<V, NV>(w, lane, k);
-            if (p < pieces) {
-                #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    out[p * V + e] = ag[k][e];
-                    out[width + p * V + e] = ab[k][e];
-                }
+            if (!cols.has(p)) continue;
+            #pragma unroll
+            for (int e = 0; e < V; e++) {
+                out[cols.at(p) + e] = ag[k][e];
+                out[width + cols.at(p) + e] = ab[k][e];
             }
         }
+        if (edge) {
+            out[cols.edge] = age;
+            out[width + cols.edge] = abe;
+        }
     } else {
+        auto add = [&](int c, float g, float b, bool first) {
+            wsum[c] = first ? g : wsum[c] + g;
+            wsum[width + c] = first ? b : wsum[width + c] + b;
+        };
         for (int t = 0; t < W; t++) {
             if (warp == t) {
                 #pragma unroll
                 for (int k = 0; k < NV; k++) {
                     const int p = piece_at<V, NV>(0, lane, k);
-                    if (p < pieces) {
-                        #pragma unroll
-                        for (int e = 0; e < V; e++) {
-                            float* c = cols + p * V + e;
-                            c[0] = t ? c[0] + ag[k][e] : ag[k][e];
-                            c[width] = t ? c[width] + ab[k][e] : ab[k][e];
-                        }
-                    }
+                    if (!cols.has(p)) continue;
+                    #pragma unroll
+                    for (int e = 0; e < V; e++) add(cols.at(p) + e, ag[k][e], ab[k][e], t == 0);
                 }
+                if (edge) add(cols.edge, age, abe, t == 0);
             }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < 2 * width; i += blockDim.x) out[i] = cols[i];
+        for (int i = threadIdx.x; i < 2 * width; i += blockDim.x) out[i] = wsum[i];
     }
 }
 
@@ -272,57 +338,78 @@ __global__ void __launch_bounds__(256) k_layer_norm_wgrad(
     }
 }
 
-// the variant of a row width: V-column pieces, NV of them per lane, W warps a
-// row (0: one warp a row, eight rows a block)
-struct Cfg { int V, NV, W; };
-Cfg cfg_of(int width, bool vec) {
+// The variant of a row width: V-column pieces, NV of them per lane, W warps a
+// row (0: one warp a row, eight rows a block).  Rows that start on 4-element
+// boundaries and a width of fours take them whole, other rows PHASED where all
+// tensors' rows start at the same phase (bf16, 4099 x 5001, both passes: 68 us
+// against 117 with single elements), the rest single elements.
+enum { SINGLE = 0, WHOLE = 1, PHASED4 = 2 };
+struct Cfg { int mode, NV, W; };
+Cfg cfg_of(int width, int mode) {
     Cfg c;
-    c.V = vec ? 4 : 1;
-    if (width > WARP_COLS) {
-        c.NV = SHARED_COLS / (32 * c.V);
-        c.W = (int)cdiv(width, SHARED_COLS);
+    c.mode = mode;
+    const int V = mode == SINGLE ? 1 : 4, w = width;
+    c.W = 0;
+    if (w > WARP_COLS) {
+        c.NV = SHARED_COLS / (32 * V);
+        c.W = (int)cdiv(w, SHARED_COLS);
         return c;
     }
-    c.W = 0;
     c.NV = 1;
-    while (c.NV * 32 * c.V < width) c.NV *= 2;
-    if (c.V == 1 && c.NV < 4) c.NV = 4;
+    while (c.NV * 32 * V < w) c.NV *= 2;
+    if (V == 1) c.NV = c.NV <= 8 ? 8 : 32;
     return c;
 }
-// blocks of the backward pass: as many as the processors hold, at most one
-// per row group, so that each leaves one partial row of the weight gradients
+// how the rows of some tensors (up to four; null: none) can be taken
+struct Rows { const void* p; int dtype; long ld; };
+int mode_of(int width, std::initializer_list<Rows> all) {
+    bool whole = width % 4 == 0, same = true;
+    long start = -1, pitch = -1;
+    for (const Rows& t : all) {
+        if (!t.p) continue;
+        const long s = (long)((uintptr_t)t.p / dt_size(t.dtype) % 4), l = t.ld % 4;
+        whole = whole && s == 0 && l == 0;
+        if (start < 0) { start = s; pitch = l; }
+        same = same && s == start && l == pitch;
+    }
+    return whole ? WHOLE : same ? PHASED4 : SINGLE;
+}
+// blocks of the backward pass: as many as the processors hold (a multiple of
+// 4, for the phases), at most one per row group, so that each leaves one
+// partial row of the weight gradients
 int bwd_blocks(long rows, const Cfg& c) {
     const long units = c.W ? rows : (rows + 7) / 8;
-    const long most = c.W ? std::max(148 * 32 / c.W, 148) : 148 * 4;
+    const long most = c.W ? std::max(148 * 32 / c.W, 148) / 4 * 4 : 148 * 4;
     return (int)(units < most ? units : most);
 }
 
-template <typename TX, typename TY, int V, int NV, bool MULTI>
+template <typename TX, typename TY, int V, int NV, bool MULTI, bool PH>
 void fwd(void* y, long ldy, float* mean, float* rstd, const void* x, long ldx, const float* gamma,
          const float* beta, long rows, int width, float eps, int W, cudaStream_t s) {
     const long units = MULTI ? rows : (rows + 7) / 8;
-    const long most = MULTI ? std::max(148 * 64 / W, 148) : 148 * 8;
+    const long most = MULTI ? std::max(148 * 64 / W, 148) / 4 * 4 : 148 * 8;
     ++g_ptcg_launches;
-    k_layer_norm_fwd<TX, TY, V, NV, MULTI><<<(unsigned)(units < most ? units : most), MULTI ? W * 32 : 256, 0, s>>>(
+    k_layer_norm_fwd<TX, TY, V, NV, MULTI, PH><<<(unsigned)(units < most ? units : most), MULTI ? W * 32 : 256, 0, s>>>(
         (TY*)y, ldy, mean, rstd, (const TX*)x, ldx, gamma, beta, rows, width, eps);
 }
+// LN(V, NV, MULTI, PHASED) of a configuration
+#define LN_BY_CFG(c) do { \
+    if ((c).mode == SINGLE) { \
+        if ((c).W) LN(1, 8, true, false); else if ((c).NV == 8) LN(1, 8, false, false); else LN(1, 32, false, false); \
+    } else if ((c).mode == WHOLE) { \
+        if ((c).W) LN(4, 2, true, false); else if ((c).NV == 1) LN(4, 1, false, false); \
+        else if ((c).NV == 2) LN(4, 2, false, false); else if ((c).NV == 4) LN(4, 4, false, false); \
+        else LN(4, 8, false, false); \
+    } else { \
+        if ((c).W) LN(4, 2, true, true); else if ((c).NV == 1) LN(4, 1, false, true); \
+        else if ((c).NV == 2) LN(4, 2, false, true); else if ((c).NV == 4) LN(4, 4, false, true); \
+        else LN(4, 8, false, true); \
+    } } while (0)
 template <typename TX, typename TY>
 void fwd(const Cfg& c, void* y, long ldy, float* mean, float* rstd, const void* x, long ldx,
          const float* gamma, const float* beta, long rows, int width, float eps, cudaStream_t s) {
-    #define LN(V, NV, M) fwd<TX, TY, V, NV, M>(y, ldy, mean, rstd, x, ldx, gamma, beta, rows, width, eps, c.W, s)
-    if (c.V == 4) {
-        if (c.W) LN(4, 2, true);
-        else if (c.NV == 1) LN(4, 1, false);
-        else if (c.NV == 2) LN(4, 2, false);
-        else if (c.NV == 4) LN(4, 4, false);
-        else LN(4, 8, false);
-    } else {
-        if (c.W) LN(1, 8, true);
-        else if (c.NV == 4) LN(1, 4, false);
-        else if (c.NV == 8) LN(1, 8, false);
-        else if (c.NV == 16) LN(1, 16, false);
-        else LN(1, 32, false);
-    }
+    #define LN(V, NV, M, PH) fwd<TX, TY, V, NV, M, PH>(y, ldy, mean, rstd, x, ldx, gamma, beta, rows, width, eps, c.W, s)
+    LN_BY_CFG(c);
     #undef LN
 }
 
@@ -331,31 +418,20 @@ struct BwdArgs {
     const void* dres; long lddres; const float* gamma; const float* mean; const float* rstd;
     long rows; int width; float* partial;
 };
-template <typename TX, typename TY, int V, int NV, bool MULTI>
+template <typename TX, typename TY, int V, int NV, bool MULTI, bool PH>
 void bwd(const BwdArgs& a, int blocks, int W, cudaStream_t s) {
     ++g_ptcg_launches;
-    k_layer_norm_bwd<TX, TY, V, NV, MULTI><<<blocks, MULTI ? W * 32 : 256, MULTI ? 0 : 8 * a.width, s>>>(
+    k_layer_norm_bwd<TX, TY, V, NV, MULTI, PH><<<blocks, MULTI ? W * 32 : 256, MULTI ? 0 : 8 * a.width, s>>>(
         (TX*)a.dx, a.lddx, (const TY*)a.dy, a.lddy, (const TX*)a.x, a.ldx, (const TX*)a.dres,
         a.lddres, a.gamma, a.mean, a.rstd, a.rows, a.width, a.partial);
 }
 template <typename TX, typename TY>
 void bwd(const Cfg& c, const BwdArgs& a, int blocks, cudaStream_t s) {
-    #define LN(V, NV, M) bwd<TX, TY, V, NV, M>(a, blocks, c.W, s)
-    if (c.V == 4) {
-        if (c.W) LN(4, 2, true);
-        else if (c.NV == 1) LN(4, 1, false);
-        else if (c.NV == 2) LN(4, 2, false);
-        else if (c.NV == 4) LN(4, 4, false);
-        else LN(4, 8, false);
-    } else {
-        if (c.W) LN(1, 8, true);
-        else if (c.NV == 4) LN(1, 4, false);
-        else if (c.NV == 8) LN(1, 8, false);
-        else if (c.NV == 16) LN(1, 16, false);
-        else LN(1, 32, false);
-    }
+    #define LN(V, NV, M, PH) bwd<TX, TY, V, NV, M, PH>(a, blocks, c.W, s)
+    LN_BY_CFG(c);
     #undef LN
 }
+#undef LN_BY_CFG
 
 }  // namespace
 
@@ -373,7 +449,7 @@ int ptcg_layer_norm_fwd(const void* x, int x_dtype, long ldx, const float* gamma
     OP_REQ(el_ok(x, x_dtype) && el_ok(y, y_dtype) && el_ok(gamma, PTCG_FP32) && el_ok(beta, PTCG_FP32) &&
            el_ok(mean, PTCG_FP32) && el_ok(rstd, PTCG_FP32), PTCG_EINVAL,
            "layer norm: pointer not aligned to its element");
-    const Cfg c = cfg_of(width, width % 4 == 0 && vec_ok(x, x_dtype, ldx, 4) && vec_ok(y, y_dtype, ldy, 4));
+    const Cfg c = cfg_of(width, mode_of(width, {{x, x_dtype, ldx}, {y, y_dtype, ldy}}));
     cudaStream_t s = (cudaStream_t)stream;
     #define LN(TX, TY) fwd<TX, TY>(c, y, ldy, mean, rstd, x, ldx, gamma, beta, rows, width, eps, s)
     if (x_dtype == PTCG_BF16) { if (y_dtype == PTCG_BF16) LN(bf16, bf16); else LN(bf16, float); }
@@ -386,8 +462,7 @@ int ptcg_layer_norm_fwd(const void* x, int x_dtype, long ldx, const float* gamma
 long ptcg_layer_norm_bwd_scratch(long rows, int width) {
     OP_REQ(rows >= 0 && width > 0 && width <= MAXW, -1,
            "layer norm gradient: bad sizes (rows %ld, width %d of at most %d)", rows, width, MAXW);
-    // the scalar and the vector variant use the same number of blocks
-    return 8L * width * bwd_blocks(rows, cfg_of(width, true));
+    return 8L * width * bwd_blocks(rows, cfg_of(width, WHOLE));    // the same for every variant
 }
 
 int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, int x_dtype,
@@ -416,8 +491,8 @@ int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, 
     const long need = ptcg_layer_norm_bwd_scratch(rows, width);
     OP_REQ(!dgamma || (scratch && scratch_bytes >= need), PTCG_ERANGE,
            "layer norm gradient: scratch of %ld bytes, %ld needed", scratch ? scratch_bytes : 0L, need);
-    const Cfg c = cfg_of(width, width % 4 == 0 && vec_ok(x, x_dtype, ldx, 4) && vec_ok(dy, dy_dtype, lddy, 4) &&
-                         vec_ok(dx, x_dtype, lddx, 4) && vec_ok(dres, x_dtype, lddres, 4));
+    const Cfg c = cfg_of(width, mode_of(width, {{x, x_dtype, ldx}, {dy, dy_dtype, lddy}, {dx, x_dtype, lddx},
+                                                {dres, x_dtype, lddres}}));
     const int blocks = bwd_blocks(rows, c);
     const BwdArgs a = {dx, lddx, dy, lddy, x, ldx, dres, lddres, gamma, mean, rstd, rows, width,
                        dgamma ? (float*)scratch : nullptr};

@@ -186,6 +186,31 @@ def test_layer_norm_plain_views_and_empty(ops):
     assert dx.shape == (0, 300) and (dg == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("xd,yd", list(itertools.product([F32, BF16], repeat=2)))
+@pytest.mark.parametrize("width", [3, 62, 127, 130, 509, 1021, 1023, 1026, 2051, 4099, 8191])
+def test_layer_norm_row_phases(ops, xd, yd, width):
+    """Rows that start anywhere: odd pitches, tensors that start off a boundary
+    together or apart, rows enough for every block to take several."""
+    g = gen(width)
+    rows = 1300 if width < 1100 else 701
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    gamma, beta = 1 + 0.3 * rand(g, width), rand(g, width)
+    for pitch, offs in ((width, 0), (width + 2, 1), (width + 5, 3), (width + 8, 2)):
+        buf = rand(g, rows * pitch + 8, dtype=xd)
+        x = buf[offs:offs + rows * pitch].view(rows, pitch)[:, :width]
+        f = ref.norm(x, gamma, beta, eps)
+        y, mean, rstd = ops.layer_norm(x, gamma, beta, out_dtype=yd)
+        ref.within(y, f["y"], f["e_y"] + ref.HALF[yd] * (f["y"].abs() + f["e_y"]), "y")
+        gb = rand(g, rows * pitch + 8, dtype=yd)
+        for o2 in (offs, (offs + 1) % 4):            # at x's phase, and at another
+            dy = gb[o2:o2 + rows * pitch].view(rows, pitch)[:, :width]
+            dx, e_dx, dg, e_dg, db, e_db = ref.norm_grad(f, dy, x, xd)
+            got = ops.layer_norm_backward(dy, x, gamma, mean, rstd, dres=x)
+            ref.within(got[0], dx, 2 * e_dx, "dx")
+            ref.within(got[1], dg, 2 * e_dg, "dgamma")
+            ref.within(got[2], db, e_db, "dbeta")
+
+
 def test_layer_norm_in_place(pkg, ops):
     """y over x, dx over dres and dx over dy through the C entry."""
     import ptcg_b200.native as n
