@@ -1587,7 +1587,9 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dq_f32(const __
 
 // dk and dv of a key tile over the stacked rows (ROWS: at most 64 of them, all
 // in one tile, and dq as well: each block then walks the key tiles and S is
-// computed once, as in k_cross_bwd_rows; BQ rows in a tile, 16 for single tokens)
+// computed once, as in k_cross_bwd_rows; tiles of BQ = 16, 32 or 64 rows, the
+// smallest that holds them: 24 rows of width 128 on 93 keys, 512 x 8 of them,
+// 1066 us in 32 against 1998 in 64)
 template <int DH, bool ROWS, int BQ>
 __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const __grid_constant__ CrossArgs a) {
     constexpr int RT = 8, BK = 64, LM = BK + 4, LQ = BQ + 4, LD = F32<DH>::LD;
@@ -1752,7 +1754,7 @@ FwdPlan fwd_plan(const PtcgCross& c) {
     const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
     p.few = rows <= 16;
     p.tc = use_tc(c, rows);
-    p.bm = p.few ? 16 : p.tc ? TC_ROWS : 64;
+    p.bm = p.few ? 16 : c.dtype == PTCG_FP32 && rows <= 32 ? 32 : p.tc ? TC_ROWS : 64;
     p.tiles = (rows + p.bm - 1) / p.bm;
     p.sp = split_of(p.tiles * probs, c.lk, p.tc);
     p.blocks = p.tiles * probs * p.sp.n;
@@ -1766,9 +1768,7 @@ BwdPlan bwd_plan(const PtcgCross& c, bool tc) {
     BwdPlan p;
     const long group = c.heads / c.kv_heads, rows = group * c.lq, probs = (long)c.nseq * c.kv_heads;
     const long tile = tc ? TC_TILE : 64;
-    // (fp32 rows of width 128 spill registers in the one-kernel form past 16
-    // rows: 61 x 93 of them 2070 us a 512 x 8 batch, some 1700 in two kernels)
-    p.rows = rows > 0 && rows <= (c.dtype == PTCG_FP32 && c.dh == 128 ? 16 : 64);
+    p.rows = rows > 0 && rows <= 64;
     p.qtiles = (rows + tile - 1) / tile;
     p.ktiles = (c.lk + tile - 1) / tile;
     // dq: split over keys; dk and dv: over rows (tcgen05: in whole blocks of a head)
@@ -1903,7 +1903,8 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
             : p.sp.n == 1 && is_short(c.lk, short_fwd_bytes(DH, c.lk)) ? launch_fwd_short<DH>(a, p.blocks, s)
             : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
     else if (!p.tc)
-        e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
+        e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s)
+            : p.bm == 32 ? launch_fwd_f32<DH, 4>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
     if (e != cudaSuccess || p.sp.n == 1) return e;
     const long nrows = (long)c.nseq * c.kv_heads * a.rows;
     ++g_ptcg_launches;
@@ -1948,7 +1949,8 @@ cudaError_t bwd_dh(CrossArgs a, const PtcgCross& c, uint8_t* scratch, cudaStream
     if (plain.rows && plain.qblocks) {
         set_tiles(a, 1, plain.qs);
         e = !bf ? (a.rows <= 16 ? launch_dkv_f32<DH, true, 16>(a, plain.qblocks, s)
-                                   : launch_dkv_f32<DH, true, DH == 128 ? 16 : 64>(a, plain.qblocks, s))
+                   : a.rows <= 32 ? launch_dkv_f32<DH, true, 32>(a, plain.qblocks, s)
+                                  : launch_dkv_f32<DH, true, 64>(a, plain.qblocks, s))
             : a.rows <= 16 ? launch_bwd_rows<DH, 1>(a, plain.qblocks, s)
             : a.rows <= 32 ? launch_bwd_rows<DH, 2>(a, plain.qblocks, s) : launch_bwd_rows<DH, 4>(a, plain.qblocks, s);
         if (e == cudaSuccess && a.nsplit > 1) sum_parts<DH>(a, bf, nrows, 0, s);

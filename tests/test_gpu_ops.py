@@ -297,7 +297,8 @@ CROSS = [  # nseq, lq, lk, heads, kv_heads, dh
     (1, 1, 1, 1, 1, 32), (4, 1, 129, 8, 8, 32), (3, 1, 700, 8, 2, 64), (2, 1, 3000, 8, 1, 128),
     (5, 64, 129, 8, 8, 32), (3, 17, 63, 4, 2, 64), (2, 65, 64, 2, 2, 128), (2, 130, 65, 4, 1, 32),
     (1, 63, 1000, 2, 1, 128), (1, 700, 33, 3, 3, 64), (1, 1500, 70, 2, 1, 32), (7, 5, 8, 6, 3, 32),
-    (2, 16, 257, 1, 1, 128), (1, 300, 520, 4, 4, 128), (300, 9, 31, 2, 1, 32)]
+    (2, 16, 257, 1, 1, 128), (1, 300, 520, 4, 4, 128), (300, 9, 31, 2, 1, 32), (4, 31, 150, 2, 2, 128),
+    (3, 10, 70, 4, 2, 64), (2, 24, 2100, 2, 2, 32)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
