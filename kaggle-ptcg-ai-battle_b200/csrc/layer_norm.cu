@@ -19,7 +19,7 @@ constexpr int MAXW = PTCG_LN_MAX_WIDTH;
 // one warp holds rows of up to 1024 columns, NV pieces of V columns per lane;
 // wider rows are shared by the warps of a block, 256 columns each, so that the
 // backward's registers per column still fit 1024 threads
-constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MAX_THREADS = MAXW / SHARED_COLS * 32;
+constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MID_THREADS = 640, MAX_THREADS = MAXW / SHARED_COLS * 32;
 
 // Bound: HBM.  A row belongs to one warp (width <= 1024, eight rows to a
 // block) or to the W warps of a block (MULTI).  Lane l of warp w owns pieces
@@ -27,15 +27,20 @@ constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MAX_THREADS = MAXW / SHARED_C
 template <int V, int NV>
 PTCG_DEV int piece_at(int w, int lane, int k) { return (w * NV + k) * 32 + lane; }
 
-// sum of v over the row's warps; `slot` alternates so that one barrier per
-// reduction is enough
-template <bool MULTI>
-PTCG_DEV float row_sum(float v, float (*red)[32], int slot, int w, int lane, int W) {
-    v = warp_sum(v);
-    if (!MULTI) return v;
-    if (lane == 0) red[slot][w] = v;
+// sums of N values over the row's warps; `slot` alternates so that one barrier
+// per reduction is enough
+template <int MULTI, int N>
+PTCG_DEV void row_sums(float (&v)[N], float (*red)[N][32], int slot, int w, int lane, int W) {
+    #pragma unroll
+    for (int i = 0; i < N; i++) v[i] = warp_sum(v[i]);
+    if (!MULTI) return;
+    if (lane == 0) {
+        #pragma unroll
+        for (int i = 0; i < N; i++) red[slot][i][w] = v[i];
+    }
     __syncthreads();
-    return warp_sum(lane < W ? red[slot][lane] : 0.f);
+    #pragma unroll
+    for (int i = 0; i < N; i++) v[i] = warp_sum(lane < W ? red[slot][i][lane] : 0.f);
 }
 
 // Columns of a row: `body` pieces of V from `head` on, and up to 2 (V - 1) single
@@ -57,18 +62,19 @@ template <int V, bool PHASED> struct Columns {
     PTCG_DEV int at(int p) const { return head + p * V; }
 };
 
-template <typename TX, typename TY, int V, int NV, bool MULTI, bool PHASED>
-__global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
+template <typename TX, typename TY, int V, int NV, int MULTI, bool PHASED>
+__global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
         TY* y, long ldy, float* mean, float* rstd, const TX* x, long ldx,
         const float* __restrict__ gamma, const float* __restrict__ beta, long rows, int width,
         float eps) {
-    __shared__ float red[4][32];
+    constexpr int R = MULTI == MID_THREADS ? 2 : 1;
+    __shared__ float red[4][R][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int w = MULTI ? warp : 0;
     const float inv = 1.f / (float)width;
     const long step = MULTI ? gridDim.x : (long)gridDim.x * W;
-    long r = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
-    const int phase = PHASED ? (int)(((uintptr_t)x / sizeof(TX) + r * ldx) & (V - 1)) : 0;
+    long r0 = MULTI ? blockIdx.x : (long)blockIdx.x * W + warp;
+    const int phase = PHASED ? (int)(((uintptr_t)x / sizeof(TX) + r0 * ldx) & (V - 1)) : 0;
     const Columns<V, PHASED> cols(phase, width, w == 0, lane);
     const bool edge = PHASED && cols.edge >= 0;
     float gm[NV][V], bt[NV][V];
@@ -82,69 +88,85 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
         }
     }
     const float ge = edge && gamma ? gamma[cols.edge] : 1.f, be = edge && beta ? beta[cols.edge] : 0.f;
-    // the next row's loads are in flight while this one is reduced, where the
-    // registers allow it
+    // R rows at a time, the next ones' loads in flight while these are reduced,
+    // where the registers allow it
     constexpr bool AHEAD = NV * V <= 8;
-    Raw<TX, V> row[NV];
-    Raw<TX, 1> single;
-    auto fetch = [&](long i) {
-        const TX* xr = x + i * ldx;
+    Raw<TX, V> row[R][NV];
+    Raw<TX, 1> single[R];
+    auto fetch = [&](long i0) {
         #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int p = piece_at<V, NV>(w, lane, k);
-            row[k].zero();
-            if (i < rows && cols.has(p)) row[k].ld(xr + cols.at(p));
-        }
-        if (PHASED) {
-            single.zero();
-            if (i < rows && edge) single.ld(xr + cols.edge);
+        for (int j = 0; j < R; j++) {
+            const long i = i0 + j * step;
+            const TX* xr = x + i * ldx;
+            #pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int p = piece_at<V, NV>(w, lane, k);
+                row[j][k].zero();
+                if (i < rows && cols.has(p)) row[j][k].ld(xr + cols.at(p));
+            }
+            if (PHASED) {
+                single[j].zero();
+                if (i < rows && edge) single[j].ld(xr + cols.edge);
+            }
         }
     };
     int slot = 0;
-    if (AHEAD) fetch(r);
-    for (; r < rows; r += step) {
-        float v[NV][V];
-        float s = 0.f;
-        if (!AHEAD) fetch(r);
+    if (AHEAD) fetch(r0);
+    for (; r0 < rows; r0 += R * step) {
+        float v[R][NV][V], s[R], mu[R], rs[R], se[R][1];
+        if (!AHEAD) fetch(r0);
         #pragma unroll
-        for (int k = 0; k < NV; k++) row[k].get(v[k]);
-        float se[1] = {0.f};
-        if (PHASED) {
-            single.get(se);
-            s = se[0];
+        for (int j = 0; j < R; j++) {
+            #pragma unroll
+            for (int k = 0; k < NV; k++) row[j][k].get(v[j][k]);
+            se[j][0] = 0.f;
+            if (PHASED) single[j].get(se[j]);
+            s[j] = se[j][0];
         }
-        if (AHEAD) fetch(r + step);
+        if (AHEAD) fetch(r0 + R * step);
         #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int j = 0; j < R; j++)
             #pragma unroll
-            for (int e = 0; e < V; e++) s += v[k][e];
-        // rounded here, so that x - mu is the same whether or not mean is stored
-        const float mu = __fmul_rn(row_sum<MULTI>(s, red, slot, w, lane, W), inv);
-        float q = 0.f;
+            for (int k = 0; k < NV; k++)
+                #pragma unroll
+                for (int e = 0; e < V; e++) s[j] += v[j][k][e];
+        row_sums<MULTI>(s, red, slot, w, lane, W);
         #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const float in = cols.has(piece_at<V, NV>(w, lane, k)) ? 1.f : 0.f;
+        for (int j = 0; j < R; j++) {
+            // rounded here, so that x - mu is the same whether or not mean is stored
+            mu[j] = __fmul_rn(s[j], inv);
+            s[j] = 0.f;
             #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = (v[k][e] - mu) * in;
-                q = fmaf(d, d, q);
+            for (int k = 0; k < NV; k++) {
+                const float in = cols.has(piece_at<V, NV>(w, lane, k)) ? 1.f : 0.f;
+                #pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float d = (v[j][k][e] - mu[j]) * in;
+                    s[j] = fmaf(d, d, s[j]);
+                }
             }
+            if (edge) s[j] = fmaf(se[j][0] - mu[j], se[j][0] - mu[j], s[j]);
         }
-        if (edge) q = fmaf(se[0] - mu, se[0] - mu, q);
-        const float rs = rsqrtf(fmaf(row_sum<MULTI>(q, red, slot + 1, w, lane, W), inv, eps));
+        row_sums<MULTI>(s, red, slot + 1, w, lane, W);
         slot ^= 2;
-        if (lane == 0 && w == 0) {
-            if (mean) mean[r] = mu;
-            if (rstd) rstd[r] = rs;
-        }
         #pragma unroll
-        for (int k = 0; k < NV; k++) {
+        for (int j = 0; j < R; j++) {
+            const long r = r0 + j * step;
+            if (j && r >= rows) break;
+            rs[j] = rsqrtf(fmaf(s[j], inv, eps));
+            if (lane == 0 && w == 0) {
+                if (mean) mean[r] = mu[j];
+                if (rstd) rstd[r] = rs[j];
+            }
             #pragma unroll
-            for (int e = 0; e < V; e++) v[k][e] = fmaf((v[k][e] - mu) * rs, gm[k][e], bt[k][e]);
-            const int p = piece_at<V, NV>(w, lane, k);
-            if (cols.has(p)) VecIO<TY, V>::st(y + r * ldy + cols.at(p), v[k]);
+            for (int k = 0; k < NV; k++) {
+                #pragma unroll
+                for (int e = 0; e < V; e++) v[j][k][e] = fmaf((v[j][k][e] - mu[j]) * rs[j], gm[k][e], bt[k][e]);
+                const int p = piece_at<V, NV>(w, lane, k);
+                if (cols.has(p)) VecIO<TY, V>::st(y + r * ldy + cols.at(p), v[j][k]);
+            }
+            if (edge) y[r * ldy + cols.edge] = from_f<TY>(fmaf((se[j][0] - mu[j]) * rs[j], ge, be));
         }
-        if (edge) y[r * ldy + cols.edge] = from_f<TY>(fmaf((se[0] - mu) * rs, ge, be));
     }
 }
 
@@ -153,13 +175,13 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_fwd(
 // warp order through shared memory, as one partial row of dgamma and dbeta;
 // k_layer_norm_wgrad adds the blocks' partials in a fixed order.  No atomics,
 // so equal inputs give equal bits.
-template <typename TX, typename TY, int V, int NV, bool MULTI, bool PHASED>
-__global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
+template <typename TX, typename TY, int V, int NV, int MULTI, bool PHASED>
+__global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_bwd(
         TX* dx, long lddx, const TY* dy, long lddy, const TX* x, long ldx,
         const TX* dres, long lddres, const float* __restrict__ gamma,
         const float* __restrict__ mean, const float* __restrict__ rstd, long rows, int width,
         float* __restrict__ partial) {
-    __shared__ float red[4][32];
+    __shared__ float red[2][2][32];
     extern __shared__ float wsum[];                 // [2][width] of a one-warp-per-row block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int w = MULTI ? warp : 0;
@@ -182,9 +204,8 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
     const float ge = edge && gamma ? gamma[cols.edge] : 1.f;
     float age = 0.f, abe = 0.f;
     int slot = 0;
-    // the next row's loads are in flight while this one is reduced, where the
-    // registers allow it
-    constexpr bool AHEAD = !MULTI && NV * V <= 8;
+    // as in the forward, a row at a time
+    constexpr bool AHEAD = MULTI != MAX_THREADS && NV * V <= 8;
     struct Row { Raw<TX, V> x[NV], r[NV]; Raw<TY, V> g[NV]; Raw<TX, 1> xe, re; Raw<TY, 1> ge; float mu, rs; } row;
     auto fetch = [&](long i) {
         #pragma unroll
@@ -210,7 +231,7 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
     };
     if (AHEAD) fetch(r);
     for (; r < rows; r += step) {
-        float h[NV][V], g[NV][V], d[NV][V];
+        float h[NV][V], g[NV][V], d[NV][V], s[2] = {0.f, 0.f};
         if (!AHEAD) fetch(r);
         const float mu = row.mu, rs = row.rs;
         #pragma unroll
@@ -226,14 +247,13 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
             row.re.get(re);
         }
         if (AHEAD) fetch(r + step);
-        float s1 = 0.f, s2 = 0.f;
         if (PHASED) {                               // 0 gradient where there is no edge column
             xe[0] = (xe[0] - mu) * rs;
             age = fmaf(gy[0], xe[0], age);
             abe += gy[0];
             gy[0] *= ge;
-            s1 = gy[0];
-            s2 = gy[0] * xe[0];
+            s[0] = gy[0];
+            s[1] = gy[0] * xe[0];
         }
         #pragma unroll
         for (int k = 0; k < NV; k++) {
@@ -244,23 +264,13 @@ __global__ void __launch_bounds__(MULTI ? MAX_THREADS : 256) k_layer_norm_bwd(
                 ab[k][e] += g[k][e];
                 g[k][e] *= gm[k][e];
                 h[k][e] = hh;
-                s1 += g[k][e];
-                s2 = fmaf(g[k][e], hh, s2);
+                s[0] += g[k][e];
+                s[1] = fmaf(g[k][e], hh, s[1]);
             }
         }
-        if (MULTI) {
-            s1 = warp_sum(s1);
-            s2 = warp_sum(s2);
-            if (lane == 0) { red[slot][w] = s1; red[slot + 1][w] = s2; }
-            __syncthreads();
-            s1 = warp_sum(lane < W ? red[slot][lane] : 0.f);
-            s2 = warp_sum(lane < W ? red[slot + 1][lane] : 0.f);
-            slot ^= 2;
-        } else {
-            s1 = warp_sum(s1);
-            s2 = warp_sum(s2);
-        }
-        const float m1 = __fmul_rn(s1, inv), m2 = __fmul_rn(s2, inv);
+        row_sums<MULTI>(s, red, slot, w, lane, W);
+        slot ^= 1;
+        const float m1 = __fmul_rn(s[0], inv), m2 = __fmul_rn(s[1], inv);
         #pragma unroll
         for (int k = 0; k < NV; k++) {
             #pragma unroll
@@ -341,8 +351,9 @@ __global__ void __launch_bounds__(256) k_layer_norm_wgrad(
 // The variant of a row width: V-column pieces, NV of them per lane, W warps a
 // row (0: one warp a row, eight rows a block).  Rows that start on 4-element
 // boundaries and a width of fours take them whole, other rows PHASED where all
-// tensors' rows start at the same phase (bf16, 4099 x 5001, both passes: 68 us
-// against 117 with single elements), the rest single elements.
+// tensors' rows start at the same phase (4099 x 5001 in bf16: 24.8 + 55.5 us
+// forward and backward against 32.5 + 59.5 with single elements; 50000 x 634
+// in fp32: 74 + 119 against 76 + 128), the rest single elements.
 enum { SINGLE = 0, WHOLE = 1, PHASED4 = 2 };
 struct Cfg { int mode, NV, W; };
 Cfg cfg_of(int width, int mode) {
@@ -374,36 +385,44 @@ int mode_of(int width, std::initializer_list<Rows> all) {
     }
     return whole ? WHOLE : same ? PHASED4 : SINGLE;
 }
+// blocks of W warps that a processor's registers hold: each then takes its
+// share of the rows in one go (a second, partial wave of blocks: 35.4
+// and 69 us at 4099 x 5001 instead of 24.7 and 55)
+int resident(int W) { return std::max(MID_THREADS / 32 / W, 1); }
 // blocks of the backward pass: as many as the processors hold (a multiple of
-// 4, for the phases), at most one per row group, so that each leaves one
+// 4, as 148 is, for the phases), at most one per row group, so that each leaves one
 // partial row of the weight gradients
 int bwd_blocks(long rows, const Cfg& c) {
     const long units = c.W ? rows : (rows + 7) / 8;
-    const long most = c.W ? std::max(148 * 32 / c.W, 148) / 4 * 4 : 148 * 4;
+    const long most = 148L * (c.W ? resident(c.W) : 4);
     return (int)(units < most ? units : most);
 }
 
-template <typename TX, typename TY, int V, int NV, bool MULTI, bool PH>
+template <typename TX, typename TY, int V, int NV, int MULTI, bool PH>
 void fwd(void* y, long ldy, float* mean, float* rstd, const void* x, long ldx, const float* gamma,
          const float* beta, long rows, int width, float eps, int W, cudaStream_t s) {
     const long units = MULTI ? rows : (rows + 7) / 8;
-    const long most = MULTI ? std::max(148 * 64 / W, 148) / 4 * 4 : 148 * 8;
+    const long most = 148L * (MULTI ? resident(W) : 8);
     ++g_ptcg_launches;
     k_layer_norm_fwd<TX, TY, V, NV, MULTI, PH><<<(unsigned)(units < most ? units : most), MULTI ? W * 32 : 256, 0, s>>>(
         (TY*)y, ldy, mean, rstd, (const TX*)x, ldx, gamma, beta, rows, width, eps);
 }
-// LN(V, NV, MULTI, PHASED) of a configuration
+// LN(V, NV, MULTI, PHASED) of a configuration; MULTI: the most threads of a
+// block whose warps share rows (a bound that leaves each its registers), 0: a
+// warp takes rows alone
+#define LN_WIDE(c, V, NV, PH) do { \
+    if ((c).W * 32 <= MID_THREADS) LN(V, NV, MID_THREADS, PH); else LN(V, NV, MAX_THREADS, PH); } while (0)
 #define LN_BY_CFG(c) do { \
     if ((c).mode == SINGLE) { \
-        if ((c).W) LN(1, 8, true, false); else if ((c).NV == 8) LN(1, 8, false, false); else LN(1, 32, false, false); \
+        if ((c).W) LN(1, 8, MAX_THREADS, false); else if ((c).NV == 8) LN(1, 8, 0, false); else LN(1, 32, 0, false); \
     } else if ((c).mode == WHOLE) { \
-        if ((c).W) LN(4, 2, true, false); else if ((c).NV == 1) LN(4, 1, false, false); \
-        else if ((c).NV == 2) LN(4, 2, false, false); else if ((c).NV == 4) LN(4, 4, false, false); \
-        else LN(4, 8, false, false); \
+        if ((c).W) LN_WIDE(c, 4, 2, false); else if ((c).NV == 1) LN(4, 1, 0, false); \
+        else if ((c).NV == 2) LN(4, 2, 0, false); else if ((c).NV == 4) LN(4, 4, 0, false); \
+        else LN(4, 8, 0, false); \
     } else { \
-        if ((c).W) LN(4, 2, true, true); else if ((c).NV == 1) LN(4, 1, false, true); \
-        else if ((c).NV == 2) LN(4, 2, false, true); else if ((c).NV == 4) LN(4, 4, false, true); \
-        else LN(4, 8, false, true); \
+        if ((c).W) LN_WIDE(c, 4, 2, true); else if ((c).NV == 1) LN(4, 1, 0, true); \
+        else if ((c).NV == 2) LN(4, 2, 0, true); else if ((c).NV == 4) LN(4, 4, 0, true); \
+        else LN(4, 8, 0, true); \
     } } while (0)
 template <typename TX, typename TY>
 void fwd(const Cfg& c, void* y, long ldy, float* mean, float* rstd, const void* x, long ldx,
@@ -418,7 +437,7 @@ struct BwdArgs {
     const void* dres; long lddres; const float* gamma; const float* mean; const float* rstd;
     long rows; int width; float* partial;
 };
-template <typename TX, typename TY, int V, int NV, bool MULTI, bool PH>
+template <typename TX, typename TY, int V, int NV, int MULTI, bool PH>
 void bwd(const BwdArgs& a, int blocks, int W, cudaStream_t s) {
     ++g_ptcg_launches;
     k_layer_norm_bwd<TX, TY, V, NV, MULTI, PH><<<blocks, MULTI ? W * 32 : 256, MULTI ? 0 : 8 * a.width, s>>>(
@@ -432,6 +451,7 @@ void bwd(const Cfg& c, const BwdArgs& a, int blocks, cudaStream_t s) {
     #undef LN
 }
 #undef LN_BY_CFG
+#undef LN_WIDE
 
 }  // namespace
 
