@@ -469,8 +469,9 @@ int ptcg_attention_bwd(int operand_dtype, const void* qkv, long ldqkv, const uns
  * model's gathers clamp theirs; a place whose id equals pad_id (>= 0; pass -1
  * for none) gives zeros and takes no gradient.  The gradient sorts the places
  * by id and writes every row of dtable (vocab x width fp32, pitch lddt) once:
- *   dtable[v, :] = scale * sum of dout[i, :] over ids[i] = v, in place order
- * (0 for a row without places; accumulate != 0 adds to what is there).
+ *   dtable[v, :] = scale * sum of dout[i, :] over ids[i] = v
+ * (0 for a row without places; accumulate != 0 adds to what is there), in an
+ * order that follows from the ids alone.  width <= 65535 * 32, n < 2^31.
  * Replaces the gathers and atomic scatter-adds of k_tok_cat / k_tok_cat_bwd
  * (native/model/ptcg_model.cu:289-321, ptcg_model2.cu:36-64) for callers with
  * their own token tables. */
@@ -516,7 +517,7 @@ int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, 
  * zero for masked keys.  Each tensor has its own strides in elements:
  * element (s, row, head, d) at p + s * seq + row * row + head * head + d.
  * bf16 runs on tensor cores with fp32 sums (P and dS are rounded to bf16 as
- * operands); fp32 is exact.  Rows must start on 16-byte boundaries (strides
+ * operands); fp32 is fp32 throughout.  scale is positive and finite.  Rows must start on 16-byte boundaries (strides
  * multiples of 16 bytes).  Beside ptcg_attention_fwd / _bwd, which take
  * packed self-attention rows of width 32. */
 typedef struct PtcgHeads { long seq, row, head; } PtcgHeads;

@@ -7,7 +7,8 @@ enqueued on that device's current stream, on outputs and scratch that come
 from torch's allocator.  Nothing waits on the host, so the calls can be
 captured in a CUDA graph.  A tensor last used on another stream has to be
 ordered before the call by the caller, as for any torch operation.  Arguments
-are checked before anything is launched; errors raise `PtcgError`.
+are checked before anything is launched; errors raise `PtcgError`.  Nothing is
+recorded for autograd: the gradients are calls of their own.
 """
 from __future__ import annotations
 
@@ -123,8 +124,8 @@ def embedding(table, ids, scale=1.0, pad_id=None, out_dtype=None):
 
 def embedding_backward(dout, ids, vocab, scale=1.0, pad_id=None, dtable=None, accumulate=False):
     """Gradient of `embedding` for its table: float32 (vocab, width), every row
-    the sum of its places' gradients in place order.  With accumulate, added
-    to dtable."""
+    the sum of its places' gradients, in an order that follows from the ids
+    alone.  With accumulate, added to dtable."""
     dev = dout.device
     ids = _ids(ids, dev)
     if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:

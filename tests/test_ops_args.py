@@ -39,7 +39,7 @@ def emb_bwd(lib, dout=A, dd=0, lddo=8, ids=A, n=2, dtable=A, lddt=8, vocab=4, wi
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(dd=3), EINVAL), (dict(vocab=-1), EINVAL), (dict(width=0), EINVAL), (dict(n=-1), EINVAL),
-    (dict(n=1 << 31), EINVAL), (dict(lddo=4), EINVAL), (dict(lddt=4), EINVAL),
+    (dict(n=1 << 31), EINVAL), (dict(width=65535 * 32 + 1, lddo=1 << 22, lddt=1 << 22), EINVAL), (dict(lddo=4), EINVAL), (dict(lddt=4), EINVAL),
     (dict(dtable=None), EINVAL), (dict(dout=None), EINVAL), (dict(ids=None), EINVAL),
     (dict(scratch=None), EINVAL), (dict(scratch=A + 4), EINVAL), (dict(dtable=A + 2), EINVAL),
     (dict(nbytes=16), ERANGE)])
@@ -53,6 +53,7 @@ def test_embedding_scratch_size(lib):
     assert lib.ptcg_embedding_bwd_scratch(-1, 10, 8) == -1
     assert lib.ptcg_embedding_bwd_scratch(1 << 31, 10, 8) == -1
     assert lib.ptcg_embedding_bwd_scratch(5, 0, 8) == -1
+    assert lib.ptcg_embedding_bwd_scratch(5, 8, 65535 * 32 + 1) == -1
     # two sets of keys and places at least
     assert lib.ptcg_embedding_bwd_scratch(1 << 21, 4096, 128) >= 16 << 21
 
