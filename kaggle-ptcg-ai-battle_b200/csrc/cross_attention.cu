@@ -107,7 +107,6 @@ PTCG_DEV float quad_sum(float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 1);
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-
 // ---------------------------------------------------------- bf16 forward
 // A block owns 16 WM stacked rows and walks its keys 64 at a time through NST
 // cp.async stages; the running maximum, sum and output rows stay in registers
@@ -525,6 +524,39 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
 }
 
 // --------------------------------------------------------- bf16 backward
+// A quad's accumulators hold two columns of each 8-column piece per lane;
+// handed around, lane t has the whole of piece t out of four and stores 16
+// bytes: the short backward below takes 932 us so, 965 with 4-byte stores (the
+// forward has a third of its stores and loses by it, 413 to 418 us).
+PTCG_DEV uint4 quad_piece(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int t) {
+    const bool odd = t & 1, hi = t & 2;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+    const uint32_t r1 = __shfl_xor_sync(0xffffffffu, odd ? v2 : v3, 1);
+    // two words of piece t & 1 and of piece 2 + (t & 1)
+    const uint32_t a0 = odd ? r0 : v0, a1 = odd ? v1 : r0, b0 = odd ? r1 : v2, b1 = odd ? v3 : r1;
+    const uint32_t c0 = __shfl_xor_sync(0xffffffffu, hi ? a0 : b0, 2);
+    const uint32_t c1 = __shfl_xor_sync(0xffffffffu, hi ? a1 : b1, 2);
+    return hi ? make_uint4(c0, c1, b0, b1) : make_uint4(a0, a1, c0, c1);
+}
+// the accumulators' upper or lower row times f as bf16; every lane takes part,
+// those with `in` store
+template <int DH>
+PTCG_DEV void put_acc(bf16* row, int t, bool in, float f, const float (&acc)[DH / 8][4], int half) {
+    #pragma unroll
+    for (int j = 0; j < DH / 8; j += 4) {
+        uint32_t v[4];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = pack_bf2(acc[j + i][2 * half] * f, acc[j + i][2 * half + 1] * f);
+        const uint4 w = quad_piece(v[0], v[1], v[2], v[3], t);
+        if (in) *(uint4*)(row + (j + t) * 8) = w;
+    }
+}
+template <int DH>
+PTCG_DEV void put_zeros(bf16* row, int t) {
+    #pragma unroll
+    for (int j = 0; j < DH / 8; j += 4) *(uint4*)(row + (j + t) * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // dq: a block owns 64 stacked rows (16 a warp) with q, dout and dq in
 // registers and walks the keys; it also writes delta = dout . out for the
 // dk / dv kernel.  S is computed again from q and k: reading stored
@@ -669,17 +701,15 @@ __global__ void __launch_bounds__(128) k_cross_dq(const __grid_constant__ CrossA
     #pragma unroll
     for (int half = 0; half < 2; half++) {
         const int r = half ? rb : ra;
-        if (r >= a.rows) continue;
+        const bool in = r < a.rows;
         if (a.nsplit > 1) {
+            if (!in) continue;
             float* p = a.part + ((row0 + r) * a.nsplit + at.part) * DH;
             #pragma unroll
             for (int i = 0; i < DH / 8; i++)
                 *(float2*)(p + i * 8 + 2 * t) = make_float2(dq[i][2 * half] * a.scale, dq[i][2 * half + 1] * a.scale);
         } else {
-            bf16* p = (bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r);
-            #pragma unroll
-            for (int i = 0; i < DH / 8; i++)
-                *(uint32_t*)(p + i * 8 + 2 * t) = pack_bf2(dq[i][2 * half] * a.scale, dq[i][2 * half + 1] * a.scale);
+            put_acc<DH>((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), t, in, a.scale, dq, half);
         }
     }
 }
@@ -822,8 +852,9 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
     #pragma unroll
     for (int half = 0; half < 2; half++) {
         const int j = j0 + warp * 16 + g + half * 8;
-        if (j >= a.lk) continue;
+        const bool in = j < a.lk;
         if (a.nsplit > 1) {
+            if (!in) continue;
             const long at_row = (((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part;
             #pragma unroll
             for (int i = 0; i < DH / 8; i++) {
@@ -831,13 +862,23 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
                 *(float2*)(a.part2 + at_row * DH + i * 8 + 2 * t) = make_float2(dv[i][2 * half], dv[i][2 * half + 1]);
             }
         } else {
-            bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, j);
-            bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, j);
-            #pragma unroll
-            for (int i = 0; i < DH / 8; i++) {
-                *(uint32_t*)(pk + i * 8 + 2 * t) = pack_bf2(dk[i][2 * half] * a.scale, dk[i][2 * half + 1] * a.scale);
-                *(uint32_t*)(pv + i * 8 + 2 * t) = pack_bf2(dv[i][2 * half], dv[i][2 * half + 1]);
-            }
+            put_acc<DH>((bf16*)a.dk + krow(a.sdk, at.seq, at.hk, j), t, in, a.scale, dk, half);
+            put_acc<DH>((bf16*)a.dv + krow(a.sdv, at.seq, at.hk, j), t, in, 1.f, dv, half);
+        }
+    }
+}
+
+// a dq row of a warp that has its 16-column pieces d0, d0 + DR, .. (all of them
+// with 64 rows)
+template <int DH, int NR, int N>
+PTCG_DEV void put_dq(bf16* row, int t, int d0, bool in, float f, const float (&dq)[N][4], int half) {
+    if constexpr (NR == 4) {
+        put_acc<DH>(row, t, in, f, dq, half);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = (d0 + (i >> 1) * (4 / NR)) * 16 + (i & 1) * 8;
+            if (in && c < DH) *(uint32_t*)(row + c + 2 * t) = pack_bf2(dq[i][2 * half] * f, dq[i][2 * half + 1] * f);
         }
     }
 }
@@ -918,11 +959,9 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
     const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
     const float sc = a.scale * LOG2E;
     const int qr = NR == 1 ? 0 : warp % NR, qd = NR == 1 ? warp : warp / NR;   // dq rows, first column piece
-    float dq[ND][2][4];
+    float dq[2 * ND][4];
     #pragma unroll
-    for (int i = 0; i < ND; i++)
-        #pragma unroll
-        for (int e = 0; e < 4; e++) dq[i][0][e] = dq[i][1][e] = 0.f;
+    for (int i = 0; i < 2 * ND; i++) dq[i][0] = dq[i][1] = dq[i][2] = dq[i][3] = 0.f;
     // 16-byte piece c (8 rows) of key row k of the dS^T tile
     auto ds_off = [&](int k, int c) {
         return sD + (uint32_t)(k * BM * 2 + ((c ^ (NT == 8 ? k & 7 : NT == 4 ? (k >> 1) & 3 : (k >> 2) & 1)) << 4));
@@ -936,8 +975,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
         const uint32_t wk = ((warp & 2 ? w1 : w0) >> ((warp & 1) * 16)) & 0xffffu;
         const uint32_t kt = sK + (j & 1) * TILE, vt = sV + (j & 1) * TILE;
         const int ja = kbeg + j * BN + warp * 16 + g;
-        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja) + 2 * t;
-        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja) + 2 * t;
+        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja);
+        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja);
         const bool ina = ja < kend, inb = ja + 8 < kend;
         if (wk) {
             float s[NT][4], p[NT][4];
@@ -999,18 +1038,12 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                 const float f = which ? a.scale : 1.f;
                 bf16* out = which ? pk : pv;
                 const long down = 8 * (which ? a.sdk.row : a.sdv.row);
-                #pragma unroll
-                for (int i = 0; i < DH / 8; i++) {
-                    if (ina) *(uint32_t*)(out + i * 8) = pack_bf2(acc[i][0] * f, acc[i][1] * f);
-                    if (inb) *(uint32_t*)(out + down + i * 8) = pack_bf2(acc[i][2] * f, acc[i][3] * f);
-                }
+                put_acc<DH>(out, t, ina, f, acc, 0);
+                put_acc<DH>(out + down, t, inb, f, acc, 1);
             }
         } else {                                 // masked keys: no gradient
-            #pragma unroll
-            for (int i = 0; i < DH / 8; i++) {
-                if (ina) { *(uint32_t*)(pk + i * 8) = 0u; *(uint32_t*)(pv + i * 8) = 0u; }
-                if (inb) { *(uint32_t*)(pk + 8 * a.sdk.row + i * 8) = 0u; *(uint32_t*)(pv + 8 * a.sdv.row + i * 8) = 0u; }
-            }
+            if (ina) { put_zeros<DH>(pk, t); put_zeros<DH>(pv, t); }
+            if (inb) { put_zeros<DH>(pk + 8 * a.sdk.row, t); put_zeros<DH>(pv + 8 * a.sdv.row, t); }
         }
         put_bits(j + 2, next);
         if (w0 | w1) {                           // the same for every warp
@@ -1026,8 +1059,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                     if (d >= KS) break;
                     uint32_t b[4];
                     frag_t<DH>(b, kt + fr, k * 16, d);
-                    mma(dq[i][0], f, b[0], b[1]);
-                    mma(dq[i][1], f, b[2], b[3]);
+                    mma(dq[2 * i], f, b[0], b[1]);
+                    mma(dq[2 * i + 1], f, b[2], b[3]);
                 }
             }
         }
@@ -1036,18 +1069,16 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
     #pragma unroll
     for (int half = 0; half < 2; half++) {
         const int r = qr * 16 + g + half * 8;
+        if (a.nsplit == 1) {
+            put_dq<DH, NR>((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), t, qd, r < a.rows, a.scale, dq, half);
+            continue;
+        }
         if (r >= a.rows) continue;
+        float* p = a.part + ((row0 + r) * a.nsplit + at.part) * DH + 2 * t;
         #pragma unroll
-        for (int i = 0; i < ND; i++) {
-            const int d = qd + i * DR;
-            if (d >= KS) break;
-            #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const float x = dq[i][n][2 * half] * a.scale, y = dq[i][n][2 * half + 1] * a.scale;
-                const int c = d * 16 + n * 8 + 2 * t;
-                if (a.nsplit > 1) *(float2*)(a.part + ((row0 + r) * a.nsplit + at.part) * DH + c) = make_float2(x, y);
-                else *(uint32_t*)((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r) + c) = pack_bf2(x, y);
-            }
+        for (int i = 0; i < 2 * ND; i++) {
+            const int c = (qd + (i >> 1) * DR) * 16 + (i & 1) * 8;
+            if (c < DH) *(float2*)(p + c) = make_float2(dq[i][2 * half] * a.scale, dq[i][2 * half + 1] * a.scale);
         }
     }
 }
@@ -1055,9 +1086,11 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
 // The same for keys that fit shared memory whole: every warp takes each fourth
 // 16-key group that has a kept key, dS^T of all of them is kept, and dq is one
 // product at the end; three barriers in all.  8192 x 8 problems of 64 rows on
-// 129 keys, width 32: 965 us (3.4 TB/s; with the forward 1378, 1730 in 64-key tiles).  Bound: shared
-// memory, whose accesses fill 78 % of their cycles: q and dout are read as
-// fragments by every warp, dS^T is written and read back.
+// 129 keys, width 32: 932 us (3.5 TB/s; with the
+// forward 1351, in 64-key tiles 1730).  Bound: 16
+// warps a processor, as shared memory allows, with 63 % of the memory pipe's
+// cycles (every warp reads q and dout as fragments, dS^T is written and read
+// back) and half of the issue slots taken.
 template <int DH, int NR>                    // 16 NR rows
 __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_bwd_short(const __grid_constant__ CrossArgs a) {
     constexpr int BM = NR * 16, KS = DH / 16, NT = BM / 8;
@@ -1137,14 +1170,11 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_
         if (((on ? turn++ : k) & 3) != warp) continue;
         const int ja = k * 16 + g;
         const bool ina = ja < a.lk, inb = ja + 8 < a.lk;
-        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja) + 2 * t;
-        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja) + 2 * t;
+        bf16* pk = (bf16*)a.dk + krow(a.sdk, at.seq, at.hk, ja);
+        bf16* pv = (bf16*)a.dv + krow(a.sdv, at.seq, at.hk, ja);
         if (!on) {                               // masked keys: no gradient
-            #pragma unroll
-            for (int i = 0; i < DH / 8; i++) {
-                if (ina) { *(uint32_t*)(pk + i * 8) = 0u; *(uint32_t*)(pv + i * 8) = 0u; }
-                if (inb) { *(uint32_t*)(pk + 8 * a.sdk.row + i * 8) = 0u; *(uint32_t*)(pv + 8 * a.sdv.row + i * 8) = 0u; }
-            }
+            if (ina) { put_zeros<DH>(pk, t); put_zeros<DH>(pv, t); }
+            if (inb) { put_zeros<DH>(pk + 8 * a.sdk.row, t); put_zeros<DH>(pv + 8 * a.sdv.row, t); }
             continue;
         }
         float s[NT][4], p[NT][4];
@@ -1204,20 +1234,15 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_
             const float f = which ? a.scale : 1.f;
             bf16* out = which ? pk : pv;
             const long down = 8 * (which ? a.sdk.row : a.sdv.row);
-            #pragma unroll
-            for (int i = 0; i < DH / 8; i++) {
-                if (ina) *(uint32_t*)(out + i * 8) = pack_bf2(acc[i][0] * f, acc[i][1] * f);
-                if (inb) *(uint32_t*)(out + down + i * 8) = pack_bf2(acc[i][2] * f, acc[i][3] * f);
-            }
+            put_acc<DH>(out, t, ina, f, acc, 0);
+            put_acc<DH>(out + down, t, inb, f, acc, 1);
         }
     }
     __syncthreads();
     const int qr = NR == 1 ? 0 : warp % NR, qd = NR == 1 ? warp : warp / NR;   // dq rows, first column piece
-    float dq[ND][2][4];
+    float dq[2 * ND][4];
     #pragma unroll
-    for (int i = 0; i < ND; i++)
-        #pragma unroll
-        for (int e = 0; e < 4; e++) dq[i][0][e] = dq[i][1][e] = 0.f;
+    for (int i = 0; i < 2 * ND; i++) dq[i][0] = dq[i][1] = dq[i][2] = dq[i][3] = 0.f;
     for (uint32_t rem = active; rem; rem &= rem - 1) {
         const int k = __ffs(rem) - 1;
         uint32_t f[4];                           // dS rows 16 qr .., keys 16 k ..
@@ -1228,23 +1253,14 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_
             if (d >= KS) break;
             uint32_t b[4];
             frag_t<DH>(b, sK + fr, k * 16, d);
-            mma(dq[i][0], f, b[0], b[1]);
-            mma(dq[i][1], f, b[2], b[3]);
+            mma(dq[2 * i], f, b[0], b[1]);
+            mma(dq[2 * i + 1], f, b[2], b[3]);
         }
     }
     #pragma unroll
     for (int half = 0; half < 2; half++) {
         const int r = qr * 16 + g + half * 8;
-        if (r >= a.rows) continue;
-        bf16* out = (bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r) + 2 * t;
-        #pragma unroll
-        for (int i = 0; i < ND; i++) {
-            const int d = qd + i * DR;
-            if (d >= KS) break;
-            #pragma unroll
-            for (int n = 0; n < 2; n++)
-                *(uint32_t*)(out + d * 16 + n * 8) = pack_bf2(dq[i][n][2 * half] * a.scale, dq[i][n][2 * half + 1] * a.scale);
-        }
+        put_dq<DH, NR>((bf16*)a.dq + qrow(a, a.sdq, at.seq, at.hk, r), t, qd, r < a.rows, a.scale, dq, half);
     }
 }
 
