@@ -34,6 +34,7 @@ struct CrossArgs {
     PtcgHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
     int nseq, lq, lk, heads, kv_heads, group, rows;      // rows = group * lq
     int tiles, nsplit, split;                      // `split` rows of the split axis per part
+    int want;                                      // or even parts (below), at most so many per key head
     FastDiv by_lq, by_tiles, by_nsplit, by_kv;
     float scale;
 };
@@ -62,6 +63,66 @@ PTCG_DEV Where where(const CrossArgs& a) {
     w.hk = d - e * a.by_kv.d;
     w.seq = e;
     return w;
+}
+
+// Even parts: caches of unequal length (kv_len) as at most `want` parts of one
+// length, so that all blocks run at once and end together.  Parts of a fixed
+// share of lk left processors idle behind the longest caches (8 caches of 12653
+// to 65181 keys, 4 key heads of width 128: 162 us, 120 in even parts).  The length is the
+// smallest multiple of 256 keys that gives no more parts; every warp works it
+// out from the lengths, which are known on the device only.
+constexpr int EVEN_KEYS = 256;
+PTCG_DEV unsigned even_units(const CrossArgs& a, int seq) {
+    return ((unsigned)kept_len(a, seq) + EVEN_KEYS - 1) / EVEN_KEYS;
+}
+PTCG_DEV unsigned warp_sum_u(unsigned v) {
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+PTCG_DEV unsigned even_length(const CrossArgs& a) {      // in units
+    const int lane = threadIdx.x & 31;
+    const unsigned want = a.want;
+    unsigned all = 0;                                    // at most 2^22 units of each of 296 sequences
+    for (int s = lane; s < a.nseq; s += 32) all += even_units(a, s);
+    all = warp_sum_u(all);
+    unsigned lo = max((all + want - 1) / want, 1u), hi = max(all / (want - a.nseq) + 1, lo);
+    while (lo < hi) {
+        const unsigned mid = (lo + hi) / 2;
+        unsigned n = 0;
+        for (int s = lane; s < a.nseq; s += 32) n += (even_units(a, s) + mid - 1) / mid;
+        if (warp_sum_u(n) <= want) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+// this block's part, and its keys; false: no part is left for it
+PTCG_DEV bool even_part(const CrossArgs& a, Where& w, int& kbeg, int& kend) {
+    const int lane = threadIdx.x & 31;
+    const unsigned len = even_length(a), i = a.by_kv.div(blockIdx.x);
+    unsigned base = 0;
+    for (int s0 = 0; s0 < a.nseq; s0 += 32) {
+        const unsigned n = s0 + lane < a.nseq ? (even_units(a, s0 + lane) + len - 1) / len : 0;
+        unsigned x = n;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, i < base + x);
+        if (m) {
+            const int at = __ffs(m) - 1;
+            w.tile = 0;
+            w.hk = blockIdx.x - i * a.by_kv.d;
+            w.seq = s0 + at;
+            w.part = i - base - __shfl_sync(0xffffffffu, x - n, at);
+            const int keys = kept_len(a, w.seq), step = (int)len * EVEN_KEYS;
+            kbeg = w.part * step;
+            kend = keys - kbeg < step ? keys : kbeg + step;
+            return true;
+        }
+        base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    return false;
 }
 
 PTCG_DEV uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

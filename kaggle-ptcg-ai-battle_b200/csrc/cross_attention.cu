@@ -114,9 +114,9 @@ PTCG_DEV float quad_sum(float v) {
 // (rounded to bf16: at most 2^-8 of each probability, the size of the output's
 // own rounding).  WN = 4 is the form for at most 16 rows (single tokens): the
 // four warps take 16 keys each of every tile and are joined at the end.
-// Bound: HBM with few rows (single tokens, 16 heads on 4, width 128, caches of up
-// to 65536 keys: 86 us for some 535 MB, 6.2 TB/s), the launch for one decision
-// (4.1 us), else issue slots around the products.
+// Bound: HBM with few rows (single tokens, 16 heads on 4, width 128: 8 caches of
+// 65536 keys 168 us, 6.4 TB/s; unequal ones of 436 MB 77 us, 5.7 TB/s), the launch
+// for one decision (4.1 us), else issue slots around the products.
 template <int DH, int WM, int WN, int NST>
 __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 5 : 1) k_cross_fwd(const __grid_constant__ CrossArgs a) {
     constexpr int THREADS = WM * WN * 32, BM = WM * 16, BN = 64, KW = BN / WN, NT = KW / 8;
@@ -127,12 +127,19 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 5 : 1) k_c
     // 0 for a kept key, -inf for a masked one: where the scores start from
     __shared__ __align__(8) float bias[NST + 1][BN];
     const uint32_t sQ = s_addr(sm), sK = sQ + BM * DH * 2, sV = sK + NST * TILE;
-    const Where at = where(a);
+    Where at = where(a);
+    int kbeg, kend;
+    if (WN == 4 && a.want) {
+        if (!even_part(a, at, kbeg, kend)) return;
+    }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t fr = lane_rows<DH>(lane), fc = lane_cols<DH>(lane);
     const int wm = WN == 1 ? warp : 0, wn = WN == 1 ? 0 : warp;
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
-    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    if (WN != 4 || !a.want) {
+        kbeg = min(at.part * a.split, len);
+        kend = min(len, kbeg + a.split);
+    }
     const int nt = (kend - kbeg + BN - 1) / BN;
     const bf16 *K = (const bf16*)a.k, *V = (const bf16*)a.v;
 
@@ -493,9 +500,16 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
     __shared__ float sy[4][DH], sl[4];
     const long row = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long b = row / a.rows;
+    const int seq = (int)(b / a.kv_heads), hk = (int)(b % a.kv_heads), r = (int)(row - b * a.rows);
+    int parts = a.nsplit;
+    if (a.want) {
+        const unsigned len = even_length(a);
+        parts = (int)((even_units(a, seq) + len - 1) / len);
+    }
     const float2* ml = a.part_ml + row * a.nsplit;
     float m = -INFINITY;
-    for (int i = lane; i < a.nsplit; i += 32) m = fmaxf(m, ml[i].x);
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml[i].x);
     m = warp_max(m);
     const float u = m == -INFINITY ? 0.f : m;
     float l = 0.f, y[C];
@@ -503,7 +517,7 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
     for (int e = 0; e < C; e++) y[e] = 0.f;
     const float* p = a.part + row * a.nsplit * DH + lane;
     #pragma unroll 8
-    for (int i = warp; i < a.nsplit; i += 4) {
+    for (int i = warp; i < parts; i += 4) {
         const float2 x = ml[i];
         const float c = ex2_approx(x.x - u);
         l = fmaf(x.y, c, l);
@@ -515,8 +529,6 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
     if (lane == 0) sl[warp] = l;
     __syncthreads();
     l = sl[0] + sl[1] + sl[2] + sl[3];
-    const long b = row / a.rows;
-    const int seq = (int)(b / a.kv_heads), hk = (int)(b % a.kv_heads), r = (int)(row - b * a.rows);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     for (int d = threadIdx.x; d < DH; d += 128)
         ((T*)a.out + qrow(a, a.so, seq, hk, r))[d] = from_f<T>((sy[0][d] + sy[1][d] + sy[2][d] + sy[3][d]) * inv);
@@ -1467,10 +1479,17 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
     float* Ks = Qs + BM * LD;        // [BN][LD]
     float* Vs = Ks + BN * LD;        // [BN][LD]
     float* Ps = Vs + BN * LD;        // [BN][LM]
-    const Where at = where(a);
+    Where at = where(a);
+    int kbeg, kend;
+    if (RT == 2 && a.want) {
+        if (!even_part(a, at, kbeg, kend)) return;
+    }
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int r0 = at.tile * BM, len = kept_len(a, at.seq);
-    const int kbeg = min(at.part * a.split, len), kend = min(len, kbeg + a.split);
+    if (RT != 2 || !a.want) {
+        kbeg = min(at.part * a.split, len);
+        kend = min(len, kbeg + a.split);
+    }
     stage_f32<DH, BM>(Qs, (const float*)a.q, [&](int r) { return q_ptr(a, a.q, a.sq, at, r0 + r, a.rows); });
     float o[RT][ND], m[RT], l[RT];
     clear(o);
@@ -1778,7 +1797,13 @@ bool use_tc(const PtcgCross& c, long rows) {
     if (c.dtype != PTCG_BF16 || !gemm_tc_available()) return false;
     return c.dh == 32 ? rows >= 384 && c.lk >= 256 : rows > 64 && c.lk > 64;
 }
-struct FwdPlan { bool few, tc; int bm; long tiles, blocks; Split sp; long o_ml, bytes; };
+// Parts of the single-token form: as many blocks as run at once (two of width
+// 128 on a processor, four of the others), twice that where the problems alone
+// are more than half of it.  Long caches of unequal length take even parts
+// instead (cross.cuh), which only pays where the blocks have more to do than
+// find their parts: from 4096 keys on (8 caches of up to 4100, 4 key heads of
+// width 128: 24.6 us either way).
+struct FwdPlan { bool few, tc; int bm; long tiles, blocks; Split sp; int want, most; long o_ml, bytes; };
 FwdPlan fwd_plan(const PtcgCross& c) {
     FwdPlan p;
     const long rows = (long)c.heads / c.kv_heads * c.lq, probs = (long)c.nseq * c.kv_heads;
@@ -1787,10 +1812,19 @@ FwdPlan fwd_plan(const PtcgCross& c) {
     p.bm = p.few ? 16 : c.dtype == PTCG_FP32 && rows <= 32 ? 32 : p.tc ? TC_ROWS : 64;
     p.tiles = (rows + p.bm - 1) / p.bm;
     p.sp = split_of(p.tiles * probs, c.lk, p.tc);
+    p.want = 0;
+    if (p.few && p.sp.n > 1) {
+        long slots = 148 * (c.dh == 128 ? 2 : 4);
+        if (2 * probs > slots) slots *= 2;
+        p.sp.len = (int)((cdiv(c.lk, std::min(slots / probs, ((long)c.lk + 255) / 256)) + 63) / 64 * 64);
+        p.sp.n = (int)cdiv(c.lk, p.sp.len);
+        if (c.lk >= 4096) p.want = (int)(slots / c.kv_heads);
+    }
     p.blocks = p.tiles * probs * p.sp.n;
-    const long parts = p.sp.n > 1 ? rows * probs * p.sp.n : 0;
+    p.most = p.want ? std::max(std::min((int)cdiv(c.lk, EVEN_KEYS), p.want), p.sp.n) : p.sp.n;
+    const long parts = p.most > 1 ? rows * probs * p.most : 0;
     p.o_ml = (4 * parts * c.dh + 255) / 256 * 256;
-    p.bytes = p.sp.n > 1 ? p.o_ml + 8 * parts : 0;
+    p.bytes = p.most > 1 ? p.o_ml + 8 * parts : 0;
     return p;
 }
 struct BwdPlan { bool rows; long qtiles, qblocks, ktiles, kblocks; Split qs, ks; long o_part, o_part2, bytes; };
@@ -1920,6 +1954,12 @@ template <int DH>
 cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream_t s) {
     cudaError_t e;
     bool taken = false;
+    long blocks = p.blocks;
+    if (p.want && a.kv_len) {
+        a.want = p.want;
+        a.nsplit = p.most;
+        blocks = (long)p.want * c.kv_heads;
+    }
     if (p.tc) {
         e = fwd_tc(DH, a, p.blocks, s, &taken);
         if (e != cudaSuccess) return e;
@@ -1929,13 +1969,13 @@ cudaError_t fwd_dh(CrossArgs a, const PtcgCross& c, const FwdPlan& p, cudaStream
         set_tiles(a, tiles, p.sp);
         e = launch_fwd<DH, 4, 1, 2>(a, tiles * c.nseq * c.kv_heads * p.sp.n, s);
     } else if (!p.tc && c.dtype == PTCG_BF16)
-        e = p.few ? launch_fwd<DH, 1, 4, 3>(a, p.blocks, s)
+        e = p.few ? launch_fwd<DH, 1, 4, 3>(a, blocks, s)
             : p.sp.n == 1 && is_short(c.lk, short_fwd_bytes(DH, c.lk)) ? launch_fwd_short<DH>(a, p.blocks, s)
             : launch_fwd<DH, 4, 1, 2>(a, p.blocks, s);
     else if (!p.tc)
-        e = p.few ? launch_fwd_f32<DH, 2>(a, p.blocks, s)
+        e = p.few ? launch_fwd_f32<DH, 2>(a, blocks, s)
             : p.bm == 32 ? launch_fwd_f32<DH, 4>(a, p.blocks, s) : launch_fwd_f32<DH, 8>(a, p.blocks, s);
-    if (e != cudaSuccess || p.sp.n == 1) return e;
+    if (e != cudaSuccess || a.nsplit == 1) return e;
     const long nrows = (long)c.nseq * c.kv_heads * a.rows;
     ++g_ptcg_launches;
     if (c.dtype == PTCG_BF16) k_cross_join<bf16, DH><<<(unsigned)nrows, 128, 0, s>>>(a);

@@ -351,6 +351,34 @@ def test_cross_attention_long_growing_scores(ops):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", ["drawn", "none", "one", "equal", "short"])
+@pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", [(5, 1, 9000, 8, 2, 64), (40, 2, 4100, 2, 1, 32),
+                                                     (3, 4, 20000, 4, 1, 128), (1, 1, 4096, 3, 3, 128),
+                                                     (147, 1, 4200, 2, 2, 32)])
+def test_cross_attention_uneven_caches(ops, dtype, lens, nseq, lq, lk, heads, kvh, dh):
+    """Single tokens over long caches of unequal lengths, which the blocks share
+    out by the lengths: empty caches, one that has all keys, few keys in all."""
+    q, k, v, _ = problem(lk, nseq, lq, lk, heads, kvh, dh, dtype, "none", "rows")
+    n = torch.randint(0, lk + 1, (nseq,), generator=torch.Generator().manual_seed(nseq), dtype=torch.int32)
+    if lens == "none":
+        n[:] = 0
+    elif lens == "one":
+        n[:] = 0
+        n[nseq // 2] = lk
+    elif lens == "equal":
+        n[:] = lk
+    elif lens == "short":
+        n %= 70
+    m = {"keep": None, "kv_len": n.cuda()}
+    out, lse = ops.cross_attention(q, k, v, **m)
+    r = ref.cross(q, k, v, **m)
+    ref.within(out, r["out"], r["e_out"], "out")
+    ref.within(lse, r["lse"], r["e_lse"], "lse")
+    again, _ = ops.cross_attention(q, k, v, **m)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("layout", ["heads", "packed"])
 @pytest.mark.parametrize("nseq,lq,lk,heads,kvh,dh", [(3, 40, 75, 4, 2, 32), (2, 1, 900, 4, 4, 64),
                                                      (2, 90, 40, 2, 2, 128)])
