@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
             int ks = 0, vs = 0;                             // stages, and their phases
             uint32_t kp = 0, vp = 0;
             for (int j = 0; ok && j <= nt; j++) {
-                // the operands of this round are waited for before the
+                // the operands of this step are waited for before the
                 // probabilities, off the path from them to the next scores
                 ok = (j == 0 || wait_warp(vready + 8 * vs, vp, abort_flag, 5)) &&
                      (j == nt || wait_warp(kfull + 8 * ks, kp, abort_flag, 7));
