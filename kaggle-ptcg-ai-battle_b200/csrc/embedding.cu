@@ -21,8 +21,8 @@ constexpr int MAX_WIDTH = 65535 * 32;
 // touch.  2 M rows of 128 from an fp32 table of 4096 to bf16: 126 us, 4.3 TB/s
 // of output and 8.5 TB/s of table rows from L2; 32768 rows of 1024, bf16 to
 // bf16, 28 us (4.8 TB/s).  LX lanes take a row's V-element pieces, 256 / LX rows to a
-// block pass, four rows in flight per thread and the next rows' ids ahead of
-// them.
+// block pass, four rows (eight of single elements) in flight per thread and the
+// next rows' ids ahead of them.
 template <typename TT, typename TO, int V>
 __global__ void __launch_bounds__(256) k_embed_fwd(
         TO* __restrict__ out, long ldo, const TT* __restrict__ table, long ldt,
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) k_embed_fwd(
         int pad_id, int has_pad) {
     const int tx = threadIdx.x & ((1 << lx_log2) - 1), ty = threadIdx.x >> lx_log2;
     const int ry = 256 >> lx_log2;
-    constexpr int U = 4;
+    constexpr int U = V == 1 ? 8 : 4;                      // rows in flight a thread
     const long step = (long)gridDim.x * ry * U;
     int next[U];
     auto fetch = [&](long r0) {
@@ -266,41 +266,44 @@ __global__ void __launch_bounds__(SORT_T) k_sort_scatter(const __grid_constant__
 }
 
 // All passes of a batch that one block holds, in one launch: for small batches
-// the launches would cost more than the sort
-constexpr int SMALL_ITEMS = 8, SMALL_N = SORT_T * SMALL_ITEMS;
+// the launches would cost more than the sort (8000 places of 4096 ids 16 us,
+// 20000 in five launches 22; with one place a thread, up to 1024, 5 us
+// where eight a thread took 14)
+constexpr int SMALL_N = SORT_T * 8;
+template <int ITEMS>
 __global__ void __launch_bounds__(SORT_T) k_sort_small(const __grid_constant__ SortArgs a, int passes) {
-    extern __shared__ uint32_t sorted[];                   // [SMALL_N] keys, [SMALL_N] places
+    extern __shared__ uint32_t sorted[];                   // [SORT_T * ITEMS] keys, as many places
     __shared__ TileSort t;
-    const int n = (int)a.n, base = (threadIdx.x >> 5) * 32 * SMALL_ITEMS + (threadIdx.x & 31);
-    uint32_t key[SMALL_ITEMS], ps[SMALL_ITEMS], to[SMALL_ITEMS];
+    const int n = (int)a.n, base = (threadIdx.x >> 5) * 32 * ITEMS + (threadIdx.x & 31);
+    uint32_t key[ITEMS], ps[ITEMS], to[ITEMS];
     #pragma unroll
-    for (int k = 0; k < SMALL_ITEMS; k++) {
+    for (int k = 0; k < ITEMS; k++) {
         const int i = base + k * 32;
         key[k] = i < n ? key_of(a.ids[i], a.vocab, a.pad_id, a.has_pad) : 0u;
         ps[k] = (uint32_t)i;
     }
     for (int p = 0; p < passes; p++) {
-        tile_places<SMALL_ITEMS>(t, to, key, n, p * a.bits, a.bits);
+        tile_places<ITEMS>(t, to, key, n, p * a.bits, a.bits);
         #pragma unroll
-        for (int k = 0; k < SMALL_ITEMS; k++) {
+        for (int k = 0; k < ITEMS; k++) {
             if (base + k * 32 < n) {
                 sorted[to[k]] = key[k];
-                sorted[SMALL_N + to[k]] = ps[k];
+                sorted[SORT_T * ITEMS + to[k]] = ps[k];
             }
         }
         __syncthreads();
         #pragma unroll
-        for (int k = 0; k < SMALL_ITEMS; k++) {
+        for (int k = 0; k < ITEMS; k++) {
             const int i = base + k * 32;
             if (i < n) {
                 key[k] = sorted[i];
-                ps[k] = sorted[SMALL_N + i];
+                ps[k] = sorted[SORT_T * ITEMS + i];
             }
         }
         __syncthreads();
     }
     #pragma unroll
-    for (int k = 0; k < SMALL_ITEMS; k++) {
+    for (int k = 0; k < ITEMS; k++) {
         const int i = base + k * 32;
         if (i < n) {
             a.keys_out[i] = key[k];
@@ -600,9 +603,15 @@ template <typename TT, typename TO>
 void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids, long n,
                int vocab, int width, float scale, int pad_id, int V, cudaStream_t s) {
     const int pieces = width / V;
+    // the lanes of a row that leave the fewest idle in its last step (100000 rows
+    // of 300 single bf16 columns: 40 us with 64, and 8 rows in flight; 53 with 256
+    // and 4)
     int lx = 0;
     while (lx < 8 && (1 << lx) < pieces) lx++;
-    const long rows = (256 >> lx) * 4L;
+    if (lx == 8)
+        for (int l = 7; l >= 5; l--)
+            if (cdiv(pieces, 1L << l) << l < cdiv(pieces, 1L << lx) << lx) lx = l;
+    const long rows = (256 >> lx) * (V == 1 ? 8L : 4L);
     const long blocks = (n + rows - 1) / rows;
     const unsigned grid = (unsigned)(blocks < 148L * 32 ? blocks : 148L * 32);
     ++g_ptcg_launches;
@@ -622,11 +631,12 @@ cudaError_t sort_pass(const SortArgs& a, int tiles, cudaStream_t s) {
     k_sort_scatter<ITEMS, FIRST><<<tiles, SORT_T, bytes, s>>>(a);
     return cudaSuccess;
 }
+template <int ITEMS>
 cudaError_t sort_small(const SortArgs& a, int passes, cudaStream_t s) {
-    constexpr int bytes = 8 * SMALL_N;
-    const cudaError_t e = cudaFuncSetAttribute(k_sort_small, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    constexpr int bytes = 8 * SORT_T * ITEMS;
+    const cudaError_t e = cudaFuncSetAttribute(k_sort_small<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    ++g_ptcg_launches, k_sort_small<<<1, SORT_T, bytes, s>>>(a, passes);
+    ++g_ptcg_launches, k_sort_small<ITEMS><<<1, SORT_T, bytes, s>>>(a, passes);
     return cudaSuccess;
 }
 
@@ -712,7 +722,7 @@ int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* i
         const int to = i & 1;
         const SortArgs sa = {(uint32_t*)(base + p.o_counts), keys[to], pos[to], keys[to ^ 1], pos[to ^ 1],
                              ids, n, i * p.bits, p.bits, vocab, pad_id, pad_id >= 0};
-        OP_CK(small ? sort_small(sa, p.passes, s)
+        OP_CK(small ? (n <= SORT_T ? sort_small<1>(sa, p.passes, s) : sort_small<8>(sa, p.passes, s))
               : p.items == 16 ? (i == 0 ? sort_pass<16, true>(sa, p.tiles, s) : sort_pass<16, false>(sa, p.tiles, s))
                               : (i == 0 ? sort_pass<4, true>(sa, p.tiles, s) : sort_pass<4, false>(sa, p.tiles, s)));
     }

@@ -59,7 +59,7 @@ GRADS = [  # n, vocab, width, how the ids fall
     (31, 5, 40, "one"), (4095, 257, 8, "any"), (4097, 255, 64, "skew"), (8192, 256, 16, "one"), (8193, 600, 12, "any"), (16385, 600, 12, "skew"),
     (5000, 65537, 24, "any"), (3000, 70000, 9, "skew"), (20000, 40, 136, "skew"),
     (12289, 11, 7, "skew"), (2500, 4000, 520, "any"), (700001, 1000, 8, "skew"),
-    (611000, 3, 1, "any")]
+    (611000, 3, 1, "any"), (1024, 70000, 8, "any"), (1025, 300, 130, "skew"), (3000, 50, 301, "any")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
