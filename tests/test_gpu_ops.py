@@ -514,6 +514,25 @@ def test_decoder_sublayer_against_autograd(ops):
         assert (a.double() - b).norm() <= 4 * 2.0 ** -8 * b.norm(), i
 
 
+def test_graph_replay_with_other_lengths(ops):
+    """A captured single-token call shares its keys out by the lengths that are
+    there when it is replayed."""
+    q, k, v, _ = problem(4, 6, 1, 7000, 4, 2, 64, BF16, "none", "heads")
+    n = torch.tensor([7000, 3, 0, 512, 4097, 6999], dtype=torch.int32, device="cuda")
+    ops.cross_attention(q, k, v, kv_len=n)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, lse = ops.cross_attention(q, k, v, kv_len=n)
+    for lens in ([1, 1, 1, 1, 1, 1], [0, 7000, 0, 0, 0, 0], [9000, 255, 256, 257, -5, 6000]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        gr.replay()
+        want, wlse = ops.cross_attention(q, k, v, kv_len=n)
+        assert torch.equal(out, want) and torch.equal(lse, wlse)
+        r = ref.cross(q, k, v, kv_len=n)
+        ref.within(out, r["out"], r["e_out"], "out")
+
+
 def test_graph_capture_and_replay(ops):
     """Two captured graphs, replayed in turn on new inputs beside eager calls,
     give the eager results bit for bit."""
