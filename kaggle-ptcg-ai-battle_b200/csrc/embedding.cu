@@ -18,13 +18,13 @@ constexpr int MAX_WIDTH = 65535 * 32;
 
 // -------------------------------------------------------------- forward
 // Bound: HBM for ids and output, L2 for the table's rows after their first
-// touch.  2 M rows of 128 from an fp32 table of 4096 to bf16: 126 us, 4.3 TB/s
-// of output and 8.5 TB/s of table rows from L2; 32768 rows of 1024, bf16 to
-// bf16, 28 us (4.8 TB/s).  LX lanes take a row's V-element pieces, 256 / LX rows to a
+// touch.  2 M rows of 128 from an fp32 table of 4096 to bf16: 117 us, 4.6 TB/s
+// of output and 9.2 TB/s of table rows from L1 and L2; 32768 rows of 1024, bf16
+// to bf16, 25 us (5.4 TB/s).  LX lanes take a row's V-element pieces, 256 / LX rows to a
 // block pass, four rows (eight of single elements) in flight per thread and the
 // next rows' ids ahead of them.
 template <typename TT, typename TO, int V>
-__global__ void __launch_bounds__(256) k_embed_fwd(
+__global__ void __launch_bounds__(256, V == 4 ? 5 : 4) k_embed_fwd(
         TO* __restrict__ out, long ldo, const TT* __restrict__ table, long ldt,
         const int* __restrict__ ids, long n, int vocab, int pieces, int lx_log2, float scale,
         int pad_id, int has_pad) {
@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(SORT_T) k_sort_small(const __grid_constant__ S
 // as a partial: the block joins its groups' partials in order through shared
 // memory, and k_embed_join joins the blocks'.  Rows without a place are
 // zeroed by extra blocks.  Bound: HBM, dout read once as gathered rows: 2 M
-// bf16 rows of 128 into 4096 120 us (4.5 TB/s), 32768 of 1024 into 65537 61 us
+// bf16 rows of 128 into 4096 111 us (4.8 TB/s; 120 with three blocks a
+// processor, which their registers would leave), 32768 of 1024 into 65537 61 us
 // (5.5 TB/s with the table's zeros).
 constexpr int MAX_CHUNK = 2048;
 enum { SEG_HEAD = 1, SEG_THROUGH = 2, SEG_TAIL = 4 };
@@ -354,7 +355,7 @@ PTCG_DEV void put_row(const SumArgs& a, uint32_t id, int piece, const float (&s)
 }
 
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(256) k_embed_sum(const __grid_constant__ SumArgs a) {
+__global__ void __launch_bounds__(256, 4) k_embed_sum(const __grid_constant__ SumArgs a) {
     constexpr int NG = 256 / G, S = G * V, U = 8;
     __shared__ float s_head[NG][S], s_tail[NG][S];
     __shared__ uint32_t s_key[MAX_CHUNK + 2], s_pos[MAX_CHUNK];
@@ -603,9 +604,8 @@ template <typename TT, typename TO>
 void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids, long n,
                int vocab, int width, float scale, int pad_id, int V, cudaStream_t s) {
     const int pieces = width / V;
-    // the lanes of a row that leave the fewest idle in its last step (100000 rows
-    // of 300 single bf16 columns: 40 us with 64, and 8 rows in flight; 53 with 256
-    // and 4)
+    // the lanes of a row that leave the fewest idle in its last step (100000 bf16
+    // rows of 301: 40 us with 64 lanes and 8 rows in flight, 53 with 256 and 4)
     int lx = 0;
     while (lx < 8 && (1 << lx) < pieces) lx++;
     if (lx == 8)
@@ -617,7 +617,9 @@ void embed_fwd(void* out, long ldo, const void* table, long ldt, const int* ids,
     ++g_ptcg_launches;
     #define EF(V) k_embed_fwd<TT, TO, V><<<grid, 256, 0, s>>>((TO*)out, ldo, (const TT*)table, ldt, \
         ids, n, vocab, pieces, lx, scale, pad_id, pad_id >= 0)
-    if (V == 8) EF(8); else EF(1);
+    if constexpr (sizeof(TO) == 2)
+        if (V == 8) { EF(8); return; }
+    if (V == 4) EF(4); else EF(1);
     #undef EF
 }
 
@@ -678,7 +680,12 @@ int ptcg_embedding_fwd(const void* table, int table_dtype, long ldt, int vocab, 
     OP_REQ(el_ok(table, table_dtype) && el_ok(out, out_dtype) && (uintptr_t)ids % 4 == 0,
            PTCG_EINVAL, "embedding: pointer not aligned to its element");
     cudaStream_t s = (cudaStream_t)stream;
-    const int V = width % 8 == 0 && vec_ok(table, table_dtype, ldt, 8) && vec_ok(out, out_dtype, ldo, 8) ? 8 : 1;
+    // pieces of 8 elements for bf16 outputs, else of 4 (2 M rows of 128: fp32 to
+    // bf16 117 us in eights, 136 in fours, but bf16 to fp32, where an eight is two
+    // stores of half sectors, 267 and 179; 100000 bf16 rows of 300: 27 us in
+    // fours, 40 in ones)
+    auto fits = [&](int v) { return width % v == 0 && vec_ok(table, table_dtype, ldt, v) && vec_ok(out, out_dtype, ldo, v); };
+    const int V = out_dtype == PTCG_BF16 && fits(8) ? 8 : fits(4) ? 4 : 1;
     #define EF(TT, TO) embed_fwd<TT, TO>(out, ldo, table, ldt, ids, n, vocab, width, scale, pad_id, V, s)
     if (table_dtype == PTCG_BF16) { if (out_dtype == PTCG_BF16) EF(bf16, bf16); else EF(bf16, float); }
     else { if (out_dtype == PTCG_BF16) EF(float, bf16); else EF(float, float); }
