@@ -1315,7 +1315,7 @@ __global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ Cross
 // last place of e^x, whose largest value over x is 2 units of the row's largest
 // probability.  Bound: the multiply-adds and the reads from shared memory that
 // feed them: 512 x 8 problems of 61 rows on up to 186 keys of width 32 take
-// 168 us forward and 402 backward (18 TFLOP/s over the kept keys).
+// 173 us forward and 406 backward (18 TFLOP/s over the kept keys).
 template <int RT> PTCG_DEV int row_of(int ty, int i) {
     return RT == 8 ? (i >> 2) * 32 + ty * 4 + (i & 3) : ty * RT + i;
 }
@@ -1404,6 +1404,20 @@ template <int RT, int NC> PTCG_DEV void clear(float (&acc)[RT][NC]) {
     for (int i = 0; i < RT; i++)
         #pragma unroll
         for (int j = 0; j < NC; j++) acc[i][j] = 0.f;
+}
+// the same, the tile's products summed by themselves first: one rounding of the
+// running sum per tile, not per row of it, so that long sums stay as exact as
+// short ones: out is off by 2.6e-7 of its size at 300 keys and at 20000 (a sum
+// over all keys grows with the root of their number); 1 to 3 % of the time
+template <int RT, int NC, int K>
+PTCG_DEV void mm_outer_add(float (&acc)[RT][NC], const float* A, int lda, const float* B, int ldb, int ty, int tx) {
+    float y[RT][NC];
+    clear(y);
+    mm_outer<RT, NC, K>(y, A, lda, B, ldb, ty, tx);
+    #pragma unroll
+    for (int i = 0; i < RT; i++)
+        #pragma unroll
+        for (int j = 0; j < NC; j++) acc[i][j] += y[i][j];
 }
 // the thread's RT values of column k into row k of a [k][row] tile
 template <int RT> PTCG_DEV void put_rows(float* T, int ld, int k, int ty, const float (&v)[RT]) {
@@ -1515,13 +1529,14 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
             #pragma unroll
             for (int i = 0; i < RT; i++) s[i][j] = live ? s[i][j] * a.scale : -INFINITY;
         }
+        float c[RT];
         #pragma unroll
         for (int i = 0; i < RT; i++) {
             float x = s[i][0];
             #pragma unroll
             for (int j = 1; j < NC; j++) x = fmaxf(x, s[i][j]);
             const float n = fmaxf(m[i], row16_max(x)), u = n == -INFINITY ? 0.f : n;
-            const float c = __expf(m[i] - u);
+            c[i] = __expf(m[i] - u);
             m[i] = n;
             float t = 0.f;
             #pragma unroll
@@ -1529,9 +1544,7 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
                 s[i][j] = __expf(s[i][j] - u);
                 t += s[i][j];
             }
-            l[i] = fmaf(l[i], c, t);
-            #pragma unroll
-            for (int j = 0; j < ND; j++) o[i][j] *= c;
+            l[i] = fmaf(l[i], c[i], t);
         }
         #pragma unroll
         for (int j = 0; j < NC; j++) {
@@ -1542,7 +1555,14 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
         }
         cp_wait<0>();
         __syncthreads();
-        mm_outer<RT, ND, BN>(o, Ps, LM, Vs, LD, ty, tx);
+        // as mm_outer_add, with the old maximum's factor
+        float y[RT][ND];
+        clear(y);
+        mm_outer<RT, ND, BN>(y, Ps, LM, Vs, LD, ty, tx);
+        #pragma unroll
+        for (int i = 0; i < RT; i++)
+            #pragma unroll
+            for (int j = 0; j < ND; j++) o[i][j] = fmaf(o[i][j], c[i], y[i][j]);
     }
     cp_wait<0>();
     #pragma unroll
@@ -1623,7 +1643,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dq_f32(const __
             put_rows<RT>(Ds, LM, tx + 16 * j, ty, v);
         }
         __syncthreads();
-        mm_outer<RT, ND, BN>(dq, Ds, LM, Ks, LD, ty, tx);
+        mm_outer_add<RT, ND, BN>(dq, Ds, LM, Ks, LD, ty, tx);
     }
     #pragma unroll
     for (int i = 0; i < RT; i++) {
@@ -1725,9 +1745,9 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
                     }
                 }
                 __syncthreads();
-                mm_outer<RT, ND, BQ>(dv, Ps, LM, Gs, LD, ty, tx);
-                if constexpr (ROWS) {
-                    mm_outer<RQ, ND, BK>(dq, Ds, LQ, Ks, LD, ty, tx);
+                if constexpr (ROWS) {                // one tile of rows: nothing to add to
+                    mm_outer<RT, ND, BQ>(dv, Ps, LM, Gs, LD, ty, tx);
+                    mm_outer_add<RQ, ND, BK>(dq, Ds, LQ, Ks, LD, ty, tx);
                     __syncthreads();
                     #pragma unroll
                     for (int j = 0; j < NC; j++) {
@@ -1739,7 +1759,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
                     __syncthreads();
                     mm_outer<RT, ND, BQ>(dk, Ps, LM, Qs, LD, ty, tx);
                 } else {
-                    mm_outer<RT, ND, BQ>(dk, Ds, LM, Qs, LD, ty, tx);
+                    mm_outer_add<RT, ND, BQ>(dv, Ps, LM, Gs, LD, ty, tx);
+                    mm_outer_add<RT, ND, BQ>(dk, Ds, LM, Qs, LD, ty, tx);
                 }
             }
             cp_wait<0>();

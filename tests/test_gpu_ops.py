@@ -422,6 +422,20 @@ def test_cross_attention_no_lengths(ops, dtype):
     assert out.shape == (0, 3, 4, 32)
 
 
+def test_cross_attention_long_sums(ops):
+    """fp32 sums over many keys or rows are as exact as short ones."""
+    for nseq, lq, lk, heads, kvh, dh in ((1, 48, 20000, 2, 2, 32), (1, 100, 20000, 2, 1, 128), (1, 6000, 100, 1, 1, 64)):
+        q, k, v, m = problem(lk, nseq, lq, lk, heads, kvh, dh, F32, "none", "rows")
+        dout, got = run_cross(ops, q, k, v, m)
+        r = ref.cross(q, k, v, dout=dout, **m)
+        for name, t in zip(("out", "dq", "dk", "dv"), (got[0], got[2], got[3], got[4])):
+            err = float((t.double() - r[name]).pow(2).mean().sqrt() / r[name].pow(2).mean().sqrt())
+            # P = exp(s - lse): s of some 4 and lse of some 10 are off by half a
+            # step each, 2^-22 + 2^-21, the products and sums by less; in the root
+            # mean square below that, so 2^-20 holds with room
+            assert err < 2.0 ** -20, (name, err)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_cross_attention_large_scores(ops, dtype):
     """Scores of hundreds: the running maximum keeps every exponential in
