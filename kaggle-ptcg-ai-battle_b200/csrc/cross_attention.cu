@@ -1098,11 +1098,10 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
 // The same for keys that fit shared memory whole: every warp takes each fourth
 // 16-key group that has a kept key, dS^T of all of them is kept, and dq is one
 // product at the end; three barriers in all.  8192 x 8 problems of 64 rows on
-// 129 keys, width 32: 932 us (3.5 TB/s; with the
-// forward 1351, in 64-key tiles 1730).  Bound: 16
-// warps a processor, as shared memory allows, with 63 % of the memory pipe's
-// cycles (every warp reads q and dout as fragments, dS^T is written and read
-// back) and half of the issue slots taken.
+// 129 keys, width 32: 932 us (3.5 TB/s; with the forward 1351, in 64-key tiles
+// 1730).  Bound: 16 warps a processor, as shared memory allows, with 63 % of the
+// memory pipe's cycles (every warp reads q and dout as fragments, dS^T is
+// written and read back) and half of the issue slots taken.
 template <int DH, int NR>                    // 16 NR rows
 __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_bwd_short(const __grid_constant__ CrossArgs a) {
     constexpr int BM = NR * 16, KS = DH / 16, NT = BM / 8;
