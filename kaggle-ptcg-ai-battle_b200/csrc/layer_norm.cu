@@ -7,7 +7,13 @@
 // (torch nn.LayerNorm; the model's own norms, ptcg/rl/model.py:70-91, run
 // kernels tied to its row layouts.)  The statistics are two passes over the
 // row in registers, so no cancellation between sums of squares; everything
-// is fp32 until the one rounding to the output's type.
+// is fp32 until the one rounding to the output's type.  An fp32 mean is off by
+// some of its last places, which in a row far from 0 are not small beside its
+// deviations or sqrt(eps) (at 12345 one of them moves a constant row's y by 0.3
+// gamma).  Such rows take the mean of the deviations as well, a third sum, and
+// are normed about both; summed beside the squares in every row it would cost
+// 3 to 20 % of the time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 121
+// by need).
 #include <algorithm>
 #include <initializer_list>
 
@@ -25,8 +31,8 @@ constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MID_THREADS = 640, MAX_THREAD
 
 // Bound: HBM (2.1 M rows of 256, fp32 to bf16: forward 500 us, 6.5 TB/s; backward
 // with the residual's gradient 1146 us, 6.6 TB/s); wide rows are bound by the
-// latency of a row's loads and barriers (50000 x 2048, fp32 to bf16: 110 us, 5.6
-// TB/s, and 225, 4.5; 4099 x 5001 in bf16: 25 us, 3.3 TB/s, and 55, 2.2).  A row
+// latency of a row's loads and barriers (50000 x 2048, fp32 to bf16: 114 us, 5.4
+// TB/s, and 225, 4.5; 4099 x 5001 in bf16: 29 us, 2.8 TB/s, and 55, 2.2).  A row
 // belongs to one warp (width <= 1024, eight rows to a block) or to the W warps
 // of a block (MULTI).  Lane l of warp w owns pieces w * 32 * NV + l, + 32, .. so
 // that a warp's accesses are contiguous.
@@ -74,7 +80,7 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
         const float* __restrict__ gamma, const float* __restrict__ beta, long rows, int width,
         float eps) {
     constexpr int R = MULTI == MID_THREADS ? 2 : 1;
-    __shared__ float red[4][R][32];
+    __shared__ float red[4][R][32], far_red[1][R][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int w = MULTI ? warp : 0;
     const float inv = 1.f / (float)width;
@@ -119,7 +125,7 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
     int slot = 0;
     if (AHEAD) fetch(r0);
     for (; r0 < rows; r0 += R * step) {
-        float v[R][NV][V], s[R], mu[R], rs[R], se[R][1];
+        float v[R][NV][V], s[R], mu[R], dm[R], se[R][1];
         if (!AHEAD) fetch(r0);
         #pragma unroll
         for (int j = 0; j < R; j++) {
@@ -155,23 +161,51 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
         }
         row_sums<MULTI>(s, red, slot + 1, w, lane, W);
         slot ^= 2;
+        // mean squares of up to 16 times the variance (+ eps): the mean's last
+        // places are below those of h itself.  The same answer in all warps of a row
+        bool far = false;
+        #pragma unroll
+        for (int j = 0; j < R; j++) {
+            dm[j] = 0.f;
+            far = far || mu[j] * mu[j] > 16.f * fmaf(s[j], inv, eps);
+        }
+        if (__builtin_expect(far, 0)) {
+            float d[R];
+            #pragma unroll
+            for (int j = 0; j < R; j++) {
+                d[j] = edge ? se[j][0] - mu[j] : 0.f;
+                #pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    const bool in = cols.has(piece_at<V, NV>(w, lane, k));
+                    #pragma unroll
+                    for (int e = 0; e < V; e++) d[j] += in ? v[j][k][e] - mu[j] : 0.f;
+                }
+            }
+            row_sums<MULTI>(d, far_red, 0, w, lane, W);
+            #pragma unroll
+            for (int j = 0; j < R; j++) {
+                dm[j] = __fmul_rn(d[j], inv);
+                s[j] = fmaf(-d[j], dm[j], s[j]);     // sum (d - dm)^2 = sum d^2 - dm sum d
+                if (s[j] < 0.f) s[j] = 0.f;
+            }
+        }
         #pragma unroll
         for (int j = 0; j < R; j++) {
             const long r = r0 + j * step;
             if (j && r >= rows) break;
-            rs[j] = rsqrtf(fmaf(s[j], inv, eps));
+            const float rs = rsqrtf(fmaf(s[j], inv, eps));
             if (lane == 0 && w == 0) {
-                if (mean) mean[r] = mu[j];
-                if (rstd) rstd[r] = rs[j];
+                if (mean) mean[r] = mu[j] + dm[j];
+                if (rstd) rstd[r] = rs;
             }
             #pragma unroll
             for (int k = 0; k < NV; k++) {
                 #pragma unroll
-                for (int e = 0; e < V; e++) v[j][k][e] = fmaf((v[j][k][e] - mu[j]) * rs[j], gm[k][e], bt[k][e]);
+                for (int e = 0; e < V; e++) v[j][k][e] = fmaf((v[j][k][e] - mu[j] - dm[j]) * rs, gm[k][e], bt[k][e]);
                 const int p = piece_at<V, NV>(w, lane, k);
                 if (cols.has(p)) VecIO<TY, V>::st(y + r * ldy + cols.at(p), v[j][k]);
             }
-            if (edge) y[r * ldy + cols.edge] = from_f<TY>(fmaf((se[j][0] - mu[j]) * rs[j], ge, be));
+            if (edge) y[r * ldy + cols.edge] = from_f<TY>(fmaf((se[j][0] - mu[j] - dm[j]) * rs, ge, be));
         }
     }
 }

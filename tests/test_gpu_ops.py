@@ -250,6 +250,45 @@ def test_layer_norm_constant_and_far_rows(ops):
                           rtol=2 ** -20)
 
 
+@pytest.mark.parametrize("xd,at", [(F32, 12345.0), (F32, -0.1), (BF16, 12352.0)])
+@pytest.mark.parametrize("width", [1, 3, 56, 60, 112, 120, 224, 240, 252, 380, 639, 1000, 1028, 2051, 5001, 8191])
+def test_layer_norm_constant_rows_of_any_width(ops, xd, at, width):
+    """Whatever the width's reciprocal rounds to: the mean is the value, the
+    deviations are 0."""
+    x = torch.full((5, width), at, device="cuda", dtype=xd)
+    y, mean, rstd = ops.layer_norm(x, None, torch.full((width,), 0.5, device="cuda"))
+    assert (mean == x[:, 0].float()).all() and (y == 0.5).all()
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    assert ((rstd.double() / eps ** -0.5 - 1).abs() <= ref.FN).all()
+
+
+@pytest.mark.parametrize("width", [1, 3, 56, 60, 120, 240, 380, 639, 1000, 1028, 2051, 5001, 8191])
+def test_layer_norm_far_rows_with_variance(ops, width):
+    """Rows some 10^4 from 0 whose deviations are a few steps of fp32 there: y
+    is as exact as the deviations' own arithmetic.  c = x - mean, e the first
+    pass's mean's error (a step per addition): x - mu is exact, its sum is off
+    by depth u of its terms' magnitudes, at most |c| + e, and the variance
+    about it likewise; the first-order error of the mean does not appear."""
+    g = gen(width)
+    rows = 9
+    x = 1e4 + 0.01 * rand(g, rows, width) * (1 + 10 * torch.rand(rows, 1, generator=g, device="cuda"))
+    gamma, beta = 1 + 0.3 * rand(g, width), rand(g, width)
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    f = ref.norm(x, gamma, beta, eps)
+    c = f["x"] - f["mean"]
+    off = f["e_mean"]
+    size = c.abs().mean(-1, keepdim=True) + off
+    e_dm = (f["depth"] + 3) * ref.U * size
+    e_var = (f["depth"] + 8) * ref.U * ((c.abs() + off) ** 2).mean(-1, keepdim=True)
+    rel_r = 0.5 * e_var / ((c * c).mean(-1, keepdim=True) + eps) + ref.FN
+    e_h = f["rstd"] * e_dm + f["h"].abs() * (rel_r + 3 * ref.U)
+    e_y = f["g"].abs() * e_h + 3 * ref.U * ((f["h"] * f["g"]).abs() + beta.double().abs())
+    y, mean, rstd = ops.layer_norm(x, gamma, beta)
+    ref.within(y, f["y"], e_y, "y")
+    ref.within(mean, f["mean"][:, 0], (e_dm + ref.U * f["mean"].abs())[:, 0], "mean")
+    ref.within(rstd, f["rstd"][:, 0], (f["rstd"] * rel_r)[:, 0], "rstd")
+
+
 # -------------------------------------------------------- cross attention
 def problem(seed, nseq, lq, lk, heads, kvh, dh, dtype, mask, layout="rows"):
     g = gen(seed)
