@@ -1310,11 +1310,12 @@ __global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ Cross
 //   mm_rows   acc[i][j] = sum_d A[row i][d] B[row tx + 16 j][d], pairs along d
 //   mm_outer  acc[i][j] += sum_k A[k][row i] B[k][col j], pairs along the rows,
 //             A a probability tile that the threads wrote with k as its row
-// Exponentials are __expf: of x <= 0, off by at most 1.17 |x| + 2 units in the
-// last place of e^x, whose largest value over x is 2 units of the row's largest
-// probability.  Bound: the multiply-adds and the reads from shared memory that
+// Exponentials are expf, right to 2 units in the last place over the whole
+// range: the intrinsic's error grows with |x| (54 half units of 2^-24 were seen
+// down to e^-82, 4 now), for 1 to 3 % less time (170 and 399 us below).
+// Bound: the multiply-adds and the reads from shared memory that
 // feed them: 512 x 8 problems of 61 rows on up to 186 keys of width 32 take
-// 173 us forward and 406 backward (18 TFLOP/s over the kept keys).
+// 176 us forward and 403 backward (18 TFLOP/s over the kept keys).
 template <int RT> PTCG_DEV int row_of(int ty, int i) {
     return RT == 8 ? (i >> 2) * 32 + ty * 4 + (i & 3) : ty * RT + i;
 }
@@ -1535,12 +1536,12 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
             #pragma unroll
             for (int j = 1; j < NC; j++) x = fmaxf(x, s[i][j]);
             const float n = fmaxf(m[i], row16_max(x)), u = n == -INFINITY ? 0.f : n;
-            c[i] = __expf(m[i] - u);
+            c[i] = expf(m[i] - u);
             m[i] = n;
             float t = 0.f;
             #pragma unroll
             for (int j = 0; j < NC; j++) {
-                s[i][j] = __expf(s[i][j] - u);
+                s[i][j] = expf(s[i][j] - u);
                 t += s[i][j];
             }
             l[i] = fmaf(l[i], c[i], t);
@@ -1636,7 +1637,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dq_f32(const __
             #pragma unroll
             for (int i = 0; i < RT; i++) {
                 const int r = row_of<RT>(ty, i);
-                const float e = live ? __expf(fmaf(s[i][j], a.scale, -s_lse[r])) : 0.f;
+                const float e = live ? expf(fmaf(s[i][j], a.scale, -s_lse[r])) : 0.f;
                 v[i] = e * (p[i][j] - s_delta[r]);
             }
             put_rows<RT>(Ds, LM, tx + 16 * j, ty, v);
@@ -1730,7 +1731,7 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
                     float v[RT];
                     #pragma unroll
                     for (int i = 0; i < RT; i++) {
-                        v[i] = ok[row_of<RT>(ty, i)] ? __expf(fmaf(s[i][j], a.scale, -x)) : 0.f;
+                        v[i] = ok[row_of<RT>(ty, i)] ? expf(fmaf(s[i][j], a.scale, -x)) : 0.f;
                         p[i][j] = v[i] * (p[i][j] - d);
                     }
                     put_rows<RT>(Ps, LM, c, ty, v);

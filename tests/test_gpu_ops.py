@@ -475,6 +475,36 @@ def test_cross_attention_long_sums(ops):
             assert err < 2.0 ** -20, (name, err)
 
 
+@pytest.mark.parametrize("lq", [1, 20, 40, 100])
+def test_cross_attention_small_probabilities(ops, lq):
+    """fp32 probabilities down to e^-82 are as exact as large ones.  The scores
+    are whole numbers, so they are exact; one is 0 and the rest below e^-20, so
+    that the sum rounds to 1 and the log-sum-exp to 0 (both true to 2^-28).  Each
+    result that is looked at is one exponential, off by 2 units of the last
+    place (4 u), times factors that are exact or off by a few u: out 3 P (u each
+    from the division and the product), dv P, dq P (dP - delta) with dP = 3 and
+    delta = 1 (2 u of it, which is u of the difference of 2, and u each from
+    the difference, the product and the last factor)."""
+    dh = 32
+    z = lambda n: torch.zeros(1, n, 1, dh, device="cuda")          # noqa: E731
+    q, k, v, dout = z(lq), z(dh), z(dh), z(lq)
+    s = torch.tensor([0.0] + [-20.0 - 2 * j for j in range(1, dh)], device="cuda")
+    q[..., 0] = 1
+    k[0, :, 0, 0] = s
+    v[0, 0, 0, 0] = 1
+    for j in range(1, dh):
+        k[0, j, 0, j], v[0, j, 0, j] = 1, 3
+    out, lse = ops.cross_attention(q, k, v, scale=1.0)
+    p = torch.softmax(s.double(), 0)
+    off = lambda got, want: ((got.double() / want - 1).abs().max() / ref.U).item()   # noqa: E731
+    assert (lse == 0).all()
+    assert off(out[0, :, 0, 1:], 3 * p[1:]) <= 7
+    dout[0, lq - 1] = 1
+    dq, dk, dv = ops.cross_attention_backward(dout, q, k, v, out, lse, scale=1.0)
+    assert off(dv[0, :, 0], p[:, None].expand(dh, dh)) <= 7
+    assert off(dq[0, lq - 1, 0, 1:], 2 * p[1:]) <= 9
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_cross_attention_large_scores(ops, dtype):
     """Scores of hundreds: the running maximum keeps every exponential in
