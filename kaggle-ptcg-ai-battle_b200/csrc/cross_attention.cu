@@ -493,10 +493,14 @@ __global__ void __launch_bounds__(128, DH == 32 ? 6 : DH == 64 ? 3 : 2) k_cross_
 
 // joins the parts of a split forward: a block per stacked row, whose warps take
 // every fourth part and are added in order (single tokens over a long cache
-// have few rows, and each has many parts)
+// have few rows, and each has many parts).  A part's maximum comes as the shift
+// that its exponentials took, of e in fp32 and of 2 in bf16: turned into the
+// other base it would be rounded, and the part's weight be off by that much (554
+// half units of 2^-24 at scores of 1000)
 template <typename T, int DH>
 __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ CrossArgs a) {
     constexpr int C = DH / 32;                      // columns a lane
+    constexpr bool F32 = sizeof(T) == 4;
     __shared__ float sy[4][DH], sl[4];
     const long row = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
     #pragma unroll 8
     for (int i = warp; i < parts; i += 4) {
         const float2 x = ml[i];
-        const float c = ex2_approx(x.x - u);
+        const float c = F32 ? expf(x.x - u) : ex2_approx(x.x - u);
         l = fmaf(x.y, c, l);
         #pragma unroll
         for (int e = 0; e < C; e++) y[e] = fmaf(p[(long)i * DH + e * 32], c, y[e]);
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
     const float inv = l == 0.f ? 0.f : 1.f / l;
     for (int d = threadIdx.x; d < DH; d += 128)
         ((T*)a.out + qrow(a, a.so, seq, hk, r))[d] = from_f<T>((sy[0][d] + sy[1][d] + sy[2][d] + sy[3][d]) * inv);
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (threadIdx.x == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : F32 ? m + logf(l) : (m + log2f(l)) * LN2;
 }
 
 // --------------------------------------------------------- bf16 backward
@@ -1311,8 +1315,8 @@ __global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ Cross
 //   mm_outer  acc[i][j] += sum_k A[k][row i] B[k][col j], pairs along the rows,
 //             A a probability tile that the threads wrote with k as its row
 // Exponentials are expf, right to 2 units in the last place over the whole
-// range: the intrinsic's error grows with |x| (54 half units of 2^-24 were seen
-// down to e^-82, 4 now), for 1 to 3 % less time (170 and 399 us below).
+// range: the intrinsic's error grows with |x| (54 half units of 2^-24 at e^-82,
+// 2 with expf), for 1 to 3 % less time (170 and 399 us below).
 // Bound: the multiply-adds and the reads from shared memory that
 // feed them: 512 x 8 problems of 61 rows on up to 186 keys of width 32 take
 // 176 us forward and 403 backward (18 TFLOP/s over the kept keys).
@@ -1576,8 +1580,7 @@ __global__ void __launch_bounds__(128, RT == 8 && DH == 32 ? 4 : 1) k_cross_fwd_
                                 : (float*)a.out + qrow(a, a.so, at.seq, at.hk, r);
         put_cols<ND>(p, tx, o[i], inv);
         if (tx == 0) {
-            // the parts carry their maximum in the log2 domain, as the bf16 kernel's do
-            if (a.nsplit > 1) a.part_ml[row * a.nsplit + at.part] = make_float2(m[i] * LOG2E, t);
+            if (a.nsplit > 1) a.part_ml[row * a.nsplit + at.part] = make_float2(m[i], t);
             else if (a.lse) a.lse[row] = t == 0.f ? -INFINITY : m[i] + logf(t);
         }
     }

@@ -505,6 +505,32 @@ def test_cross_attention_small_probabilities(ops, lq):
     assert off(dq[0, lq - 1, 0, 1:], 2 * p[1:]) <= 9
 
 
+@pytest.mark.parametrize("even", [False, True])
+@pytest.mark.parametrize("lq", [1, 20, 100])
+def test_cross_attention_parts_of_large_scores(ops, even, lq):
+    """fp32 keys that are split into parts and joined keep what scores of 1000
+    have left: eight scores that are exact, one in every eighth of the cache.
+    Per column one part counts: its weight is one exponential (4 u, the
+    difference in it exact), over the sum of eight (4 u, and u for each of seven
+    additions in some order), and u each for the reciprocal and the product;
+    where parts hold several of the keys their own sums and factors come to
+    another 12 u at most."""
+    dh, lk, n = 32, 8192, 8
+    q, k, v = (torch.zeros(1, r, 1, dh, device="cuda") for r in (lq, lk, lk))
+    keep = torch.zeros(1, lk, dtype=torch.bool, device="cuda")
+    s = torch.tensor([1000 - 1.375 * ((3 * b) % n) for b in range(n)], device="cuda")
+    q[..., 0] = 1
+    for b in range(n):
+        at = b * (lk // n) + 5
+        keep[0, at], k[0, at, 0, 0], v[0, at, 0, b] = True, s[b], 1
+    kv_len = torch.tensor([lk], dtype=torch.int32, device="cuda") if even else None
+    out, lse = ops.cross_attention(q, k, v, keep=keep, kv_len=kv_len, scale=1.0)
+    p = torch.softmax(s.double(), 0)
+    assert ((out[..., :n].double() / p - 1).abs() <= 29 * ref.U).all()
+    want = torch.logsumexp(s.double(), 0)
+    assert ((lse.double() - want).abs() <= ref.U * want + 16 * ref.U).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_cross_attention_large_scores(ops, dtype):
     """Scores of hundreds: the running maximum keeps every exponential in
