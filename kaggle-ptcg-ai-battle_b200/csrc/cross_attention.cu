@@ -12,7 +12,8 @@
 // Masked keys never reach a sum: their K and V rows become zeros in shared
 // memory (not loaded, or cleared after a tile's TMA copy) and their
 // probabilities are set to 0, so whatever they hold (NaN, infinities, rows
-// never written) has no effect.
+// never written) has no effect.  Their own gradients are written as zeros, not
+// as the sums of zeros times dout, which may hold infinities.
 #include <algorithm>
 
 #include "cross.cuh"
@@ -554,16 +555,17 @@ PTCG_DEV uint4 quad_piece(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, in
     const uint32_t c1 = __shfl_xor_sync(0xffffffffu, hi ? a1 : b1, 2);
     return hi ? make_uint4(c0, c1, b0, b1) : make_uint4(a0, a1, c0, c1);
 }
-// the accumulators' upper or lower row times f as bf16; every lane takes part,
-// those with `in` store
+// the accumulators' upper or lower row times f as bf16 (zeros where `keep` is not
+// all ones); every lane takes part, those with `in` store
 template <int DH>
-PTCG_DEV void put_acc(bf16* row, int t, bool in, float f, const float (&acc)[DH / 8][4], int half) {
+PTCG_DEV void put_acc(bf16* row, int t, bool in, float f, const float (&acc)[DH / 8][4], int half,
+                      uint32_t keep = 0xffffffffu) {
     #pragma unroll
     for (int j = 0; j < DH / 8; j += 4) {
         uint32_t v[4];
         #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = pack_bf2(acc[j + i][2 * half] * f, acc[j + i][2 * half + 1] * f);
-        const uint4 w = quad_piece(v[0], v[1], v[2], v[3], t);
+        const uint4 w = quad_piece(v[0] & keep, v[1] & keep, v[2] & keep, v[3] & keep, t);
         if (in) *(uint4*)(row + (j + t) * 8) = w;
     }
 }
@@ -783,14 +785,14 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
         dv[i][0] = dv[i][1] = dv[i][2] = dv[i][3] = 0.f;
     }
     const int g = lane >> 2, t = lane & 3;
+    const uint32_t wk = (warp & 2 ? w1 : w0) >> ((warp & 1) * 16);
+    const bool ka = (wk >> g) & 1, kb = (wk >> (g + 8)) & 1;
     if (any) {
         stage_k<DH, BK, THREADS>(sK, (const bf16*)a.k, a.sk, at.seq, at.hk, j0, bits);
         stage_k<DH, BK, THREADS>(sV, (const bf16*)a.v, a.sv, at.seq, at.hk, j0, bits);
         load(0);
         load_stat(0);
         const float sc = a.scale * LOG2E;
-        const uint32_t wk = warp & 2 ? w1 : w0;
-        const bool ka = (wk >> ((warp & 1) * 16 + g)) & 1, kb = (wk >> ((warp & 1) * 16 + g + 8)) & 1;
         uint32_t kf[REGS ? KS : 1][4], vf[REGS ? KS : 1][4];
         for (int j = 0; j < nt; j++) {
             put_stat(j);
@@ -868,18 +870,20 @@ __global__ void __launch_bounds__(128) k_cross_dkv(const __grid_constant__ Cross
     #pragma unroll
     for (int half = 0; half < 2; half++) {
         const int j = j0 + warp * 16 + g + half * 8;
-        const bool in = j < a.lk;
+        const bool in = j < a.lk, live = half ? kb : ka;
         if (a.nsplit > 1) {
             if (!in) continue;
             const long at_row = (((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part;
             #pragma unroll
             for (int i = 0; i < DH / 8; i++) {
-                *(float2*)(a.part + at_row * DH + i * 8 + 2 * t) = make_float2(dk[i][2 * half] * a.scale, dk[i][2 * half + 1] * a.scale);
-                *(float2*)(a.part2 + at_row * DH + i * 8 + 2 * t) = make_float2(dv[i][2 * half], dv[i][2 * half + 1]);
+                const float2 z = make_float2(0.f, 0.f);
+                *(float2*)(a.part + at_row * DH + i * 8 + 2 * t) = live ? make_float2(dk[i][2 * half] * a.scale, dk[i][2 * half + 1] * a.scale) : z;
+                *(float2*)(a.part2 + at_row * DH + i * 8 + 2 * t) = live ? make_float2(dv[i][2 * half], dv[i][2 * half + 1]) : z;
             }
         } else {
-            put_acc<DH>((bf16*)a.dk + krow(a.sdk, at.seq, at.hk, j), t, in, a.scale, dk, half);
-            put_acc<DH>((bf16*)a.dv + krow(a.sdv, at.seq, at.hk, j), t, in, 1.f, dv, half);
+            const uint32_t keep = live ? 0xffffffffu : 0u;
+            put_acc<DH>((bf16*)a.dk + krow(a.sdk, at.seq, at.hk, j), t, in, a.scale, dk, half, keep);
+            put_acc<DH>((bf16*)a.dv + krow(a.sdv, at.seq, at.hk, j), t, in, 1.f, dv, half, keep);
         }
     }
 }
@@ -1054,8 +1058,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
                 const float f = which ? a.scale : 1.f;
                 bf16* out = which ? pk : pv;
                 const long down = 8 * (which ? a.sdk.row : a.sdv.row);
-                put_acc<DH>(out, t, ina, f, acc, 0);
-                put_acc<DH>(out + down, t, inb, f, acc, 1);
+                put_acc<DH>(out, t, ina, f, acc, 0, (wk >> g) & 1 ? 0xffffffffu : 0u);
+                put_acc<DH>(out + down, t, inb, f, acc, 1, (wk >> (g + 8)) & 1 ? 0xffffffffu : 0u);
             }
         } else {                                 // masked keys: no gradient
             if (ina) { put_zeros<DH>(pk, t); put_zeros<DH>(pv, t); }
@@ -1249,8 +1253,8 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_
             const float f = which ? a.scale : 1.f;
             bf16* out = which ? pk : pv;
             const long down = 8 * (which ? a.sdk.row : a.sdv.row);
-            put_acc<DH>(out, t, ina, f, acc, 0);
-            put_acc<DH>(out + down, t, inb, f, acc, 1);
+            put_acc<DH>(out, t, ina, f, acc, 0, ma == 0.f ? 0xffffffffu : 0u);
+            put_acc<DH>(out + down, t, inb, f, acc, 1, mb == 0.f ? 0xffffffffu : 0u);
         }
     }
     __syncthreads();
@@ -1772,6 +1776,10 @@ __global__ void __launch_bounds__(128, DH == 32 ? 3 : 1) k_cross_dkv_f32(const _
         for (int i = 0; i < RT; i++) {
             const int j = j0 + row_of<RT>(ty, i);
             if (j >= kto) continue;
+            if (!ok[j - j0]) {
+                #pragma unroll
+                for (int c = 0; c < ND; c++) dk[i][c] = dv[i][c] = 0.f;
+            }
             const bool parts = !ROWS && a.nsplit > 1;
             const long part = ((((long)at.seq * a.kv_heads + at.hk) * a.lk + j) * a.nsplit + at.part) * DH;
             put_cols<ND>(parts ? a.part + part : (float*)a.dk + krow(a.sdk, at.seq, at.hk, j), tx, dk[i], a.scale);

@@ -446,6 +446,26 @@ def test_cross_attention_masked_keys_may_hold_anything(ops, dtype, lq):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nseq,lq,lk,dh", [(2, 20, 50, 64), (2, 20, 600, 64), (2, 100, 50, 64), (2, 100, 200, 128),
+                                           (1, 3000, 60, 32), (2, 600, 700, 64), (1, 7, 3000, 32)])
+def test_cross_attention_masked_keys_take_no_gradient(ops, dtype, nseq, lq, lk, dh):
+    """Nor where dout holds infinities or NaN: 0 times those is not 0."""
+    q, k, v, m = problem(lq, nseq, lq, lk, 4, 2, dh, dtype, "keep len")
+    live = ref.live_keys(nseq, lk, m["keep"], m["kv_len"], "cuda")
+    if nseq == 1:                                # problem() empties the only one
+        m["keep"][:] = torch.rand(1, lk, generator=gen(3), device="cuda") < 0.6
+        m["kv_len"][:] = lk - 7
+        live = ref.live_keys(nseq, lk, m["keep"], m["kv_len"], "cuda")
+    dout = rand(gen(5), *q.shape, dtype=dtype)
+    dout[0, lq // 2, 1, 5], dout[0, lq - 1, 3, dh - 1] = math.inf, math.nan
+    out, lse = ops.cross_attention(q, k, v, **m)
+    dq, dk, dv = ops.cross_attention_backward(dout, q, k, v, out, lse, **m)
+    assert live.any() and not live.all()
+    assert (dk[~live] == 0).all() and (dv[~live] == 0).all()
+    assert not dv[live].isfinite().all()         # a kept key does take them
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_cross_attention_no_lengths(ops, dtype):
     z = lambda *s: torch.zeros(*s, device="cuda", dtype=dtype)     # noqa: E731
     out, lse = ops.cross_attention(z(2, 3, 4, 32), z(2, 0, 2, 32), z(2, 0, 2, 32))
