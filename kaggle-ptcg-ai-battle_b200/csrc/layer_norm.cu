@@ -10,9 +10,9 @@
 // is fp32 until the one rounding to the output's type.  An fp32 mean is off by
 // some of its last places, which in a row far from 0 are not small beside its
 // deviations or sqrt(eps) (at 12345 one of them moves a constant row's y by 0.3
-// gamma).  Such rows take the mean of the deviations as well, a third sum, and
-// are normed about both; summed beside the squares in every row it would cost
-// 3 to 20 % of the time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 121
+// gamma) or, squared, lie past its range.  Such rows take the mean of the
+// deviations as well, a third sum, and are normed about both, their variance too; summed beside the squares in every row it would cost
+// 3 to 20 % of the time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 124
 // by need).
 #include <algorithm>
 #include <initializer_list>
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
         const float* __restrict__ gamma, const float* __restrict__ beta, long rows, int width,
         float eps) {
     constexpr int R = MULTI == MID_THREADS ? 2 : 1;
-    __shared__ float red[4][R][32], far_red[1][R][32];
+    __shared__ float red[4][R][32], far_red[2][R][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
     const int w = MULTI ? warp : 0;
     const float inv = 1.f / (float)width;
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
         #pragma unroll
         for (int j = 0; j < R; j++) {
             dm[j] = 0.f;
-            far = far || mu[j] * mu[j] > 16.f * fmaf(s[j], inv, eps);
+            const float t = fmaf(s[j], inv, eps);
+            far = far || mu[j] * mu[j] > 16.f * t || t == INFINITY;
         }
         if (__builtin_expect(far, 0)) {
             float d[R];
@@ -184,10 +185,21 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
             row_sums<MULTI>(d, far_red, 0, w, lane, W);
             #pragma unroll
             for (int j = 0; j < R; j++) {
-                dm[j] = __fmul_rn(d[j], inv);
-                s[j] = fmaf(-d[j], dm[j], s[j]);     // sum (d - dm)^2 = sum d^2 - dm sum d
-                if (s[j] < 0.f) s[j] = 0.f;
+                // divided, so that equal deviations (a constant row) leave nothing
+                dm[j] = d[j] / (float)width;
+                s[j] = edge ? se[j][0] - mu[j] - dm[j] : 0.f;
+                s[j] *= s[j];
+                #pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    const bool in = cols.has(piece_at<V, NV>(w, lane, k));
+                    #pragma unroll
+                    for (int e = 0; e < V; e++) {
+                        const float x = in ? v[j][k][e] - mu[j] - dm[j] : 0.f;
+                        s[j] = fmaf(x, x, s[j]);
+                    }
+                }
             }
+            row_sums<MULTI>(s, far_red, 1, w, lane, W);
         }
         #pragma unroll
         for (int j = 0; j < R; j++) {

@@ -289,6 +289,18 @@ def test_layer_norm_far_rows_with_variance(ops, width):
     ref.within(rstd, f["rstd"][:, 0], (f["rstd"] * rel_r)[:, 0], "rstd")
 
 
+@pytest.mark.parametrize("width", [1, 37, 62, 100, 127, 130])
+@pytest.mark.parametrize("at", [3e19, -2e36])
+def test_layer_norm_huge_constant_rows(ops, at, width):
+    """One last place of the mean, squared, is past fp32's range there; the
+    variance is 0 all the same."""
+    x = torch.full((5, width), at, device="cuda")
+    y, mean, rstd = ops.layer_norm(x)
+    assert (y == 0).all() and (mean == x[:, 0]).all()
+    eps = float(torch.tensor(1e-5, dtype=F32))
+    assert ((rstd.double() / eps ** -0.5 - 1).abs() <= ref.FN).all()
+
+
 # -------------------------------------------------------- cross attention
 def problem(seed, nseq, lq, lk, heads, kvh, dh, dtype, mask, layout="rows"):
     g = gen(seed)
