@@ -299,8 +299,9 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_bwd(
             row.re.get(re);
         }
         if (AHEAD) fetch(r + step);
+        // past the row g is 0, but mu rs need not be finite: no h there in the sums
         if (PHASED) {                               // 0 gradient where there is no edge column
-            xe[0] = (xe[0] - mu) * rs;
+            xe[0] = (xe[0] - mu) * (edge ? rs : 0.f);
             age = fmaf(gy[0], xe[0], age);
             abe += gy[0];
             gy[0] *= ge;
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_bwd(
                 g[k][e] *= gm[k][e];
                 h[k][e] = hh;
                 s[0] += g[k][e];
-                s[1] = fmaf(g[k][e], hh, s[1]);
+                s[1] = cols.has(piece_at<V, NV>(w, lane, k)) ? fmaf(g[k][e], hh, s[1]) : s[1];
             }
         }
         row_sums<MULTI>(s, red, slot, w, lane, W);

@@ -301,6 +301,23 @@ def test_layer_norm_huge_constant_rows(ops, at, width):
     assert ((rstd.double() / eps ** -0.5 - 1).abs() <= ref.FN).all()
 
 
+@pytest.mark.parametrize("width,pitch,offset", [(37, 37, 0), (100, 100, 0), (37, 39, 1), (62, 62, 2), (130, 130, 0)])
+def test_layer_norm_gradient_of_huge_rows(ops, width, pitch, offset):
+    """Constant rows so large that mean * rstd is past fp32's range: h is 0, and
+    dx is the gradient less its mean, times rstd."""
+    buf = torch.full((3 * pitch + 4,), 2e36, device="cuda")
+    x = buf[offset:offset + 3 * pitch].view(3, pitch)[:, :width]
+    y, mean, rstd = ops.layer_norm(x)
+    assert (y == 0).all()
+    dy = rand(gen(width), 3 * pitch + 4)[offset:offset + 3 * pitch].view(3, pitch)[:, :width]
+    f = ref.norm(torch.zeros(3, width, device="cuda"), None, None, float(torch.tensor(1e-5, dtype=F32)))
+    dx, e_dx, dg, e_dg, db, e_db = ref.norm_grad(f, dy, None, F32)
+    got = ops.layer_norm_backward(dy, x, None, mean, rstd)
+    ref.within(got[0], dx, 2 * e_dx, "dx")
+    assert (got[1] == 0).all()
+    ref.within(got[2], db, e_db, "dbeta")
+
+
 # -------------------------------------------------------- cross attention
 def problem(seed, nseq, lq, lk, heads, kvh, dh, dtype, mask, layout="rows"):
     g = gen(seed)
