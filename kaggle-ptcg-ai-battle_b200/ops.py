@@ -171,6 +171,8 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dres=None, dgamma=None, dbeta=
     are new, or written or (accumulate) added to where given; with
     weight_grads=False they are None."""
     dev, width = x.device, x.shape[-1] if x.dim() else 0
+    if mean is None or rstd is None:
+        _bad("mean and rstd are the forward's (layer_norm with stats=True), not None")
     xr, n, ldx = _rows(x, width, "x")
     if dy.shape != x.shape or (dres is not None and (dres.shape != x.shape or dres.dtype != x.dtype)):
         _bad("dy and dres must have x's shape, and dres its type")
@@ -275,6 +277,8 @@ def cross_attention_backward(dout, q, k, v, out, lse, keep=None, kv_len=None, sc
     if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
         _bad("dout and out must have q's shape and type")
     _on(dev, dout=dout, out=out)
+    if lse is None:
+        _bad("lse is the forward's, not None")
     _f32(dev, (nseq, heads, lq), lse=lse)
     dq = torch.empty(nseq, lq, heads, dh, dtype=q.dtype, device=dev)
     dk = torch.empty(nseq, lk, kvh, dh, dtype=q.dtype, device=dev)

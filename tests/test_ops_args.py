@@ -211,3 +211,17 @@ def test_torch_calls_refuse(pkg):
             lambda: ops.cross_attention_backward(o, q, k, k, o.bfloat16(), lse)]:
         with pytest.raises(PtcgError):
             call()
+
+
+def test_torch_calls_refuse_missing_statistics(pkg):
+    """What layer_norm(stats=False) returns is no argument of the backward."""
+    import ptcg_b200.ops as ops
+    from ptcg_b200.native import PtcgError
+    t, s, one = torch.zeros(4, 8), torch.zeros(4), torch.zeros(8)
+    q, k = torch.zeros(2, 3, 4, 32), torch.zeros(2, 5, 2, 32)
+    for call in [lambda: ops.layer_norm_backward(t, t, one, None, None),
+                 lambda: ops.layer_norm_backward(t, t, one, s, None),
+                 lambda: ops.layer_norm_backward(t, t, one, None, s, weight_grads=False),
+                 lambda: ops.cross_attention_backward(q, q, k, k, q, None)]:
+        with pytest.raises(PtcgError, match="not None"):
+            call()
