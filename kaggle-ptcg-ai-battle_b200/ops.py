@@ -28,6 +28,12 @@ def _bad(msg):
     raise PtcgError(msg)
 
 
+def _fits(what, *sizes):
+    """The C entries take these as 32-bit ints; ctypes would cut them off."""
+    if max(sizes) > 0x7fffffff:
+        _bad(f"{what}: sizes {sizes} do not all fit 32 bits")
+
+
 def _dt(t, what):
     d = _DT.get(t.dtype)
     if d is None:
@@ -100,8 +106,8 @@ def _ids(ids, dev):
 def _pad(pad_id):
     if pad_id is None:
         return -1
-    if pad_id < 0:
-        _bad("pad_id must be None or at least 0")
+    if not 0 <= pad_id <= 0x7fffffff:
+        _bad(f"pad_id {pad_id} must be None or an id of 32 bits, at least 0")
     return int(pad_id)
 
 
@@ -112,12 +118,14 @@ def embedding(table, ids, scale=1.0, pad_id=None, out_dtype=None):
     if table.dim() != 2:
         _bad("table must be (vocab, width)")
     dev = table.device
-    ids = _ids(ids, dev)
     vocab, width = table.shape
+    _fits("table", vocab, width)
+    pad_id = _pad(pad_id)
+    ids = _ids(ids, dev)
     tab, _, ldt = _rows(table, width, "table")
     out = torch.empty(*ids.shape, width, dtype=out_dtype or table.dtype, device=dev)
     _call(dev, native.lib().ptcg_embedding_fwd, tab.data_ptr(), _dt(table, "table"), ldt, vocab,
-          width, ids.data_ptr(), ids.numel(), scale, _pad(pad_id), out.data_ptr(),
+          width, ids.data_ptr(), ids.numel(), scale, pad_id, out.data_ptr(),
           _dt(out, "out"), width)
     return out
 
@@ -131,6 +139,10 @@ def embedding_backward(dout, ids, vocab, scale=1.0, pad_id=None, dtable=None, ac
     if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
         _bad(f"dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)}")
     width = dout.shape[-1]
+    _fits("dout", vocab, width)
+    if vocab <= 0:
+        _bad(f"vocab {vocab} must be at least 1")
+    pad_id = _pad(pad_id)
     g, n, ldg = _rows(dout, width, "dout")
     if dtable is None:
         if accumulate:
@@ -143,7 +155,7 @@ def embedding_backward(dout, ids, vocab, scale=1.0, pad_id=None, dtable=None, ac
     nbytes = lib.ptcg_embedding_bwd_scratch(n, vocab, width)
     scratch = _scratch(nbytes, dev)
     _call(dev, lib.ptcg_embedding_bwd, g.data_ptr(), _dt(dout, "dout"), ldg, ids.data_ptr(), n,
-          scale, _pad(pad_id), dtable.data_ptr(), dtable.stride(0) if vocab > 1 else width, vocab,
+          scale, pad_id, dtable.data_ptr(), dtable.stride(0) if vocab > 1 else width, vocab,
           width, int(accumulate), _ptr(scratch), nbytes)
     return dtable
 
@@ -154,6 +166,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out_dtype=None, stats=True):
     float32 or None (1 / 0).  mean and rstd (float32, x.shape[:-1]) are what
     the backward takes; stats=False leaves them out (None)."""
     dev, width = x.device, x.shape[-1] if x.dim() else 0
+    _fits("x", width)
     xr, n, ldx = _rows(x, width, "x")
     _f32(dev, (width,), gamma=gamma, beta=beta)
     y = torch.empty(*x.shape, dtype=out_dtype or x.dtype, device=dev)
@@ -171,6 +184,7 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dres=None, dgamma=None, dbeta=
     are new, or written or (accumulate) added to where given; with
     weight_grads=False they are None."""
     dev, width = x.device, x.shape[-1] if x.dim() else 0
+    _fits("x", width)
     if mean is None or rstd is None:
         _bad("mean and rstd are the forward's (layer_norm with stats=True), not None")
     xr, n, ldx = _rows(x, width, "x")
@@ -231,6 +245,7 @@ def _cross_args(q, k, v, keep, kv_len, scale):
     dev, dt = q.device, _dt(q, "q")
     nseq, lq, heads, dh = q.shape
     lk, kvh = k.shape[1], k.shape[2]
+    _fits("q, k", nseq, lq, lk, heads, kvh, dh)
     if k.shape[0] != nseq or k.shape[3] != dh or v.shape != k.shape:
         _bad(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     if k.dtype != q.dtype or v.dtype != q.dtype:

@@ -225,3 +225,29 @@ def test_torch_calls_refuse_missing_statistics(pkg):
                  lambda: ops.cross_attention_backward(q, q, k, k, q, None)]:
         with pytest.raises(PtcgError, match="not None"):
             call()
+
+
+def test_torch_calls_refuse_sizes_past_32_bits(pkg):
+    """They are ints in C, and what is above 2^31 would be cut off."""
+    import ptcg_b200.ops as ops
+    from ptcg_b200.native import PtcgError
+    big = (1 << 32) + 5
+    i32, one = torch.zeros(3, dtype=torch.int32), torch.zeros(1)
+    q, k = torch.zeros(1, 1, 1, 32), torch.zeros(1, 1, 1, 32)
+    row = one.expand(big)
+    for call in [lambda: ops.embedding(torch.zeros(4, 8), i32, pad_id=big),
+                 lambda: ops.embedding(torch.zeros(4, 8), i32, pad_id=1 << 31),
+                 lambda: ops.embedding(one.expand(big, 1), i32),
+                 lambda: ops.embedding(one.expand(1, big), i32),
+                 lambda: ops.embedding_backward(torch.zeros(3, 8), i32, big),
+                 lambda: ops.embedding_backward(torch.zeros(3, 8), i32, 4, pad_id=big),
+                 lambda: ops.embedding_backward(one.expand(3, big), i32, 4),
+                 lambda: ops.layer_norm(row),
+                 lambda: ops.layer_norm_backward(row, row, None, one, one),
+                 lambda: ops.cross_attention(q, k.expand(1, big, 1, 32), k.expand(1, big, 1, 32)),
+                 lambda: ops.cross_attention(q.expand(1, big, 1, 32), k, k),
+                 lambda: ops.cross_attention(q.expand(big, 1, 1, 32), *[k.expand(big, 1, 1, 32)] * 2)]:
+        with pytest.raises(PtcgError, match="32 bits"):
+            call()
+    with pytest.raises(PtcgError, match="at least 1"):
+        ops.embedding_backward(torch.zeros(3, 8), i32, -1)
