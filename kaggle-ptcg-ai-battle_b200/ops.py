@@ -8,7 +8,10 @@ from torch's allocator.  Nothing waits on the host, so the calls can be
 captured in a CUDA graph.  A tensor last used on another stream has to be
 ordered before the call by the caller, as for any torch operation.  Arguments
 are checked before anything is launched; errors raise `PtcgError`.  Nothing is
-recorded for autograd: the gradients are calls of their own.
+recorded for autograd: the gradients are calls of their own.  A forward whose
+inputs, or a backward whose incoming gradients, require grad is refused while
+autograd records (its outputs would be cut off without a word); under
+`torch.no_grad()`, in an `autograd.Function` and on detached tensors they run.
 """
 from __future__ import annotations
 
@@ -26,6 +29,14 @@ _BYTES = (torch.bool, torch.uint8)
 
 def _bad(msg):
     raise PtcgError(msg)
+
+
+def _records_nothing(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _bad("an input requires grad, but the operators record nothing for autograd: "
+                     "call them under torch.no_grad() or on detached tensors")
 
 
 def _fits(what, *sizes):
@@ -117,6 +128,7 @@ def embedding(table, ids, scale=1.0, pad_id=None, out_dtype=None):
     zeros."""
     if table.dim() != 2:
         _bad("table must be (vocab, width)")
+    _records_nothing(table)
     dev = table.device
     vocab, width = table.shape
     _fits("table", vocab, width)
@@ -134,6 +146,7 @@ def embedding_backward(dout, ids, vocab, scale=1.0, pad_id=None, dtable=None, ac
     """Gradient of `embedding` for its table: float32 (vocab, width), every row
     the sum of its places' gradients, in an order that follows from the ids
     alone.  With accumulate, added to dtable."""
+    _records_nothing(dout)
     dev = dout.device
     ids = _ids(ids, dev)
     if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
@@ -165,6 +178,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out_dtype=None, stats=True):
     """(y, mean, rstd) of a layer norm over the last dimension; gamma / beta
     float32 or None (1 / 0).  mean and rstd (float32, x.shape[:-1]) are what
     the backward takes; stats=False leaves them out (None)."""
+    _records_nothing(x, gamma, beta)
     dev, width = x.device, x.shape[-1] if x.dim() else 0
     _fits("x", width)
     xr, n, ldx = _rows(x, width, "x")
@@ -183,6 +197,7 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dres=None, dgamma=None, dbeta=
     gradient that reaches x past the norm, x's type) if given.  dgamma / dbeta
     are new, or written or (accumulate) added to where given; with
     weight_grads=False they are None."""
+    _records_nothing(dy, dres)
     dev, width = x.device, x.shape[-1] if x.dim() else 0
     _fits("x", width)
     if mean is None or rstd is None:
@@ -270,6 +285,7 @@ def cross_attention(q, k, v, keep=None, kv_len=None, scale=None):
     (nseq, lk) bool / uint8 and kv_len (nseq,) int32 mask keys; scale defaults
     to dh ** -0.5.  out is q's shape and type; lse (nseq, heads, lq) float32
     is what the backward takes (-inf, with out 0, where no key is kept)."""
+    _records_nothing(q, k, v)
     dev, dt, dims, keep, kv_len, scale = _cross_args(q, k, v, keep, kv_len, scale)
     nseq, lq, lk, heads, kvh, dh = dims
     out = torch.empty(nseq, lq, heads, dh, dtype=q.dtype, device=dev)
@@ -287,6 +303,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, keep=None, kv_len=None, sc
     """(dq, dk, dv) of `cross_attention`, contiguous, in the inputs' type and
     shapes; out and lse are the forward's.  dk and dv are summed over the query
     heads of a group and are zero for masked keys."""
+    _records_nothing(dout)
     dev, dt, dims, keep, kv_len, scale = _cross_args(q, k, v, keep, kv_len, scale)
     nseq, lq, lk, heads, kvh, dh = dims
     if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:

@@ -738,6 +738,31 @@ def test_two_streams_at_once(ops):
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
 
 
+def test_under_an_autograd_function(ops):
+    """The calls as the two passes of a Function: its leaves get the gradients
+    that the calls return."""
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, gamma, beta):
+            y, mean, rstd = ops.layer_norm(x, gamma, beta)
+            ctx.save_for_backward(x, gamma, mean, rstd)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            return ops.layer_norm_backward(dy, *ctx.saved_tensors)
+
+    g = gen(71)
+    leaves = [t.requires_grad_() for t in (rand(g, 40, 96), rand(g, 96), rand(g, 96))]
+    dy = rand(g, 40, 96)
+    y = Norm.apply(*leaves)
+    y.backward(dy)
+    with torch.no_grad():
+        y2, mean, rstd = ops.layer_norm(*leaves)
+        want = ops.layer_norm_backward(dy, leaves[0], leaves[1], mean, rstd)
+    assert torch.equal(y, y2) and all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
 def test_launches_are_counted(pkg, ops):
     import ptcg_b200.native as n
     lib = n.lib()

@@ -251,3 +251,29 @@ def test_torch_calls_refuse_sizes_past_32_bits(pkg):
             call()
     with pytest.raises(PtcgError, match="at least 1"):
         ops.embedding_backward(torch.zeros(3, 8), i32, -1)
+
+
+def test_torch_calls_refuse_what_autograd_would_lose(pkg):
+    import ptcg_b200.ops as ops
+    from ptcg_b200.native import PtcgError
+    z = lambda *s, need=False: torch.zeros(*s, requires_grad=need)     # noqa: E731
+    i32, s, one, lse = torch.zeros(3, dtype=torch.int32), z(4), z(8), z(2, 4, 3)
+    q, k, t = z(2, 3, 4, 32), z(2, 5, 2, 32), z(4, 8)
+    calls = [lambda n: ops.embedding(z(4, 8, need=n), i32),
+             lambda n: ops.embedding_backward(z(3, 8, need=n), i32, 4),
+             lambda n: ops.layer_norm(z(4, 8, need=n)),
+             lambda n: ops.layer_norm(t, z(8, need=n)),
+             lambda n: ops.layer_norm(t, one, z(8, need=n)),
+             lambda n: ops.layer_norm_backward(z(4, 8, need=n), t, one, s, s),
+             lambda n: ops.layer_norm_backward(t, t, one, s, s, dres=z(4, 8, need=n)),
+             lambda n: ops.cross_attention(z(2, 3, 4, 32, need=n), k, k),
+             lambda n: ops.cross_attention(q, z(2, 5, 2, 32, need=n), k),
+             lambda n: ops.cross_attention(q, k, z(2, 5, 2, 32, need=n)),
+             lambda n: ops.cross_attention_backward(z(2, 3, 4, 32, need=n), q, k, k, q, lse)]
+    for call in calls:
+        with pytest.raises(PtcgError, match="records? nothing for autograd"):
+            call(True)
+        with pytest.raises(PtcgError, match="CUDA"):                   # past that check
+            call(False)
+        with torch.no_grad(), pytest.raises(PtcgError, match="CUDA"):
+            call(True)
