@@ -572,14 +572,18 @@ long up256(long x) { return (x + 255) / 256 * 256; }
 // for before the call; the alignment-dependent choices do not change it.
 Plan plan(long n, int vocab, int width) {
     Plan p;
-    // 16 places a thread fill the SMs from 2.4 M places on; below, 4 give
-    // four times the blocks
-    p.items = n > 148L * SORT_T * 4 ? 16 : 4;
-    p.tiles = (int)cdiv(n, (long)SORT_T * p.items);
     int bits = 1;
     while (bits < 31 && (1L << bits) <= vocab) bits++;      // keys 0 .. vocab
     p.passes = (bits + MAX_BITS - 1) / MAX_BITS;
     p.bits = (bits + p.passes - 1) / p.passes;
+    // 4 places a thread give four times the blocks of 16, but sixteen times the
+    // counters that all blocks read, tiles^2 x bins: they are taken for one
+    // block a processor, or two where the digits have at most 7 bits.  Whole
+    // gradients of width 16 by 4 / 16 places, us: 4096 ids (7-bit digits) 600000
+    // places 70 / 107, 1.2 M 108 / 123, 1.6 M 145 / 129, 4 M 387 / 277; 65537 ids (9-bit
+    // digits) 600000 87 / 123, 620000 119 / 125, 1.2 M 156 / 139, 4 M 781 / 330
+    p.items = n > 148L * SORT_T * 4 * (p.bits <= 7 ? 2 : 1) ? 16 : 4;
+    p.tiles = (int)cdiv(n, (long)SORT_T * p.items);
     // about eight blocks a processor over all column slices, at least 8
     // places a lane group
     const int slices = (int)cdiv(width, 256);

@@ -90,6 +90,32 @@ def test_embedding_gradient(ops, dtype, n, vocab, width, how):
         assert torch.equal(acc[still], base[still])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,vocab,width,how", [
+    (9000, 2, 40, "any"), (300001, 5, 24, "any"), (605000, 70000, 3, "skew"), (620000, 70000, 8, "skew"),
+    (700001, 1000, 8, "skew"), (1212417, 3, 1, "any"), (1300001, 4096, 8, "skew"), (1 << 21, 1, 16, "any"),
+    (1 << 21, 4096, 40, "skew")])
+def test_embedding_gradient_exact_sums(ops, dtype, n, vocab, width, how):
+    """Whole numbers of -3 to 3, whose sums stay below 2^24 and so are exact in
+    fp32 in any order: not one place of a million may be lost or counted
+    twice.  On both sides of the sort's tile sizes."""
+    g = gen(n)
+    if how == "any":
+        ids = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    else:
+        ids = (torch.exp(torch.rand(n, generator=g, device="cuda") * math.log(vocab)).int() - 1).clamp(0, vocab - 1)
+    dout = torch.randint(-3, 4, (n, width), generator=g, device="cuda").to(dtype)
+    want = torch.zeros(vocab, width, dtype=torch.float64, device="cuda").index_add_(0, ids.long(), dout.double())
+    assert want.abs().max() * 4 < 2 ** 24 and 3 * n < 2 ** 24
+    got = ops.embedding_backward(dout, ids, vocab, scale=4.0)
+    assert torch.equal(got.double(), 4 * want)
+    pad = vocab // 3
+    base = torch.randint(-99, 99, (vocab, width), generator=g, device="cuda").float()
+    acc = ops.embedding_backward(dout, ids, vocab, pad_id=pad, dtable=base.clone(), accumulate=True)
+    want[pad] = 0
+    assert torch.equal(acc.double(), base.double() + want)
+
+
 def test_embedding_gradient_views(ops):
     g = gen(3)
     ids = torch.randint(0, 50, (6, 100), generator=g, device="cuda", dtype=torch.int32)
