@@ -133,11 +133,12 @@ __global__ void __launch_bounds__(SORT_T) k_sort_count(const __grid_constant__ S
 // place among the tile's places of that digit; the digits' first places.
 struct TileSort {
     uint16_t wcnt[SORT_T / 32][MAX_BINS];
-    uint32_t start[MAX_BINS], total[MAX_BINS], wsum[MAX_BINS / 32];
+    uint32_t start[MAX_BINS], wsum[MAX_BINS / 32];
 };
 // Where each of this thread's ITEMS places goes in its tile sorted by the digit
-// (stable: a warp holds 32 * ITEMS consecutive places, lane by lane).  Ends
-// with a barrier; t.start and t.total hold the digits' first places and counts.
+// (stable: a warp holds 32 * ITEMS consecutive places, lane by lane).  t.start
+// holds the digits' first places.  It is read, as t.wcnt is, after the last
+// barrier in here: a caller synchronises before it writes t or calls again.
 template <int ITEMS>
 PTCG_DEV void tile_places(TileSort& t, uint32_t (&to)[ITEMS], const uint32_t (&key)[ITEMS], int n, int shift, int bits) {
     constexpr int NW = SORT_T / 32;
@@ -167,7 +168,6 @@ PTCG_DEV void tile_places(TileSort& t, uint32_t (&to)[ITEMS], const uint32_t (&k
                 t.wcnt[w][tid] = (uint16_t)all;            // below the tile's 16384 places
                 all += v;
             }
-            t.total[tid] = all;
         }
         x = all;
         #pragma unroll
