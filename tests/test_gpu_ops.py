@@ -327,6 +327,21 @@ def test_layer_norm_huge_constant_rows(ops, at, width):
     assert ((rstd.double() / eps ** -0.5 - 1).abs() <= ref.FN).all()
 
 
+@pytest.mark.parametrize("xd,yd", list(itertools.product([F32, BF16], repeat=2)))
+@pytest.mark.parametrize("rows,width", [(1, 3), (70001, 64), (70001, 5), (6001, 1024), (40000, 255), (5003, 2050),
+                                        (3001, 5001), (2000, 8192)])
+def test_layer_norm_weight_gradients_exact_sums(ops, xd, yd, rows, width):
+    """Whole numbers of -3 to 3 with mean 0 and rstd 1 given, so that h = x and
+    all sums stay below 2^24: exact in any order, and no row may be missing."""
+    g = gen(rows)
+    x, dy = (torch.randint(-3, 4, (rows, width), generator=g, device="cuda").to(t) for t in (xd, yd))
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    _, dg, db = ops.layer_norm_backward(dy, x, None, mean, rstd)
+    assert 9 * rows < 2 ** 24
+    assert torch.equal(dg.double(), (dy.double() * x.double()).sum(0))
+    assert torch.equal(db.double(), dy.double().sum(0))
+
+
 @pytest.mark.parametrize("width,pitch,offset", [(37, 37, 0), (100, 100, 0), (37, 39, 1), (62, 62, 2), (130, 130, 0)])
 def test_layer_norm_gradient_of_huge_rows(ops, width, pitch, offset):
     """Constant rows so large that mean * rstd is past fp32's range: h is 0, and
