@@ -779,6 +779,75 @@ def test_two_streams_at_once(ops):
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
 
 
+def large_inputs(seed):
+    """Problems whose kernels have something to collide over: tcgen05 with all
+    of TMEM and split axes, single tokens in parts, a sort of several tiles."""
+    g = gen(seed)
+    q, k, v, _ = problem(seed, 1, 400, 2100, 2, 1, 128, BF16, "none")
+    q1, k1, v1, _ = problem(seed + 1, 3, 1, 9000, 8, 2, 64, BF16, "none")
+    n = torch.randint(0, 9001, (3,), generator=g, device="cuda", dtype=torch.int32)
+    ids = torch.randint(0, 700, (20000,), generator=g, device="cuda", dtype=torch.int32)
+    return [q, k, v, rand(g, *q.shape, dtype=BF16), q1, k1, v1, n, ids, rand(g, 20000, 48, dtype=BF16)]
+
+
+def large_calls(ops, q, k, v, dout, q1, k1, v1, n, ids, demb):
+    out, lse = ops.cross_attention(q, k, v)
+    grads = ops.cross_attention_backward(dout, q, k, v, out, lse)
+    return (out, lse, *grads, *ops.cross_attention(q1, k1, v1, kv_len=n),
+            ops.embedding_backward(demb, ids, 700))
+
+
+def test_two_streams_at_once_large(pkg, ops):
+    """Large calls that overlap on two streams share nothing."""
+    import ptcg_b200.native as n
+    sets = [large_inputs(s) for s in (81, 91)]
+    want = [large_calls(ops, *s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(large_calls(ops, *sets[i]))
+    torch.cuda.synchronize()
+    assert n.lib().ptcg_device_error() == 0
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_two_graphs_at_once_large(pkg, ops):
+    """Two captured graphs of large calls, replayed on two streams at the same
+    time, on inputs that were not there at the capture."""
+    import ptcg_b200.native as n
+    sets = [large_inputs(s) for s in (101, 111)]
+    want = [large_calls(ops, *s) for s in sets]
+    graphs = []
+    for _ in range(2):
+        inputs = large_inputs(121)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            large_calls(ops, *inputs)
+        torch.cuda.current_stream().wait_stream(side)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs = large_calls(ops, *inputs)
+        graphs.append((gr, inputs, outs, side))
+    for turn in range(4):
+        for i, (gr, inputs, outs, side) in enumerate(graphs):
+            for a, b in zip(inputs, sets[(i + turn) % 2]):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for gr, _, _, side in graphs:
+            with torch.cuda.stream(side):
+                gr.replay()
+        torch.cuda.synchronize()
+        assert n.lib().ptcg_device_error() == 0
+        for i, (gr, inputs, outs, side) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[(i + turn) % 2]))
+
+
 def test_under_an_autograd_function(ops):
     """The calls as the two passes of a Function: its leaves get the gradients
     that the calls return."""
