@@ -25,8 +25,10 @@ constexpr int MAXW = PTCG_LN_MAX_WIDTH;
 // one warp holds rows of up to 1024 columns, NV pieces of V columns per lane;
 // wider rows are shared by the warps of a block, 256 columns each, so that the
 // backward's registers per column still fit 1024 threads; blocks of up to 640
-// have registers for two rows at once (forward) or the next row's loads
-// (backward): 39 -> 35 and 72 -> 69 us at 4099 x 5001
+// have registers, 96 each, for two rows at once (forward) or the next row's
+// loads (backward): 47 + 90 us at 8192 x 5120 in bf16 against 58 + 118 under the
+// bound of 1024.  A bound of 672 threads, which would leave 96 registers too, takes
+// 57 + 111 there and no less at 5376
 constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MID_THREADS = 640, MAX_THREADS = MAXW / SHARED_COLS * 32;
 
 // Bound: HBM (2.1 M rows of 256, fp32 to bf16: forward 500 us, 6.5 TB/s; backward
@@ -442,12 +444,15 @@ int mode_of(int width, std::initializer_list<Rows> all) {
 // share of the rows in one go (a second, partial wave of blocks: 35.4
 // and 69 us at 4099 x 5001 instead of 24.7 and 55)
 int resident(int W) { return std::max(MID_THREADS / 32 / W, 1); }
-// blocks of the backward pass: as many as the processors hold (a multiple of
-// 4, as 148 is, for the phases), at most one per row group, so that each leaves one
-// partial row of the weight gradients
-int bwd_blocks(long rows, const Cfg& c) {
-    const long units = c.W ? rows : (rows + 7) / 8;
-    const long most = 148L * (c.W ? resident(c.W) : 4);
+// blocks of the backward pass: as many as the registers of a processor hold, some
+// 128 a thread up to 512 columns and 250 above (a multiple of 4, as 148 is, for
+// the phases), at most one per row group, so that each leaves one partial row of
+// the weight gradients.  1 / 2 / 4 blocks a processor, us: 2.1 M x 256, fp32 to
+// bf16, 1413 / 969 / 978; 100000 x 512 129 / 100 / 111; 50000 x 634 113 / 125 / 145; 50000
+// x 1024 113 / 129 / 158
+int bwd_blocks(long rows, int width) {
+    const long units = width > WARP_COLS ? rows : (rows + 7) / 8;
+    const long most = 148L * (width > WARP_COLS ? resident((int)cdiv(width, SHARED_COLS)) : width > 512 ? 1 : 2);
     return (int)(units < most ? units : most);
 }
 
@@ -535,7 +540,7 @@ int ptcg_layer_norm_fwd(const void* x, int x_dtype, long ldx, const float* gamma
 long ptcg_layer_norm_bwd_scratch(long rows, int width) {
     OP_REQ(rows >= 0 && width > 0 && width <= MAXW, -1,
            "layer norm gradient: bad sizes (rows %ld, width %d of at most %d)", rows, width, MAXW);
-    return 8L * width * bwd_blocks(rows, cfg_of(width, WHOLE));    // the same for every variant
+    return 8L * width * bwd_blocks(rows, width);    // the same for every variant
 }
 
 int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, int x_dtype,
@@ -566,7 +571,7 @@ int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, 
            "layer norm gradient: scratch of %ld bytes, %ld needed", scratch ? scratch_bytes : 0L, need);
     const Cfg c = cfg_of(width, mode_of(width, {{x, x_dtype, ldx}, {dy, dy_dtype, lddy}, {dx, x_dtype, lddx},
                                                 {dres, x_dtype, lddres}}));
-    const int blocks = bwd_blocks(rows, c);
+    const int blocks = bwd_blocks(rows, width);
     const BwdArgs a = {dx, lddx, dy, lddy, x, ldx, dres, lddres, gamma, mean, rstd, rows, width,
                        dgamma ? (float*)scratch : nullptr};
     if (x_dtype == PTCG_BF16) { if (dy_dtype == PTCG_BF16) bwd<bf16, bf16>(c, a, blocks, s); else bwd<bf16, float>(c, a, blocks, s); }
