@@ -517,9 +517,11 @@ int ptcg_layer_norm_bwd(const void* dy, int dy_dtype, long lddy, const void* x, 
  * zero for masked keys.  Each tensor has its own strides in elements:
  * element (s, row, head, d) at p + s * seq + row * row + head * head + d.
  * bf16 runs on tensor cores with fp32 sums (P and dS are rounded to bf16 as
- * operands); fp32 is fp32 throughout.  scale is positive and finite.  Rows must start on 16-byte boundaries (strides
- * multiples of 16 bytes).  Beside ptcg_attention_fwd / _bwd, which take
- * packed self-attention rows of width 32. */
+ * operands, and delta = dout . out comes from the rounded out); fp32 is fp32
+ * throughout.  scale is positive and finite, scale * log2 e too.  Rows must
+ * start on 16-byte boundaries (strides multiples of 16 bytes).  Beside
+ * ptcg_attention_fwd / _bwd, which take packed self-attention rows of width
+ * 32. */
 typedef struct PtcgHeads { long seq, row, head; } PtcgHeads;
 typedef struct PtcgCross {
     int dtype, nseq, lq, lk, heads, kv_heads, dh;

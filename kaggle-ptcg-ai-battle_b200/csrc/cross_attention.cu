@@ -2110,7 +2110,9 @@ int check(const PtcgCross* c) {
            c->lk, c->heads, c->kv_heads);
     OP_REQ(c->dh == 32 || c->dh == 64 || c->dh == 128, PTCG_EINVAL,
            "cross attention: head width %d is not 32, 64 or 128", c->dh);
-    OP_REQ(c->scale > 0.f && c->scale < INFINITY, PTCG_EINVAL, "cross attention: scale must be positive and finite");
+    // the exponentials are of 2
+    OP_REQ(c->scale > 0.f && c->scale * LOG2E < INFINITY, PTCG_EINVAL,
+           "cross attention: scale must be positive and finite, scale * log2 e too");
     const long rows = (long)c->heads / c->kv_heads * c->lq;
     OP_REQ(rows <= (1L << 30) && c->lk <= (1 << 30), PTCG_EINVAL, "cross attention: more than 2^30 rows");
     return PTCG_OK;

@@ -277,3 +277,10 @@ def test_torch_calls_refuse_what_autograd_would_lose(pkg):
             call(False)
         with torch.no_grad(), pytest.raises(PtcgError, match="CUDA"):
             call(True)
+
+
+def test_cross_attention_refuses_scales_that_overflow_in_base_2(lib):
+    c = desc(scale=3e38)
+    assert cross_fwd(lib, c) == EINVAL and b"scale" in lib.ptcg_last_error()
+    assert cross_bwd(lib, c) == EINVAL and lib.ptcg_cross_attention_fwd_scratch(c) == -1
+    assert lib.ptcg_cross_attention_fwd_scratch(desc(scale=2e38)) >= 0
