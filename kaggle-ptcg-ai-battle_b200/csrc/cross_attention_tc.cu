@@ -149,6 +149,16 @@ PTCG_DEV void stage_q(uint32_t dst, const CrossArgs& a, const Where& at, int r0,
     cp_wait<0>();
 }
 
+// start and end of a block's life with TMEM; warp 10 allocates and frees
+PTCG_DEV void tmem_alloc(uint32_t* slot) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(s_addr(slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+PTCG_DEV void tmem_free(uint32_t tmem) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
+}
+
 // ------------------------------------------------------------------ forward
 // One block per SM takes two 128-row tiles of the stacked rows and walks the
 // keys 128 at a time.  Warps 0-3 and 4-7 are the softmax of one tile each (a
@@ -162,7 +172,9 @@ PTCG_DEV void stage_q(uint32_t dst, const CrossArgs& a, const Where& at, int r0,
 // once S_t(j+1) is there, PV_t(j) is done and O_t may be rescaled.  A row's
 // maximum is raised (and O_t rescaled) only when it grew by more than 2^8:
 // until then the probabilities are at most 2^8 and the sum stays exact enough
-// in fp32, and the final division takes the common factor out.
+// in fp32, and the final division takes the common factor out.  P is rounded to
+// bf16 as an operand, at most 2^-8 of each probability, the size of the output's
+// own rounding; its sum is taken before that.
 // TMEM: S_0 0-127, S_1 128-255, O_0 256.., O_1 256 + DH.. .
 // Bound: the exponentials (16 a clock and SM) and, at DH 128, equally the
 // tensor core: 2048 clocks each per 256 x 128 scores.  131232 stacked rows on
@@ -228,11 +240,7 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
-    if (warp == 10) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     :: "r"(s_addr(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 10) tmem_alloc(tmem_slot);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -451,8 +459,7 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 10)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
+    if (warp == 10) tmem_free(tmem);
 }
 
 // ----------------------------------------------------------------- backward
@@ -462,7 +469,8 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
 // across blocks).  In both, blocks of 64 of the walked axis alternate between
 // two TMEM buffers, each with its own warpgroup, so that one block's products
 // run while the other's probabilities are computed; P and dS go to TMEM as
-// bf16 over the scores and are the A operands of the products after them.
+// bf16 (2^-8 of each, as the gradients' own rounding) over the scores and are the
+// A operands of the products after them.
 // Warps 0-3 and 4-7 compute (a TMEM lane per thread), a lane of warp 8 loads
 // by TMA, warp 9 prepares, warp 10 issues the MMAs.
 // Bound: the tensor core; a block of 128 x 64 scores takes 1024 clocks of
@@ -510,16 +518,6 @@ PTCG_DEV void write32(uint32_t taddr, float f, bool live, bool in, bf16* out, fl
                                           pack_bf2(o[8 * i + 4], o[8 * i + 5]), pack_bf2(o[8 * i + 6], o[8 * i + 7]));
     }
 }
-// start and end of a block's life with TMEM; warp 10 allocates and frees
-PTCG_DEV void tmem_alloc(uint32_t* slot) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(s_addr(slot)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-PTCG_DEV void tmem_free(uint32_t tmem) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
-}
-
 // dk, dv of 128 keys (M, a TMEM lane each).  Row blocks are taken per query
 // head (TMA fills rows past lq with zeros; their log-sum-exp counts as +inf).
 //   S^T = K Q^T, dP^T = V dO^T (N = 64 rows);  dV += P^T dO, dK += dS^T Q
