@@ -453,9 +453,10 @@ int ptcg_attention_bwd(int operand_dtype, const void* qkv, long ldqkv, const uns
                        void* dqkv, long lddqkv, float* dbias, int nseq, int L, int H,
                        void* stream);
 /* ---- decoder operators ------------------------------------------------------
- * The operators of a decoder that reads this model's encoder rows (options,
- * beams or drafted decks as queries, the board as states), for callers that
- * build one beside the policy: embedding, layer norm and cross attention,
+ * The operators of a decoder for callers that build one beside the policy
+ * (options, beams or drafted decks as queries; encoder rows or a cache of the
+ * caller's as states: the model calls return no trunk rows and take no gradient
+ * for them): embedding, layer norm and cross attention,
  * forward and backward.  They take no model; they run on the current device
  * and on `stream`, allocate nothing, wait for nothing on the host and can be
  * captured in a CUDA graph.  Element types are PTCG_FP32 / PTCG_BF16;
@@ -486,7 +487,9 @@ int ptcg_embedding_bwd(const void* dout, int dout_dtype, long lddo, const int* i
 /* Layer norm over rows of `width` <= PTCG_LN_MAX_WIDTH elements:
  * y = (x - mean) * rstd * gamma + beta, rstd = (var + eps)^(-1/2).  gamma /
  * beta NULL mean 1 / 0; mean / rstd (one float per row, what the backward
- * needs) may be NULL.  y may be x when the types and pitches agree.
+ * needs) may be NULL.  y may be x when the types and pitches agree.  The
+ * forward norms about the mean itself; the backward about the stored one, which
+ * is rounded to fp32 (half a last place of it, times rstd, in every h).
  * Backward: dx (x's type) = the gradient through the norm, plus dres (x's
  * type, may be NULL: the residual stream's own gradient); dgamma / dbeta
  * (fp32, both or neither) are written, or added to with accumulate != 0.
