@@ -335,7 +335,8 @@ __global__ void __launch_bounds__(WM * WN * 32, DH == 32 && WN == 1 ? 5 : 1) k_c
 // spends some 390 instructions a warp on every 64 keys besides the groups' own
 // 45 (staging, barriers, stages, masked groups' maxima); here that is paid once:
 // 1024 x 8 problems of 64 rows on 129 keys, width 32, 58 us against 75, 8192 x 8
-// of them 413 us (3.9 TB/s).  Bound: issue slots and shared memory about equally.
+// of them 413 us (3.9 TB/s).  Bound: issue slots (69 % taken) and shared memory
+// (42 % of its wavefronts).
 constexpr int SHORT_KEYS = 256;
 
 // mask words and score offsets of all keys (a multiple of 32 of them, up to
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(128) k_cross_join(const __grid_constant__ Cros
 // --------------------------------------------------------- bf16 backward
 // A quad's accumulators hold two columns of each 8-column piece per lane;
 // handed around, lane t has the whole of piece t out of four and stores 16
-// bytes: the short backward below takes 932 us so, 965 with 4-byte stores (the
+// bytes: the short backward below took 932 us so, 965 with 4-byte stores (the
 // forward has a third of its stores and loses by it, 413 to 418 us).
 PTCG_DEV uint4 quad_piece(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int t) {
     const bool odd = t & 1, hi = t & 2;
@@ -909,7 +910,9 @@ PTCG_DEV void put_dq(bf16* row, int t, int d0, bool in, float f, const float (&d
 // a key tile's dk and dv are finished at once.  S^T and dP^T have keys as rows
 // (16 a warp); dS^T goes through shared memory, from where the warps take it
 // transposed as the left operand of dq += dS k (16 rows and a share of the
-// columns each), which stays in registers over all keys.
+// columns each), which stays in registers over all keys.  512 x 8 problems of 64
+// rows on 600 keys of width 64, some 350 of them kept: 416 us (the tiled forward
+// 222); bound by latency: two blocks a processor, by their registers.
 template <int DH, int NR>                    // 16 NR rows
 __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const __grid_constant__ CrossArgs a) {
     constexpr int THREADS = 128, BM = NR * 16, BN = 64, KS = DH / 16, TILE = BN * DH * 2;
@@ -1106,10 +1109,10 @@ __global__ void __launch_bounds__(128, DH == 32 ? 4 : 1) k_cross_bwd_rows(const 
 // The same for keys that fit shared memory whole: every warp takes each fourth
 // 16-key group that has a kept key, dS^T of all of them is kept, and dq is one
 // product at the end; three barriers in all.  8192 x 8 problems of 64 rows on
-// 129 keys, width 32: 932 us (3.5 TB/s; with the forward 1351, in 64-key tiles
-// 1730).  Bound: 16 warps a processor, as shared memory allows, with 63 % of the
-// memory pipe's cycles (every warp reads q and dout as fragments, dS^T is
-// written and read back) and half of the issue slots taken.
+// 129 keys, width 32: 915 us (3.6 TB/s; with the forward 1318, in 64-key tiles
+// 1730).  Bound: 16 warps a processor, as shared memory allows, with half of
+// shared memory's wavefronts (every warp reads q and dout as fragments, dS^T is
+// written and read back) and of the issue slots taken, the tensor pipe at 25 %.
 template <int DH, int NR>                    // 16 NR rows
 __global__ void __launch_bounds__(128, DH == 32 ? 4 : DH == 64 ? 2 : 1) k_cross_bwd_short(const __grid_constant__ CrossArgs a) {
     constexpr int BM = NR * 16, KS = DH / 16, NT = BM / 8;
@@ -1323,7 +1326,9 @@ __global__ void __launch_bounds__(256) k_cross_sum(const __grid_constant__ Cross
 // 2 with expf), for 1 to 3 % less time (170 and 399 us below).
 // Bound: the multiply-adds and the reads from shared memory that
 // feed them: 512 x 8 problems of 61 rows on up to 186 keys of width 32 take
-// 176 us forward and 403 backward (18 TFLOP/s over the kept keys).
+// 176 us forward and 403 backward (18 TFLOP/s over the kept keys); single
+// tokens, 8 of them on caches of up to 20000 keys (8 heads on 2 of width 128),
+// 86 us, as 16 rows are computed for the 4 there are.
 template <int RT> PTCG_DEV int row_of(int ty, int i) {
     return RT == 8 ? (i >> 2) * 32 + ty * 4 + (i & 3) : ty * RT + i;
 }

@@ -178,7 +178,9 @@ PTCG_DEV void tmem_free(uint32_t tmem) {
 // TMEM: S_0 0-127, S_1 128-255, O_0 256.., O_1 256 + DH.. .
 // Bound: the exponentials (16 a clock and SM) and, at DH 128, equally the
 // tensor core: 2048 clocks each per 256 x 128 scores.  131232 stacked rows on
-// 8191 keys of width 128: 508 us, 1083 TFLOP/s, under the power cap.
+// 8191 keys of width 128: 508 us, 1083 TFLOP/s; the tensor and the exponentials'
+// pipes are busy 69 % each.  In a loop with the backward the power cap holds the
+// clock at 1792 of 1965 MHz.
 template <int DH> struct Fwd {
     static constexpr int NS = DH == 128 ? 2 : DH == 64 ? 4 : 7;       // K and V stages
     using T = Tile<DH, 128>;
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(Fwd<DH>::THREADS, 1) k_cross_fwd_tc(
 // Bound: the tensor core; a block of 128 x 64 scores takes 1024 clocks of
 // products in the first kernel and 768 in the second, 512 of exponentials.
 // The rows and keys above: dk and dv 1068 us (1030 TFLOP/s of its own four
-// products), dq 757 us (1090 of three).
+// products), dq 757 us (1090 of three); the tensor pipe is busy 62 and 59 %.
 constexpr int BB = 64;                       // rows or keys of a block
 constexpr int ONE_PER_SM = 120 * 1024;       // shared memory that keeps a second block off the processor
 

@@ -31,10 +31,11 @@ constexpr int MAXW = PTCG_LN_MAX_WIDTH;
 // 57 + 111 there and no less at 5376
 constexpr int WARP_COLS = 1024, SHARED_COLS = 256, MID_THREADS = 640, MAX_THREADS = MAXW / SHARED_COLS * 32;
 
-// Bound: HBM (2.1 M rows of 256, fp32 to bf16: forward 500 us, 6.5 TB/s; backward
-// with the residual's gradient 1146 us, 6.6 TB/s); wide rows are bound by the
-// latency of a row's loads and barriers (50000 x 2048, fp32 to bf16: 114 us, 5.4
-// TB/s, and 225, 4.5; 4099 x 5001 in bf16: 29 us, 2.8 TB/s, and 55, 2.2).  A row
+// Bound: HBM (2.1 M rows of 256, fp32 to bf16: forward 502 us, 6.5 TB/s; backward
+// with the residual's gradient 1146 us, 6.6 TB/s); wider rows are bound by the
+// latency of a row's loads and barriers (fp32 to bf16, 50000 x 1024: 54 us, 5.7
+// TB/s, and 101, 5.1; 50000 x 2048: 123, 5.0, and 237, 4.3; in bf16, 4099 x 5001:
+// 31, 2.7, and 57, 2.2; 8192 x 8192: 78, 3.5, and 133, 3.0).  A row
 // belongs to one warp (width <= 1024, eight rows to a block) or to the W warps
 // of a block (MULTI).  Lane l of warp w owns pieces w * 32 * NV + l, + 32, .. so
 // that a warp's accesses are contiguous.
@@ -406,9 +407,10 @@ __global__ void __launch_bounds__(256) k_layer_norm_wgrad(
 // The variant of a row width: V-column pieces, NV of them per lane, W warps a
 // row (0: one warp a row, eight rows a block).  Rows that start on 4-element
 // boundaries and a width of fours take them whole, other rows PHASED where all
-// tensors' rows start at the same phase (4099 x 5001 in bf16: 24.8 + 55.5 us
-// forward and backward against 32.5 + 59.5 with single elements; 50000 x 634
-// in fp32: 74 + 119 against 76 + 128), the rest single elements.
+// tensors' rows start at the same phase (4099 x 5001 fp32 to bf16: 39 + 64 us
+// forward and backward against 43 + 82 with single elements, in bf16 31 + 71
+// against 43 + 72; 50000 x 634 in fp32: 78 + 121 against 90 + 113), the rest
+// single elements.
 enum { SINGLE = 0, WHOLE = 1, PHASED4 = 2 };
 struct Cfg { int mode, NV, W; };
 Cfg cfg_of(int width, int mode) {
@@ -441,8 +443,9 @@ int mode_of(int width, std::initializer_list<Rows> all) {
     return whole ? WHOLE : same ? PHASED4 : SINGLE;
 }
 // blocks of W warps that a processor's registers hold: each then takes its
-// share of the rows in one go (a second, partial wave of blocks: 35.4
-// and 69 us at 4099 x 5001 instead of 24.7 and 55)
+// share of the rows in one go (twice as many blocks, fp32 to bf16: 41 + 70 us
+// forward and backward at 4099 x 5001 instead of 39 + 64, 133 + 280 at 50000 x 2048
+// instead of 123 + 237)
 int resident(int W) { return std::max(MID_THREADS / 32 / W, 1); }
 // blocks of the backward pass: as many as the registers of a processor hold, some
 // 128 a thread up to 512 columns and 250 above (a multiple of 4, as 148 is, for
