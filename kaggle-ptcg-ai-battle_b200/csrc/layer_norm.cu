@@ -13,7 +13,7 @@
 // gamma) or, squared, lie past its range.  Such rows take the mean of the
 // deviations as well, a third sum, and are normed about both, their variance too; summed beside the squares in every row it would cost
 // 3 to 20 % of the time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 124
-// by need).
+// by need, or 156 where every row lies 100 deviations from 0; 2.1 M x 256 508 and 518).
 #include <algorithm>
 #include <initializer_list>
 
@@ -186,23 +186,34 @@ __global__ void __launch_bounds__(MULTI ? MULTI : 256) k_layer_norm_fwd(
                 }
             }
             row_sums<MULTI>(d, far_red, 0, w, lane, W);
+            // sum (d - dm)^2 = sum d^2 - dm sum d, or summed again where little is
+            // left of it or it was past fp32's range
+            bool again = false;
             #pragma unroll
             for (int j = 0; j < R; j++) {
                 // divided, so that equal deviations (a constant row) leave nothing
                 dm[j] = d[j] / (float)width;
-                s[j] = edge ? se[j][0] - mu[j] - dm[j] : 0.f;
-                s[j] *= s[j];
+                const float left = fmaf(-d[j], dm[j], s[j]);
+                again = again || !(left >= 0.25f * s[j]) || s[j] == INFINITY;
+                s[j] = left;
+            }
+            if (again) {
                 #pragma unroll
-                for (int k = 0; k < NV; k++) {
-                    const bool in = cols.has(piece_at<V, NV>(w, lane, k));
+                for (int j = 0; j < R; j++) {
+                    s[j] = edge ? se[j][0] - mu[j] - dm[j] : 0.f;
+                    s[j] *= s[j];
                     #pragma unroll
-                    for (int e = 0; e < V; e++) {
-                        const float x = in ? v[j][k][e] - mu[j] - dm[j] : 0.f;
-                        s[j] = fmaf(x, x, s[j]);
+                    for (int k = 0; k < NV; k++) {
+                        const bool in = cols.has(piece_at<V, NV>(w, lane, k));
+                        #pragma unroll
+                        for (int e = 0; e < V; e++) {
+                            const float x = in ? v[j][k][e] - mu[j] - dm[j] : 0.f;
+                            s[j] = fmaf(x, x, s[j]);
+                        }
                     }
                 }
+                row_sums<MULTI>(s, far_red, 1, w, lane, W);
             }
-            row_sums<MULTI>(s, far_red, 1, w, lane, W);
         }
         #pragma unroll
         for (int j = 0; j < R; j++) {
