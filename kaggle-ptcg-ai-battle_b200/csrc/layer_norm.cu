@@ -11,9 +11,10 @@
 // some of its last places, which in a row far from 0 are not small beside its
 // deviations or sqrt(eps) (at 12345 one of them moves a constant row's y by 0.3
 // gamma) or, squared, lie past its range.  Such rows take the mean of the
-// deviations as well, a third sum, and are normed about both, their variance too; summed beside the squares in every row it would cost
-// 3 to 20 % of the time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 124
-// by need, or 156 where every row lies 100 deviations from 0; 2.1 M x 256 508 and 518).
+// deviations as well, a third sum, and are normed about both, their variance
+// too; summed beside the squares in every row it would cost 3 to 20 % of the
+// time (50000 x 2048, fp32 to bf16: 117 us without it, 137 so, 124 by need, or 156
+// where every row lies 100 deviations from 0; 2.1 M x 256 508 and 518).
 #include <algorithm>
 #include <initializer_list>
 
