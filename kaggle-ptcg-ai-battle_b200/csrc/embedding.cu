@@ -321,10 +321,10 @@ __global__ void __launch_bounds__(SORT_T) k_sort_small(const __grid_constant__ S
 // as a partial: the block joins its groups' partials in order through shared
 // memory, and k_embed_join joins the blocks'.  Rows without a place are
 // zeroed by extra blocks.  Bound: HBM, dout read once as gathered rows: 2 M
-// bf16 rows of 128 into 4096 103 us (5.2 TB/s; 111 with three blocks a
+// bf16 rows of 128 into 4096 111 us (4.8 TB/s; 120 with three blocks a
 // processor, which their registers would leave), as many fp32 rows 166 us (6.5
-// TB/s), 32768 bf16 rows of 1024 into 65537 62 us
-// (5.5 TB/s with the table's zeros).
+// TB/s), 32768 bf16 rows of 1024 into 65537 61 us (5.5 TB/s with the table's
+// zeros).
 constexpr int MAX_CHUNK = 2048;
 enum { SEG_HEAD = 1, SEG_THROUGH = 2, SEG_TAIL = 4 };
 
